@@ -21,7 +21,8 @@
  *    text). Device-side anomalies (a bounded wait that ran out) are written to *status
  *    (a zero-initialised device uint32, optional) as (code << 24 | detail); see pith_status_string.
  *    Codes: 1 a barrier wait inside a kernel ran out, 2 unexpected TMEM allocation, 3 a wait for a ring neighbour
- *    ran out, 4 a kernel found its shared-memory window misaligned. A launch that finds the word non-zero does no work.
+ *    ran out, 4 a kernel found its shared-memory window misaligned, 5 a slot, page, length or position given to a
+ *    latent-cache entry was out of range (nothing outside the tensors is touched). A launch that finds the word non-zero does no work.
  *  - Re-entrant; no internal threads; no global mutable state besides, per device, one side stream with two
  *    events used by pith_attn_bwd (created on first use) and the device address of the scratch area of
  *    pith_attn_bwd_noalloc (looked up on its first call; it does not survive cudaDeviceReset).
@@ -65,6 +66,7 @@ extern "C" {
 /* element types for pith_combine_args.out*_dtype */
 #define PITH_DTYPE_BF16 0
 #define PITH_DTYPE_F32 1
+#define PITH_DTYPE_E4M3 2 /* pith_latent_cache.dtype only */
 
 typedef struct pith_attn_fwd_args {
   const void* q;          /* [B][Sq][Hq][Dqk] bf16 */
@@ -338,6 +340,57 @@ typedef struct pith_mla_assemble_args {
  */
 int pith_mla_assemble_fwd(const pith_mla_assemble_args* args, void* stream);
 int pith_mla_assemble_bwd(const pith_mla_assemble_args* args, void* stream);
+
+/*
+ * ---- Latent cache of multi-head latent attention (MLA) ----
+ * Per token the cache holds the normalised 512-wide latent vector from which the layer's kv_b_proj produces k_nope and v
+ * of every head, and the 64-wide rotated key that all heads share. No counterpart in the reference, which trains and
+ * keeps no cache; the arithmetic in front is that of pithtrain/models/deepseek_v2_lite.py:426-454.
+ */
+typedef struct pith_latent_cache {
+  void* latent;              /* [pages][page_size][512]: bf16, or e4m3 with one factor a row */
+  void* rope;                /* [pages][page_size][64] bf16, de-interleaved and rotated */
+  float* scale;              /* [pages][page_size] fp32, e4m3 only: row = stored * scale */
+  int32_t dtype;             /* PITH_DTYPE_BF16 or PITH_DTYPE_E4M3 */
+  int32_t pages, page_size;  /* page_size 16, 32 or a multiple of 64 */
+  int64_t latent_stride[2], rope_stride[2], scale_stride[2]; /* page, row (elements); innermost contiguous */
+} pith_latent_cache;
+
+typedef struct pith_latent_write_args {
+  pith_latent_cache cache;
+  const void* compressed_kv; /* [B][S][512] bf16, before the norm */
+  const void* k_pe;          /* [B][S][64] bf16, interleaved rotary pairs */
+  const void* norm_weight;   /* [512] weight_dtype */
+  const void* cos;           /* [table_rows][64] cs_dtype with `positions`, else [B or 1][S][64] */
+  const void* sin;
+  const int64_t* slots;      /* [B][S]: page * page_size + row; negative = this token is not stored */
+  const int64_t* positions;  /* optional [B][S]: rows of cos / sin */
+  uint32_t* status;
+  int32_t B, S;
+  int32_t weight_dtype, cs_dtype; /* PITH_DTYPE_BF16 or PITH_DTYPE_F32 */
+  int64_t table_rows;
+  float eps;
+  int64_t kv_stride[2], k_pe_stride[2], cs_stride[2], slots_stride[2], positions_stride[2]; /* b, s (elements) */
+} pith_latent_write_args;
+
+/*
+ * RMSNorm of the compressed latent, rotary embedding of k_pe (as pith_mla_assemble_fwd) and the store of both at
+ * `slots`, in one pass: fp32 arithmetic with one rounding. An e4m3 row gets the least power of two as its factor with
+ * which no value passes 448. The slots of one call have to differ.
+ */
+int pith_latent_write(const pith_latent_write_args* args, void* stream);
+
+typedef struct pith_latent_read_args {
+  pith_latent_cache cache;
+  const int64_t* slots;  /* [n] contiguous; negative = zeros */
+  void* latent;          /* [n][512] bf16, written */
+  void* k_pe;            /* [n][64] bf16, written */
+  uint32_t* status;
+  int64_t n;
+} pith_latent_read_args;
+
+/* Gathers rows of the cache as bf16 (an e4m3 row times its power-of-two factor is exact in bf16). */
+int pith_latent_read(const pith_latent_read_args* args, void* stream);
 
 /* Text of the last host-side rejection on the calling thread. */
 const char* pith_last_error(void);

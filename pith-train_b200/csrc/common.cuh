@@ -21,7 +21,9 @@ enum : uint32_t {
   kErrWaitTimeout = 1u,   // an mbarrier wait ran out of cycles
   kErrTmemAlloc = 2u,     // TMEM allocation returned an unexpected base
   kErrSmemAlign = 4u,     // the dynamic shared-memory window does not start on a 1024-byte boundary (3 = peer wait)
+  kErrIndex = 5u,         // an index given to a latent-cache entry is out of range; detail = kIdx*
 };
+enum : uint32_t { kIdxSlot = 1u, kIdxPosition = 2u, kIdxPage = 3u, kIdxLength = 4u };
 
 struct AbortCtl {
   uint32_t* status;         // global status word (may be nullptr)

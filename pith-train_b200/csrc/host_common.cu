@@ -60,7 +60,9 @@ int make_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int64_t 
                            (cuuint64_t)(sb * elem_bytes)};
   cuuint32_t box[4] = {(cuuint32_t)box_d, 1u, (cuuint32_t)box_rows, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  CUtensorMapDataType dt = elem_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                           : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = fn(out, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(kErrCuda, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
@@ -86,6 +88,10 @@ const char* pith_status_string(uint32_t status) {
     snprintf(buf, sizeof buf, "unexpected TMEM allocation (0x%06x)", detail);
   else if (code == pith::kErrSmemAlign)
     snprintf(buf, sizeof buf, "shared-memory window not 1024-byte aligned (offset 0x%06x)", detail);
+  else if (code == pith::kErrIndex)
+    snprintf(buf, sizeof buf, "%s given to a latent-cache operator is out of range",
+             detail == pith::kIdxSlot ? "a slot" : detail == pith::kIdxPosition ? "a position" :
+             detail == pith::kIdxPage ? "a page of the block table" : "a sequence length");
   else
     snprintf(buf, sizeof buf, "unknown device status 0x%08x", status);
   return buf;

@@ -9,6 +9,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include "../../include/pith_b200.h"
+
 namespace pith {
 
 enum : int {
@@ -46,9 +48,12 @@ int require_sm100();
 
 // Builds a 4-D tiled tensor map over a [B][S][H][D] tensor (dims given innermost first:
 // D, H, S, B) with a {box_d, 1, box_rows, 1} box and the 128-byte shared-memory swizzle.
-// strides_elems = {b, s, h}. elem_bytes = 2 (bf16) or 4 (fp32).
+// strides_elems = {b, s, h}. elem_bytes = 1 (8-bit), 2 (bf16) or 4 (fp32).
 int make_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int64_t B, int64_t S, int64_t H, int64_t D,
                     const int64_t strides_elems[3], int box_d, int box_rows);
+
+// Checks the planes of a latent cache (pointers, alignment, strides, sizes). Defined in latent_cache.cu.
+int check_latent_cache(const pith_latent_cache& c);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -121,6 +121,33 @@ class MlaAssembleArgs(Structure):
     ]
 
 
+class LatentCacheArgs(Structure):
+    _fields_ = [
+        ("latent", c_void_p), ("rope", c_void_p), ("scale", c_void_p),
+        ("dtype", c_int32), ("pages", c_int32), ("page_size", c_int32),
+        ("latent_stride", I64x2), ("rope_stride", I64x2), ("scale_stride", I64x2),
+    ]
+
+
+class LatentWriteArgs(Structure):
+    _fields_ = [
+        ("cache", LatentCacheArgs),
+        ("compressed_kv", c_void_p), ("k_pe", c_void_p), ("norm_weight", c_void_p), ("cos", c_void_p),
+        ("sin", c_void_p), ("slots", c_void_p), ("positions", c_void_p), ("status", c_void_p),
+        ("B", c_int32), ("S", c_int32), ("weight_dtype", c_int32), ("cs_dtype", c_int32),
+        ("table_rows", c_int64), ("eps", c_float),
+        ("kv_stride", I64x2), ("k_pe_stride", I64x2), ("cs_stride", I64x2), ("slots_stride", I64x2),
+        ("positions_stride", I64x2),
+    ]
+
+
+class LatentReadArgs(Structure):
+    _fields_ = [
+        ("cache", LatentCacheArgs), ("slots", c_void_p), ("latent", c_void_p), ("k_pe", c_void_p),
+        ("status", c_void_p), ("n", c_int64),
+    ]
+
+
 NOALLOC_SCRATCH_BYTES = 32 << 20
 FWD_O_FP32 = 1
 BWD_SERIAL = 1
@@ -132,6 +159,7 @@ FWD_CTA_PAIR = 8
 COMBINE_NATURAL = 1
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_E4M3 = 2
 
 # Every symbol include/pith_b200.h declares: name -> (restype, argtypes)
 EXPORTS = {
@@ -155,6 +183,8 @@ EXPORTS = {
     "pith_qk_norm_rope_bwd": (c_int, [POINTER(QkNormRopeArgs), c_void_p]),
     "pith_mla_assemble_fwd": (c_int, [POINTER(MlaAssembleArgs), c_void_p]),
     "pith_mla_assemble_bwd": (c_int, [POINTER(MlaAssembleArgs), c_void_p]),
+    "pith_latent_write": (c_int, [POINTER(LatentWriteArgs), c_void_p]),
+    "pith_latent_read": (c_int, [POINTER(LatentReadArgs), c_void_p]),
     "pith_last_error": (c_char_p, []),
     "pith_status_string": (c_char_p, [c_uint32]),
     "pith_abi_version": (c_int, []),

@@ -423,3 +423,104 @@ def mla_assemble_bwd(cos, sin, dquery, dkey, dvalue):
     _lib.check(_lib.load().pith_mla_assemble_bwd(ctypes.byref(a), _stream(dquery)), "pith_mla_assemble_bwd")
     _count(1 if dq.numel() else 0)
     return dq, dkv, dk_pe
+
+
+# --------------------------------------------------------------------------- MLA latent cache
+_NUMBER = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
+def _one_device(device, **ts):
+    """CUDA tensors of one device: a kernel launched on `device` reads and writes all of them."""
+    for name, t in ts.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device.type != "cuda":
+        raise RuntimeError("pith_b200 operators run on CUDA tensors only (no CPU fallback)")
+
+
+def _bs(t: torch.Tensor) -> I64x2:
+    """b and s strides of a [B or 1, S, ...] tensor; a batch of one is broadcast."""
+    return I64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1))
+
+
+def _rotary(a, cos, sin, position_ids, B: int, S: int) -> None:
+    """Fills cos / sin / positions of an argument struct after checking them: tables [rows, 64] with position_ids
+    [B or 1, S], or [B or 1, S, 64] (or tables: rows 0 .. S - 1) without."""
+    if cos.dtype not in _NUMBER or sin.dtype != cos.dtype:
+        raise TypeError("cos and sin must both be bfloat16 or float32")
+    if cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(-1) != 1 or cos.shape[-1] != 64:
+        raise ValueError("cos and sin must be [..., 64] with a contiguous last dimension, equal shapes and strides")
+    if position_ids is not None:
+        if cos.dim() != 2:
+            raise ValueError(f"with position_ids, cos and sin are tables [rows, 64], got {tuple(cos.shape)}")
+        if position_ids.dtype != torch.int64:
+            raise TypeError("position_ids must be int64")
+        if position_ids.dim() != 2 or position_ids.shape[0] not in (1, B) or position_ids.shape[1] != S:
+            raise ValueError(f"position_ids has shape {tuple(position_ids.shape)}, expected {(B, S)}")
+        a.positions, a.positions_stride = position_ids.data_ptr(), _bs(position_ids)
+        a.cs_stride = I64x2(0, cos.stride(0))
+        a.table_rows = cos.shape[0]
+    elif cos.dim() == 2:
+        if cos.shape[0] < S:
+            raise ValueError(f"cos and sin have {cos.shape[0]} rows, {S} are needed")
+        a.cs_stride = I64x2(0, cos.stride(0))
+    else:
+        if cos.dim() != 3 or cos.shape[0] not in (1, B) or cos.shape[1] != S:
+            raise ValueError(f"cos and sin have shape {tuple(cos.shape)}, expected [B or 1, {S}, 64]")
+        a.cs_stride = _bs(cos)
+    a.cos, a.sin, a.cs_dtype = cos.data_ptr(), sin.data_ptr(), _NUMBER[cos.dtype]
+
+
+def latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps: float, position_ids=None) -> None:
+    """RMSNorm + rotary embedding of new tokens and their store in the cache; see ``pith_latent_write``."""
+    if k_pe.dim() == 4 and k_pe.shape[2] == 1:
+        k_pe = k_pe[:, :, 0]
+    if compressed_kv.dim() != 3 or compressed_kv.shape[2] != 512 or compressed_kv.stride(2) != 1:
+        raise ValueError(f"compressed_kv must be [B,S,512] with a contiguous last dimension, got "
+                         f"{tuple(compressed_kv.shape)}")
+    B, S, _ = compressed_kv.shape
+    if tuple(k_pe.shape) != (B, S, 64) or k_pe.stride(2) != 1:
+        raise ValueError(f"k_pe must be [B,S,64] or [B,S,1,64] with a contiguous last dimension, got {tuple(k_pe.shape)}")
+    if compressed_kv.dtype != torch.bfloat16 or k_pe.dtype != torch.bfloat16:
+        raise TypeError("compressed_kv and k_pe must be bfloat16")
+    if norm_weight.dtype not in _NUMBER:
+        raise TypeError("norm_weight must be bfloat16 or float32")
+    if tuple(norm_weight.shape) != (512,) or not norm_weight.is_contiguous():
+        raise ValueError("norm_weight must be contiguous [512]")
+    if slots.dtype != torch.int64:
+        raise TypeError("slots must be int64")
+    _expect(slots, (B, S), "slots")
+    a = _lib.LatentWriteArgs()
+    _rotary(a, cos, sin, position_ids, B, S)
+    dev = compressed_kv.device
+    _one_device(dev, k_pe=k_pe, norm_weight=norm_weight, cos=cos, sin=sin, slots=slots, position_ids=position_ids,
+                cache=cache.latent)
+    a.cache = cache.args
+    a.compressed_kv, a.k_pe, a.norm_weight = compressed_kv.data_ptr(), k_pe.data_ptr(), norm_weight.data_ptr()
+    a.slots, a.status = slots.data_ptr(), status_word(dev).data_ptr()
+    a.B, a.S, a.eps, a.weight_dtype = B, S, float(eps), _NUMBER[norm_weight.dtype]
+    a.kv_stride = I64x2(compressed_kv.stride(0), compressed_kv.stride(1))
+    a.k_pe_stride = I64x2(k_pe.stride(0), k_pe.stride(1))
+    a.slots_stride = I64x2(slots.stride(0), slots.stride(1))
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pith_latent_write(ctypes.byref(a), _stream(slots)), "pith_latent_write")
+    _count(1 if B * S else 0)
+
+
+def latent_read(cache, slots):
+    """(latent bf16 [..., 512], k_pe bf16 [..., 64]) of the given slots; see ``pith_latent_read``."""
+    if slots.dtype != torch.int64:
+        raise TypeError("slots must be int64")
+    dev = slots.device
+    _one_device(dev, cache=cache.latent)
+    slots = slots.contiguous()
+    latent = torch.empty((*slots.shape, 512), dtype=torch.bfloat16, device=dev)
+    k_pe = torch.empty((*slots.shape, 64), dtype=torch.bfloat16, device=dev)
+    a = _lib.LatentReadArgs()
+    a.cache = cache.args
+    a.slots, a.latent, a.k_pe = slots.data_ptr(), latent.data_ptr(), k_pe.data_ptr()
+    a.status, a.n = status_word(dev).data_ptr(), slots.numel()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pith_latent_read(ctypes.byref(a), _stream(slots)), "pith_latent_read")
+    _count(1 if a.n else 0)
+    return latent, k_pe

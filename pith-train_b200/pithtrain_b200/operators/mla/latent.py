@@ -1,0 +1,112 @@
+"""Sampling from an MLA layer: a paged cache of the shared latent vectors, and attention in the absorbed form over it.
+
+The training path expands every token's 512-wide latent vector into keys and values of all heads
+(``kv_b_proj``, pithtrain/models/deepseek_v2_lite.py:426-454) and attends to those (``MLA``). Token by token that would
+recompute or store ``16 * (192 + 128)`` values a token. Here a token costs 512 + 64: its normalised latent vector ``c``
+and the rotated key ``r`` that all heads share. With ``W_k[h] [128, 512]`` and ``W_v[h] [128, 512]`` the two halves of
+head h's block of ``kv_b_proj.weight``,
+
+    q_nope . (W_k c) = (q_nope W_k) . c        and        sum_n p_n W_v c_n = W_v (sum_n p_n c_n),
+
+so the query takes ``W_k`` in, attention runs on the latent vectors themselves, and its result goes through ``W_v``.
+
+These operators have no gradients (training keeps the expanded form): under grad mode, inputs that require one are
+refused. Sizes are DeepSeek-V2-Lite's (latent 512, rope 64, nope 128, v 128), any number of heads; bf16, CUDA only.
+Indices are read on the device, so a slot, page, position or length out of range cannot raise at the call: nothing
+outside the tensors is touched, the error is recorded, later kernels of the library skip their work, and
+``pithtrain_b200.kernels.check_device_status()`` raises. A sampling loop calls it where it fetches its tokens.
+"""
+
+from __future__ import annotations
+
+import torch
+
+
+def _kernels():
+    from ... import kernels
+    return kernels
+
+
+def _no_gradient(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+class LatentCache:
+    """Planes of a paged latent cache: ``latent`` [pages, page_size, 512] (bfloat16 or float8_e4m3fn), ``rope``
+    [pages, page_size, 64] bfloat16, and for float8_e4m3fn ``scale`` [pages, page_size] float32 (a row's values are
+    stored * scale). A slot is ``page * page_size + row``. ``page_size`` is 16, 32 or a multiple of 64; planes may be
+    strided (a layer of a larger tensor) as long as rows are contiguous. The object keeps no state besides the tensors.
+    """
+
+    def __init__(self, latent: torch.Tensor, rope: torch.Tensor, scale: torch.Tensor | None = None):
+        if latent.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or rope.dtype != torch.bfloat16:
+            raise TypeError("latent must be bfloat16 or float8_e4m3fn, rope bfloat16")
+        if latent.dim() != 3 or latent.shape[2] != 512 or latent.stride(2) != 1:
+            raise ValueError(f"latent must be [pages, page_size, 512] with a contiguous last dimension, got "
+                             f"{tuple(latent.shape)}")
+        pages, page_size, _ = latent.shape
+        if pages < 1 or not (page_size in (16, 32) or (page_size > 0 and page_size % 64 == 0)):
+            raise ValueError(f"page_size must be 16, 32 or a multiple of 64, got {pages} pages of {page_size}")
+        if pages * page_size >= 2 ** 31:
+            raise ValueError(f"{pages} pages of {page_size} rows: a cache holds at most 2^31 - 1 rows")
+        if tuple(rope.shape) != (pages, page_size, 64) or rope.stride(2) != 1:
+            raise ValueError(f"rope must be {(pages, page_size, 64)} with a contiguous last dimension, got "
+                             f"{tuple(rope.shape)}")
+        if (scale is None) != (latent.dtype == torch.bfloat16):
+            raise ValueError("an 8-bit cache has a scale plane, a bfloat16 cache has none")
+        if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != (pages, page_size)):
+            raise ValueError(f"scale must be float32 {(pages, page_size)}")
+        for name, t in (("rope", rope), ("scale", scale)):
+            if t is not None and t.device != latent.device:
+                raise ValueError(f"{name} is on {t.device}, latent on {latent.device}")
+        self.latent, self.rope, self.scale = latent, rope, scale
+        from ... import _lib
+        a = self.args = _lib.LatentCacheArgs()
+        a.latent, a.rope = latent.data_ptr(), rope.data_ptr()
+        a.scale = scale.data_ptr() if scale is not None else None
+        a.dtype = _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3
+        a.pages, a.page_size = pages, page_size
+        a.latent_stride = _lib.I64x2(latent.stride(0), latent.stride(1))
+        a.rope_stride = _lib.I64x2(rope.stride(0), rope.stride(1))
+        if scale is not None:
+            a.scale_stride = _lib.I64x2(scale.stride(0), scale.stride(1))
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        """A cache of zeroed planes; ``dtype`` bfloat16 (1152 bytes a token) or float8_e4m3fn (644)."""
+        scale = torch.ones((num_pages, page_size), dtype=torch.float32, device=device) \
+            if dtype == torch.float8_e4m3fn else None
+        return cls(torch.zeros((num_pages, page_size, 512), dtype=dtype, device=device),
+                   torch.zeros((num_pages, page_size, 64), dtype=torch.bfloat16, device=device), scale)
+
+    @property
+    def num_pages(self) -> int:
+        return self.latent.shape[0]
+
+    @property
+    def page_size(self) -> int:
+        return self.latent.shape[1]
+
+
+def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: torch.Tensor, k_pe: torch.Tensor,
+                       norm_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, eps: float,
+                       position_ids: torch.Tensor | None = None) -> None:
+    """Normalises (RMSNorm), rotates and stores new tokens: compressed_kv ``[B,S,512]`` and k_pe ``[B,S,64]`` or
+    ``[B,S,1,64]`` bf16 are the two parts of ``kv_a_proj_with_mqa``'s output (views are fine), ``norm_weight`` / ``eps``
+    those of ``kv_a_layernorm``; slots int64 ``[B,S]``, negative for tokens that are not to be stored. The slots of one
+    call have to differ, as the indices of ``torch.Tensor.index_put_``.
+
+    cos / sin (bf16 or fp32): tables ``[rows, 64]`` with ``position_ids`` int64 ``[B or 1, S]``, or ``[B or 1, S, 64]``
+    already gathered. fp32 arithmetic, one rounding to the cache's type; an 8-bit row gets the least power of two as its
+    scale with which no value passes 448.
+    """
+    _no_gradient("latent_cache_write", compressed_kv, k_pe, norm_weight)
+    _kernels().latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
+
+
+def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
+    """Rows of the cache as bf16, ``(latent [*slots.shape, 512], k_pe [*slots.shape, 64])``: what the expanded form of a
+    prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
+    give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
+    return _kernels().latent_read(cache, slots)

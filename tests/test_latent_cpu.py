@@ -1,0 +1,128 @@
+"""Argument checks of the MLA latent-cache operators that need no GPU: the Python layer and the C ABI."""
+
+import ctypes
+
+import pytest
+import torch
+
+from pithtrain_b200.operators import mla
+
+BF = torch.bfloat16
+
+
+def cache(dtype=BF, pages=2, page=16):
+    return mla.LatentCache.allocate(pages, page, dtype, device="cpu")
+
+
+def write_args(B=1, S=2):
+    return dict(slots=torch.zeros(B, S, dtype=torch.int64), compressed_kv=torch.zeros(B, S, 512, dtype=BF),
+                k_pe=torch.zeros(B, S, 64, dtype=BF), norm_weight=torch.ones(512), cos=torch.ones(8, 64),
+                sin=torch.zeros(8, 64), eps=1e-6)
+
+
+def test_cache_planes_are_checked():
+    c = cache(torch.float8_e4m3fn, 3, 32)
+    assert (c.num_pages, c.page_size) == (3, 32) and c.scale.shape == (3, 32)
+    lat, rope, scale = torch.zeros(2, 16, 512, dtype=BF), torch.zeros(2, 16, 64, dtype=BF), torch.ones(2, 16)
+    with pytest.raises(ValueError, match="page_size"):
+        cache(page=48)
+    with pytest.raises(ValueError, match="has none"):
+        mla.LatentCache(lat, rope, scale)
+    with pytest.raises(ValueError, match="scale plane"):
+        mla.LatentCache(lat.to(torch.float8_e4m3fn), rope)
+    with pytest.raises(ValueError, match="512"):
+        mla.LatentCache(lat[..., :256], rope)
+    with pytest.raises(ValueError, match="rope must be"):
+        mla.LatentCache(lat, rope[:1])
+    with pytest.raises(TypeError, match="bfloat16"):
+        mla.LatentCache(lat.float(), rope)
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(compressed_kv=torch.zeros(1, 2, 256, dtype=BF)), ValueError, "compressed_kv must be"),
+    (dict(compressed_kv=torch.zeros(1, 2, 512)), TypeError, "must be bfloat16"),
+    (dict(k_pe=torch.zeros(1, 3, 64, dtype=BF)), ValueError, "k_pe must be"),
+    (dict(slots=torch.zeros(1, 2, dtype=torch.int32)), TypeError, "slots must be int64"),
+    (dict(slots=torch.zeros(2, 1, dtype=torch.int64)), ValueError, "slots has shape"),
+    (dict(norm_weight=torch.ones(64)), ValueError, "norm_weight"),
+    (dict(cos=torch.ones(1, 64), sin=torch.ones(1, 64)), ValueError, "rows"),
+    (dict(cos=torch.ones(8, 64), sin=torch.ones(8, 64, dtype=BF)), TypeError, "cos and sin"),
+    (dict(cos=torch.ones(1, 2, 64), sin=torch.ones(1, 2, 64), position_ids=torch.zeros(1, 2, dtype=torch.int64)),
+     ValueError, "tables"),
+    (dict(position_ids=torch.zeros(1, 3, dtype=torch.int64)), ValueError, "position_ids has shape"),
+    (dict(position_ids=torch.zeros(1, 2, dtype=torch.int32)), TypeError, "position_ids must be int64"),
+    (dict(), RuntimeError, "no CPU fallback"),
+])
+def test_write_refuses(change, error, text):
+    with pytest.raises(error, match=text):
+        mla.latent_cache_write(cache(), **{**write_args(), **change})
+
+
+def test_read_refuses():
+    with pytest.raises(TypeError, match="int64"):
+        mla.latent_cache_read(cache(), torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mla.latent_cache_read(cache(), torch.zeros(2, dtype=torch.int64))
+
+
+def test_inputs_that_need_gradients_are_refused():
+    a = write_args()
+    a["norm_weight"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mla.latent_cache_write(cache(), **a)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        mla.latent_cache_write(cache(), **a)
+
+
+def cabi_cache(a):
+    a.cache.latent = a.cache.rope = 0x1000
+    a.cache.dtype, a.cache.pages, a.cache.page_size = 0, 2, 16
+    for s, d in ((a.cache.latent_stride, 512), (a.cache.rope_stride, 64)):
+        s[0], s[1] = 16 * d, d
+
+
+def test_cabi_refuses_on_the_host(built_library):
+    from pithtrain_b200 import _lib
+    lib = _lib.load()
+    assert lib.pith_latent_write(None, None) < 0 and b"null args" in lib.pith_last_error()
+    w = _lib.LatentWriteArgs()
+    w.B, w.S = 1, 2
+    cabi_cache(w)
+    assert lib.pith_latent_write(ctypes.byref(w), None) < 0 and b"null tensor" in lib.pith_last_error()
+    w.cache.page_size = 24
+    assert lib.pith_latent_write(ctypes.byref(w), None) < 0 and b"page_size" in lib.pith_last_error()
+    w.cache.page_size, w.cache.dtype = 16, 2
+    assert lib.pith_latent_write(ctypes.byref(w), None) < 0 and b"null cache plane" in lib.pith_last_error()
+    w.cache.dtype, w.cache.latent = 0, 0x1008
+    assert lib.pith_latent_write(ctypes.byref(w), None) < 0 and b"16-byte aligned" in lib.pith_last_error()
+    w.cache.latent, w.S = 0x1000, 0
+    assert lib.pith_latent_write(ctypes.byref(w), None) == 0               # no tokens: nothing to do
+    r = _lib.LatentReadArgs()
+    cabi_cache(r)
+    assert lib.pith_latent_read(ctypes.byref(r), None) == 0
+    r.n = 1
+    assert lib.pith_latent_read(ctypes.byref(r), None) < 0 and b"null tensor" in lib.pith_last_error()
+
+
+def test_struct_sizes_match_the_header(built_library):
+    import subprocess
+    import tempfile
+    from pathlib import Path
+    from pithtrain_b200 import _lib
+    root = Path(__file__).resolve().parent.parent
+    names = {"pith_latent_cache": _lib.LatentCacheArgs, "pith_latent_write_args": _lib.LatentWriteArgs,
+             "pith_latent_read_args": _lib.LatentReadArgs}
+    src = '#include <stdio.h>\n#include "pith_b200.h"\nint main(void) {%s return 0; }' % "".join(
+        f'printf("%zu\\n", sizeof({n}));' for n in names)
+    with tempfile.TemporaryDirectory() as d:
+        (Path(d) / "s.c").write_text(src)
+        subprocess.run(["gcc", "-I", str(root / "include"), f"{d}/s.c", "-o", f"{d}/s"], check=True)
+        got = subprocess.run([f"{d}/s"], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(x) for x in got] == [ctypes.sizeof(t) for t in names.values()]
+
+
+def test_status_string_of_an_index(built_library):
+    from pithtrain_b200 import _lib
+    lib = _lib.load()
+    for detail, text in ((1, b"a slot"), (2, b"a position"), (3, b"a page"), (4, b"a sequence length")):
+        assert text in lib.pith_status_string((5 << 24) | detail)
