@@ -392,6 +392,33 @@ typedef struct pith_latent_read_args {
 /* Gathers rows of the cache as bf16 (an e4m3 row times its power-of-two factor is exact in bf16). */
 int pith_latent_read(const pith_latent_read_args* args, void* stream);
 
+typedef struct pith_latent_attn_args {
+  pith_latent_cache cache;
+  const void* q;              /* [B][Sq][H][576] bf16: absorbed latent part (512) | rotated part (64) */
+  void* out;                  /* [B][Sq][H][512] bf16, contiguous */
+  float* lse;                 /* optional [B][H][Sq] fp32, contiguous, log2 domain */
+  const int32_t* block_table; /* [B][table_cols]: pages of a sequence in order */
+  const int32_t* seq_lens;    /* [B]: keys of a sequence, its new tokens among them; 0 .. table_cols * page_size */
+  const int32_t* query_lens;  /* optional [B]: new tokens of a sequence, 0 .. Sq (default: Sq) */
+  const uint8_t* tree_mask;   /* optional [B][Sq][Sq]: non-zero = new token i sees new token j */
+  void* workspace;            /* pith_latent_attn_workspace_bytes(...), not shared with a call that may run beside this one */
+  uint32_t* status;
+  size_t workspace_bytes;
+  int32_t B, Sq, H, table_cols;
+  float softmax_scale;
+  int64_t q_stride[3];        /* b, s, h (elements) */
+  int64_t table_stride, tree_stride[2];
+} pith_latent_attn_args;
+
+/*
+ * Attention in the absorbed MLA form over the cache: all H heads of the Sq new tokens of a sequence read the same keys.
+ * With n keys and m new tokens, token i sees key k iff k <= n - m + i, or with a tree mask iff k < n - m or
+ * tree_mask[i][k - (n - m)]. A row that sees nothing, or has no token, gives out 0, lse -inf. Keys are read up to
+ * seq_lens only: pages behind it need not exist. Two launches (one when no sequence can pass 64 keys).
+ */
+int pith_latent_attn(const pith_latent_attn_args* args, void* stream);
+size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t cache_dtype);
+
 /* Text of the last host-side rejection on the calling thread. */
 const char* pith_last_error(void);
 /* Human-readable form of a device status word. Returns a pointer to a thread-local buffer. */

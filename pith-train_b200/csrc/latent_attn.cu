@@ -1,0 +1,896 @@
+// Attention in the absorbed MLA form over a paged latent cache: keys are [c | r] (512 + 64), values are c, shared by all
+// heads, so the rows of one sequence are its (new token, head) pairs and all of them read the same keys:
+//
+//   s[m][n] = scale (q_c[m] . c_n + q_r[m] . r_n),   out[m] = sum_n softmax_n(s[m])[n] c_n,   512 outputs a row.
+//
+// Decoding has few rows (16 heads) and many keys, so both GEMMs run transposed, with the keys or the output dimensions on
+// the 128 lanes of the tensor core and the rows as its N:
+//   S^T[128 keys x NT rows] = [c | r]_tile * Q^T         A = cache tile, K-major, as it lies in memory
+//   O^T[128 dims x NT rows] += c_tile^T * P^T            A = the same tile read MN-major; four of these make the 512
+// A tile of 128 keys is thus read from HBM once, staged once by TMA and used by both. At NT = 16 a tile costs 68 MMAs of
+// a narrow N beside the 147 KB (bf16) that HBM delivers to one SM in ~6000 cycles: the kernel is bound by HBM until a
+// sequence has more than ~64 rows.
+//
+// An 8-bit cache stays 8-bit up to the tensor core (kind::f8f6f4). The bf16 query is split into two e4m3 terms
+// q 2^-k = hi + lo / 16 (8 significant bits, exact down to 2^-22 of the row's largest element), the weights likewise, and hi and lo
+// are separate columns of the same MMA (N = 2 NT costs no more than NT here). The row factor of a key enters the score in
+// registers and the weight as w_n = 2^(s_n + log2 scale_n - ref): ref is the running maximum of s_n + log2 scale_n, so
+// the split always covers the keys that matter; weights below 2^-22 of the reference are dropped.
+//
+// Work split: the (sequence, row tile, 64 keys) units of the launch form one line which is cut into one equal piece per
+// CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device). A piece that
+// covers a row tile completely stores its result; the others store an fp32 partial (O, ref, l), at most two per CTA, and
+// the merge kernel adds them in key order.
+//
+// Roles (256 threads): warp 0 TMA producer (one lane per page), warp 1 MMA issuer, warps 4-7 softmax and epilogue
+// (thread = key, then = output dimension). The running maximum is moved only when a score exceeds the reference by more
+// than 2^8 (8-bit: 2^2), decided by one barrier reduction per tile.
+#include "common.cuh"
+#include "host_common.h"
+
+namespace pith {
+
+constexpr int kLat = 512, kRp = 64;
+constexpr int kTile = 128;  // keys per tile
+constexpr int kUnit = 64;   // keys per unit of work
+constexpr int kLatThreads = 256;
+constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
+constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit); O^T starts at 0
+
+template <int NT, bool FP8>
+struct LatCfg {
+  static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
+  static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
+  static constexpr int kRopeSlots = FP8 ? 2 : 1;         // 128 keys x 64 dims
+  static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
+  static constexpr int kQ = kQLat + NT * 128;
+  static constexpr int kP = NT * 256;
+  static constexpr int kMisc = NT == 16 ? 1024 : 4096;
+  // bf16: P overlays the rope tile, which the score GEMM has finished with when P is written
+  static constexpr int kFixed = kRopeSlots * 16384 + kQ + (FP8 ? kP : 0) + kMisc;
+  static constexpr int NS = (232448 - kFixed) / kSlot;
+  static constexpr int kRopeOff = NS * kSlot;
+  static constexpr int kQOff = kRopeOff + kRopeSlots * 16384;
+  static constexpr int kPOff = FP8 ? kQOff + kQ : kRopeOff;
+  static constexpr int kMiscOff = FP8 ? kPOff + kP : kQOff + kQ;
+  static constexpr int kAlloc = kMiscOff + kMisc;
+  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 4;
+  static_assert(NS >= 4, "a tile's four latent slots must fit at once");
+  static_assert(kBars * 8 + 16 + 96 + NT * 40 <= kMisc, "misc area too small");
+  static_assert(kAlloc <= 232448, "shared memory");
+  static_assert(4 * NC <= kColS && kColS + NC <= kColR, "TMEM columns");
+};
+
+struct LatAttnParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;  // [B][Sq][H][512] contiguous
+  float* lse;          // [B][H][Sq] contiguous, log2 domain, optional
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* qlens;
+  const uint8_t* tree;
+  const float* scale;
+  float* part_o;      // [2 G][NT][512]
+  float2* part_ml;    // [2 G][NT]: reference, sum
+  int4* part_info;    // [G]: entry continued from the previous CTA, entry begun and not finished, its slot
+  uint32_t* status;
+  int B, Sq, H, R, RT, pages, page_size, max_keys;
+  float scale_log2;
+  int64_t qs[3], table_stride, tree_stride[2], scale_stride[2];
+};
+
+// One entry of the work line: row tile rt of sequence b.
+struct LatEntry {
+  int b, r0, len, nq, keys;  // keys: how many its rows can see at most
+};
+template <int NT>
+__device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
+  LatEntry x;
+  x.b = e / p.RT;
+  x.r0 = (e - x.b * p.RT) * NT;
+  x.len = min(max(__ldg(p.lens + x.b), 0), p.max_keys);
+  x.nq = p.qlens != nullptr ? min(max(__ldg(p.qlens + x.b), 0), p.Sq) : p.Sq;
+  const int last = min((min(x.r0 + NT, p.R) - 1) / p.H, x.nq - 1);
+  x.keys = x.r0 / p.H >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
+  return x;
+}
+__device__ __forceinline__ int lat_units(int keys) { return max((keys + kUnit - 1) / kUnit, 1); }
+
+// Walks the pieces of this CTA's share of the line. Every role keeps its own copy.
+template <int NT>
+struct LatWalk {
+  int e, off;
+  int64_t left;
+  LatEntry x;
+  int k0, k1;   // keys [k0, k1) of the entry
+  bool begins, ends;
+  __device__ __forceinline__ bool next(const LatAttnParams& p) {
+    if (left <= 0) return false;
+    x = lat_entry<NT>(p, e);
+    const int n = lat_units(x.keys);
+    const int take = static_cast<int>(min(static_cast<int64_t>(n - off), left));
+    k0 = off * kUnit;
+    k1 = min(x.keys, (off + take) * kUnit);
+    begins = off == 0;
+    ends = off + take == n;
+    left -= take;
+    if (ends) { ++e; off = 0; } else { off += take; }
+    return true;
+  }
+  __device__ __forceinline__ int tiles() const { return (k1 - k0 + kTile - 1) / kTile; }
+};
+
+__device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor for kind::f8f6f4 with e4m3 inputs (format 0) and fp32 accumulation.
+constexpr uint32_t make_idesc_e4m3(int m, int n, bool a_mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
+  static_assert(N == 16 || N % 32 == 0, "columns");
+  if (N == 16) tmem_ld16(addr, r);
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) tmem_ld32(addr + 32 * i, r + 32 * i);
+}
+template <int N>
+__device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t* r) {
+  if (N == 16) tmem_st16(addr, r);
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) tmem_st32(addr + 32 * i, r + 32 * i);
+}
+__device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred a, b;\n\t"
+      "setp.ne.u32 a, %1, 0;\n\t"
+      "bar.red.or.pred b, %2, %3, a;\n\t"
+      "selp.u32 %0, 1, 0, b;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(pred)), "r"(id), "r"(nthreads)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void e4m3x2_f32(uint16_t v, float& lo, float& hi) {
+  asm("{\n\t.reg .b32 h;\n\t.reg .b16 a, b;\n\tcvt.rn.f16x2.e4m3x2 h, %2;\n\tmov.b32 {a, b}, h;\n\t"
+      "cvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+      : "=f"(lo), "=f"(hi) : "h"(v));
+}
+
+// Shared-memory scalars behind the tiles.
+template <int NT, bool FP8>
+struct LatShared {
+  using L = LatCfg<NT, FP8>;
+  uint8_t* base;
+  uint64_t* bars;
+  __device__ explicit LatShared(uint8_t* smem) : base(smem), bars(reinterpret_cast<uint64_t*>(smem + L::kMiscOff)) {}
+  __device__ uint64_t* full(int i) const { return bars + i; }
+  __device__ uint64_t* empty(int i) const { return bars + L::NS + i; }
+  __device__ uint64_t* rfull(int i) const { return bars + 2 * L::NS + i; }
+  __device__ uint64_t* rempty(int i) const { return bars + 2 * L::NS + L::kRopeSlots + i; }
+  __device__ uint64_t* q_full() const { return bars + L::kBars - 4; }
+  __device__ uint64_t* s_full() const { return bars + L::kBars - 3; }
+  __device__ uint64_t* p_full() const { return bars + L::kBars - 2; }
+  __device__ uint64_t* o_full() const { return bars + L::kBars - 1; }
+  __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
+  __device__ int64_t* scan() const { return reinterpret_cast<int64_t*>(bars + L::kBars + 2); }      // [8 warps] + share
+  __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 14); }         // 10 NT words
+  __device__ float* ref() const { return cols(); }
+  __device__ float* fac() const { return cols() + NT; }
+  __device__ float* qk() const { return cols() + 2 * NT; }
+  __device__ float* red() const { return cols() + 3 * NT; }  // [4][NT]
+  __device__ int* lim() const { return reinterpret_cast<int*>(cols() + 7 * NT); }
+  __device__ int* tok() const { return reinterpret_cast<int*>(cols() + 8 * NT); }
+};
+
+// Query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle).
+template <int NT, bool FP8>
+__device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const LatEntry& x, int t) {
+  using L = LatCfg<NT, FP8>;
+  uint8_t* sq = sm.base + L::kQOff;
+  if (!FP8) {
+    for (int i = t; i < NT * 72; i += 128) {
+      const int row = i / 72, ch = i - row * 72;
+      const int r = x.r0 + row;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < p.R) {
+        const int tok = r / p.H, h = r - tok * p.H;
+        v = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]) + ch);
+      }
+      *reinterpret_cast<uint4*>(sq + (ch >> 3) * (NT * 128) + row * 128 + (((ch ^ row) & 7) << 4)) = v;
+    }
+    return;
+  }
+  // 128 / NT neighbouring threads share a row: its largest element decides the power of two in front of the split
+  constexpr int TPR = 128 / NT, CH = 64 / TPR;  // 16-byte chunks of the latent part per thread
+  const int row = t / TPR, sub = t % TPR, r = x.r0 + row;
+  const int tok = r / p.H, h = r - tok * p.H;
+  const uint4* src = reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]);
+  uint4 v[CH];
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) v[i] = r < p.R ? __ldg(src + i * TPR + sub) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
+  }
+#pragma unroll
+  for (int o = TPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  const uint32_t bits = __float_as_uint(top);
+  int k = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x600000u ? 7 : 8);
+  k = top == 0.f ? 0 : min(max(k, -100), 100);
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  if (sub == 0)  // an infinite element makes the row's scores NaN
+    sm.qk()[row] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int ch = i * TPR + sub;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    uint32_t hi[2], lo[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t hw = 0, lw = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float a = __uint_as_float(w[2 * j + u] << 16) * inv, b = __uint_as_float(w[2 * j + u] & 0xFFFF0000u) * inv;
+        const uint16_t hv = cvt_e4m3x2(a, b);
+        float ha, hb;
+        e4m3x2_f32(hv, ha, hb);
+        hw |= static_cast<uint32_t>(hv) << (16 * u);
+        lw |= static_cast<uint32_t>(cvt_e4m3x2((a - ha) * 16.f, (b - hb) * 16.f)) << (16 * u);
+      }
+      hi[j] = hw;
+      lo[j] = lw;
+    }
+    uint8_t* blk = sq + (ch >> 4) * (2 * NT * 128);
+    const int c16 = (ch & 15) >> 1, half = (ch & 1) * 8;
+    *reinterpret_cast<uint2*>(blk + row * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(hi[0], hi[1]);
+    *reinterpret_cast<uint2*>(blk + (NT + row) * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(lo[0], lo[1]);
+  }
+  for (int i = t; i < NT * 8; i += 128) {
+    const int rr = i >> 3, ch = i & 7, r2 = x.r0 + rr;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (r2 < p.R) {
+      const int tk = r2 / p.H, hh = r2 - tk * p.H;
+      w = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tk * p.qs[1] + hh * p.qs[2]) + 64 + ch);
+    }
+    *reinterpret_cast<uint4*>(sq + L::kQLat + rr * 128 + (((ch ^ rr) & 7) << 4)) = w;
+  }
+}
+
+// Row `t` of the current latent tile (four slots): whether it holds a value that is not finite; and zeroing it.
+template <bool FP8>
+__device__ __forceinline__ bool row_not_finite(const uint8_t* slot, int t) {
+  bool bad = false;
+#pragma unroll
+  for (int blk = 0; blk < (FP8 ? 1 : 2); ++blk) {
+    const uint4* r = reinterpret_cast<const uint4*>(slot + blk * 16384 + t * 128);
+    for (int i = 0; i < 8; ++i) {
+      const uint4 v = r[i];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      for (int j = 0; j < 4; ++j) {
+        if (FP8) {
+          for (int u = 0; u < 32; u += 8) bad |= ((w[j] >> u) & 0x7Fu) == 0x7Fu;
+        } else {
+          bad |= (w[j] & 0x7F80u) == 0x7F80u || (w[j] & 0x7F800000u) == 0x7F800000u;
+        }
+      }
+    }
+  }
+  return bad;
+}
+template <bool FP8>
+__device__ __forceinline__ void zero_row(uint8_t* slot, int t) {
+#pragma unroll
+  for (int blk = 0; blk < (FP8 ? 1 : 2); ++blk) {
+    uint4* r = reinterpret_cast<uint4*>(slot + blk * 16384 + t * 128);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <int NT, bool FP8>
+__device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const AbortCtl& ctl,
+                                            LatWalk<NT> walk, uint32_t tmem, int t) {
+  using L = LatCfg<NT, FP8>;
+  constexpr int NC = L::NC;
+  constexpr float kRise = FP8 ? 2.f : 8.f;  // how far (log2) a score may exceed the reference
+  const int w = t >> 5, lane = t & 31;
+  const uint32_t tl = tmem + (static_cast<uint32_t>(w << 5) << 16);
+  uint32_t s_phase = 0, o_phase = 0, slot0 = 0;
+  int piece = 0;
+  int4 info = make_int4(-1, -1, -1, 0);
+  while (walk.next(p)) {
+    const LatEntry x = walk.x;
+    const int tiles = walk.tiles();
+    const bool whole = walk.begins && walk.ends;
+    const int slot = 2 * blockIdx.x + (piece > 0 ? 1 : 0);
+    if (!walk.begins) info.x = x.b * p.RT + x.r0 / NT;
+    if (walk.begins && !walk.ends) { info.y = x.b * p.RT + x.r0 / NT; info.z = slot; }
+    ++piece;
+    named_bar_sync(1, 128);  // everybody has finished with the previous piece's columns and query
+    const int prefix = max(x.len - x.nq, 0);
+    if (t < NT) {
+      const int r = x.r0 + t, tok = r / p.H;
+      sm.tok()[t] = tok;
+      // keys below the limit are visible; rows without a query are stored as zeros or not at all, whatever they see
+      sm.lim()[t] = r >= p.R || tok >= x.nq ? 0x7FFFFFFF : p.tree != nullptr ? prefix : max(x.len - x.nq + tok + 1, 0);
+      sm.ref()[t] = kNoRef;
+    }
+    if (tiles > 0) {
+      load_query<NT, FP8>(p, sm, x, t);
+      fence_proxy_async_smem();
+      mbar_arrive(sm.q_full());
+    }
+    named_bar_sync(1, 128);
+    int min_lim = 0x7FFFFFFF;
+#pragma unroll 8
+    for (int c = 0; c < NT; ++c) min_lim = min(min_lim, sm.lim()[c]);
+    float l[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) l[c] = 0.f;
+
+    for (int j = 0; j < tiles; ++j) {
+      const int n0 = walk.k0 + j * kTile, n = n0 + t;
+      float ks = 1.f, lk = 0.f, iks = 1.f;
+      if (FP8 && n < walk.k1) {
+        const int pg = __ldg(p.table + x.b * p.table_stride + n / p.page_size);
+        if (pg >= 0 && pg < p.pages) ks = p.scale[pg * p.scale_stride[0] + (n % p.page_size) * p.scale_stride[1]];
+        ks = ks < 1e-30f ? 1e-30f : ks;
+        lk = fast_log2(ks);
+        iks = 1.f / ks;
+      }
+      mbar_wait(sm.s_full(), s_phase, ctl, 0x700);
+      s_phase ^= 1;
+      tc_fence_after_sync();
+      float s[NT];
+      if (FP8) {
+        uint32_t a[NC], rp[NT];
+        tmem_ld_cols<NC>(tl + kColS, a);
+        tmem_ld_cols<NT>(tl + kColR, rp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+          s[c] = fmaf(fmaf(__uint_as_float(a[NT + c]), 0.0625f, __uint_as_float(a[c])), sm.qk()[c] * ks,
+                      __uint_as_float(rp[c])) * p.scale_log2 + lk;
+      } else {
+        uint32_t a[NT];
+        tmem_ld_cols<NT>(tl + kColS, a);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < NT; ++c) s[c] = __uint_as_float(a[c]) * p.scale_log2;
+      }
+      const int end = min(walk.k1, n0 + kTile);
+      if (n0 + kTile > min(min_lim, walk.k1)) {
+        // Masked tile. Rows of the tile that hold no key of this piece are zeroed (0 * NaN would reach every output);
+        // a key that is hidden from some rows and not finite is taken out of the tile and makes the rows that see it NaN.
+        bool poison = false;
+        if (n >= end || n >= min_lim) {
+          bool bad = n >= end;
+          for (int i = 0; i < 4 && !bad; ++i) bad = row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+          poison = bad && n < end;
+          if (bad)
+            for (int i = 0; i < 4; ++i) zero_row<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+        }
+        const uint8_t* mask = p.tree != nullptr ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : nullptr;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          bool seen = n < end;
+          if (seen && n >= sm.lim()[c]) {
+            const int tok = sm.tok()[c];
+            seen = mask != nullptr && tok < x.nq && mask[tok * p.tree_stride[1]] != 0;
+          }
+          s[c] = !seen ? -INFINITY : poison ? __uint_as_float(0x7FC00000u) : s[c];
+        }
+        __syncwarp();
+      }
+      bool rise = false;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) rise |= s[c] > sm.ref()[c] + kRise;
+      if (named_bar_or(2, 128, rise)) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          float m = s[c];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+          if (lane == 0) sm.red()[w * NT + c] = m;
+        }
+        named_bar_sync(1, 128);
+        if (t < NT) {
+          const float old = sm.ref()[t];
+          const float m = fmaxf(fmaxf(fmaxf(sm.red()[t], sm.red()[NT + t]), fmaxf(sm.red()[2 * NT + t], sm.red()[3 * NT + t])), old);
+          sm.ref()[t] = m;
+          sm.fac()[t] = fast_exp2(old - m);
+        }
+        named_bar_sync(1, 128);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) l[c] *= sm.fac()[c];
+        if (j > 0) {  // the score GEMM of this tile was issued behind the previous tile's output GEMMs: O^T is complete
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            uint32_t o[NC];
+            tmem_ld_cols<NC>(tl + mt * NC, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * sm.fac()[c % NT]);
+            tmem_st_cols<NC>(tl + mt * NC, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      uint8_t* sp = sm.base + L::kPOff;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const float pw = fast_exp2(s[c] - sm.ref()[c]);
+        if (FP8) {
+          // weights in (0, 4] -> (0, 256]; the remainder of the first rounding is at most 16, times 16
+          l[c] += pw > 0.f ? pw * iks : pw;
+          const float a = pw * 64.f;
+          const uint16_t hi = cvt_e4m3x2(a, 0.f);
+          float ha, hz;
+          e4m3x2_f32(hi, ha, hz);
+          const uint16_t lo = cvt_e4m3x2((a - ha) * 16.f, 0.f);
+          sp[c * 128 + ((((t >> 4) ^ c) & 7) << 4) + (t & 15)] = static_cast<uint8_t>(hi);
+          sp[(NT + c) * 128 + ((((t >> 4) ^ c) & 7) << 4) + (t & 15)] = static_cast<uint8_t>(lo);
+        } else {
+          l[c] += pw;
+          *reinterpret_cast<__nv_bfloat16*>(sp + (t >> 6) * (NT * 128) + c * 128 + (((((t & 63) >> 3) ^ c) & 7) << 4) +
+                                            (t & 7) * 2) = __float2bfloat16_rn(pw);
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before_sync();
+      mbar_arrive(sm.p_full());
+      slot0 = (slot0 + 4) % L::NS;
+    }
+
+    // ---- epilogue: thread = output dimension
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], o);
+      if (lane == 0) sm.red()[w * NT + c] = l[c];
+    }
+    named_bar_sync(1, 128);
+    if (t < NT) {
+      const bool query = sm.tok()[t] < x.nq;
+      sm.fac()[t] = query ? (sm.red()[t] + sm.red()[NT + t]) + (sm.red()[2 * NT + t] + sm.red()[3 * NT + t]) : 0.f;
+      if (!query) sm.ref()[t] = kNoRef;
+    }
+    named_bar_sync(1, 128);
+    if (tiles > 0) {
+      mbar_wait(sm.o_full(), o_phase, ctl, 0x800);
+      o_phase ^= 1;
+      tc_fence_after_sync();
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      uint32_t o[NC];
+      if (tiles > 0) {
+        tmem_ld_cols<NC>(tl + mt * NC, o);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) o[c] = 0u;
+      }
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        float v = __uint_as_float(o[c]);
+        if (FP8) v = fmaf(__uint_as_float(o[NC - NT + c]), 0.0625f, v) * 0.015625f;
+        if (whole) {
+          const float sum = sm.fac()[c];
+          const float y = sum == 0.f ? 0.f : v / sum;
+          if (x.r0 + c < p.R)
+            p.out[(static_cast<int64_t>(x.b) * p.R + x.r0 + c) * kLat + mt * 128 + t] = __float2bfloat16_rn(y);
+        } else {
+          p.part_o[(static_cast<int64_t>(slot) * NT + c) * kLat + mt * 128 + t] = v;
+        }
+      }
+    }
+    if (t < NT) {
+      const float sum = sm.fac()[t];
+      const int r = x.r0 + t;
+      if (!whole) {
+        p.part_ml[slot * NT + t] = make_float2(sm.ref()[t], sum);
+      } else if (p.lse != nullptr && r < p.R) {
+        const int tok = r / p.H;
+        p.lse[static_cast<int64_t>(x.b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
+            sum == 0.f ? -INFINITY : sm.ref()[t] + log2f(sum);
+      }
+    }
+    tc_fence_before_sync();
+  }
+  if (t == 0) p.part_info[blockIdx.x] = info;
+}
+
+template <int NT, bool FP8>
+__global__ void __launch_bounds__(kLatThreads, 1)
+    latent_attn_kernel(const __grid_constant__ CUtensorMap tm_lat, const __grid_constant__ CUtensorMap tm_rope,
+                       const LatAttnParams p) {
+  using L = LatCfg<NT, FP8>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const LatShared<NT, FP8> sm(smem);
+  uint32_t* tmem_slot = sm.tmem_slot();
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortCtl ctl{p.status, abort_flag};
+
+  if (threadIdx.x == 0) {
+    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
+    for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
+    for (int i = 0; i < L::kRopeSlots; ++i) { mbar_init(sm.rfull(i), 1); mbar_init(sm.rempty(i), 1); }
+    mbar_init(sm.q_full(), 128);
+    mbar_init(sm.s_full(), 1);
+    mbar_init(sm.p_full(), 128);
+    mbar_init(sm.o_full(), 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  // This CTA's share of the work line: every thread counts a run of entries, then a scan over the CTA.
+  const int entries = p.B * p.RT;
+  const int run = (entries + kLatThreads - 1) / kLatThreads;
+  const int e_begin = min(static_cast<int>(threadIdx.x) * run, entries), e_end = min(e_begin + run, entries);
+  int64_t mine = 0;
+  for (int e = e_begin; e < e_end; ++e) {
+    const LatEntry x = lat_entry<NT>(p, e);
+    mine += lat_units(x.keys);
+    if (blockIdx.x == 0 && x.r0 == 0) {
+      const int len = __ldg(p.lens + x.b);
+      if (len < 0 || len > p.max_keys || (p.qlens != nullptr && (__ldg(p.qlens + x.b) < 0 || __ldg(p.qlens + x.b) > p.Sq)))
+        if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxLength);
+    }
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  int64_t* scan = sm.scan();
+  if (lane == 31) scan[warp] = incl;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kLatThreads / 32; ++i) {
+    if (i < warp) before += scan[i];
+    total += scan[i];
+  }
+  // with fewer units than CTAs the first ones get one each: the CTAs of an entry are always neighbours
+  const int64_t busy = min(total, static_cast<int64_t>(gridDim.x)), me = min(static_cast<int64_t>(blockIdx.x), busy);
+  const int64_t u0 = total * me / busy, u1 = total * min(me + 1, busy) / busy;
+  {
+    int64_t at = before + incl - mine;  // units in front of this thread's entries
+    if (u0 < u1 && at <= u0 && u0 < at + mine) {
+      int e = e_begin;
+      while (true) {
+        const int n = lat_units(lat_entry<NT>(p, e).keys);
+        if (u0 < at + n) break;
+        at += n;
+        ++e;
+      }
+      scan[8] = e;
+      scan[9] = u0 - at;
+    }
+  }
+  __syncthreads();
+  LatWalk<NT> walk;
+  walk.e = u0 < u1 ? static_cast<int>(scan[8]) : 0;
+  walk.off = u0 < u1 ? static_cast<int>(scan[9]) : 0;
+  walk.left = u1 - u0;
+  bool healthy = *abort_flag == 0u;
+  if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzled tiles need a 1024-byte aligned window
+    if (threadIdx.x == 0) report_error(ctl, kErrSmemAlign, smem_u32(smem));
+    healthy = false;
+  }
+  if (!healthy) walk.left = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer: one lane per page of the tile
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_lat);
+      tma_prefetch_desc(&tm_rope);
+    }
+    const int box = min(p.page_size, kUnit);
+    uint32_t it = 0, tile = 0;
+    while (walk.next(p)) {
+      for (int j = 0; j < walk.tiles(); ++j, ++tile) {
+        const int n0 = walk.k0 + j * kTile;
+        const int boxes = (min(kTile, walk.k1 - n0) + box - 1) / box;
+        int page = 0, row = 0;
+        if (lane < boxes) {
+          const int n = n0 + lane * box;
+          page = __ldg(p.table + walk.x.b * p.table_stride + n / p.page_size);
+          row = n % p.page_size;
+          if (page < 0 || page >= p.pages) {
+            if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPage);
+            page = 0;
+          }
+        }
+        for (int i = 0; i < 4; ++i, ++it) {
+          const uint32_t s = it % L::NS;
+          mbar_wait(sm.empty(s), ((it / L::NS) & 1) ^ 1, ctl, 0x100 + s);
+          if (lane == 0) mbar_arrive_expect_tx(sm.full(s), boxes * box * (FP8 ? 128 : 256));
+          __syncwarp();
+          if (lane < boxes) {
+            uint8_t* dst = smem + s * L::kSlot + lane * box * 128;
+            tma_load_4d(dst, &tm_lat, sm.full(s), i * 128, 0, row, page);
+            if (!FP8) tma_load_4d(dst + 16384, &tm_lat, sm.full(s), i * 128 + 64, 0, row, page);
+          }
+        }
+        const uint32_t rs = tile % L::kRopeSlots;
+        mbar_wait(sm.rempty(rs), ((tile / L::kRopeSlots) & 1) ^ 1, ctl, 0x200 + rs);
+        if (lane == 0) mbar_arrive_expect_tx(sm.rfull(rs), boxes * box * 128);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(smem + L::kRopeOff + rs * 16384 + lane * box * 128, &tm_rope, sm.rfull(rs), 0, 0, row, page);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    constexpr uint32_t id_rope = make_idesc_bf16(128, NT, false, false);
+    constexpr uint32_t id_qk = FP8 ? make_idesc_e4m3(128, L::NC, false) : id_rope;
+    constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, false);
+    const uint64_t q_desc = make_smem_desc(smem_u32(smem + L::kQOff), 16, 1024);
+    const uint64_t qr_desc = make_smem_desc(smem_u32(smem + L::kQOff + L::kQLat), 16, 1024);
+    const uint64_t p_desc = make_smem_desc(smem_u32(smem + L::kPOff), 16, 1024);
+    const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
+    const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
+    const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
+    uint32_t it = 0, tile = 0, q_phase = 0;
+    while (walk.next(p)) {
+      const int tiles = walk.tiles();
+      if (tiles > 0) {
+        mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
+        q_phase ^= 1;
+      }
+      for (int j = 0; j < tiles; ++j, ++tile) {
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t s = (it + i) % L::NS;
+          mbar_wait(sm.full(s), ((it + i) / L::NS) & 1, ctl, 0x400 + s);
+          tc_fence_after_sync();
+          if (leader) {
+            if (FP8) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_ss_f8(tmem + kColS, desc_advance(k_desc, s * L::kSlot + k * 32),
+                           desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_ss(tmem + kColS, desc_advance(k_desc, s * L::kSlot + (k >> 2) * 16384 + (k & 3) * 32),
+                        desc_advance(q_desc, (2 * i + (k >> 2)) * (NT * 128) + (k & 3) * 32), id_qk,
+                        (i > 0 || k > 0) ? 1u : 0u);
+            }
+          }
+        }
+        const uint32_t rs = tile % L::kRopeSlots;
+        mbar_wait(sm.rfull(rs), (tile / L::kRopeSlots) & 1, ctl, 0x500 + rs);
+        tc_fence_after_sync();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_ss(tmem + (FP8 ? kColR : kColS), desc_advance(r_desc, rs * 16384 + k * 32), desc_advance(qr_desc, k * 32),
+                    id_rope, (!FP8 || k > 0) ? 1u : 0u);
+          umma_commit(sm.s_full());
+          if (FP8) umma_commit(sm.rempty(rs));
+        }
+        mbar_wait(sm.p_full(), tile & 1, ctl, 0x600);
+        tc_fence_after_sync();
+        for (int i = 0; i < 4; ++i, ++it) {
+          const uint32_t s = it % L::NS;
+          if (leader) {
+            if (FP8) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_ss_f8(tmem + i * L::NC, desc_advance(v_desc, s * L::kSlot + k * 4096), desc_advance(p_desc, k * 32),
+                           id_pv, (j > 0 || k > 0) ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_ss(tmem + i * L::NC, desc_advance(v_desc, s * L::kSlot + k * 2048),
+                        desc_advance(p_desc, (k >> 2) * (NT * 128) + (k & 3) * 32), id_pv, (j > 0 || k > 0) ? 1u : 0u);
+            }
+            umma_commit(sm.empty(s));
+          }
+        }
+        if (leader) {
+          if (!FP8) umma_commit(sm.rempty(0));
+          if (j + 1 == tiles) umma_commit(sm.o_full());
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, static_cast<int>(threadIdx.x) - 128);
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0u) {  // let copies and MMAs still in flight drain before shared memory and TMEM are handed back
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Merge of a row tile that several CTAs worked on: out = sum_i 2^(ref_i - M) O_i / sum_i 2^(ref_i - M) l_i, in key order.
+// Block (c, column): the entry that CTA c began and did not finish; most blocks find none and leave.
+template <int NT>
+__global__ void __launch_bounds__(128) latent_merge_kernel(const LatAttnParams p, int ctas) {
+  __shared__ float wt[1024];
+  __shared__ float part[8];
+  const int c = blockIdx.x, col = blockIdx.y, t = threadIdx.x;
+  if (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) return;
+  const int4 info = p.part_info[c];
+  if (info.y < 0) return;
+  const int b = info.y / p.RT, r = (info.y - b * p.RT) * NT + col;
+  if (r >= p.R) return;
+  int n = 1;
+  for (int base = c + 1; base < ctas; base += 128) {
+    const int i = base + t;
+    const int k = __syncthreads_count(i < ctas && p.part_info[i].x == info.y);
+    n += k;
+    if (k < 128) break;
+  }
+  // parts of the entry: slot info.z, then the first slot of each following CTA
+  float top = kNoRef;
+  for (int i = t; i < n; i += 128) top = fmaxf(top, p.part_ml[(i == 0 ? info.z : 2 * (c + i)) * NT + col].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  if ((t & 31) == 0) part[t >> 5] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  float sum = 0.f;
+  for (int i = t; i < n; i += 128) {
+    const float2 ml = p.part_ml[(i == 0 ? info.z : 2 * (c + i)) * NT + col];
+    const float w = fast_exp2(ml.x - top);
+    wt[i] = w;
+    sum += w * ml.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if ((t & 31) == 0) part[4 + (t >> 5)] = sum;
+  __syncthreads();
+  sum = (part[4] + part[5]) + (part[6] + part[7]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
+    const float w = wt[i];
+    const float4 v = *(reinterpret_cast<const float4*>(
+        p.part_o + (static_cast<int64_t>(i == 0 ? info.z : 2 * (c + i)) * NT + col) * kLat) + t);
+    acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+  }
+  const float inv = 1.f / sum;
+  if (sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no key, or no query
+  else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  *(reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(b) * p.R + r) * kLat) + t) =
+      make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
+  if (t == 0 && p.lse != nullptr) {
+    const int tok = r / p.H;
+    p.lse[static_cast<int64_t>(b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
+        sum == 0.f ? -INFINITY : top + log2f(sum);
+  }
+}
+
+// Rows per tile: the least that holds a sequence's rows. 64 (8-bit: 32, its columns count twice) is what TMEM and shared
+// memory hold beside a whole 128-key tile.
+static int lat_rows(int64_t rows, bool fp8) { return rows <= 16 ? 16 : rows <= 32 || fp8 ? 32 : 64; }
+
+static int lat_ctas(int64_t entries, int64_t max_keys, int* ctas) {
+  int dev = 0, sms = 148;
+  PITH_CUDA(cudaGetDevice(&dev));
+  PITH_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int64_t units = entries * (max_keys <= kUnit ? 1 : (max_keys + kUnit - 1) / kUnit);
+  *ctas = static_cast<int>(units < sms ? units : sms);
+  return kOk;
+}
+
+template <int NT, bool FP8>
+static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, int ctas, cudaStream_t st) {
+  using L = LatCfg<NT, FP8>;
+  CUtensorMap tl, tr;
+  const pith_latent_cache& c = a->cache;
+  const int64_t ls[3] = {c.latent_stride[0], c.latent_stride[1], kLat}, rs[3] = {c.rope_stride[0], c.rope_stride[1], kRp};
+  const int box = c.page_size < kUnit ? c.page_size : kUnit;
+  if (int rc = make_tensor_map(&tl, c.latent, FP8 ? 1 : 2, c.pages, c.page_size, 1, kLat, ls, FP8 ? 128 : 64, box)) return rc;
+  if (int rc = make_tensor_map(&tr, c.rope, 2, c.pages, c.page_size, 1, kRp, rs, 64, box)) return rc;
+  auto kern = latent_attn_kernel<NT, FP8>;
+  PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
+  kern<<<ctas, kLatThreads, L::kAlloc, st>>>(tl, tr, p);
+  PITH_CUDA(cudaGetLastError());
+  if (p.max_keys > kUnit) {  // an entry of one unit is never cut
+    latent_merge_kernel<NT><<<dim3(ctas, NT), 128, 0, st>>>(p, ctas);
+    PITH_CUDA(cudaGetLastError());
+  }
+  return kOk;
+}
+
+}  // namespace pith
+
+using namespace pith;
+
+extern "C" size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t dtype) {
+  if (B <= 0 || Sq <= 0 || H <= 0) return 0;
+  const int nt = lat_rows(static_cast<int64_t>(Sq) * H, dtype == PITH_DTYPE_E4M3);
+  int ctas = 0;
+  if (lat_ctas(static_cast<int64_t>(B) * ((static_cast<int64_t>(Sq) * H + nt - 1) / nt), max_keys, &ctas)) return 0;
+  return static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16;
+}
+
+extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
+  PITH_REQUIRE(a != nullptr, "null args");
+  PITH_REQUIRE(a->B >= 0 && a->Sq >= 0 && a->H >= 0, "negative size");
+  if (int rc = check_latent_cache(a->cache)) return rc;
+  PITH_REQUIRE(a->softmax_scale > 0.f, "softmax_scale must be positive");
+  if (a->B == 0 || a->Sq == 0 || a->H == 0) return kOk;
+  PITH_REQUIRE(a->q && a->out && a->block_table && a->seq_lens && a->workspace, "null tensor pointer");
+  PITH_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->workspace) && a->q_stride[0] % 8 == 0 &&
+                   a->q_stride[1] % 8 == 0 && a->q_stride[2] % 8 == 0,
+               "q, out and workspace must be 16-byte aligned, q with strides that are multiples of 8 elements");
+  PITH_REQUIRE(a->table_cols >= 0 && static_cast<int64_t>(a->table_cols) * a->cache.page_size < 2147483647 - 256,
+               "the block table covers too many keys");
+  const int64_t rows = static_cast<int64_t>(a->Sq) * a->H;
+  PITH_REQUIRE(rows < 2147483647 - 256, "too many query rows");
+  const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
+  const int nt = lat_rows(rows, fp8);
+  const int64_t rt = (rows + nt - 1) / nt;
+  PITH_REQUIRE(rt * a->B < 2147483647 - 1024, "too many query rows");
+  if (int rc = require_sm100()) return rc;
+  LatAttnParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.lse = a->lse;
+  p.table = a->block_table; p.lens = a->seq_lens; p.qlens = a->query_lens; p.tree = a->tree_mask;
+  p.scale = a->cache.scale; p.status = a->status;
+  p.B = a->B; p.Sq = a->Sq; p.H = a->H; p.R = static_cast<int>(rows); p.RT = static_cast<int>(rt);
+  p.pages = a->cache.pages; p.page_size = a->cache.page_size;
+  p.max_keys = a->table_cols * a->cache.page_size;
+  p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i];
+  p.table_stride = a->table_stride;
+  for (int i = 0; i < 2; ++i) { p.tree_stride[i] = a->tree_stride[i]; p.scale_stride[i] = a->cache.scale_stride[i]; }
+  int ctas = 1;
+  if (int rc = lat_ctas(rt * a->B, p.max_keys, &ctas)) return rc;
+  PITH_REQUIRE(a->workspace_bytes >= static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16,
+               "workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += static_cast<size_t>(ctas) * 2 * nt * kLat * 4;
+  p.part_info = reinterpret_cast<int4*>(ws);
+  ws += static_cast<size_t>(ctas) * 16;
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (fp8) return nt == 16 ? launch_latent_attn<16, true>(a, p, ctas, st) : launch_latent_attn<32, true>(a, p, ctas, st);
+  if (nt == 16) return launch_latent_attn<16, false>(a, p, ctas, st);
+  if (nt == 32) return launch_latent_attn<32, false>(a, p, ctas, st);
+  return launch_latent_attn<64, false>(a, p, ctas, st);
+}

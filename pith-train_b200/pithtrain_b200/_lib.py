@@ -148,6 +148,16 @@ class LatentReadArgs(Structure):
     ]
 
 
+class LatentAttnArgs(Structure):
+    _fields_ = [
+        ("cache", LatentCacheArgs), ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("block_table", c_void_p),
+        ("seq_lens", c_void_p), ("query_lens", c_void_p), ("tree_mask", c_void_p), ("workspace", c_void_p),
+        ("status", c_void_p), ("workspace_bytes", ctypes.c_size_t),
+        ("B", c_int32), ("Sq", c_int32), ("H", c_int32), ("table_cols", c_int32), ("softmax_scale", c_float),
+        ("q_stride", I64x3), ("table_stride", c_int64), ("tree_stride", I64x2),
+    ]
+
+
 NOALLOC_SCRATCH_BYTES = 32 << 20
 FWD_O_FP32 = 1
 BWD_SERIAL = 1
@@ -185,6 +195,8 @@ EXPORTS = {
     "pith_mla_assemble_bwd": (c_int, [POINTER(MlaAssembleArgs), c_void_p]),
     "pith_latent_write": (c_int, [POINTER(LatentWriteArgs), c_void_p]),
     "pith_latent_read": (c_int, [POINTER(LatentReadArgs), c_void_p]),
+    "pith_latent_attn": (c_int, [POINTER(LatentAttnArgs), c_void_p]),
+    "pith_latent_attn_workspace_bytes": (ctypes.c_size_t, [c_int32, c_int32, c_int32, c_int64, c_int32]),
     "pith_last_error": (c_char_p, []),
     "pith_status_string": (c_char_p, [c_uint32]),
     "pith_abi_version": (c_int, []),

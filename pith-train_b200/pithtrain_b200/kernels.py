@@ -524,3 +524,62 @@ def latent_read(cache, slots):
         _lib.check(_lib.load().pith_latent_read(ctypes.byref(a), _stream(slots)), "pith_latent_read")
     _count(1 if a.n else 0)
     return latent, k_pe
+
+
+def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query_lens=None, tree_mask=None,
+                return_lse: bool = False):
+    """(out bf16 [B,Sq,H,512], lse fp32 log2 [B,H,Sq] or None) over the paged latent cache; see ``pith_latent_attn``."""
+    if query.dim() != 4 or query.shape[3] != 576 or query.stride(3) != 1:
+        raise ValueError(f"query must be [B,S,H,576] with a contiguous last dimension, got {tuple(query.shape)}")
+    if query.dtype != torch.bfloat16:
+        raise TypeError("query must be bfloat16")
+    B, S, H, _ = query.shape
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("block_table and seq_lens must be int32")
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or \
+            (B and block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError(f"block_table must be [{B}, pages] with contiguous rows, got {tuple(block_table.shape)}")
+    _expect(seq_lens, (B,), "seq_lens")
+    if not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous")
+    if query_lens is not None:
+        if query_lens.dtype != torch.int32:
+            raise TypeError("query_lens must be int32")
+        _expect(query_lens, (B,), "query_lens")
+        if not query_lens.is_contiguous():
+            raise ValueError("query_lens must be contiguous")
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.bool:
+            raise TypeError("tree_mask must be bool")
+        _expect(tree_mask, (B, S, S), "tree_mask")
+        if S > 1 and tree_mask.stride(2) != 1:
+            raise ValueError("tree_mask must have a contiguous last dimension")
+    if not softmax_scale > 0:
+        raise ValueError("softmax_scale must be positive")
+    dev = query.device
+    _one_device(dev, cache=cache.latent, block_table=block_table, seq_lens=seq_lens, query_lens=query_lens,
+                tree_mask=tree_mask)
+    out = torch.empty((B, S, H, 512), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((B, H, S), dtype=torch.float32, device=dev) if return_lse else None
+    lib = _lib.load()
+    a = _lib.LatentAttnArgs()
+    a.cache = cache.args
+    a.q, a.out, a.block_table, a.seq_lens = query.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    if query_lens is not None:
+        a.query_lens = query_lens.data_ptr()
+    if tree_mask is not None:
+        a.tree_mask, a.tree_stride = tree_mask.data_ptr(), I64x2(tree_mask.stride(0), tree_mask.stride(1))
+    a.status = status_word(dev).data_ptr()
+    a.B, a.Sq, a.H, a.table_cols, a.softmax_scale = B, S, H, block_table.shape[1], float(softmax_scale)
+    a.q_stride, a.table_stride = I64x3(*query.stride()[:3]), block_table.stride(0)
+    max_keys = block_table.shape[1] * cache.page_size
+    with torch.cuda.device(dev):
+        # allocated per call on the current stream: calls on other streams and captured graphs each have their own
+        a.workspace_bytes = lib.pith_latent_attn_workspace_bytes(B, S, H, max_keys, a.cache.dtype)
+        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
+        a.workspace = workspace.data_ptr()
+        _lib.check(lib.pith_latent_attn(ctypes.byref(a), _stream(query)), "pith_latent_attn")
+    _count((2 if max_keys > 64 else 1) if out.numel() else 0)
+    return out, lse

@@ -110,3 +110,30 @@ def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
     prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
     give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
     return _kernels().latent_read(cache, slots)
+
+
+def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                     softmax_scale: float, *, query_lens: torch.Tensor | None = None,
+                     tree_mask: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of new tokens over the cached latent vectors, absorbed form: query ``[B,S,H,576]`` bf16
+    (``latent_query``; strided views are fine) -> ``[B,S,H,512]`` bf16, the weighted means of the latent vectors, for
+    ``latent_output``. The new tokens' own rows have been written to the cache before.
+
+    * ``block_table`` int32 ``[B, pages]``: the pages of each sequence in order; entries behind its last key are not read.
+    * ``seq_lens`` int32 ``[B]``: keys of a sequence, its new tokens included. 0 is a sequence without keys.
+    * ``query_lens`` int32 ``[B]``: how many of the S tokens a sequence has (a padded batch); default all. Rows behind
+      them give 0.
+    * default mask: causal, the new tokens being the last ones of the sequence. ``tree_mask`` bool ``[B,S,S]``: new token i
+      sees the whole prefix and the new tokens j with ``tree_mask[b, i, j]`` (a tree of drafted tokens: its ancestors
+      and itself).
+    * ``return_lse``: also the log2-domain LSE, fp32 ``[B,H,S]`` (-inf for a row that sees no key), the convention of
+      this library's other operators.
+
+    Lengths and tables are read on the device: the call can be captured once and replayed with other contents. The
+    results do not depend on the other sequences of the batch by more than fp32 rounding of partial sums, and repeat
+    bit for bit for the same inputs.
+    """
+    _no_gradient("latent_attention", query)
+    out, lse = _kernels().latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask,
+                                      return_lse)
+    return (out, lse) if return_lse else out

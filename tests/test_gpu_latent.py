@@ -169,3 +169,318 @@ def test_indices_out_of_range_are_reported(cuda_device):
         kernels.check_device_status()
     assert (cache.latent.float()[0, 2:] == 1).all() and (cache.latent.float()[1] == 1).all()
     check()
+
+
+# ---------------------------------------------------------------------------------------------------- attention
+def quantised(latent):
+    """e4m3 rows and their power-of-two factors."""
+    scale = 2.0 ** torch.ceil(torch.log2(latent.abs().amax(-1).clamp_min(1e-30) / 448))
+    return (latent / scale[..., None]).to(E4M3), scale
+
+
+def filled_cache(g, lens, page, dtype, spare=3, spread=1.0):
+    """A cache with random rows for sequences of the given lengths, in random pages; every row that no sequence owns is
+    NaN, and so are the table's entries behind a sequence's last page out of range. Returns (cache, table)."""
+    cache = make_cache(sum(-(-n // page) for n in lens) + spare, page, dtype)
+    order = torch.randperm(cache.num_pages, generator=g, device="cuda").int()
+    cols = max(1, max(-(-n // page) for n in lens)) + 1
+    table = torch.full((len(lens), cols), 1 << 30, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(lens):
+        need = -(-n // page)
+        table[b, :need] = order[at: at + need]
+        at += need
+        rows = slots_of(table[b], n, page)
+        c = torch.randn(n, 512, generator=g, device="cuda") * (1 + spread * torch.rand(n, 1, generator=g, device="cuda"))
+        if dtype == E4M3 and n:
+            c8, scale = quantised(c)
+            cache.latent.view(torch.uint8).view(-1, 512)[rows] = c8.view(torch.uint8)
+            cache.scale.view(-1)[rows] = scale
+        elif n:
+            cache.latent.view(-1, 512)[rows] = c.bfloat16()
+        if n:
+            cache.rope.view(-1, 64)[rows] = torch.randn(n, 64, generator=g, device="cuda").bfloat16()
+    return cache, table
+
+
+def slots_of(pages, n, page):
+    i = torch.arange(n, device="cuda")
+    return pages[i // page].long() * page + i % page
+
+
+def visible(S, n, nq, tree=None):
+    """bool [S, n]: which keys a sequence's token sees."""
+    i, k = torch.arange(S, device="cuda")[:, None], torch.arange(n, device="cuda")
+    if tree is None:
+        seen = k <= n - nq + i
+    else:
+        j = k - (n - nq)
+        seen = (j < 0) | tree[:, j.clamp(0, S - 1)]
+    return seen & (i < nq)
+
+
+def attention_reference(query, cache, table, lens, scale, query_lens=None, tree=None):
+    """fp64 (out, log2 lse) and a bound of the kernel's error for every element of out, and for lse.
+
+    Weights: rounded once to 8 significant bits (2^-8 relative); scores: fp32 sums of 576 products, relative to the sum of
+    their magnitudes 576 * 2^-24, times two for numerator and denominator; exp2, log2 and the scaling: 2^-18. With an 8-bit
+    cache the split query is exact to 2^-21 of its largest element, and a weight to 2^-20 of the largest of its row (2^-18
+    where row factors differ by up to 4). The result is rounded to bf16: 2^-8."""
+    B, S, H, _ = query.shape
+    out = torch.zeros(B, S, H, 512, dtype=torch.float64, device="cuda")
+    lse = torch.full((B, H, S), -math.inf, dtype=torch.float64, device="cuda")
+    tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    c_all, r_all = stored(cache)
+    for b, n in enumerate(lens):
+        nq = S if query_lens is None else query_lens[b]
+        if n == 0 or nq == 0:
+            continue
+        rows = slots_of(table[b], n, cache.page_size)
+        c, r = c_all[rows], r_all[rows]
+        keys = torch.cat([c, r], -1)
+        seen = visible(S, n, nq, None if tree is None else tree[b])
+        for h in range(H):
+            q = query[b, :, h].double()
+            s = (q @ keys.T * scale).masked_fill(~seen, -math.inf)
+            size = (q.abs() @ keys.abs().T * scale).masked_fill(~seen, 0).amax(-1)
+            delta = size * 576 * 2.0 ** -24 + 2.0 ** -18
+            floor = 0.0
+            if cache.scale is not None:
+                delta = delta + scale * 512 * 2.0 ** -21 * q[:, :512].abs().amax(-1) * c.abs().max()
+                floor = 2.0 ** -18
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - torch.where(top.isinf(), 0, top))
+            total = p.sum(-1, keepdim=True)
+            some = (total > 0)
+            total = torch.where(some, total, 1)
+            out[b, :, h] = p @ c / total
+            lse[b, h] = torch.where(some[:, 0], (top[:, 0] + total[:, 0].log()) / math.log(2), -math.inf)
+            tol[b, :, h] = 2.0 ** -8 * out[b, :, h].abs() + (2.0 ** -8 + 2 * delta[:, None]) * (p @ c.abs()) / total \
+                + floor * (seen.double() @ c.abs()) / total
+            tol_lse[b, h] = 2 * delta + 2.0 ** -20 * lse[b, h].abs().nan_to_num(0, 0, 0)
+    return out, lse, tol, tol_lse
+
+
+def run_attention(query, cache, table, lens, scale, query_lens=None, tree=None):
+    from pithtrain_b200.operators.mla import latent_attention
+    i32 = lambda v: None if v is None else torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    return latent_attention(query, cache, table, i32(lens), scale, query_lens=i32(query_lens), tree_mask=tree,
+                            return_lse=True)
+
+
+def assert_attention(query, cache, table, lens, scale, query_lens=None, tree=None, got=None):
+    o, l = run_attention(query, cache, table, lens, scale, query_lens, tree) if got is None else got
+    check()
+    ro, rl, tol, tol_lse = attention_reference(query, cache, table, lens, scale, query_lens, tree)
+    assert not o.isnan().any(), "NaN in the output"
+    assert ((o.double() - ro).abs() - tol).max().item() <= 0, ((o.double() - ro).abs() - tol).max().item()
+    fin = rl.isfinite()
+    assert torch.equal(l.isfinite(), fin) and not l.isnan().any()
+    assert ((l.double() - rl)[fin].abs() <= tol_lse[fin]).all()
+    return o, l
+
+
+def random_tree(g, B, S):
+    """Ancestors of every node (and itself) of random trees."""
+    mask = torch.zeros(B, S, S, dtype=torch.bool)
+    parent = torch.rand(B, S, generator=g)
+    for b in range(B):
+        for j in range(S):
+            if j:
+                mask[b, j] = mask[b, int(parent[b, j] * j)]
+            mask[b, j, j] = True
+    return mask.cuda()
+
+
+SCALE = 192 ** -0.5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S,H,lens,page", [
+    (1, 16, [1], 16), (1, 16, [77], 64), (1, 16, [64, 0, 65, 1, 128, 129, 63], 32), (1, 16, [4097, 3, 1500], 64),
+    (1, 1, [300, 2], 16), (1, 2, [129], 192), (3, 5, [40, 3, 700], 128), (2, 16, [5, 1100], 32), (4, 16, [260, 4], 64),
+    (1, 128, [513, 90], 64), (7, 16, [900, 7, 8], 16), (100, 4, [100], 64), (33, 16, [33, 2000], 128),
+    (1, 16, list(range(1, 400, 2)), 16)])
+def test_attention_causal(cuda_device, dtype, S, H, lens, page):
+    g = torch.Generator(device="cuda").manual_seed(1000 * S + H + len(lens))
+    cache, table = filled_cache(g, lens, page, dtype)
+    q = torch.randn(len(lens), S, H, 576, generator=g, device="cuda").bfloat16()
+    assert_attention(q, cache, table, lens, SCALE)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S,H,lens,qlens,page", [
+    (13, 16, [13, 500, 1025], None, 64), (5, 2, [5, 64, 66], None, 16), (48, 16, [300], None, 32),
+    (9, 16, [200, 9, 3, 0], [9, 4, 0, 0], 64), (20, 8, [20, 129, 260], [20, 1, 7], 128)])
+def test_attention_tree(cuda_device, dtype, S, H, lens, qlens, page):
+    g = torch.Generator(device="cuda").manual_seed(S + H)
+    cache, table = filled_cache(g, lens, page, dtype)
+    q = torch.randn(len(lens), S, H, 576, generator=g, device="cuda").bfloat16()
+    tree = random_tree(torch.Generator().manual_seed(S), len(lens), S)
+    assert_attention(q, cache, table, lens, SCALE, qlens, tree)
+    tree = torch.rand(tree.shape, generator=g, device="cuda") < 0.3       # any mask; rows that see only the prefix
+    assert_attention(q, cache, table, lens, SCALE, qlens, tree)
+    assert_attention(q, cache, table, lens, SCALE, qlens, torch.zeros_like(tree))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attention_of_a_padded_batch(cuda_device, dtype):
+    """Sequences with fewer new tokens than the batch's S, with none, and with more tokens than keys (rows that see
+    nothing); queries without a token are NaN."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    lens, qlens = [300, 65, 0, 3, 1000], [5, 1, 0, 5, 0]
+    cache, table = filled_cache(g, lens, 32, dtype)
+    q = torch.randn(5, 5, 8, 576, generator=g, device="cuda").bfloat16()
+    for b, n in enumerate(qlens):
+        q[b, n:] = float("nan")
+    o, l = run_attention(q, cache, table, lens, SCALE, qlens)
+    assert_attention(q.nan_to_num(0), cache, table, lens, SCALE, qlens, got=(o, l))
+    for b, n in enumerate(qlens):
+        assert not o[b, n:].any() and (l[b, :, n:] == -math.inf).all()
+    assert not o[3, :2].any() and o[3, 2:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attention_with_large_scores_and_one_key_above_all(cuda_device, dtype):
+    """Scores of several hundred, a maximum that rises late and often, and one key that outweighs all others."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    lens = [3000]
+    cache, table = filled_cache(g, lens, 64, dtype)
+    q = torch.randn(1, 1, 16, 576, generator=g, device="cuda").bfloat16()
+    q[0, 0, 8:] *= 30
+    rows = slots_of(table[0], 3000, 64)
+    top = q[0, 0, 0, 512:] * 3                                           # key 2900 agrees with head 0
+    cache.rope.view(-1, 64)[rows[2900]] = top
+    rising = torch.linspace(0, 6, 3000, device="cuda")[:, None] * q[0, 0, 1, 512:].float()
+    cache.rope.view(-1, 64)[rows] += rising.bfloat16()
+    assert_attention(q, cache, table, lens, SCALE)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_a_key_that_is_not_finite_reaches_only_the_rows_that_see_it(cuda_device, dtype):
+    g = torch.Generator(device="cuda").manual_seed(12)
+    S, H, lens = 6, 16, [150, 64]
+    cache, table = filled_cache(g, lens, 64, dtype)
+    q = torch.randn(2, S, H, 576, generator=g, device="cuda").bfloat16()
+    tree = random_tree(torch.Generator().manual_seed(2), 2, S)
+    tree[:, 5, :5] = False                                               # token 5 sees itself only
+    want = assert_attention(q, cache, table, lens, SCALE, None, tree)[0]
+    for b in range(2):                                                   # new token 5's row of both sequences
+        row = slots_of(table[b], lens[b], 64)[lens[b] - 1]
+        cache.latent.view(-1, 512).view(torch.uint8)[row] = 0x7F if dtype == E4M3 else 0xFF
+    o = run_attention(q, cache, table, lens, SCALE, None, tree)[0]
+    check()
+    assert torch.equal(o[:, :5], want[:, :5]) and o[:, 5].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attention_takes_strided_inputs_and_repeats_to_the_bit(cuda_device, dtype):
+    from pithtrain_b200.operators.mla import LatentCache
+    g = torch.Generator(device="cuda").manual_seed(13)
+    lens = [700, 1, 2100]
+    cache, table = filled_cache(g, lens, 64, dtype)
+    q = torch.randn(3, 2, 16, 576, generator=g, device="cuda").bfloat16()
+    o, l = assert_attention(q, cache, table, lens, SCALE)
+    again = run_attention(q, cache, table, lens, SCALE)
+    assert torch.equal(o, again[0]) and torch.equal(l, again[1])
+    wide_q = torch.zeros(2, 3, 17, 640, device="cuda", dtype=torch.bfloat16)[:, :, 1:, 32:608].transpose(0, 1)
+    wide_q.copy_(q)
+    wide_t = torch.full((3, table.shape[1] + 5), -1, dtype=torch.int32, device="cuda")[:, 2:2 + table.shape[1]]
+    wide_t.copy_(table)
+    lat = torch.zeros(cache.num_pages, 2, 64, 512, device="cuda").to(dtype)
+    rope = torch.zeros(cache.num_pages, 2, 64, 64, device="cuda", dtype=torch.bfloat16)
+    lat[:, 1] = cache.latent
+    rope[:, 1] = cache.rope
+    scale = None
+    if cache.scale is not None:
+        scale = torch.zeros(cache.num_pages, 64, 2, device="cuda")[..., 1]
+        scale.copy_(cache.scale)
+    layer = LatentCache(lat[:, 1], rope[:, 1], scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run_attention(wide_q, layer, wide_t, lens, SCALE)
+    torch.cuda.current_stream().wait_stream(side)
+    check()
+    assert torch.equal(o, other[0]) and torch.equal(l, other[1])
+
+
+def test_attention_in_a_graph_and_beside_another_call(cuda_device):
+    """One captured call, replayed with other lengths, pages and queries; a second captured call replayed beside it."""
+    from pithtrain_b200.operators.mla import latent_attention
+    g = torch.Generator(device="cuda").manual_seed(14)
+    cache, table = filled_cache(g, [2000, 1500], 64, torch.bfloat16)
+    cache8, table8 = filled_cache(g, [1800, 900], 64, E4M3)
+    q = torch.randn(2, 1, 16, 576, generator=g, device="cuda").bfloat16()
+    lens = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    latent_attention(q, cache, table, lens, SCALE)
+    latent_attention(q, cache8, table8, lens, SCALE)
+    torch.cuda.synchronize()
+    graphs = []
+    for c, t in ((cache, table), (cache8, table8)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = latent_attention(q, c, t, lens, SCALE, return_lse=True)
+        graphs.append((graph, res))
+    side = torch.cuda.Stream()
+    for step in ([1700, 800], [0, 65], [1000, 900]):
+        lens.copy_(torch.tensor(step, dtype=torch.int32))
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(5):
+                graphs[1][0].replay()
+        for _ in range(5):
+            graphs[0][0].replay()
+        torch.cuda.synchronize()
+        assert_attention(q, cache, table, step, SCALE, got=graphs[0][1])
+        assert_attention(q, cache8, table8, step, SCALE, got=graphs[1][1])
+
+
+def test_pages_and_lengths_out_of_range_are_reported(cuda_device):
+    from pithtrain_b200 import kernels
+    from pithtrain_b200.operators.mla import latent_attention
+    g = torch.Generator(device="cuda").manual_seed(15)
+    cache, table = filled_cache(g, [100, 50], 64, torch.bfloat16)
+    q = torch.randn(2, 1, 16, 576, generator=g, device="cuda").bfloat16()
+    lens = torch.tensor([100, 50], dtype=torch.int32, device="cuda")
+    for bad in (-1, cache.num_pages, 1 << 30):
+        t = table.clone()
+        t[0, 1] = bad
+        latent_attention(q, cache, t, lens, SCALE)
+        with pytest.raises(RuntimeError, match="a page of the block table"):
+            kernels.check_device_status()
+    for bad in ([100, -1], [table.shape[1] * 64 + 1, 50]):
+        t = table.clamp(max=cache.num_pages - 1)
+        latent_attention(q, cache, t, torch.tensor(bad, dtype=torch.int32, device="cuda"), SCALE)
+        with pytest.raises(RuntimeError, match="a sequence length"):
+            kernels.check_device_status()
+    latent_attention(q, cache, table, lens, SCALE, query_lens=torch.tensor([2, 0], dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="a sequence length"):
+        kernels.check_device_status()
+    assert_attention(q, cache, table, [100, 50], SCALE)
+
+
+def test_a_cache_of_more_than_2_31_elements(cuda_device):
+    """Offsets behind 2^32 bytes and 2^31 elements, written, read and attended to."""
+    from pithtrain_b200.operators.mla import LatentCache, latent_cache_read, latent_cache_write
+    pages, page = 68000, 64
+    cache = LatentCache(torch.empty(pages, page, 512, dtype=torch.bfloat16, device="cuda"),
+                        torch.empty(pages, page, 64, dtype=torch.bfloat16, device="cuda"))
+    g = torch.Generator(device="cuda").manual_seed(16)
+    n = 300
+    table = (pages - 1 - torch.arange(5, device="cuda")).int()[None]
+    slots = slots_of(table[0], n, page)[None]
+    assert slots.min().item() * 512 > 2 ** 31
+    x = torch.randn(1, n, 576, generator=g, device="cuda").bfloat16()
+    cos, sin = tables(n)
+    latent_cache_write(cache, slots, x[..., :512], x[..., 512:], torch.ones(512, device="cuda"), cos, sin, 1e-6)
+    lat, pe = latent_cache_read(cache, slots)
+    check()
+    assert torch.equal(lat[0], cache.latent.view(-1, 512)[slots[0]])
+    q = torch.randn(1, 1, 16, 576, generator=g, device="cuda").bfloat16()
+    o, l = run_attention(q, cache, table, [n], SCALE)
+    small, t = filled_cache(g, [n], page, torch.bfloat16)
+    small.latent.view(-1, 512)[slots_of(t[0], n, page)] = lat[0]
+    small.rope.view(-1, 64)[slots_of(t[0], n, page)] = pe[0]
+    assert_attention(q, small, t, [n], SCALE, got=(o, l))

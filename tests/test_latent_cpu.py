@@ -111,7 +111,7 @@ def test_struct_sizes_match_the_header(built_library):
     from pithtrain_b200 import _lib
     root = Path(__file__).resolve().parent.parent
     names = {"pith_latent_cache": _lib.LatentCacheArgs, "pith_latent_write_args": _lib.LatentWriteArgs,
-             "pith_latent_read_args": _lib.LatentReadArgs}
+             "pith_latent_read_args": _lib.LatentReadArgs, "pith_latent_attn_args": _lib.LatentAttnArgs}
     src = '#include <stdio.h>\n#include "pith_b200.h"\nint main(void) {%s return 0; }' % "".join(
         f'printf("%zu\\n", sizeof({n}));' for n in names)
     with tempfile.TemporaryDirectory() as d:
@@ -126,3 +126,49 @@ def test_status_string_of_an_index(built_library):
     lib = _lib.load()
     for detail, text in ((1, b"a slot"), (2, b"a position"), (3, b"a page"), (4, b"a sequence length")):
         assert text in lib.pith_status_string((5 << 24) | detail)
+
+
+def attn_args(B=2, S=3, H=4):
+    return dict(query=torch.zeros(B, S, H, 576, dtype=BF), block_table=torch.zeros(B, 2, dtype=torch.int32),
+                seq_lens=torch.zeros(B, dtype=torch.int32), softmax_scale=0.1)
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(query=torch.zeros(2, 3, 4, 512, dtype=BF)), ValueError, "query must be"),
+    (dict(query=torch.zeros(2, 3, 4, 576)), TypeError, "query must be bfloat16"),
+    (dict(block_table=torch.zeros(2, 2, dtype=torch.int64)), TypeError, "int32"),
+    (dict(block_table=torch.zeros(1, 2, dtype=torch.int32)), ValueError, "block_table must be"),
+    (dict(block_table=torch.zeros(2, 0, dtype=torch.int32)), ValueError, "block_table must be"),
+    (dict(block_table=torch.zeros(2, 4, dtype=torch.int32)[:, ::2]), ValueError, "block_table must be"),
+    (dict(seq_lens=torch.zeros(3, dtype=torch.int32)), ValueError, "seq_lens has shape"),
+    (dict(query_lens=torch.zeros(2, dtype=torch.int64)), TypeError, "query_lens must be int32"),
+    (dict(query_lens=torch.zeros(1, dtype=torch.int32)), ValueError, "query_lens has shape"),
+    (dict(tree_mask=torch.zeros(2, 3, 3)), TypeError, "tree_mask must be bool"),
+    (dict(tree_mask=torch.zeros(2, 3, 4, dtype=torch.bool)), ValueError, "tree_mask has shape"),
+    (dict(softmax_scale=0.0), ValueError, "softmax_scale"),
+    (dict(softmax_scale=float("nan")), ValueError, "softmax_scale"),
+    (dict(), RuntimeError, "no CPU fallback"),
+])
+def test_attention_refuses(change, error, text):
+    a = {**attn_args(), **change}
+    with pytest.raises(error, match=text):
+        mla.latent_attention(a.pop("query"), cache(), a.pop("block_table"), a.pop("seq_lens"), a.pop("softmax_scale"), **a)
+
+
+def test_cabi_attention_refuses_on_the_host(built_library):
+    from pithtrain_b200 import _lib
+    lib = _lib.load()
+    assert lib.pith_latent_attn(None, None) < 0 and b"null args" in lib.pith_last_error()
+    a = _lib.LatentAttnArgs()
+    cabi_cache(a)
+    a.B, a.Sq, a.H, a.table_cols = 1, 1, 16, 4
+    assert lib.pith_latent_attn(ctypes.byref(a), None) < 0 and b"softmax_scale" in lib.pith_last_error()
+    a.softmax_scale = 0.1
+    assert lib.pith_latent_attn(ctypes.byref(a), None) < 0 and b"null tensor" in lib.pith_last_error()
+    a.q = a.out = a.block_table = a.seq_lens = a.workspace = 0x1000
+    a.q_stride[2] = 4
+    assert lib.pith_latent_attn(ctypes.byref(a), None) < 0 and b"16-byte aligned" in lib.pith_last_error()
+    a.q_stride[2], a.table_cols = 576, 1 << 30
+    assert lib.pith_latent_attn(ctypes.byref(a), None) < 0 and b"too many keys" in lib.pith_last_error()
+    a.H = 0
+    assert lib.pith_latent_attn(ctypes.byref(a), None) == 0
