@@ -419,6 +419,30 @@ typedef struct pith_latent_attn_args {
 int pith_latent_attn(const pith_latent_attn_args* args, void* stream);
 size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t cache_dtype);
 
+typedef struct pith_latent_proj_args {
+  const void* x;       /* query: [B][S][H][192] bf16 (nope | rope, interleaved pairs); output: [B][S][H][512] bf16 */
+  const void* weight;  /* kv_b_proj.weight [H * 256][512] bf16: per head 128 rows of k_nope, 128 rows of v */
+  void* out;           /* query: [B][S][H][576] bf16; output: [B][S][H][128] bf16; contiguous */
+  const void* cos;     /* query only, as in pith_latent_write_args */
+  const void* sin;
+  const int64_t* positions;
+  uint32_t* status;
+  int32_t B, S, H;
+  int32_t cs_dtype;
+  int64_t table_rows;
+  int64_t x_stride[3]; /* b, s, h (elements) */
+  int64_t weight_stride;
+  int64_t cs_stride[2], positions_stride[2];
+} pith_latent_proj_args;
+
+/*
+ * pith_latent_query: folds the key half of kv_b_proj into the query (k_nope = W_k c is never formed) and rotates its rope
+ *   part: the input of pith_latent_attn.
+ * pith_latent_output: the value half of kv_b_proj applied to pith_latent_attn's result: what o_proj takes.
+ */
+int pith_latent_query(const pith_latent_proj_args* args, void* stream);
+int pith_latent_output(const pith_latent_proj_args* args, void* stream);
+
 /* Text of the last host-side rejection on the calling thread. */
 const char* pith_last_error(void);
 /* Human-readable form of a device status word. Returns a pointer to a thread-local buffer. */

@@ -1,0 +1,299 @@
+// The two projections around latent attention, per head h with W = kv_b_proj.weight [H * 256][512]:
+//
+//   query:   out[t][h][0:512]   = q[t][h][0:128] W[h*256 : h*256+128, :]      (K = 128, N = 512)
+//            out[t][h][512:576] = rotary embedding of q[t][h][128:192]
+//   output:  out[t][h][v]       = sum_r a[t][h][r] W[h*256+128+v, r]          (K = 512, N = 128)
+//
+// W is used as the layer holds it: the query's B operand is read MN-major, the output's K-major. One CTA makes a tile of
+// 128 tokens of one head with tcgen05 (accumulators in TMEM) and stores it by TMA, which clips the rows behind the last
+// token. Both are bound by HBM at prompt sizes (a row moves 1.5 KB / 1.3 KB for 131 kFLOP) and by latency at decode sizes;
+// two CTAs share an SM, so one tile's loads run under the other's MMAs and stores. Few tokens take narrower tiles: more
+// CTAs then share the reading of W.
+#include "../../include/pith_b200.h"
+#include "common.cuh"
+#include "host_common.h"
+
+namespace pith {
+
+struct LatProjParams {
+  const __nv_bfloat16* q;  // query only: rope parts
+  __nv_bfloat16* out;
+  const void* cos;
+  const void* sin;
+  const int64_t* pos;
+  uint32_t* status;
+  int H, rows, S0;          // rows of the flattened (or per-batch) token axis; tokens per sequence of the caller's view
+  int cs_f32;
+  int64_t table_rows;
+  int64_t qs[3], cs[2], pos_s[2];
+};
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* smem_src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+__device__ __forceinline__ void lat_load4(const void* base, int f32, int64_t off, float* f) {
+  if (f32) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + off));
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  } else {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + off));
+    f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+  }
+}
+
+// Rotary part of one query row: lane l8 of eight turns inputs [8 l8, 8 l8 + 8) into outputs [4 l8, +4) and [32 + 4 l8, +4).
+__device__ __forceinline__ void lat_rope_row(const LatProjParams& p, int64_t g, int h, int l8) {
+  const int64_t b = g / p.S0, s = g - b * p.S0;
+  int64_t cs = b * p.cs[0] + s * p.cs[1];
+  if (p.pos != nullptr) {
+    const int64_t row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
+    if (row < 0 || row >= p.table_rows) {
+      if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPosition);
+      return;
+    }
+    cs = row * p.cs[1];
+  }
+  float cl[4], ch[4], sl[4], sh[4];
+  lat_load4(p.cos, p.cs_f32, cs + 4 * l8, cl);
+  lat_load4(p.cos, p.cs_f32, cs + 32 + 4 * l8, ch);
+  lat_load4(p.sin, p.cs_f32, cs + 4 * l8, sl);
+  lat_load4(p.sin, p.cs_f32, cs + 32 + 4 * l8, sh);
+  const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs[0] + s * p.qs[1] + h * p.qs[2] + 128) + l8);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  float lo[4], hi[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float even = __uint_as_float(w[i] << 16), odd = __uint_as_float(w[i] & 0xFFFF0000u);
+    lo[i] = even * cl[i] - odd * sl[i];
+    hi[i] = odd * ch[i] + even * sh[i];
+  }
+  __nv_bfloat16* d = p.out + (g * p.H + h) * 576 + 512;
+  *reinterpret_cast<uint2*>(d + 4 * l8) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+  *reinterpret_cast<uint2*>(d + 32 + 4 * l8) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
+}
+
+// A [128 tokens x K] K-major, B [NT columns x K] (query: MN-major), K in blocks of 64 through ST stages.
+template <bool QUERY, int NT, int ST>
+struct ProjCfg {
+  static constexpr int KB = QUERY ? 2 : 8;             // K blocks of 64
+  static constexpr int kA = 128 * 128;                 // bytes of an A block
+  static constexpr int kB = NT * 128;                  // bytes of a B block
+  static constexpr int kStage = kA + kB;
+  static constexpr int kOut = NT * 256;                // staged result
+  static constexpr int kTiles = ST * kStage > kOut ? ST * kStage : kOut;
+  static constexpr int kBars = 2 * ST + 1;
+  static constexpr int kAlloc = kTiles + kBars * 8 + 16;
+  static constexpr int kCols = NT < 32 ? 32 : NT;
+};
+
+template <bool QUERY, int NT, int ST>
+__global__ void __launch_bounds__(128)
+    latent_proj_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                       const __grid_constant__ CUtensorMap tm_out, const LatProjParams p) {
+  using L = ProjCfg<QUERY, NT, ST>;
+  constexpr int NN = (QUERY ? 512 : 128) / NT;  // column tiles
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kTiles);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + ST;
+  uint64_t* done = bars + 2 * ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortCtl ctl{p.status, abort_flag};
+  const int nt = blockIdx.x % NN, m0 = (blockIdx.x / NN) * 128, h = blockIdx.y, b = blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
+    for (int i = 0; i < ST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(done, 1);
+    mbar_fence_init();
+    if ((smem_u32(smem) & 1023u) != 0u) report_error(ctl, kErrSmemAlign, smem_u32(smem));
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  const bool healthy = *abort_flag == 0u;
+
+  if (healthy) {
+    if (warp == 0 && lane == 0) {
+      for (int k = 0; k < L::KB; ++k) {
+        const int s = k % ST;
+        mbar_wait(&empty[s], ((k / ST) & 1) ^ 1, ctl, 0x100 + s);
+        uint8_t* st = smem + s * L::kStage;
+        mbar_arrive_expect_tx(&full[s], L::kStage);
+        tma_load_4d(st, &tm_a, &full[s], k * 64, h, m0, b);
+        if (QUERY) {  // 64 rows of W (the K block) x NT columns, as [64 rows][64 columns] blocks
+#pragma unroll
+          for (int i = 0; i < NT / 64; ++i)
+            tma_load_4d(st + L::kA + i * 8192, &tm_w, &full[s], nt * NT + i * 64, 0, h * 256 + k * 64, 0);
+        } else {  // NT rows of W x 64 columns (the K block)
+          tma_load_4d(st + L::kA, &tm_w, &full[s], k * 64, 0, h * 256 + 128 + nt * NT, 0);
+        }
+      }
+    }
+    __syncwarp();
+    if (warp == 1) {
+      const bool leader = elect_one();
+      constexpr uint32_t idesc = make_idesc_bf16(128, NT, false, QUERY);
+      for (int k = 0; k < L::KB; ++k) {
+        const int s = k % ST;
+        mbar_wait(&full[s], (k / ST) & 1, ctl, 0x400 + s);
+        tc_fence_after_sync();
+        if (leader) {
+          const uint64_t ad = make_smem_desc(smem_u32(smem) + s * L::kStage, 16, 1024);
+          const uint64_t bd = make_smem_desc(smem_u32(smem) + s * L::kStage + L::kA, QUERY ? 8192 : 16, 1024);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            umma_ss(tmem, desc_advance(ad, i * 32), desc_advance(bd, QUERY ? i * 2048 : i * 32), idesc,
+                    (k > 0 || i > 0) ? 1u : 0u);
+          umma_commit(&empty[s]);
+          if (k + 1 == L::KB) umma_commit(done);
+        }
+      }
+    }
+    __syncwarp();
+    if (QUERY) {  // this column tile's share of the rotary parts, while the MMAs run
+      constexpr int RR = 128 / NN;
+#pragma unroll
+      for (int i = 0; i < (RR + 15) / 16; ++i) {
+        const int row = m0 + nt * RR + i * 16 + (threadIdx.x >> 3);
+        if (row < p.rows) lat_rope_row(p, static_cast<int64_t>(b) * p.rows + row, h, threadIdx.x & 7);
+      }
+      __syncwarp();
+    }
+    {
+      mbar_wait(done, 0, ctl, 0x800);
+      tc_fence_after_sync();
+      const int t = threadIdx.x;
+      const uint32_t tl = tmem + (static_cast<uint32_t>(warp << 5) << 16);
+#pragma unroll
+      for (int c = 0; c < NT / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(tl + c * 32, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t* v = r + 8 * i;
+          const uint4 y = make_uint4(pack_bf16(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                                     pack_bf16(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                                     pack_bf16(__uint_as_float(v[4]), __uint_as_float(v[5])),
+                                     pack_bf16(__uint_as_float(v[6]), __uint_as_float(v[7])));
+          if (NT >= 64) {
+            const int ch = (c & 1) * 4 + i;
+            *reinterpret_cast<uint4*>(smem + (c >> 1) * 16384 + t * 128 + (((ch ^ t) & 7) << 4)) = y;
+          } else if (m0 + t < p.rows) {
+            *(reinterpret_cast<uint4*>(p.out + ((static_cast<int64_t>(b) * p.rows + m0 + t) * p.H + h) * 128 + nt * NT) + i) = y;
+          }
+        }
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (NT >= 64 && *abort_flag == 0u && threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) tma_store_4d(&tm_out, smem + i * 16384, nt * NT + i * 64, h, m0, b);
+    tma_store_commit();
+    tma_store_wait_read();  // the shared memory may go once it has been read
+  }
+  if (*abort_flag != 0u) {  // let copies and MMAs still in flight drain before shared memory and TMEM are handed back
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+  }
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, L::kCols);
+  }
+}
+
+template <bool QUERY, int NT, int ST>
+static int launch_proj(const CUtensorMap& ta, const pith_latent_proj_args* a, const LatProjParams& p, int64_t B, int64_t S,
+                       cudaStream_t st) {
+  using L = ProjCfg<QUERY, NT, ST>;
+  constexpr int kIn = QUERY ? 576 : 128, NN = (QUERY ? 512 : 128) / NT;
+  CUtensorMap tw, to;
+  const int64_t ws[3] = {static_cast<int64_t>(a->H) * 256 * a->weight_stride, a->weight_stride, 512};
+  if (int rc = make_tensor_map(&tw, a->weight, 2, 1, static_cast<int64_t>(a->H) * 256, 1, 512, ws, 64, QUERY ? 64 : NT)) return rc;
+  const int64_t os[3] = {S * a->H * kIn, static_cast<int64_t>(a->H) * kIn, kIn};
+  if (int rc = make_tensor_map(&to, a->out, 2, B, S, a->H, kIn, os, 64, 128)) return rc;
+  auto kern = latent_proj_kernel<QUERY, NT, ST>;
+  PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
+  const int64_t mt = (S + 127) / 128;
+  PITH_REQUIRE(mt * NN < 2147483647 && a->H <= 65535 && B <= 65535, "too many tokens, heads or sequences");
+  kern<<<dim3(static_cast<unsigned>(mt * NN), a->H, static_cast<unsigned>(B)), 128, L::kAlloc, st>>>(ta, tw, to, p);
+  PITH_CUDA(cudaGetLastError());
+  return kOk;
+}
+
+template <bool QUERY>
+static int latent_proj(const pith_latent_proj_args* a, void* stream) {
+  PITH_REQUIRE(a != nullptr, "null args");
+  PITH_REQUIRE(a->B >= 0 && a->S >= 0 && a->H >= 0, "negative size");
+  if (a->B == 0 || a->S == 0 || a->H == 0) return kOk;
+  PITH_REQUIRE(a->x && a->weight && a->out, "null tensor pointer");
+  PITH_REQUIRE(aligned16(a->out), "out must be 16-byte aligned");
+  if (QUERY) {
+    PITH_REQUIRE(a->cos && a->sin, "null tensor pointer");
+    PITH_REQUIRE(aligned16(a->cos) && aligned16(a->sin) && a->cs_stride[0] % 4 == 0 && a->cs_stride[1] % 4 == 0,
+                 "cos / sin must be 16-byte aligned with strides that are multiples of 4 elements");
+    PITH_REQUIRE(a->cs_dtype == PITH_DTYPE_BF16 || a->cs_dtype == PITH_DTYPE_F32, "cos / sin must be bf16 or fp32");
+    PITH_REQUIRE(aligned16(a->x) && a->x_stride[0] % 8 == 0 && a->x_stride[1] % 8 == 0 && a->x_stride[2] % 8 == 0,
+                 "q must be 16-byte aligned with strides that are multiples of 8 elements");
+  }
+  if (int rc = require_sm100()) return rc;
+  // One token axis where the strides allow it: a batch of single tokens fills the tiles.
+  int64_t B = a->B, S = a->S;
+  int64_t xs[3] = {a->x_stride[0], a->x_stride[1], a->x_stride[2]};
+  if (S == 1 || B == 1 || xs[0] == S * xs[1]) {
+    if (S == 1) xs[1] = xs[0];
+    S *= B;
+    B = 1;
+    xs[0] = S * xs[1];
+  }
+  if (a->H == 1) xs[2] = QUERY ? 192 : 512;  // strides of axes of one element say nothing
+  if (S == 1) xs[1] = a->H * xs[2];
+  if (B == 1) xs[0] = S * xs[1];
+  PITH_REQUIRE(S < 2147483647 - 256, "too many tokens");
+  CUtensorMap ta;
+  if (int rc = make_tensor_map(&ta, a->x, 2, B, S, a->H, QUERY ? 192 : 512, xs, 64, 128)) return rc;
+  LatProjParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(a->x);
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  p.cos = a->cos; p.sin = a->sin; p.pos = a->positions; p.status = a->status;
+  p.H = a->H; p.rows = static_cast<int>(S); p.S0 = a->S; p.cs_f32 = a->cs_dtype == PITH_DTYPE_F32;
+  p.table_rows = a->table_rows;
+  for (int i = 0; i < 3; ++i) p.qs[i] = a->x_stride[i];
+  for (int i = 0; i < 2; ++i) { p.cs[i] = a->cs_stride[i]; p.pos_s[i] = a->positions_stride[i]; }
+  int dev = 0, sms = 148;
+  PITH_CUDA(cudaGetDevice(&dev));
+  PITH_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = (S + 127) / 128 * B * a->H;
+  // narrow tiles while the wide ones would leave SMs without a CTA
+  if constexpr (QUERY) {
+    if (tiles * 2 < sms) return launch_proj<true, 64, 2>(ta, a, p, B, S, st);
+    return launch_proj<true, 256, 2>(ta, a, p, B, S, st);
+  } else {
+    if (tiles < sms) return launch_proj<false, 32, 8>(ta, a, p, B, S, st);
+    return launch_proj<false, 128, 3>(ta, a, p, B, S, st);
+  }
+}
+
+}  // namespace pith
+
+extern "C" int pith_latent_query(const pith_latent_proj_args* a, void* stream) { return pith::latent_proj<true>(a, stream); }
+extern "C" int pith_latent_output(const pith_latent_proj_args* a, void* stream) { return pith::latent_proj<false>(a, stream); }

@@ -158,6 +158,15 @@ class LatentAttnArgs(Structure):
     ]
 
 
+class LatentProjArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("weight", c_void_p), ("out", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("positions", c_void_p), ("status", c_void_p),
+        ("B", c_int32), ("S", c_int32), ("H", c_int32), ("cs_dtype", c_int32), ("table_rows", c_int64),
+        ("x_stride", I64x3), ("weight_stride", c_int64), ("cs_stride", I64x2), ("positions_stride", I64x2),
+    ]
+
+
 NOALLOC_SCRATCH_BYTES = 32 << 20
 FWD_O_FP32 = 1
 BWD_SERIAL = 1
@@ -197,6 +206,8 @@ EXPORTS = {
     "pith_latent_read": (c_int, [POINTER(LatentReadArgs), c_void_p]),
     "pith_latent_attn": (c_int, [POINTER(LatentAttnArgs), c_void_p]),
     "pith_latent_attn_workspace_bytes": (ctypes.c_size_t, [c_int32, c_int32, c_int32, c_int64, c_int32]),
+    "pith_latent_query": (c_int, [POINTER(LatentProjArgs), c_void_p]),
+    "pith_latent_output": (c_int, [POINTER(LatentProjArgs), c_void_p]),
     "pith_last_error": (c_char_p, []),
     "pith_status_string": (c_char_p, [c_uint32]),
     "pith_abi_version": (c_int, []),

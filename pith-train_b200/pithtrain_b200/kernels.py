@@ -583,3 +583,45 @@ def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query
         _lib.check(lib.pith_latent_attn(ctypes.byref(a), _stream(query)), "pith_latent_attn")
     _count((2 if max_keys > 64 else 1) if out.numel() else 0)
     return out, lse
+
+
+def _proj_args(x, weight, width: int, name: str):
+    if x.dim() != 4 or x.shape[3] != width or x.stride(3) != 1:
+        raise ValueError(f"{name} must be [B,S,H,{width}] with a contiguous last dimension, got {tuple(x.shape)}")
+    if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"{name} and kv_b_weight must be bfloat16")
+    B, S, H, _ = x.shape
+    if tuple(weight.shape) != (H * 256, 512) or weight.stride(1) != 1:
+        raise ValueError(f"kv_b_weight must be [{H * 256}, 512] with contiguous rows, got {tuple(weight.shape)}")
+    a = _lib.LatentProjArgs()
+    a.B, a.S, a.H = B, S, H
+    a.x, a.weight = x.data_ptr(), weight.data_ptr()
+    a.x_stride, a.weight_stride = I64x3(*x.stride()[:3]), weight.stride(0)
+    return a
+
+
+def latent_query(q, weight, cos, sin, position_ids=None):
+    """[B,S,H,576] bf16: the query with the key half of kv_b_proj folded in, and rotated; see ``pith_latent_query``."""
+    a = _proj_args(q, weight, 192, "q")
+    _rotary(a, cos, sin, position_ids, a.B, a.S)
+    dev = q.device
+    _one_device(dev, kv_b_weight=weight, cos=cos, sin=sin, position_ids=position_ids)
+    out = torch.empty((a.B, a.S, a.H, 576), dtype=torch.bfloat16, device=dev)
+    a.out, a.status = out.data_ptr(), status_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pith_latent_query(ctypes.byref(a), _stream(q)), "pith_latent_query")
+    _count(1 if out.numel() else 0)
+    return out
+
+
+def latent_output(attn, weight):
+    """[B,S,H,128] bf16: the value half of kv_b_proj applied to latent attention's result; see ``pith_latent_output``."""
+    a = _proj_args(attn, weight, 512, "attn")
+    dev = attn.device
+    _one_device(dev, kv_b_weight=weight)
+    out = torch.empty((a.B, a.S, a.H, 128), dtype=torch.bfloat16, device=dev)
+    a.out, a.status = out.data_ptr(), status_word(dev).data_ptr()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().pith_latent_output(ctypes.byref(a), _stream(attn)), "pith_latent_output")
+    _count(1 if out.numel() else 0)
+    return out

@@ -78,7 +78,9 @@ def _mla_bwd_dq(q, k, v, dout, lse, delta, softmax_scale: float, causal: bool = 
 
 
 from .assemble import MLAAssembleFunc, mla_assemble  # noqa: E402
-from .latent import LatentCache, latent_attention, latent_cache_read, latent_cache_write  # noqa: E402
+from .latent import (LatentCache, latent_attention, latent_cache_read, latent_cache_write,  # noqa: E402
+                     latent_output, latent_query)
 
 __all__ = ["MLA", "_mla_fwd", "_mla_bwd_preprocess", "_mla_bwd_dk_dv", "_mla_bwd_dq", "MLAAssembleFunc", "mla_assemble",
-           "LatentCache", "latent_cache_write", "latent_cache_read", "latent_attention"]
+           "LatentCache", "latent_cache_write", "latent_cache_read", "latent_query", "latent_attention",
+           "latent_output"]

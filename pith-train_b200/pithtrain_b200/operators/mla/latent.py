@@ -137,3 +137,20 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     out, lse = _kernels().latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask,
                                       return_lse)
     return (out, lse) if return_lse else out
+
+
+def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                 position_ids: torch.Tensor | None = None) -> torch.Tensor:
+    """The query that ``latent_attention`` takes: q ``[B,S,H,192]`` = ``[q_nope | q_pe]`` bf16 (the projection output,
+    viewed per head; strided views are fine) -> ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
+    ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
+    cos / sin / position_ids as in ``latent_cache_write``."""
+    _no_gradient("latent_query", q, kv_b_weight)
+    return _kernels().latent_query(q, kv_b_weight, cos, sin, position_ids)
+
+
+def latent_output(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor:
+    """``latent_attention``'s result ``[B,S,H,512]`` times head h's value rows of ``kv_b_weight``: ``[B,S,H,128]`` bf16,
+    contiguous, which the layer views as ``[B,S,H * 128]`` for ``o_proj``."""
+    _no_gradient("latent_output", attn, kv_b_weight)
+    return _kernels().latent_output(attn, kv_b_weight)

@@ -484,3 +484,168 @@ def test_a_cache_of_more_than_2_31_elements(cuda_device):
     small.latent.view(-1, 512)[slots_of(t[0], n, page)] = lat[0]
     small.rope.view(-1, 64)[slots_of(t[0], n, page)] = pe[0]
     assert_attention(q, small, t, [n], SCALE, got=(o, l))
+
+
+# ---------------------------------------------------------------------------------------------------- projections
+# One rounding to bf16 (2^-8 of the value) behind an fp32 sum of K products (K * 2^-24 of the sum of their magnitudes).
+def assert_product(got, x, w, what):
+    want = torch.einsum("bshk,hkn->bshn", x.double(), w.double())
+    size = torch.einsum("bshk,hkn->bshn", x.double().abs(), w.double().abs())
+    excess = (got.double() - want).abs() - (2.0 ** -8 * want.abs() + x.shape[-1] * 2.0 ** -24 * size)
+    assert excess.max().item() <= 0, (what, excess.max().item())
+
+
+@pytest.mark.parametrize("B,S,H", [(1, 1, 16), (1, 1, 1), (3, 1, 16), (33, 1, 5), (2, 65, 16), (1, 129, 2), (1, 700, 16),
+                                   (3, 130, 16), (64, 5, 16), (1, 300, 128)])
+def test_query_and_output_projections(cuda_device, B, S, H):
+    from pithtrain_b200.operators.mla import latent_output, latent_query
+    g = torch.Generator(device="cuda").manual_seed(B * S + H)
+    w = (torch.randn(H * 256, 512, generator=g, device="cuda") / 20).bfloat16()
+    heads = w.view(H, 256, 512)
+    q = torch.randn(B, S, H, 192, generator=g, device="cuda").bfloat16()
+    cos, sin = tables(3000)
+    pos = torch.randint(0, 3000, (B, S), generator=g, device="cuda")
+    out = latent_query(q, w, cos, sin, position_ids=pos)
+    check()
+    assert out.shape == (B, S, H, 576) and out.is_contiguous()
+    assert_product(out[..., :512], q[..., :128], heads[:, :128], "query")
+    turned = rotated(q[..., 128:], cos[pos][:, :, None], sin[pos][:, :, None])
+    assert_rounded(out[..., 512:], turned, 2.0 ** -8, "rope", floor=2.0 ** -20)
+    a = torch.randn(B, S, H, 512, generator=g, device="cuda").bfloat16()
+    y = latent_output(a, w)
+    check()
+    assert y.shape == (B, S, H, 128) and y.is_contiguous()
+    assert_product(y, a, heads[:, 128:].transpose(1, 2), "output")
+
+
+@pytest.mark.parametrize("cs", [torch.float32, torch.bfloat16])
+def test_projections_take_strided_views(cuda_device, cs):
+    """Head and sequence slices of larger tensors, tables gathered beforehand, a weight with padded rows."""
+    from pithtrain_b200.operators.mla import latent_output, latent_query
+    g = torch.Generator(device="cuda").manual_seed(21)
+    B, S, H = 3, 150, 4
+    w = torch.randn(H * 256, 640, generator=g, device="cuda").div(20).bfloat16()[:, 64:576]
+    q = torch.randn(S, B, 9, 200, generator=g, device="cuda").bfloat16()[:, :, 3:7, 8:].transpose(0, 1)
+    cos, sin = (t[None] for t in tables(S, cs))
+    out = latent_query(q, w, cos, sin)
+    a = torch.randn(B, 2 * S, H, 512, generator=g, device="cuda").bfloat16()[:, S:]
+    y = latent_output(a, w)
+    check()
+    heads = w.reshape(H, 256, 512)
+    assert_product(out[..., :512], q[..., :128], heads[:, :128], "query")
+    assert_rounded(out[..., 512:], rotated(q[..., 128:], cos[:, :, None], sin[:, :, None]), 2.0 ** -8, "rope",
+                   floor=2.0 ** -20)
+    assert_product(y, a, heads[:, 128:].transpose(1, 2), "output")
+
+
+def test_projection_reports_a_position_out_of_range(cuda_device):
+    from pithtrain_b200 import kernels
+    from pithtrain_b200.operators.mla import latent_query
+    cos, sin = tables(10)
+    w = torch.zeros(256, 512, device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros(1, 2, 1, 192, device="cuda", dtype=torch.bfloat16)
+    for bad in (10, -1, 1 << 40):
+        latent_query(q, w, cos, sin, position_ids=torch.tensor([[0, bad]], device="cuda"))
+        with pytest.raises(RuntimeError, match="a position given"):
+            kernels.check_device_status()
+
+
+# ---------------------------------------------------------------------------------------------------- all together
+class Layer:
+    """The weights of an MLA layer between its input projections and o_proj, and the expanded form in 64 bits."""
+
+    def __init__(self, g, H):
+        self.H = H
+        self.norm = (1 + 0.1 * torch.randn(512, generator=g, device="cuda")).bfloat16()
+        self.kv_b = torch.randn(H * 256, 512, generator=g, device="cuda").div(512 ** 0.5).bfloat16()
+        self.cos, self.sin = tables(4096)
+
+    def expanded(self, q, proj, seen, pos):
+        """q [n, H, 192], proj [n, 576] of all n tokens of a sequence, seen [n, n], pos [n] -> [n, H, 128]."""
+        x = proj[:, :512].double()
+        c = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * self.norm.double()
+        kv = torch.einsum("nr,hdr->nhd", c, self.kv_b.double().view(self.H, 256, 512))
+        cos, sin = self.cos[pos], self.sin[pos]
+        r = rotated(proj[:, 512:], cos, sin)
+        qr = rotated(q[..., 128:], cos[:, None], sin[:, None])
+        s = torch.einsum("ihd,nhd->hin", q[..., :128].double(), kv[..., :128]) + torch.einsum("ihd,nd->hin", qr, r)
+        return torch.einsum("hin,nhd->ihd", torch.softmax((s * SCALE).masked_fill(~seen, -math.inf), -1), kv[..., 128:])
+
+
+def close_to(got, want, dtype, what):
+    """Against the expanded form in 64 bits. Four bf16 roundings in a row (latent, query, weights and result of attention,
+    output) of half a step each, 2^-8 relative, act on sums of many terms whose rounding errors are independent, so that
+    the relative 2-norm error is at most 4 * 2^-8 (all in the same direction); an 8-bit latent row adds 2^-4."""
+    rel = ((got.double() - want).norm() / want.norm()).item()
+    bound = 4 * 2.0 ** -8 + (2.0 ** -4 if dtype == E4M3 else 0)
+    assert rel <= bound, (what, rel, bound)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_prompt_tokens_drafts_and_the_expanded_form(cuda_device, dtype):
+    """A ragged batch as a sampling loop runs it: prompts in two chunks, three single tokens, then a tree of drafts over
+    everything so far; each compared with the expanded form over all tokens of the sequence."""
+    from pithtrain_b200.operators import mla
+    g = torch.Generator(device="cuda").manual_seed(30)
+    H, page, B, D = 16, 32, 2, 6
+    layer = Layer(g, H)
+    prompts, total = [75, 130], [75 + 3 + D, 130 + 3 + D]
+    pages = [-(-n // page) for n in total]
+    cache = make_cache(sum(pages) + 1, page, dtype)
+    order = torch.randperm(cache.num_pages, generator=g, device="cuda").int()
+    table = torch.full((B, max(pages)), -1, dtype=torch.int32, device="cuda")
+    table[0, : pages[0]], table[1, : pages[1]] = order[: pages[0]], order[pages[0]: sum(pages)]
+    q = [torch.randn(n, H, 192, generator=g, device="cuda").bfloat16() for n in total]
+    proj = [torch.randn(n, 576, generator=g, device="cuda").bfloat16() for n in total]
+    tree = random_tree(torch.Generator().manual_seed(4), B, D)
+    depth = tree.sum(-1) - 1
+
+    def step(first, counts, mask=None, positions=None):
+        S = max(counts)
+        take = lambda xs: torch.stack([torch.cat([x[f:f + n], x.new_zeros(S - n, *x.shape[1:])])  # noqa: E731
+                                       for x, f, n in zip(xs, first, counts)])
+        qs, ps = take(q), take(proj)
+        at = torch.tensor(first, device="cuda")[:, None] + torch.arange(S, device="cuda")
+        pos = at if positions is None else positions
+        real = torch.arange(S, device="cuda") < torch.tensor(counts, device="cuda")[:, None]
+        slot = torch.gather(table.long(), 1, (at // page).clamp(max=table.shape[1] - 1)) * page + at % page
+        mla.latent_cache_write(cache, torch.where(real, slot, -1), ps[..., :512], ps[..., 512:], layer.norm, layer.cos,
+                               layer.sin, 1e-6, position_ids=pos)
+        query = mla.latent_query(qs, layer.kv_b, layer.cos, layer.sin, position_ids=pos)
+        lens = torch.tensor([f + n for f, n in zip(first, counts)], dtype=torch.int32, device="cuda")
+        attn = mla.latent_attention(query, cache, table, lens, SCALE, tree_mask=mask,
+                                    query_lens=torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        return mla.latent_output(attn, layer.kv_b)
+
+    results = [[], []]
+    for first, counts in (([0, 0], [64, 64]), ([64, 64], [11, 66])):          # the prompts' chunks
+        y = step(first, counts)
+        for b in range(B):
+            results[b].append(y[b, : counts[b]])
+    for i in range(3):
+        y = step([n + i for n in prompts], [1, 1])
+        for b in range(B):
+            results[b].append(y[b])
+    base = [n + 3 for n in prompts]
+    y = step(base, [D, D], tree, torch.tensor(base, device="cuda")[:, None] + depth)
+    check()
+    for b in range(B):
+        results[b].append(y[b])
+        n = total[b]
+        seen = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+        seen[base[b]:, base[b]:] = tree[b]
+        pos = torch.arange(n, device="cuda")
+        pos[base[b]:] = base[b] + depth[b]
+        want = layer.expanded(q[b], proj[b], seen, pos)
+        close_to(torch.cat(results[b]), want, dtype, f"sequence {b}")
+
+    # the expanded form of the library over the cached prefix agrees with what was decoded from the cache
+    b, n = 1, prompts[1]
+    latent, pe = mla.latent_cache_read(cache, slots_of(table[b], n, page)[None])
+    kv = (latent @ layer.kv_b.T).view(1, n, H, 256)
+    key = torch.cat([kv[..., :128], pe[:, :, None].expand(1, n, H, 64)], -1)
+    cos, sin = layer.cos[:n, None], layer.sin[:n, None]
+    query = torch.cat([q[b][:n, :, :128], rotated(q[b][:n, :, 128:], cos, sin).bfloat16()], -1)[None]
+    got = mla.MLA(H, 192, 128, SCALE)(query, key, kv[..., 128:].contiguous())
+    check()
+    close_to(got[0], torch.cat(results[b])[:n].double(), torch.bfloat16, "expanded over the cache")

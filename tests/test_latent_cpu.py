@@ -111,7 +111,8 @@ def test_struct_sizes_match_the_header(built_library):
     from pithtrain_b200 import _lib
     root = Path(__file__).resolve().parent.parent
     names = {"pith_latent_cache": _lib.LatentCacheArgs, "pith_latent_write_args": _lib.LatentWriteArgs,
-             "pith_latent_read_args": _lib.LatentReadArgs, "pith_latent_attn_args": _lib.LatentAttnArgs}
+             "pith_latent_read_args": _lib.LatentReadArgs, "pith_latent_attn_args": _lib.LatentAttnArgs,
+             "pith_latent_proj_args": _lib.LatentProjArgs}
     src = '#include <stdio.h>\n#include "pith_b200.h"\nint main(void) {%s return 0; }' % "".join(
         f'printf("%zu\\n", sizeof({n}));' for n in names)
     with tempfile.TemporaryDirectory() as d:
@@ -172,3 +173,46 @@ def test_cabi_attention_refuses_on_the_host(built_library):
     assert lib.pith_latent_attn(ctypes.byref(a), None) < 0 and b"too many keys" in lib.pith_last_error()
     a.H = 0
     assert lib.pith_latent_attn(ctypes.byref(a), None) == 0
+
+
+@pytest.mark.parametrize("change,error,text", [
+    (dict(q=torch.zeros(1, 2, 4, 128, dtype=BF)), ValueError, "q must be"),
+    (dict(q=torch.zeros(1, 2, 4, 192)), TypeError, "must be bfloat16"),
+    (dict(kv_b_weight=torch.zeros(4 * 256, 512)), TypeError, "must be bfloat16"),
+    (dict(kv_b_weight=torch.zeros(3 * 256, 512, dtype=BF)), ValueError, "kv_b_weight must be"),
+    (dict(cos=torch.ones(2, 64), sin=torch.ones(2, 32)), ValueError, "cos and sin"),
+    (dict(position_ids=torch.zeros(2, 2, dtype=torch.int64)), ValueError, "position_ids has shape"),
+    (dict(), RuntimeError, "no CPU fallback"),
+])
+def test_query_projection_refuses(change, error, text):
+    a = dict(q=torch.zeros(1, 2, 4, 192, dtype=BF), kv_b_weight=torch.zeros(4 * 256, 512, dtype=BF),
+             cos=torch.ones(8, 64), sin=torch.ones(8, 64))
+    with pytest.raises(error, match=text):
+        mla.latent_query(**{**a, **change})
+
+
+def test_output_projection_refuses():
+    w = torch.zeros(4 * 256, 512, dtype=BF)
+    with pytest.raises(ValueError, match="attn must be"):
+        mla.latent_output(torch.zeros(1, 2, 4, 576, dtype=BF), w)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mla.latent_output(torch.zeros(1, 2, 4, 512, dtype=BF), w)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        mla.latent_output(torch.zeros(1, 2, 4, 512, dtype=BF), w.requires_grad_())
+
+
+def test_cabi_projections_refuse_on_the_host(built_library):
+    from pithtrain_b200 import _lib
+    lib = _lib.load()
+    a = _lib.LatentProjArgs()
+    for entry in (lib.pith_latent_query, lib.pith_latent_output):
+        assert entry(None, None) < 0 and b"null args" in lib.pith_last_error()
+        a.B, a.S, a.H = 1, 0, 4
+        assert entry(ctypes.byref(a), None) == 0
+        a.S = 1
+        assert entry(ctypes.byref(a), None) < 0 and b"null tensor" in lib.pith_last_error()
+    a.x = a.weight = a.out = a.cos = a.sin = 0x1000
+    a.cs_stride[1] = 2
+    assert lib.pith_latent_query(ctypes.byref(a), None) < 0 and b"multiples of 4" in lib.pith_last_error()
+    a.cs_stride[1], a.cs_dtype = 64, 2
+    assert lib.pith_latent_query(ctypes.byref(a), None) < 0 and b"bf16 or fp32" in lib.pith_last_error()
