@@ -99,8 +99,7 @@ __device__ __forceinline__ int lat_units(int keys) { return max((keys + kUnit - 
 // Walks the pieces of this CTA's share of the line. Every role keeps its own copy.
 template <int NT>
 struct LatWalk {
-  int e, off;
-  int64_t left;
+  int e, off, left;
   LatEntry x;
   int k0, k1;   // keys [k0, k1) of the entry
   bool begins, ends;
@@ -108,7 +107,7 @@ struct LatWalk {
     if (left <= 0) return false;
     x = lat_entry<NT>(p, e);
     const int n = lat_units(x.keys);
-    const int take = static_cast<int>(min(static_cast<int64_t>(n - off), left));
+    const int take = min(n - off, left);
     k0 = off * kUnit;
     k1 = min(x.keys, (off + take) * kUnit);
     begins = off == 0;
@@ -174,6 +173,50 @@ __device__ __forceinline__ void e4m3x2_f32(uint16_t v, float& lo, float& hi) {
       : "=f"(lo), "=f"(hi) : "h"(v));
 }
 
+// A value that is the same in all lanes, in a form the compiler knows to be so (descriptors then stay in uniform registers).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
+
+__device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Reduces N per-lane columns over the 32 lanes: halves of the columns are exchanged for halves of the lanes until a lane
+// holds max(N / 32, 1) columns, about N shuffles in all. Afterwards v[i] of a lane is column i + first_column(lane).
+template <int N, bool MAX>
+__device__ __forceinline__ void reduce_cols(float* v, int lane) {
+  int n = N;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool upper = (lane & o) != 0;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (i < n) {
+          const float other = __shfl_xor_sync(0xFFFFFFFFu, upper ? v[i] : v[i + n], o);
+          const float own = upper ? v[i + n] : v[i];
+          v[i] = MAX ? fmaxf(own, other) : own + other;
+        }
+      }
+    } else {
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+      v[0] = MAX ? fmaxf(v[0], other) : v[0] + other;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ int first_column(int lane) {
+  int c = 0, n = N;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (n > 1) {
+      n >>= 1;
+      if (lane & o) c += n;
+    }
+  return c;
+}
+
 // Shared-memory scalars behind the tiles.
 template <int NT, bool FP8>
 struct LatShared {
@@ -190,7 +233,7 @@ struct LatShared {
   __device__ uint64_t* p_full() const { return bars + L::kBars - 2; }
   __device__ uint64_t* o_full() const { return bars + L::kBars - 1; }
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
-  __device__ int64_t* scan() const { return reinterpret_cast<int64_t*>(bars + L::kBars + 2); }      // [8 warps] + share
+  __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 2); }              // [8 warps] + share
   __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 14); }         // 10 NT words
   __device__ float* ref() const { return cols(); }
   __device__ float* fac() const { return cols() + NT; }
@@ -205,47 +248,52 @@ template <int NT, bool FP8>
 __device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const LatEntry& x, int t) {
   using L = LatCfg<NT, FP8>;
   uint8_t* sq = sm.base + L::kQOff;
+  // Eight threads copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
+  constexpr int kBlocks = FP8 ? 1 : 9;  // 8-bit: only the rope part as it is
+#pragma unroll 1
+  for (int row = t >> 3; row < NT; row += 16) {
+    const int r = x.r0 + row, ch = t & 7;
+    const int tok = r / p.H, h = r - tok * p.H;
+    const bool there = r < p.R;
+    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + ch * 8 + (FP8 ? kLat : 0) : p.q;
+    const uint32_t dst = smem_u32(sq) + (FP8 ? L::kQLat : 0) + row * 128 + (((ch ^ row) & 7) << 4);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) cp_async16(dst + i * (NT * 128), src + (there ? i * 64 : 0), there ? 16u : 0u);
+  }
   if (!FP8) {
-    for (int i = t; i < NT * 72; i += 128) {
-      const int row = i / 72, ch = i - row * 72;
-      const int r = x.r0 + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < p.R) {
-        const int tok = r / p.H, h = r - tok * p.H;
-        v = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]) + ch);
-      }
-      *reinterpret_cast<uint4*>(sq + (ch >> 3) * (NT * 128) + row * 128 + (((ch ^ row) & 7) << 4)) = v;
-    }
+    cp_async_wait_all();
     return;
   }
   // 128 / NT neighbouring threads share a row: its largest element decides the power of two in front of the split
   constexpr int TPR = 128 / NT, CH = 64 / TPR;  // 16-byte chunks of the latent part per thread
   const int row = t / TPR, sub = t % TPR, r = x.r0 + row;
   const int tok = r / p.H, h = r - tok * p.H;
-  const uint4* src = reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]);
+  const bool there = r < p.R;
+  const uint4* src = reinterpret_cast<const uint4*>(there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] : p.q) + sub;
   uint4 v[CH];
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < CH; ++i) v[i] = r < p.R ? __ldg(src + i * TPR + sub) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < CH; ++i) v[i] = __ldg(src + i * TPR);
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u))));
+      top = fmax3(top, fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u)));
   }
 #pragma unroll
   for (int o = TPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   const uint32_t bits = __float_as_uint(top);
   int k = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x600000u ? 7 : 8);
   k = top == 0.f ? 0 : min(max(k, -100), 100);
-  const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  const float inv = there ? __uint_as_float(static_cast<uint32_t>(127 - k) << 23) : 0.f;
   if (sub == 0)  // an infinite element makes the row's scores NaN
     sm.qk()[row] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-#pragma unroll
+#pragma unroll 2
   for (int i = 0; i < CH; ++i) {
     const int ch = i * TPR + sub;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    const uint4 y = __ldg(src + i * TPR);  // read a second time (it is in L1): a loop stays small in the instruction cache
+    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
     uint32_t hi[2], lo[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -267,46 +315,28 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShar
     *reinterpret_cast<uint2*>(blk + row * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(hi[0], hi[1]);
     *reinterpret_cast<uint2*>(blk + (NT + row) * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(lo[0], lo[1]);
   }
-  for (int i = t; i < NT * 8; i += 128) {
-    const int rr = i >> 3, ch = i & 7, r2 = x.r0 + rr;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (r2 < p.R) {
-      const int tk = r2 / p.H, hh = r2 - tk * p.H;
-      w = __ldg(reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tk * p.qs[1] + hh * p.qs[2]) + 64 + ch);
-    }
-    *reinterpret_cast<uint4*>(sq + L::kQLat + rr * 128 + (((ch ^ rr) & 7) << 4)) = w;
-  }
+  cp_async_wait_all();
 }
 
-// Row `t` of the current latent tile (four slots): whether it holds a value that is not finite; and zeroing it.
+// Row t of one slot of the current latent tile: whether it holds a value that is not finite.
 template <bool FP8>
 __device__ __forceinline__ bool row_not_finite(const uint8_t* slot, int t) {
   bool bad = false;
+#pragma unroll 1
+  for (int i = 0; i < (FP8 ? 8 : 16); ++i) {
+    const uint4 v = *reinterpret_cast<const uint4*>(slot + (i >> 3) * 16384 + t * 128 + (((i ^ t) & 7) << 4));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int blk = 0; blk < (FP8 ? 1 : 2); ++blk) {
-    const uint4* r = reinterpret_cast<const uint4*>(slot + blk * 16384 + t * 128);
-    for (int i = 0; i < 8; ++i) {
-      const uint4 v = r[i];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      for (int j = 0; j < 4; ++j) {
-        if (FP8) {
-          for (int u = 0; u < 32; u += 8) bad |= ((w[j] >> u) & 0x7Fu) == 0x7Fu;
-        } else {
-          bad |= (w[j] & 0x7F80u) == 0x7F80u || (w[j] & 0x7F800000u) == 0x7F800000u;
-        }
+    for (int j = 0; j < 4; ++j) {
+      if (FP8) {  // a byte 0x7F or 0xFF
+#pragma unroll
+        for (int u = 0; u < 32; u += 8) bad |= ((w[j] >> u) & 0x7Fu) == 0x7Fu;
+      } else {
+        bad |= (w[j] & 0x7F80u) == 0x7F80u || (w[j] & 0x7F800000u) == 0x7F800000u;
       }
     }
   }
   return bad;
-}
-template <bool FP8>
-__device__ __forceinline__ void zero_row(uint8_t* slot, int t) {
-#pragma unroll
-  for (int blk = 0; blk < (FP8 ? 1 : 2); ++blk) {
-    uint4* r = reinterpret_cast<uint4*>(slot + blk * 16384 + t * 128);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = make_uint4(0, 0, 0, 0);
-  }
 }
 
 template <int NT, bool FP8>
@@ -314,6 +344,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
                                             LatWalk<NT> walk, uint32_t tmem, int t) {
   using L = LatCfg<NT, FP8>;
   constexpr int NC = L::NC;
+  constexpr int kStep = FP8 ? 32 : 16;      // keys of one MMA of the output GEMM
   constexpr float kRise = FP8 ? 2.f : 8.f;  // how far (log2) a score may exceed the reference
   const int w = t >> 5, lane = t & 31;
   const uint32_t tl = tmem + (static_cast<uint32_t>(w << 5) << 16);
@@ -382,15 +413,25 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       }
       const int end = min(walk.k1, n0 + kTile);
       if (n0 + kTile > min(min_lim, walk.k1)) {
-        // Masked tile. Rows of the tile that hold no key of this piece are zeroed (0 * NaN would reach every output);
-        // a key that is hidden from some rows and not finite is taken out of the tile and makes the rows that see it NaN.
+        // Masked tile. The output GEMM takes the keys in steps of 16 (8-bit: 32); the rows of its last step that hold no
+        // key of this piece are zeroed (0 * NaN would reach every output). A key that is hidden from some rows and not
+        // finite is taken out of the tile and makes the rows that see it NaN.
+        const int rows = (kStep - (end - n0) % kStep) % kStep;
+#pragma unroll 1
+        for (int i = t; i < rows * (FP8 ? 32 : 64); i += 128) {
+          const int row = end - n0 + i / (FP8 ? 32 : 64), ch = i % (FP8 ? 32 : 64);
+          *reinterpret_cast<uint4*>(sm.base + ((slot0 + ch / (FP8 ? 8 : 16)) % L::NS) * L::kSlot +
+                                    (FP8 ? 0 : (ch >> 3 & 1) * 16384) + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
         bool poison = false;
-        if (n >= end || n >= min_lim) {
-          bool bad = n >= end;
-          for (int i = 0; i < 4 && !bad; ++i) bad = row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
-          poison = bad && n < end;
-          if (bad)
-            for (int i = 0; i < 4; ++i) zero_row<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+        if (n >= min_lim && n < end) {
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) poison |= row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+          if (poison)
+#pragma unroll 1
+            for (int i = 0; i < (FP8 ? 32 : 64); ++i)
+              *reinterpret_cast<uint4*>(sm.base + ((slot0 + i / (FP8 ? 8 : 16)) % L::NS) * L::kSlot +
+                                        (FP8 ? 0 : (i >> 3 & 1) * 16384) + t * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         const uint8_t* mask = p.tree != nullptr ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : nullptr;
 #pragma unroll
@@ -408,12 +449,14 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
 #pragma unroll
       for (int c = 0; c < NT; ++c) rise |= s[c] > sm.ref()[c] + kRise;
       if (named_bar_or(2, 128, rise)) {
+        {
+          float m[NT];
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          float m = s[c];
+          for (int c = 0; c < NT; ++c) m[c] = s[c];
+          reduce_cols<NT, true>(m, lane);
+          constexpr int kOwn = NT > 32 ? NT / 32 : 1;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-          if (lane == 0) sm.red()[w * NT + c] = m;
+          for (int i = 0; i < kOwn; ++i) sm.red()[w * NT + first_column<NT>(lane) + i] = m[i];
         }
         named_bar_sync(1, 128);
         if (t < NT) {
@@ -423,39 +466,54 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           sm.fac()[t] = fast_exp2(old - m);
         }
         named_bar_sync(1, 128);
-#pragma unroll
-        for (int c = 0; c < NT; ++c) l[c] *= sm.fac()[c];
         if (j > 0) {  // the score GEMM of this tile was issued behind the previous tile's output GEMMs: O^T is complete
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            uint32_t o[NC];
-            tmem_ld_cols<NC>(tl + mt * NC, o);
+          for (int c = 0; c < NT; ++c) l[c] *= sm.fac()[c];
+#pragma unroll 1
+          for (int i = 0; i < 4 * NC; i += 16) {
+            uint32_t o[16];
+            tmem_ld16(tl + i, o);
             tmem_wait_ld();
+            const float* f = sm.fac() + i % NT;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * sm.fac()[c % NT]);
-            tmem_st_cols<NC>(tl + mt * NC, o);
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f[c]);
+            tmem_st16(tl + i, o);
           }
           tmem_wait_st();
         }
       }
+      // sixteen columns at a time: references and weights in registers first, so that no load waits for a store
       uint8_t* sp = sm.base + L::kPOff;
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        const float pw = fast_exp2(s[c] - sm.ref()[c]);
+      for (int c0 = 0; c0 < NT; c0 += 16) {
+        float pw[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(s[c0 + c] - sm.ref()[c0 + c]);
         if (FP8) {
           // weights in (0, 4] -> (0, 256]; the remainder of the first rounding is at most 16, times 16
-          l[c] += pw > 0.f ? pw * iks : pw;
-          const float a = pw * 64.f;
-          const uint16_t hi = cvt_e4m3x2(a, 0.f);
-          float ha, hz;
-          e4m3x2_f32(hi, ha, hz);
-          const uint16_t lo = cvt_e4m3x2((a - ha) * 16.f, 0.f);
-          sp[c * 128 + ((((t >> 4) ^ c) & 7) << 4) + (t & 15)] = static_cast<uint8_t>(hi);
-          sp[(NT + c) * 128 + ((((t >> 4) ^ c) & 7) << 4) + (t & 15)] = static_cast<uint8_t>(lo);
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            l[c0 + c] += pw[c] > 0.f ? pw[c] * iks : pw[c];
+            l[c0 + c + 1] += pw[c + 1] > 0.f ? pw[c + 1] * iks : pw[c + 1];
+            const float a = pw[c] * 64.f, b = pw[c + 1] * 64.f;
+            const uint16_t hi = cvt_e4m3x2(a, b);
+            float ha, hb;
+            e4m3x2_f32(hi, ha, hb);
+            const uint16_t lo = cvt_e4m3x2((a - ha) * 16.f, (b - hb) * 16.f);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint8_t* d = sp + (c0 + c + u) * 128 + ((((t >> 4) ^ (c + u)) & 7) << 4) + (t & 15);
+              d[0] = static_cast<uint8_t>(hi >> (8 * u));
+              d[NT * 128] = static_cast<uint8_t>(lo >> (8 * u));
+            }
+          }
         } else {
-          l[c] += pw;
-          *reinterpret_cast<__nv_bfloat16*>(sp + (t >> 6) * (NT * 128) + c * 128 + (((((t & 63) >> 3) ^ c) & 7) << 4) +
-                                            (t & 7) * 2) = __float2bfloat16_rn(pw);
+          uint8_t* d = sp + (t >> 6) * (NT * 128) + c0 * 128 + (t & 7) * 2;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            l[c0 + c] += pw[c];
+            *reinterpret_cast<__nv_bfloat16*>(d + c * 128 + (((((t & 63) >> 3) ^ c) & 7) << 4)) = __float2bfloat16_rn(pw[c]);
+          }
         }
       }
       fence_proxy_async_smem();
@@ -465,17 +523,17 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     }
 
     // ---- epilogue: thread = output dimension
+    reduce_cols<NT, false>(l, lane);
+    constexpr int kOwn = NT > 32 ? NT / 32 : 1;
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], o);
-      if (lane == 0) sm.red()[w * NT + c] = l[c];
-    }
+    for (int i = 0; i < kOwn; ++i) sm.red()[w * NT + first_column<NT>(lane) + i] = l[i];
     named_bar_sync(1, 128);
+    float sum = 0.f;
     if (t < NT) {
       const bool query = sm.tok()[t] < x.nq;
-      sm.fac()[t] = query ? (sm.red()[t] + sm.red()[NT + t]) + (sm.red()[2 * NT + t] + sm.red()[3 * NT + t]) : 0.f;
+      sum = query ? (sm.red()[t] + sm.red()[NT + t]) + (sm.red()[2 * NT + t] + sm.red()[3 * NT + t]) : 0.f;
       if (!query) sm.ref()[t] = kNoRef;
+      sm.fac()[t] = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
     }
     named_bar_sync(1, 128);
     if (tiles > 0) {
@@ -483,32 +541,37 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       o_phase ^= 1;
       tc_fence_after_sync();
     }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      uint32_t o[NC];
+    // A rolled loop: the code runs once per piece, and unrolled it waited for the instruction cache at every store.
+    const int rows = min(p.R - x.r0, NT);
+#pragma unroll 1
+    for (int i = 0; i < 4 * NT; i += 16) {
+      const int mt = i / NT, c0 = i % NT;
+      uint32_t o[16], lo[16];
       if (tiles > 0) {
-        tmem_ld_cols<NC>(tl + mt * NC, o);
+        tmem_ld16(tl + mt * NC + c0, o);
+        if (FP8) tmem_ld16(tl + mt * NC + NT + c0, lo);
         tmem_wait_ld();
-      } else {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) o[c] = 0u;
       }
+      float y[16];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
+      for (int c = 0; c < 16; ++c) {
         float v = __uint_as_float(o[c]);
-        if (FP8) v = fmaf(__uint_as_float(o[NC - NT + c]), 0.0625f, v) * 0.015625f;
-        if (whole) {
-          const float sum = sm.fac()[c];
-          const float y = sum == 0.f ? 0.f : v / sum;
-          if (x.r0 + c < p.R)
-            p.out[(static_cast<int64_t>(x.b) * p.R + x.r0 + c) * kLat + mt * 128 + t] = __float2bfloat16_rn(y);
-        } else {
-          p.part_o[(static_cast<int64_t>(slot) * NT + c) * kLat + mt * 128 + t] = v;
-        }
+        if (FP8) v = fmaf(__uint_as_float(lo[c]), 0.0625f, v) * 0.015625f;
+        const float f = sm.fac()[c0 + c];
+        y[c] = tiles == 0 || f == 0.f ? 0.f : v * f;  // no key, or no query (whose scores may be anything)
+      }
+      if (whole) {
+        __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0) * kLat + mt * 128 + t;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < rows) d[c * kLat] = __float2bfloat16_rn(y[c]);
+      } else {
+        float* d = p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat + mt * 128 + t;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) d[c * kLat] = y[c];
       }
     }
     if (t < NT) {
-      const float sum = sm.fac()[t];
       const int r = x.r0 + t;
       if (!whole) {
         p.part_ml[slot * NT + t] = make_float2(sm.ref()[t], sum);
@@ -553,7 +616,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
   const int entries = p.B * p.RT;
   const int run = (entries + kLatThreads - 1) / kLatThreads;
   const int e_begin = min(static_cast<int>(threadIdx.x) * run, entries), e_end = min(e_begin + run, entries);
-  int64_t mine = 0;
+  int mine = 0;
   for (int e = e_begin; e < e_end; ++e) {
     const LatEntry x = lat_entry<NT>(p, e);
     mine += lat_units(x.keys);
@@ -563,29 +626,30 @@ __global__ void __launch_bounds__(kLatThreads, 1)
         if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxLength);
     }
   }
-  int64_t incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
     if (lane >= o) incl += v;
   }
-  int64_t* scan = sm.scan();
+  int* scan = sm.scan();
   if (lane == 31) scan[warp] = incl;
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  int64_t before = 0, total = 0;
+  int before = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < kLatThreads / 32; ++i) {
     if (i < warp) before += scan[i];
     total += scan[i];
   }
   // with fewer units than CTAs the first ones get one each: the CTAs of an entry are always neighbours
-  const int64_t busy = min(total, static_cast<int64_t>(gridDim.x)), me = min(static_cast<int64_t>(blockIdx.x), busy);
-  const int64_t u0 = total * me / busy, u1 = total * min(me + 1, busy) / busy;
+  const int busy = min(total, static_cast<int>(gridDim.x)), me = static_cast<int>(blockIdx.x);
+  const int share = total / busy, more = total - share * busy;
+  const int u0 = me < busy ? me * share + min(me, more) : total, u1 = me < busy ? u0 + share + (me < more ? 1 : 0) : total;
   {
-    int64_t at = before + incl - mine;  // units in front of this thread's entries
+    int at = before + incl - mine;  // units in front of this thread's entries
     if (u0 < u1 && at <= u0 && u0 < at + mine) {
       int e = e_begin;
       while (true) {
@@ -600,8 +664,8 @@ __global__ void __launch_bounds__(kLatThreads, 1)
   }
   __syncthreads();
   LatWalk<NT> walk;
-  walk.e = u0 < u1 ? static_cast<int>(scan[8]) : 0;
-  walk.off = u0 < u1 ? static_cast<int>(scan[9]) : 0;
+  walk.e = u0 < u1 ? scan[8] : 0;
+  walk.off = u0 < u1 ? scan[9] : 0;
   walk.left = u1 - u0;
   bool healthy = *abort_flag == 0u;
   if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzled tiles need a 1024-byte aligned window
@@ -663,67 +727,76 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
     const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
     const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
-    uint32_t it = 0, tile = 0, q_phase = 0;
-    while (walk.next(p)) {
-      const int tiles = walk.tiles();
+    uint32_t slot = 0, phase = 0, rs = 0, rphase = 0, tile_phase = 0, q_phase = 0;
+    while (__any_sync(0xFFFFFFFFu, walk.next(p))) {
+      const int tiles = uniform(walk.tiles()), keys = uniform(walk.k1 - walk.k0);
       if (tiles > 0) {
         mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
         q_phase ^= 1;
       }
-      for (int j = 0; j < tiles; ++j, ++tile) {
+      for (int j = 0; j < tiles; ++j) {
+        uint32_t s = slot, ph = phase;
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t s = (it + i) % L::NS;
-          mbar_wait(sm.full(s), ((it + i) / L::NS) & 1, ctl, 0x400 + s);
+          mbar_wait(sm.full(s), ph, ctl, 0x400 + s);
           tc_fence_after_sync();
-          if (leader) {
-            if (FP8) {
+          const uint64_t kd = desc_advance(k_desc, uniform(s) * L::kSlot);
+          if (FP8) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_ss_f8(tmem + kColS, desc_advance(k_desc, s * L::kSlot + k * 32),
-                           desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
-            } else {
+            for (int k = 0; k < 4; ++k)
+              if (leader)
+                umma_ss_f8(tmem + kColS, desc_advance(kd, k * 32), desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk,
+                           (i > 0 || k > 0) ? 1u : 0u);
+          } else {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                umma_ss(tmem + kColS, desc_advance(k_desc, s * L::kSlot + (k >> 2) * 16384 + (k & 3) * 32),
+            for (int k = 0; k < 8; ++k)
+              if (leader)
+                umma_ss(tmem + kColS, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
                         desc_advance(q_desc, (2 * i + (k >> 2)) * (NT * 128) + (k & 3) * 32), id_qk,
                         (i > 0 || k > 0) ? 1u : 0u);
-            }
           }
+          if (++s == L::NS) { s = 0; ph ^= 1; }
         }
-        const uint32_t rs = tile % L::kRopeSlots;
-        mbar_wait(sm.rfull(rs), (tile / L::kRopeSlots) & 1, ctl, 0x500 + rs);
+        mbar_wait(sm.rfull(rs), rphase, ctl, 0x500 + rs);
         tc_fence_after_sync();
-        if (leader) {
+        const uint64_t rd = desc_advance(r_desc, uniform(rs) * 16384);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(tmem + (FP8 ? kColR : kColS), desc_advance(r_desc, rs * 16384 + k * 32), desc_advance(qr_desc, k * 32),
-                    id_rope, (!FP8 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k)
+          if (leader)
+            umma_ss(tmem + (FP8 ? kColR : kColS), desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope,
+                    (!FP8 || k > 0) ? 1u : 0u);
+        if (leader) {
           umma_commit(sm.s_full());
           if (FP8) umma_commit(sm.rempty(rs));
         }
-        mbar_wait(sm.p_full(), tile & 1, ctl, 0x600);
+        const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
+        mbar_wait(sm.p_full(), tile_phase, ctl, 0x600);
+        tile_phase ^= 1;
         tc_fence_after_sync();
-        for (int i = 0; i < 4; ++i, ++it) {
-          const uint32_t s = it % L::NS;
-          if (leader) {
-            if (FP8) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_ss_f8(tmem + i * L::NC, desc_advance(v_desc, s * L::kSlot + k * 4096), desc_advance(p_desc, k * 32),
-                           id_pv, (j > 0 || k > 0) ? 1u : 0u);
-            } else {
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t vd = desc_advance(v_desc, uniform(slot) * L::kSlot);
+          if (FP8) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                umma_ss(tmem + i * L::NC, desc_advance(v_desc, s * L::kSlot + k * 2048),
+            for (int k = 0; k < 4; ++k)
+              if (leader && k < steps)
+                umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(p_desc, k * 32), id_pv,
+                           (j > 0 || k > 0) ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (leader && k < steps)
+                umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048),
                         desc_advance(p_desc, (k >> 2) * (NT * 128) + (k & 3) * 32), id_pv, (j > 0 || k > 0) ? 1u : 0u);
-            }
-            umma_commit(sm.empty(s));
           }
+          if (leader) umma_commit(sm.empty(slot));
+          if (++slot == L::NS) { slot = 0; phase ^= 1; }
         }
         if (leader) {
           if (!FP8) umma_commit(sm.rempty(0));
           if (j + 1 == tiles) umma_commit(sm.o_full());
         }
+        if (++rs == L::kRopeSlots) { rs = 0; rphase ^= 1; }
       }
     }
   } else if (warp >= 4) {
@@ -863,7 +936,8 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
   const int nt = lat_rows(rows, fp8);
   const int64_t rt = (rows + nt - 1) / nt;
-  PITH_REQUIRE(rt * a->B < 2147483647 - 1024, "too many query rows");
+  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2) < 2147483647 - 1024,
+               "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
   LatAttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->q);
