@@ -6,6 +6,8 @@ All functions enqueue on the current CUDA stream of the tensors' device and retu
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 
 import torch
 
@@ -426,202 +428,206 @@ def mla_assemble_bwd(cos, sin, dquery, dkey, dvalue):
 
 
 # --------------------------------------------------------------------------- MLA latent cache
+# Operators of a few microseconds: every attribute of a tensor is fetched once, and the argument struct is packed in one
+# go (fields in the order of the ctypes mirrors in _lib).
 _NUMBER = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_WRITE = _lib.packer(_lib.LatentWriteArgs).pack
+_READ = _lib.packer(_lib.LatentReadArgs).pack
+_ATTN = _lib.packer(_lib.LatentAttnArgs).pack
+_PROJ = _lib.packer(_lib.LatentProjArgs).pack
+_INT32_MAX = 2 ** 31 - 1
 
 
-def _one_device(device, **ts):
-    """CUDA tensors of one device: a kernel launched on `device` reads and writes all of them."""
-    for name, t in ts.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if device.type != "cuda":
+def _device_index(what: str, first: torch.Tensor, *others) -> int:
+    """Index of the CUDA device that holds all of the given tensors."""
+    idx = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}, expected one device")
+    if idx < 0:
         raise RuntimeError("pith_b200 operators run on CUDA tensors only (no CPU fallback)")
+    return idx
 
 
-def _bs(t: torch.Tensor) -> I64x2:
-    """b and s strides of a [B or 1, S, ...] tensor; a batch of one is broadcast."""
-    return I64x2(t.stride(0) if t.shape[0] > 1 else 0, t.stride(1))
+def _enqueue(entry: str, args: bytes, idx: int, launches: int) -> None:
+    """Calls an entry on the current stream of device `idx`, whichever device is current."""
+    global launch_count
+    fn = _lib.packed_entry(entry)
+    if torch.cuda.current_device() == idx:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _lib.check(rc, entry)
+    launch_count += launches
 
 
-def _rotary(a, cos, sin, position_ids, B: int, S: int) -> None:
-    """Fills cos / sin / positions of an argument struct after checking them: tables [rows, 64] with position_ids
-    [B or 1, S], or [B or 1, S, 64] (or tables: rows 0 .. S - 1) without."""
-    if cos.dtype not in _NUMBER or sin.dtype != cos.dtype:
+def _status_ptr(idx: int) -> int:
+    w = _status_words.get(idx)
+    return (w if w is not None else status_word(torch.device("cuda", idx))).data_ptr()
+
+
+def _rotary(cos, sin, position_ids, B: int, S: int):
+    """Checks cos / sin / position_ids: tables [rows, 64] with position_ids [B or 1, S], or [B or 1, S, 64] (or tables: rows
+    0 .. S - 1) without. Returns (cos, sin, positions pointers, dtype number, table rows, cs strides, position strides)."""
+    number = _NUMBER.get(cos.dtype)
+    if number is None or sin.dtype != cos.dtype:
         raise TypeError("cos and sin must both be bfloat16 or float32")
-    if cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(-1) != 1 or cos.shape[-1] != 64:
+    shape, strides = cos.shape, cos.stride()
+    if sin.shape != shape or sin.stride() != strides or shape[-1] != 64 or strides[-1] != 1:
         raise ValueError("cos and sin must be [..., 64] with a contiguous last dimension, equal shapes and strides")
     if position_ids is not None:
-        if cos.dim() != 2:
-            raise ValueError(f"with position_ids, cos and sin are tables [rows, 64], got {tuple(cos.shape)}")
+        if len(shape) != 2:
+            raise ValueError(f"with position_ids, cos and sin are tables [rows, 64], got {tuple(shape)}")
         if position_ids.dtype != torch.int64:
             raise TypeError("position_ids must be int64")
-        if position_ids.dim() != 2 or position_ids.shape[0] not in (1, B) or position_ids.shape[1] != S:
-            raise ValueError(f"position_ids has shape {tuple(position_ids.shape)}, expected {(B, S)}")
-        a.positions, a.positions_stride = position_ids.data_ptr(), _bs(position_ids)
-        a.cs_stride = I64x2(0, cos.stride(0))
-        a.table_rows = cos.shape[0]
-    elif cos.dim() == 2:
-        if cos.shape[0] < S:
-            raise ValueError(f"cos and sin have {cos.shape[0]} rows, {S} are needed")
-        a.cs_stride = I64x2(0, cos.stride(0))
-    else:
-        if cos.dim() != 3 or cos.shape[0] not in (1, B) or cos.shape[1] != S:
-            raise ValueError(f"cos and sin have shape {tuple(cos.shape)}, expected [B or 1, {S}, 64]")
-        a.cs_stride = _bs(cos)
-    a.cos, a.sin, a.cs_dtype = cos.data_ptr(), sin.data_ptr(), _NUMBER[cos.dtype]
+        pshape = position_ids.shape
+        if len(pshape) != 2 or pshape[0] not in (1, B) or pshape[1] != S:
+            raise ValueError(f"position_ids has shape {tuple(pshape)}, expected {(B, S)}")
+        pb, ps = position_ids.stride()
+        return (cos.data_ptr(), sin.data_ptr(), position_ids.data_ptr(), number, shape[0], 0, strides[0],
+                pb if pshape[0] > 1 else 0, ps)
+    if len(shape) == 2:
+        if shape[0] < S:
+            raise ValueError(f"cos and sin have {shape[0]} rows, {S} are needed")
+        return cos.data_ptr(), sin.data_ptr(), 0, number, 0, 0, strides[0], 0, 0
+    if len(shape) != 3 or shape[0] not in (1, B) or shape[1] != S:
+        raise ValueError(f"cos and sin have shape {tuple(shape)}, expected [B or 1, {S}, 64]")
+    return cos.data_ptr(), sin.data_ptr(), 0, number, 0, strides[0] if shape[0] > 1 else 0, strides[1], 0, 0
 
 
 def latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps: float, position_ids=None) -> None:
     """RMSNorm + rotary embedding of new tokens and their store in the cache; see ``pith_latent_write``."""
-    if k_pe.dim() == 4 and k_pe.shape[2] == 1:
-        k_pe = k_pe[:, :, 0]
-    if compressed_kv.dim() != 3 or compressed_kv.shape[2] != 512 or compressed_kv.stride(2) != 1:
-        raise ValueError(f"compressed_kv must be [B,S,512] with a contiguous last dimension, got "
-                         f"{tuple(compressed_kv.shape)}")
-    B, S, _ = compressed_kv.shape
-    if tuple(k_pe.shape) != (B, S, 64) or k_pe.stride(2) != 1:
-        raise ValueError(f"k_pe must be [B,S,64] or [B,S,1,64] with a contiguous last dimension, got {tuple(k_pe.shape)}")
+    shape, kv_stride = compressed_kv.shape, compressed_kv.stride()
+    if len(shape) != 3 or shape[2] != 512 or kv_stride[2] != 1:
+        raise ValueError(f"compressed_kv must be [B,S,512] with a contiguous last dimension, got {tuple(shape)}")
+    B, S, _ = shape
+    pe_shape, pe_stride = k_pe.shape, k_pe.stride()
+    if pe_shape != (B, S, 64) and pe_shape != (B, S, 1, 64) or pe_stride[-1] != 1:
+        raise ValueError(f"k_pe must be [B,S,64] or [B,S,1,64] with a contiguous last dimension, got {tuple(pe_shape)}")
     if compressed_kv.dtype != torch.bfloat16 or k_pe.dtype != torch.bfloat16:
         raise TypeError("compressed_kv and k_pe must be bfloat16")
-    if norm_weight.dtype not in _NUMBER:
+    w_number = _NUMBER.get(norm_weight.dtype)
+    if w_number is None:
         raise TypeError("norm_weight must be bfloat16 or float32")
-    if tuple(norm_weight.shape) != (512,) or not norm_weight.is_contiguous():
+    if norm_weight.shape != (512,) or not norm_weight.is_contiguous():
         raise ValueError("norm_weight must be contiguous [512]")
     if slots.dtype != torch.int64:
         raise TypeError("slots must be int64")
-    _expect(slots, (B, S), "slots")
-    a = _lib.LatentWriteArgs()
-    _rotary(a, cos, sin, position_ids, B, S)
-    dev = compressed_kv.device
-    _one_device(dev, k_pe=k_pe, norm_weight=norm_weight, cos=cos, sin=sin, slots=slots, position_ids=position_ids,
-                cache=cache.latent)
-    a.cache = cache.args
-    a.compressed_kv, a.k_pe, a.norm_weight = compressed_kv.data_ptr(), k_pe.data_ptr(), norm_weight.data_ptr()
-    a.slots, a.status = slots.data_ptr(), status_word(dev).data_ptr()
-    a.B, a.S, a.eps, a.weight_dtype = B, S, float(eps), _NUMBER[norm_weight.dtype]
-    a.kv_stride = I64x2(compressed_kv.stride(0), compressed_kv.stride(1))
-    a.k_pe_stride = I64x2(k_pe.stride(0), k_pe.stride(1))
-    a.slots_stride = I64x2(slots.stride(0), slots.stride(1))
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pith_latent_write(ctypes.byref(a), _stream(slots)), "pith_latent_write")
-    _count(1 if B * S else 0)
+    if slots.shape != (B, S):
+        raise ValueError(f"slots has shape {tuple(slots.shape)}, expected {(B, S)}")
+    cp, sp, pp, cs_number, rows, cs0, cs1, ps0, ps1 = _rotary(cos, sin, position_ids, B, S)
+    idx = _device_index("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, slots, position_ids,
+                        cache.latent)
+    sl0, sl1 = slots.stride()
+    args = _WRITE(*cache.flat, compressed_kv.data_ptr(), k_pe.data_ptr(), norm_weight.data_ptr(), cp, sp,
+                  slots.data_ptr(), pp, _status_ptr(idx), B, S, w_number, cs_number, rows, eps,
+                  kv_stride[0], kv_stride[1], pe_stride[0], pe_stride[1], cs0, cs1, sl0, sl1, ps0, ps1)
+    _enqueue("pith_latent_write", args, idx, 1 if B * S else 0)
 
 
 def latent_read(cache, slots):
     """(latent bf16 [..., 512], k_pe bf16 [..., 64]) of the given slots; see ``pith_latent_read``."""
     if slots.dtype != torch.int64:
         raise TypeError("slots must be int64")
-    dev = slots.device
-    _one_device(dev, cache=cache.latent)
-    slots = slots.contiguous()
-    latent = torch.empty((*slots.shape, 512), dtype=torch.bfloat16, device=dev)
-    k_pe = torch.empty((*slots.shape, 64), dtype=torch.bfloat16, device=dev)
-    a = _lib.LatentReadArgs()
-    a.cache = cache.args
-    a.slots, a.latent, a.k_pe = slots.data_ptr(), latent.data_ptr(), k_pe.data_ptr()
-    a.status, a.n = status_word(dev).data_ptr(), slots.numel()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pith_latent_read(ctypes.byref(a), _stream(slots)), "pith_latent_read")
-    _count(1 if a.n else 0)
+    idx = _device_index("latent_cache_read", slots, cache.latent)
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    shape, n = slots.shape, slots.numel()
+    latent = cache.rope.new_empty((*shape, 512))
+    k_pe = cache.rope.new_empty((*shape, 64))
+    args = _READ(*cache.flat, slots.data_ptr(), latent.data_ptr(), k_pe.data_ptr(), _status_ptr(idx), n)
+    _enqueue("pith_latent_read", args, idx, 1 if n else 0)
     return latent, k_pe
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_workspace(idx: int, B: int, S: int, H: int, max_keys: int, dtype: int) -> int:
+    with torch.cuda.device(idx):
+        return _lib.load().pith_latent_attn_workspace_bytes(B, S, H, max_keys, dtype)
 
 
 def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query_lens=None, tree_mask=None,
                 return_lse: bool = False):
     """(out bf16 [B,Sq,H,512], lse fp32 log2 [B,H,Sq] or None) over the paged latent cache; see ``pith_latent_attn``."""
-    if query.dim() != 4 or query.shape[3] != 576 or query.stride(3) != 1:
-        raise ValueError(f"query must be [B,S,H,576] with a contiguous last dimension, got {tuple(query.shape)}")
+    shape, q_stride = query.shape, query.stride()
+    if len(shape) != 4 or shape[3] != 576 or q_stride[3] != 1:
+        raise ValueError(f"query must be [B,S,H,576] with a contiguous last dimension, got {tuple(shape)}")
     if query.dtype != torch.bfloat16:
         raise TypeError("query must be bfloat16")
-    B, S, H, _ = query.shape
+    B, S, H, _ = shape
     if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise TypeError("block_table and seq_lens must be int32")
-    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or \
-            (B and block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise ValueError(f"block_table must be [{B}, pages] with contiguous rows, got {tuple(block_table.shape)}")
-    _expect(seq_lens, (B,), "seq_lens")
-    if not seq_lens.is_contiguous():
-        raise ValueError("seq_lens must be contiguous")
+    t_shape = block_table.shape
+    if len(t_shape) != 2 or t_shape[0] != B or t_shape[1] < 1 or (block_table.stride(1) != 1 and t_shape[1] > 1):
+        raise ValueError(f"block_table must be [{B}, pages] with contiguous rows, got {tuple(t_shape)}")
+    if seq_lens.shape != (B,) or not seq_lens.is_contiguous():
+        raise ValueError(f"seq_lens has shape {tuple(seq_lens.shape)}, expected contiguous {(B,)}")
+    ql = tm = tm0 = tm1 = 0
     if query_lens is not None:
         if query_lens.dtype != torch.int32:
             raise TypeError("query_lens must be int32")
-        _expect(query_lens, (B,), "query_lens")
-        if not query_lens.is_contiguous():
-            raise ValueError("query_lens must be contiguous")
+        if query_lens.shape != (B,) or not query_lens.is_contiguous():
+            raise ValueError(f"query_lens has shape {tuple(query_lens.shape)}, expected contiguous {(B,)}")
+        ql = query_lens.data_ptr()
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool:
             raise TypeError("tree_mask must be bool")
-        _expect(tree_mask, (B, S, S), "tree_mask")
-        if S > 1 and tree_mask.stride(2) != 1:
+        if tree_mask.shape != (B, S, S):
+            raise ValueError(f"tree_mask has shape {tuple(tree_mask.shape)}, expected {(B, S, S)}")
+        tm0, tm1, last = tree_mask.stride()
+        if S > 1 and last != 1:
             raise ValueError("tree_mask must have a contiguous last dimension")
-    if not softmax_scale > 0:
-        raise ValueError("softmax_scale must be positive")
-    dev = query.device
-    _one_device(dev, cache=cache.latent, block_table=block_table, seq_lens=seq_lens, query_lens=query_lens,
-                tree_mask=tree_mask)
-    out = torch.empty((B, S, H, 512), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((B, H, S), dtype=torch.float32, device=dev) if return_lse else None
-    lib = _lib.load()
-    a = _lib.LatentAttnArgs()
-    a.cache = cache.args
-    a.q, a.out, a.block_table, a.seq_lens = query.data_ptr(), out.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr()
-    if lse is not None:
-        a.lse = lse.data_ptr()
-    if query_lens is not None:
-        a.query_lens = query_lens.data_ptr()
-    if tree_mask is not None:
-        a.tree_mask, a.tree_stride = tree_mask.data_ptr(), I64x2(tree_mask.stride(0), tree_mask.stride(1))
-    a.status = status_word(dev).data_ptr()
-    a.B, a.Sq, a.H, a.table_cols, a.softmax_scale = B, S, H, block_table.shape[1], float(softmax_scale)
-    a.q_stride, a.table_stride = I64x3(*query.stride()[:3]), block_table.stride(0)
-    max_keys = block_table.shape[1] * cache.page_size
-    with torch.cuda.device(dev):
-        # allocated per call on the current stream: calls on other streams and captured graphs each have their own
-        a.workspace_bytes = lib.pith_latent_attn_workspace_bytes(B, S, H, max_keys, a.cache.dtype)
-        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=dev)
-        a.workspace = workspace.data_ptr()
-        _lib.check(lib.pith_latent_attn(ctypes.byref(a), _stream(query)), "pith_latent_attn")
-    _count((2 if max_keys > 64 else 1) if out.numel() else 0)
+        tm = tree_mask.data_ptr()
+    if not 0.0 < softmax_scale < math.inf:
+        raise ValueError("softmax_scale must be positive and finite")
+    max_keys = t_shape[1] * cache.page_size
+    if max_keys > _INT32_MAX:
+        raise ValueError(f"block_table covers {max_keys} keys a sequence")
+    idx = _device_index("latent_attention", query, cache.latent, block_table, seq_lens, query_lens, tree_mask)
+    out = query.new_empty((B, S, H, 512))
+    lse = query.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
+    # allocated per call on the current stream: calls on other streams and captured graphs each have their own
+    nbytes = _attn_workspace(idx, B, S, H, max_keys, cache.flat[3])
+    workspace = query.new_empty(nbytes, dtype=torch.uint8)
+    args = _ATTN(*cache.flat, query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                 block_table.data_ptr(), seq_lens.data_ptr(), ql, tm, workspace.data_ptr(), _status_ptr(idx), nbytes,
+                 B, S, H, t_shape[1], softmax_scale, q_stride[0], q_stride[1], q_stride[2], block_table.stride(0), tm0, tm1)
+    _enqueue("pith_latent_attn", args, idx, (2 if max_keys > 64 else 1) if B * S * H else 0)
     return out, lse
 
 
-def _proj_args(x, weight, width: int, name: str):
-    if x.dim() != 4 or x.shape[3] != width or x.stride(3) != 1:
-        raise ValueError(f"{name} must be [B,S,H,{width}] with a contiguous last dimension, got {tuple(x.shape)}")
+def _proj_check(x, weight, width: int, name: str):
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 4 or shape[3] != width or stride[3] != 1:
+        raise ValueError(f"{name} must be [B,S,H,{width}] with a contiguous last dimension, got {tuple(shape)}")
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise TypeError(f"{name} and kv_b_weight must be bfloat16")
-    B, S, H, _ = x.shape
-    if tuple(weight.shape) != (H * 256, 512) or weight.stride(1) != 1:
-        raise ValueError(f"kv_b_weight must be [{H * 256}, 512] with contiguous rows, got {tuple(weight.shape)}")
-    a = _lib.LatentProjArgs()
-    a.B, a.S, a.H = B, S, H
-    a.x, a.weight = x.data_ptr(), weight.data_ptr()
-    a.x_stride, a.weight_stride = I64x3(*x.stride()[:3]), weight.stride(0)
-    return a
+    w_shape, w_stride = weight.shape, weight.stride()
+    if w_shape != (shape[2] * 256, 512) or w_stride[1] != 1:
+        raise ValueError(f"kv_b_weight must be [{shape[2] * 256}, 512] with contiguous rows, got {tuple(w_shape)}")
+    return shape, stride, w_stride[0]
 
 
 def latent_query(q, weight, cos, sin, position_ids=None):
     """[B,S,H,576] bf16: the query with the key half of kv_b_proj folded in, and rotated; see ``pith_latent_query``."""
-    a = _proj_args(q, weight, 192, "q")
-    _rotary(a, cos, sin, position_ids, a.B, a.S)
-    dev = q.device
-    _one_device(dev, kv_b_weight=weight, cos=cos, sin=sin, position_ids=position_ids)
-    out = torch.empty((a.B, a.S, a.H, 576), dtype=torch.bfloat16, device=dev)
-    a.out, a.status = out.data_ptr(), status_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pith_latent_query(ctypes.byref(a), _stream(q)), "pith_latent_query")
-    _count(1 if out.numel() else 0)
+    (B, S, H, _), stride, w_stride = _proj_check(q, weight, 192, "q")
+    cp, sp, pp, cs_number, rows, cs0, cs1, ps0, ps1 = _rotary(cos, sin, position_ids, B, S)
+    idx = _device_index("latent_query", q, weight, cos, sin, position_ids)
+    out = q.new_empty((B, S, H, 576))
+    args = _PROJ(q.data_ptr(), weight.data_ptr(), out.data_ptr(), cp, sp, pp, _status_ptr(idx), B, S, H, cs_number, rows,
+                 stride[0], stride[1], stride[2], w_stride, cs0, cs1, ps0, ps1)
+    _enqueue("pith_latent_query", args, idx, 1 if B * S * H else 0)
     return out
 
 
 def latent_output(attn, weight):
     """[B,S,H,128] bf16: the value half of kv_b_proj applied to latent attention's result; see ``pith_latent_output``."""
-    a = _proj_args(attn, weight, 512, "attn")
-    dev = attn.device
-    _one_device(dev, kv_b_weight=weight)
-    out = torch.empty((a.B, a.S, a.H, 128), dtype=torch.bfloat16, device=dev)
-    a.out, a.status = out.data_ptr(), status_word(dev).data_ptr()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().pith_latent_output(ctypes.byref(a), _stream(attn)), "pith_latent_output")
-    _count(1 if out.numel() else 0)
+    (B, S, H, _), stride, w_stride = _proj_check(attn, weight, 512, "attn")
+    idx = _device_index("latent_output", attn, weight)
+    out = attn.new_empty((B, S, H, 128))
+    args = _PROJ(attn.data_ptr(), weight.data_ptr(), out.data_ptr(), 0, 0, 0, _status_ptr(idx), B, S, H, 0, 0,
+                 stride[0], stride[1], stride[2], w_stride, 0, 0, 0, 0)
+    _enqueue("pith_latent_output", args, idx, 1 if B * S * H else 0)
     return out

@@ -21,15 +21,11 @@ from __future__ import annotations
 
 import torch
 
-
-def _kernels():
-    from ... import kernels
-    return kernels
+from ... import _lib, kernels
 
 
-def _no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+def _refuse(what: str) -> None:
+    raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 class LatentCache:
@@ -61,16 +57,10 @@ class LatentCache:
             if t is not None and t.device != latent.device:
                 raise ValueError(f"{name} is on {t.device}, latent on {latent.device}")
         self.latent, self.rope, self.scale = latent, rope, scale
-        from ... import _lib
-        a = self.args = _lib.LatentCacheArgs()
-        a.latent, a.rope = latent.data_ptr(), rope.data_ptr()
-        a.scale = scale.data_ptr() if scale is not None else None
-        a.dtype = _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3
-        a.pages, a.page_size = pages, page_size
-        a.latent_stride = _lib.I64x2(latent.stride(0), latent.stride(1))
-        a.rope_stride = _lib.I64x2(rope.stride(0), rope.stride(1))
-        if scale is not None:
-            a.scale_stride = _lib.I64x2(scale.stride(0), scale.stride(1))
+        # the fields of pith_latent_cache, in order
+        self.flat = (latent.data_ptr(), rope.data_ptr(), scale.data_ptr() if scale is not None else 0,
+                     _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, pages, page_size,
+                     *latent.stride()[:2], *rope.stride()[:2], *(scale.stride() if scale is not None else (0, 0)))
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -101,15 +91,16 @@ def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: t
     already gathered. fp32 arithmetic, one rounding to the cache's type; an 8-bit row gets the least power of two as its
     scale with which no value passes 448.
     """
-    _no_gradient("latent_cache_write", compressed_kv, k_pe, norm_weight)
-    _kernels().latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
+    if torch.is_grad_enabled() and (compressed_kv.requires_grad or k_pe.requires_grad or norm_weight.requires_grad):
+        _refuse("latent_cache_write")
+    kernels.latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
 
 
 def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
     """Rows of the cache as bf16, ``(latent [*slots.shape, 512], k_pe [*slots.shape, 64])``: what the expanded form of a
     prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
     give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
-    return _kernels().latent_read(cache, slots)
+    return kernels.latent_read(cache, slots)
 
 
 def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -133,9 +124,9 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     results do not depend on the other sequences of the batch by more than fp32 rounding of partial sums, and repeat
     bit for bit for the same inputs.
     """
-    _no_gradient("latent_attention", query)
-    out, lse = _kernels().latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask,
-                                      return_lse)
+    if torch.is_grad_enabled() and query.requires_grad:
+        _refuse("latent_attention")
+    out, lse = kernels.latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -145,12 +136,14 @@ def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, 
     viewed per head; strided views are fine) -> ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
     ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
     cos / sin / position_ids as in ``latent_cache_write``."""
-    _no_gradient("latent_query", q, kv_b_weight)
-    return _kernels().latent_query(q, kv_b_weight, cos, sin, position_ids)
+    if torch.is_grad_enabled() and (q.requires_grad or kv_b_weight.requires_grad):
+        _refuse("latent_query")
+    return kernels.latent_query(q, kv_b_weight, cos, sin, position_ids)
 
 
 def latent_output(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor:
     """``latent_attention``'s result ``[B,S,H,512]`` times head h's value rows of ``kv_b_weight``: ``[B,S,H,128]`` bf16,
     contiguous, which the layer views as ``[B,S,H * 128]`` for ``o_proj``."""
-    _no_gradient("latent_output", attn, kv_b_weight)
-    return _kernels().latent_output(attn, kv_b_weight)
+    if torch.is_grad_enabled() and (attn.requires_grad or kv_b_weight.requires_grad):
+        _refuse("latent_output")
+    return kernels.latent_output(attn, kv_b_weight)
