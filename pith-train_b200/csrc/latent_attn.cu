@@ -33,32 +33,38 @@ namespace pith {
 constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
 constexpr int kUnit = 64;   // keys per unit of work
-constexpr int kLatThreads = 256;
+constexpr int kExtra = 2;   // units of work that another piece costs a CTA
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
-constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit); O^T starts at 0
+constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
 
 template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
+  static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
+  static constexpr int CW = NT / G;
+  static constexpr int kThreads = 128 + 128 * G;
   static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
   static constexpr int kRopeSlots = FP8 ? 2 : 1;         // 128 keys x 64 dims
   static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
   static constexpr int kQ = kQLat + NT * 128;
   static constexpr int kP = NT * 256;
   static constexpr int kMisc = NT == 16 ? 1024 : 4096;
-  // bf16: P overlays the rope tile, which the score GEMM has finished with when P is written
-  static constexpr int kFixed = kRopeSlots * 16384 + kQ + (FP8 ? kP : 0) + kMisc;
+  // bf16: P overlays the rope tile, which the score GEMM has finished with when P is written; 8-bit: two buffers
+  static constexpr int kFixed = kRopeSlots * 16384 + kQ + (FP8 ? 2 * kP : 0) + kMisc;
   static constexpr int NS = (232448 - kFixed) / kSlot;
+  // Slots of the next tile whose score GEMM may run before this tile's output GEMM: what the ring holds beyond one tile.
+  static constexpr int kAhead = NS >= 8 ? 4 : NS - 4;
   static constexpr int kRopeOff = NS * kSlot;
   static constexpr int kQOff = kRopeOff + kRopeSlots * 16384;
   static constexpr int kPOff = FP8 ? kQOff + kQ : kRopeOff;
-  static constexpr int kMiscOff = FP8 ? kPOff + kP : kQOff + kQ;
+  static constexpr int kMiscOff = FP8 ? kPOff + 2 * kP : kQOff + kQ;
   static constexpr int kAlloc = kMiscOff + kMisc;
-  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 4;
+  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 6;
   static_assert(NS >= 4, "a tile's four latent slots must fit at once");
-  static_assert(kBars * 8 + 16 + 96 + NT * 40 <= kMisc, "misc area too small");
+  static_assert(!FP8 || kAhead == 4, "the 8-bit pipeline holds two tiles");
+  static_assert(kBars * 8 + 16 + 48 + NT * 40 <= kMisc, "misc area too small");
   static_assert(kAlloc <= 232448, "shared memory");
-  static_assert(4 * NC <= kColS && kColS + NC <= kColR, "TMEM columns");
+  static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
 };
 
 struct LatAttnParams {
@@ -96,25 +102,28 @@ __device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
 }
 __device__ __forceinline__ int lat_units(int keys) { return max((keys + kUnit - 1) / kUnit, 1); }
 
-// Walks the pieces of this CTA's share of the line. Every role keeps its own copy.
+// Walks the pieces of this CTA's share of the line. Every role keeps its own copy. An entry takes `extra` places of the line
+// in front of its units: what beginning another piece costs a CTA.
 template <int NT>
 struct LatWalk {
-  int e, off, left;
+  int e, off, left, extra;  // off: place inside entry e
   LatEntry x;
   int k0, k1;   // keys [k0, k1) of the entry
   bool begins, ends;
   __device__ __forceinline__ bool next(const LatAttnParams& p) {
-    if (left <= 0) return false;
-    x = lat_entry<NT>(p, e);
-    const int n = lat_units(x.keys);
-    const int take = min(n - off, left);
-    k0 = off * kUnit;
-    k1 = min(x.keys, (off + take) * kUnit);
-    begins = off == 0;
-    ends = off + take == n;
-    left -= take;
-    if (ends) { ++e; off = 0; } else { off += take; }
-    return true;
+    while (left > 0) {
+      x = lat_entry<NT>(p, e);
+      const int n = lat_units(x.keys) + extra;
+      const int take = min(n - off, left), u0 = max(off - extra, 0), u1 = off + take - extra;
+      k0 = u0 * kUnit;
+      k1 = min(x.keys, u1 * kUnit);
+      begins = u0 == 0;
+      ends = off + take == n;
+      left -= take;
+      if (ends) { ++e; off = 0; } else { off += take; }
+      if (u1 > u0) return true;  // else the share ends in front of the entry's first unit
+    }
+    return false;
   }
   __device__ __forceinline__ int tiles() const { return (k1 - k0 + kTile - 1) / kTile; }
 };
@@ -228,30 +237,32 @@ struct LatShared {
   __device__ uint64_t* empty(int i) const { return bars + L::NS + i; }
   __device__ uint64_t* rfull(int i) const { return bars + 2 * L::NS + i; }
   __device__ uint64_t* rempty(int i) const { return bars + 2 * L::NS + L::kRopeSlots + i; }
-  __device__ uint64_t* q_full() const { return bars + L::kBars - 4; }
-  __device__ uint64_t* s_full() const { return bars + L::kBars - 3; }
+  __device__ uint64_t* q_full() const { return bars + L::kBars - 6; }
+  __device__ uint64_t* q_empty() const { return bars + L::kBars - 5; }
+  __device__ uint64_t* s_full(int i) const { return bars + L::kBars - 4 + i; }
   __device__ uint64_t* p_full() const { return bars + L::kBars - 2; }
-  __device__ uint64_t* o_full() const { return bars + L::kBars - 1; }
+  __device__ uint64_t* o_full() const { return bars + L::kBars - 1; }  // a tile's output GEMMs have completed
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
-  __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 2); }              // [8 warps] + share
-  __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 14); }         // 10 NT words
+  __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 1); }             // [12 warps] + start
+  __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 10 NT words
   __device__ float* ref() const { return cols(); }
   __device__ float* fac() const { return cols() + NT; }
-  __device__ float* qk() const { return cols() + 2 * NT; }
-  __device__ float* red() const { return cols() + 3 * NT; }  // [4][NT]
-  __device__ int* lim() const { return reinterpret_cast<int*>(cols() + 7 * NT); }
-  __device__ int* tok() const { return reinterpret_cast<int*>(cols() + 8 * NT); }
+  __device__ float* qk(int i) const { return cols() + (2 + i) * NT; }
+  __device__ float* red(int g) const { return cols() + 4 * NT + g * 4 * L::CW; }  // [4 warps][CW]
+  __device__ int* lim() const { return reinterpret_cast<int*>(cols() + 8 * NT); }
+  __device__ int* tok() const { return reinterpret_cast<int*>(cols() + 9 * NT); }
 };
 
-// Query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle).
+// Query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle), by 64 threads.
 template <int NT, bool FP8>
-__device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const LatEntry& x, int t) {
+__device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const LatEntry& x, int t,
+                                           int parity) {
   using L = LatCfg<NT, FP8>;
   uint8_t* sq = sm.base + L::kQOff;
   // Eight threads copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
   constexpr int kBlocks = FP8 ? 1 : 9;  // 8-bit: only the rope part as it is
 #pragma unroll 1
-  for (int row = t >> 3; row < NT; row += 16) {
+  for (int row = t >> 3; row < NT; row += 8) {
     const int r = x.r0 + row, ch = t & 7;
     const int tok = r / p.H, h = r - tok * p.H;
     const bool there = r < p.R;
@@ -264,22 +275,25 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShar
     cp_async_wait_all();
     return;
   }
-  // 128 / NT neighbouring threads share a row: its largest element decides the power of two in front of the split
-  constexpr int TPR = 128 / NT, CH = 64 / TPR;  // 16-byte chunks of the latent part per thread
+  // 64 / NT neighbouring threads share a row: its largest element decides the power of two in front of the split
+  constexpr int TPR = 64 / NT, CH = 64 / TPR;  // 16-byte chunks of the latent part per thread
   const int row = t / TPR, sub = t % TPR, r = x.r0 + row;
   const int tok = r / p.H, h = r - tok * p.H;
   const bool there = r < p.R;
   const uint4* src = reinterpret_cast<const uint4*>(there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] : p.q) + sub;
-  uint4 v[CH];
   float top = 0.f;
+#pragma unroll 1
+  for (int i0 = 0; i0 < CH; i0 += 16) {
+    uint4 v[16];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) v[i] = __ldg(src + i * TPR);
+    for (int i = 0; i < 16; ++i) v[i] = __ldg(src + (i0 + i) * TPR);
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      top = fmax3(top, fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u)));
+      for (int j = 0; j < 4; ++j)
+        top = fmax3(top, fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u)));
+    }
   }
 #pragma unroll
   for (int o = TPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -288,8 +302,9 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShar
   k = top == 0.f ? 0 : min(max(k, -100), 100);
   const float inv = there ? __uint_as_float(static_cast<uint32_t>(127 - k) << 23) : 0.f;
   if (sub == 0)  // an infinite element makes the row's scores NaN
-    sm.qk()[row] = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-#pragma unroll 2
+    sm.qk(parity)[row] =
+        bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
+#pragma unroll 4
   for (int i = 0; i < CH; ++i) {
     const int ch = i * TPR + sub;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
     const uint4 y = __ldg(src + i * TPR);  // read a second time (it is in L1): a loop stays small in the instruction cache
@@ -339,17 +354,20 @@ __device__ __forceinline__ bool row_not_finite(const uint8_t* slot, int t) {
   return bad;
 }
 
+// Softmax and epilogue of warpgroup g: columns [g CW, g CW + CW) of the row tile, thread = key of the tile (then output
+// dimension) = TMEM lane.
 template <int NT, bool FP8>
 __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const AbortCtl& ctl,
-                                            LatWalk<NT> walk, uint32_t tmem, int t) {
+                                            LatWalk<NT> walk, uint32_t tmem, int g, int t) {
   using L = LatCfg<NT, FP8>;
-  constexpr int NC = L::NC;
+  constexpr int NC = L::NC, CW = L::CW;
   constexpr int kStep = FP8 ? 32 : 16;      // keys of one MMA of the output GEMM
   constexpr float kRise = FP8 ? 2.f : 8.f;  // how far (log2) a score may exceed the reference
-  const int w = t >> 5, lane = t & 31;
+  constexpr int kOwn = CW > 32 ? CW / 32 : 1;
+  const int w = t >> 5, lane = t & 31, cb = g * CW;
+  const uint32_t bar = 1 + g;               // named barrier of this warpgroup; 3 = all softmax warpgroups
   const uint32_t tl = tmem + (static_cast<uint32_t>(w << 5) << 16);
-  uint32_t s_phase = 0, o_phase = 0, slot0 = 0;
-  int piece = 0;
+  uint32_t tile = 0, slot0 = 0, piece = 0;
   int4 info = make_int4(-1, -1, -1, 0);
   while (walk.next(p)) {
     const LatEntry x = walk.x;
@@ -358,31 +376,28 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     const int slot = 2 * blockIdx.x + (piece > 0 ? 1 : 0);
     if (!walk.begins) info.x = x.b * p.RT + x.r0 / NT;
     if (walk.begins && !walk.ends) { info.y = x.b * p.RT + x.r0 / NT; info.z = slot; }
-    ++piece;
-    named_bar_sync(1, 128);  // everybody has finished with the previous piece's columns and query
+    named_bar_sync(3, 128 * L::G);  // everybody has finished with the previous piece's columns
     const int prefix = max(x.len - x.nq, 0);
-    if (t < NT) {
-      const int r = x.r0 + t, tok = r / p.H;
-      sm.tok()[t] = tok;
+    if (t < CW) {
+      const int c = cb + t, r = x.r0 + c, tok = r / p.H;
+      sm.tok()[c] = tok;
       // keys below the limit are visible; rows without a query are stored as zeros or not at all, whatever they see
-      sm.lim()[t] = r >= p.R || tok >= x.nq ? 0x7FFFFFFF : p.tree != nullptr ? prefix : max(x.len - x.nq + tok + 1, 0);
-      sm.ref()[t] = kNoRef;
+      sm.lim()[c] = r >= p.R || tok >= x.nq ? 0x7FFFFFFF : p.tree != nullptr ? prefix : max(x.len - x.nq + tok + 1, 0);
+      sm.ref()[c] = kNoRef;
     }
-    if (tiles > 0) {
-      load_query<NT, FP8>(p, sm, x, t);
-      fence_proxy_async_smem();
-      mbar_arrive(sm.q_full());
-    }
-    named_bar_sync(1, 128);
+    named_bar_sync(3, 128 * L::G);
     int min_lim = 0x7FFFFFFF;
 #pragma unroll 8
     for (int c = 0; c < NT; ++c) min_lim = min(min_lim, sm.lim()[c]);
-    float l[NT];
+    const float* qk = sm.qk(piece & 1) + cb;
+    ++piece;
+    float l[CW];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) l[c] = 0.f;
+    for (int c = 0; c < CW; ++c) l[c] = 0.f;
 
-    for (int j = 0; j < tiles; ++j) {
+    for (int j = 0; j < tiles; ++j, ++tile) {
       const int n0 = walk.k0 + j * kTile, n = n0 + t;
+      const uint32_t buf = L::kAhead > 0 ? tile & 1 : 0;
       float ks = 1.f, lk = 0.f, iks = 1.f;
       if (FP8 && n < walk.k1) {
         const int pg = __ldg(p.table + x.b * p.table_stride + n / p.page_size);
@@ -391,25 +406,25 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         lk = fast_log2(ks);
         iks = 1.f / ks;
       }
-      mbar_wait(sm.s_full(), s_phase, ctl, 0x700);
-      s_phase ^= 1;
+      mbar_wait(sm.s_full(buf), (L::kAhead > 0 ? tile >> 1 : tile) & 1, ctl, 0x700);
       tc_fence_after_sync();
-      float s[NT];
+      float s[CW];
       if (FP8) {
-        uint32_t a[NC], rp[NT];
-        tmem_ld_cols<NC>(tl + kColS, a);
-        tmem_ld_cols<NT>(tl + kColR, rp);
+        uint32_t a[CW], b[CW], rp[CW];
+        tmem_ld_cols<CW>(tl + kColS + buf * NC + cb, a);
+        tmem_ld_cols<CW>(tl + kColS + buf * NC + NT + cb, b);
+        tmem_ld_cols<CW>(tl + kColR + buf * NT + cb, rp);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-          s[c] = fmaf(fmaf(__uint_as_float(a[NT + c]), 0.0625f, __uint_as_float(a[c])), sm.qk()[c] * ks,
-                      __uint_as_float(rp[c])) * p.scale_log2 + lk;
+        for (int c = 0; c < CW; ++c)
+          s[c] = fmaf(fmaf(__uint_as_float(b[c]), 0.0625f, __uint_as_float(a[c])), qk[c] * ks, __uint_as_float(rp[c])) *
+                     p.scale_log2 + lk;
       } else {
-        uint32_t a[NT];
-        tmem_ld_cols<NT>(tl + kColS, a);
+        uint32_t a[CW];
+        tmem_ld_cols<CW>(tl + kColS + buf * NC + cb, a);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < NT; ++c) s[c] = __uint_as_float(a[c]) * p.scale_log2;
+        for (int c = 0; c < CW; ++c) s[c] = __uint_as_float(a[c]) * p.scale_log2;
       }
       const int end = min(walk.k1, n0 + kTile);
       if (n0 + kTile > min(min_lim, walk.k1)) {
@@ -424,9 +439,12 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
                                     (FP8 ? 0 : (ch >> 3 & 1) * 16384) + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         bool poison = false;
-        if (n >= min_lim && n < end) {
+        if (end > min_lim) {
+          if (n >= min_lim && n < end)
 #pragma unroll 1
-          for (int i = 0; i < 4; ++i) poison |= row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+            for (int i = 0; i < 4; ++i) poison |= row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
+          __syncwarp();
+          if (L::G > 1) named_bar_sync(3, 128 * L::G);  // both warpgroups have looked before either takes a key out
           if (poison)
 #pragma unroll 1
             for (int i = 0; i < (FP8 ? 32 : 64); ++i)
@@ -435,10 +453,10 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         }
         const uint8_t* mask = p.tree != nullptr ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : nullptr;
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
+        for (int c = 0; c < CW; ++c) {
           bool seen = n < end;
-          if (seen && n >= sm.lim()[c]) {
-            const int tok = sm.tok()[c];
+          if (seen && n >= sm.lim()[cb + c]) {
+            const int tok = sm.tok()[cb + c];
             seen = mask != nullptr && tok < x.nq && mask[tok * p.tree_stride[1]] != 0;
           }
           s[c] = !seen ? -INFINITY : poison ? __uint_as_float(0x7FC00000u) : s[c];
@@ -447,34 +465,38 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       }
       bool rise = false;
 #pragma unroll
-      for (int c = 0; c < NT; ++c) rise |= s[c] > sm.ref()[c] + kRise;
-      if (named_bar_or(2, 128, rise)) {
+      for (int c = 0; c < CW; ++c) rise |= s[c] > sm.ref()[cb + c] + kRise;
+      if (named_bar_or(bar, 128, rise)) {
         {
-          float m[NT];
+          float m[CW];
 #pragma unroll
-          for (int c = 0; c < NT; ++c) m[c] = s[c];
-          reduce_cols<NT, true>(m, lane);
-          constexpr int kOwn = NT > 32 ? NT / 32 : 1;
+          for (int c = 0; c < CW; ++c) m[c] = s[c];
+          reduce_cols<CW, true>(m, lane);
 #pragma unroll
-          for (int i = 0; i < kOwn; ++i) sm.red()[w * NT + first_column<NT>(lane) + i] = m[i];
+          for (int i = 0; i < kOwn; ++i) sm.red(g)[w * CW + first_column<CW>(lane) + i] = m[i];
         }
-        named_bar_sync(1, 128);
-        if (t < NT) {
-          const float old = sm.ref()[t];
-          const float m = fmaxf(fmaxf(fmaxf(sm.red()[t], sm.red()[NT + t]), fmaxf(sm.red()[2 * NT + t], sm.red()[3 * NT + t])), old);
-          sm.ref()[t] = m;
-          sm.fac()[t] = fast_exp2(old - m);
+        named_bar_sync(bar, 128);
+        if (t < CW) {
+          const float old = sm.ref()[cb + t];
+          const float* red = sm.red(g) + t;
+          const float m = fmaxf(fmaxf(fmaxf(red[0], red[CW]), fmaxf(red[2 * CW], red[3 * CW])), old);
+          sm.ref()[cb + t] = m;
+          sm.fac()[cb + t] = fast_exp2(old - m);
         }
-        named_bar_sync(1, 128);
-        if (j > 0) {  // the score GEMM of this tile was issued behind the previous tile's output GEMMs: O^T is complete
+        named_bar_sync(bar, 128);
+        if (j > 0) {
 #pragma unroll
-          for (int c = 0; c < NT; ++c) l[c] *= sm.fac()[c];
+          for (int c = 0; c < CW; ++c) l[c] *= sm.fac()[cb + c];
+          mbar_wait(sm.o_full(), (tile - 1) & 1, ctl, 0x780);  // O^T of the tiles so far
+          tc_fence_after_sync();
 #pragma unroll 1
           for (int i = 0; i < 4 * NC; i += 16) {
+            const int c0 = i % NT;  // hi and lo columns alike
+            if (L::G > 1 && c0 / CW != g) continue;
             uint32_t o[16];
             tmem_ld16(tl + i, o);
             tmem_wait_ld();
-            const float* f = sm.fac() + i % NT;
+            const float* f = sm.fac() + c0;
 #pragma unroll
             for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f[c]);
             tmem_st16(tl + i, o);
@@ -483,12 +505,12 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         }
       }
       // sixteen columns at a time: references and weights in registers first, so that no load waits for a store
-      uint8_t* sp = sm.base + L::kPOff;
+      uint8_t* sp = sm.base + L::kPOff + (FP8 ? (tile & 1) * L::kP : 0) + cb * 128;
 #pragma unroll
-      for (int c0 = 0; c0 < NT; c0 += 16) {
+      for (int c0 = 0; c0 < CW; c0 += 16) {
         float pw[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(s[c0 + c] - sm.ref()[c0 + c]);
+        for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(s[c0 + c] - sm.ref()[cb + c0 + c]);
         if (FP8) {
           // weights in (0, 4] -> (0, 256]; the remainder of the first rounding is at most 16, times 16
 #pragma unroll
@@ -523,29 +545,28 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     }
 
     // ---- epilogue: thread = output dimension
-    reduce_cols<NT, false>(l, lane);
-    constexpr int kOwn = NT > 32 ? NT / 32 : 1;
+    reduce_cols<CW, false>(l, lane);
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) sm.red()[w * NT + first_column<NT>(lane) + i] = l[i];
-    named_bar_sync(1, 128);
+    for (int i = 0; i < kOwn; ++i) sm.red(g)[w * CW + first_column<CW>(lane) + i] = l[i];
+    named_bar_sync(bar, 128);
     float sum = 0.f;
-    if (t < NT) {
-      const bool query = sm.tok()[t] < x.nq;
-      sum = query ? (sm.red()[t] + sm.red()[NT + t]) + (sm.red()[2 * NT + t] + sm.red()[3 * NT + t]) : 0.f;
-      if (!query) sm.ref()[t] = kNoRef;
-      sm.fac()[t] = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+    if (t < CW) {
+      const float* red = sm.red(g) + t;
+      const bool query = sm.tok()[cb + t] < x.nq;
+      sum = query ? (red[0] + red[CW]) + (red[2 * CW] + red[3 * CW]) : 0.f;
+      if (!query) sm.ref()[cb + t] = kNoRef;
+      sm.fac()[cb + t] = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
     }
-    named_bar_sync(1, 128);
+    named_bar_sync(bar, 128);
     if (tiles > 0) {
-      mbar_wait(sm.o_full(), o_phase, ctl, 0x800);
-      o_phase ^= 1;
+      mbar_wait(sm.o_full(), (tile - 1) & 1, ctl, 0x800);
       tc_fence_after_sync();
     }
     // A rolled loop: the code runs once per piece, and unrolled it waited for the instruction cache at every store.
     const int rows = min(p.R - x.r0, NT);
 #pragma unroll 1
-    for (int i = 0; i < 4 * NT; i += 16) {
-      const int mt = i / NT, c0 = i % NT;
+    for (int i = 0; i < 4 * CW; i += 16) {
+      const int mt = i / CW, c0 = cb + i % CW;
       uint32_t o[16], lo[16];
       if (tiles > 0) {
         tmem_ld16(tl + mt * NC + c0, o);
@@ -571,23 +592,37 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         for (int c = 0; c < 16; ++c) d[c * kLat] = y[c];
       }
     }
-    if (t < NT) {
-      const int r = x.r0 + t;
+    if (t < CW) {
+      const int c = cb + t, r = x.r0 + c;
       if (!whole) {
-        p.part_ml[slot * NT + t] = make_float2(sm.ref()[t], sum);
+        p.part_ml[slot * NT + c] = make_float2(sm.ref()[c], sum);
       } else if (p.lse != nullptr && r < p.R) {
         const int tok = r / p.H;
         p.lse[static_cast<int64_t>(x.b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
-            sum == 0.f ? -INFINITY : sm.ref()[t] + log2f(sum);
+            sum == 0.f ? -INFINITY : sm.ref()[c] + log2f(sum);
       }
     }
     tc_fence_before_sync();
   }
-  if (t == 0) p.part_info[blockIdx.x] = info;
+  if (g == 0 && t == 0) p.part_info[blockIdx.x] = info;
+}
+
+__device__ __forceinline__ bool mbar_test_all(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __all_sync(0xFFFFFFFFu, ok != 0);
 }
 
 template <int NT, bool FP8>
-__global__ void __launch_bounds__(kLatThreads, 1)
+__global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap tm_lat, const __grid_constant__ CUtensorMap tm_rope,
                        const LatAttnParams p) {
   using L = LatCfg<NT, FP8>;
@@ -602,9 +637,11 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
     for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
     for (int i = 0; i < L::kRopeSlots; ++i) { mbar_init(sm.rfull(i), 1); mbar_init(sm.rempty(i), 1); }
-    mbar_init(sm.q_full(), 128);
-    mbar_init(sm.s_full(), 1);
-    mbar_init(sm.p_full(), 128);
+    mbar_init(sm.q_full(), 64);
+    mbar_init(sm.q_empty(), 1);
+    mbar_init(sm.s_full(0), 1);
+    mbar_init(sm.s_full(1), 1);
+    mbar_init(sm.p_full(), 128 * L::G);
     mbar_init(sm.o_full(), 1);
     mbar_fence_init();
   }
@@ -615,7 +652,7 @@ __global__ void __launch_bounds__(kLatThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge kernel may be set up; it waits for this grid's end
   // This CTA's share of the work line: every thread counts a run of entries, then a scan over the CTA.
   const int entries = p.B * p.RT;
-  const int run = (entries + kLatThreads - 1) / kLatThreads;
+  const int run = (entries + L::kThreads - 1) / L::kThreads;
   const int e_begin = min(static_cast<int>(threadIdx.x) * run, entries), e_end = min(e_begin + run, entries);
   int mine = 0;
   for (int e = e_begin; e < e_end; ++e) {
@@ -639,35 +676,40 @@ __global__ void __launch_bounds__(kLatThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_slot;
-  int before = 0, total = 0;
+  int before = 0, units = 0;
 #pragma unroll
-  for (int i = 0; i < kLatThreads / 32; ++i) {
+  for (int i = 0; i < L::kThreads / 32; ++i) {
     if (i < warp) before += scan[i];
-    total += scan[i];
+    units += scan[i];
   }
-  // with fewer units than CTAs the first ones get one each: the CTAs of an entry are always neighbours
+  // Every entry takes kExtra more places; not where every unit can have a CTA of its own.
+  const int extra = units <= static_cast<int>(gridDim.x) ? 0 : kExtra;
+  const int total = units + extra * entries;
+  // with fewer places than CTAs the first ones get one each: the CTAs of an entry are always neighbours
   const int busy = min(total, static_cast<int>(gridDim.x)), me = static_cast<int>(blockIdx.x);
   const int share = total / busy, more = total - share * busy;
   const int u0 = me < busy ? me * share + min(me, more) : total, u1 = me < busy ? u0 + share + (me < more ? 1 : 0) : total;
   {
-    int at = before + incl - mine;  // units in front of this thread's entries
+    mine += extra * (e_end - e_begin);
+    int at = before + incl + extra * e_end - mine;  // places in front of this thread's entries
     if (u0 < u1 && at <= u0 && u0 < at + mine) {
       int e = e_begin;
       while (true) {
-        const int n = lat_units(lat_entry<NT>(p, e).keys);
+        const int n = lat_units(lat_entry<NT>(p, e).keys) + extra;
         if (u0 < at + n) break;
         at += n;
         ++e;
       }
-      scan[8] = e;
-      scan[9] = u0 - at;
+      scan[12] = e;
+      scan[13] = u0 - at;
     }
   }
   __syncthreads();
   LatWalk<NT> walk;
-  walk.e = u0 < u1 ? scan[8] : 0;
-  walk.off = u0 < u1 ? scan[9] : 0;
+  walk.e = u0 < u1 ? scan[12] : 0;
+  walk.off = u0 < u1 ? scan[13] : 0;
   walk.left = u1 - u0;
+  walk.extra = extra;
   bool healthy = *abort_flag == 0u;
   if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzled tiles need a 1024-byte aligned window
     if (threadIdx.x == 0) report_error(ctl, kErrSmemAlign, smem_u32(smem));
@@ -728,80 +770,117 @@ __global__ void __launch_bounds__(kLatThreads, 1)
     const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
     const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
     const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
-    uint32_t slot = 0, phase = 0, rs = 0, rphase = 0, tile_phase = 0, q_phase = 0;
+    uint32_t ks = 0, kph = 0;       // slot and phase of the next score GEMM step
+    uint32_t vs = 0;                // slot of the next output GEMM step
+    uint32_t rs = 0, rph = 0;       // rope slot of the next score GEMM
+    uint32_t tile = 0, q_phase = 0;
+    // One step of the score GEMM of tile `number`: 128 latent dimensions, or (i = 4) the rope part.
+    const auto score_step = [&](int i, uint32_t number) {
+      const uint32_t d = tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
+      if (i < 4) {
+        const uint64_t kd = desc_advance(k_desc, uniform(ks) * L::kSlot);
+        const uint64_t qd = desc_advance(q_desc, uniform(i) * (2 * NT * 128));
+        if (FP8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (leader) umma_ss_f8(d, desc_advance(kd, k * 32), desc_advance(qd, k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (leader)
+              umma_ss(d, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
+                      desc_advance(qd, (k >> 2) * (NT * 128) + (k & 3) * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+        }
+        if (++ks == L::NS) { ks = 0; kph ^= 1; }
+      } else {
+        const uint64_t rd = desc_advance(r_desc, uniform(rs) * 16384);
+        const uint32_t dr = FP8 ? tmem + kColR + (number & 1) * NT : d;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (leader) umma_ss(dr, desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
+        if (leader) {
+          umma_commit(sm.s_full(L::kAhead > 0 ? number & 1 : 0));
+          if (FP8) umma_commit(sm.rempty(rs));
+        }
+        if (++rs == L::kRopeSlots) { rs = 0; rph ^= 1; }
+      }
+    };
     while (__any_sync(0xFFFFFFFFu, walk.next(p))) {
       const int tiles = uniform(walk.tiles()), keys = uniform(walk.k1 - walk.k0);
       if (tiles > 0) {
         mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
         q_phase ^= 1;
       }
-      for (int j = 0; j < tiles; ++j) {
-        uint32_t s = slot, ph = phase;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          mbar_wait(sm.full(s), ph, ctl, 0x400 + s);
+      int done = 0;  // score steps of tile j that were issued ahead
+      for (int j = 0; j < tiles; ++j, ++tile) {
+#pragma unroll 1
+        for (; done < 5; ++done) {
+          if (done < 4) mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
+          else mbar_wait(sm.rfull(rs), rph, ctl, 0x500 + rs);
           tc_fence_after_sync();
-          const uint64_t kd = desc_advance(k_desc, uniform(s) * L::kSlot);
-          if (FP8) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (leader)
-                umma_ss_f8(tmem + kColS, desc_advance(kd, k * 32), desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk,
-                           (i > 0 || k > 0) ? 1u : 0u);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (leader)
-                umma_ss(tmem + kColS, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
-                        desc_advance(q_desc, (2 * i + (k >> 2)) * (NT * 128) + (k & 3) * 32), id_qk,
-                        (i > 0 || k > 0) ? 1u : 0u);
-          }
-          if (++s == L::NS) { s = 0; ph ^= 1; }
+          score_step(done, tile);
         }
-        mbar_wait(sm.rfull(rs), rphase, ctl, 0x500 + rs);
-        tc_fence_after_sync();
-        const uint64_t rd = desc_advance(r_desc, uniform(rs) * 16384);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (leader)
-            umma_ss(tmem + (FP8 ? kColR : kColS), desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope,
-                    (!FP8 || k > 0) ? 1u : 0u);
-        if (leader) {
-          umma_commit(sm.s_full());
-          if (FP8) umma_commit(sm.rempty(rs));
+        if (j + 1 == tiles && leader) umma_commit(sm.q_empty());
+        done = 0;
+        if (L::kAhead > 0 && j + 1 < tiles) {
+          // While this tile's softmax runs: the next tile's score GEMM, as far as its slots have arrived.
+          constexpr int kSteps = FP8 ? 5 : L::kAhead;
+          const long long t0 = clock64();
+          while (done < kSteps && !mbar_test_all(sm.p_full(), tile & 1)) {
+            if (mbar_test_all(done < 4 ? sm.full(ks) : sm.rfull(rs), done < 4 ? kph : rph)) {
+              tc_fence_after_sync();
+              score_step(done, tile + 1);
+              ++done;
+            } else if (clock64() - t0 > kWaitCycleLimit) {
+              break;  // the wait below reports it
+            }
+          }
         }
         const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
-        mbar_wait(sm.p_full(), tile_phase, ctl, 0x600);
-        tile_phase ^= 1;
+        mbar_wait(sm.p_full(), tile & 1, ctl, 0x600);
         tc_fence_after_sync();
+        const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint64_t vd = desc_advance(v_desc, uniform(slot) * L::kSlot);
+          const uint64_t vd = desc_advance(v_desc, uniform(vs) * L::kSlot);
           if (FP8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               if (leader && k < steps)
-                umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(p_desc, k * 32), id_pv,
+                umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(pd, k * 32), id_pv,
                            (j > 0 || k > 0) ? 1u : 0u);
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
               if (leader && k < steps)
-                umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048),
-                        desc_advance(p_desc, (k >> 2) * (NT * 128) + (k & 3) * 32), id_pv, (j > 0 || k > 0) ? 1u : 0u);
+                umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048), desc_advance(pd, (k >> 2) * (NT * 128) + (k & 3) * 32),
+                        id_pv, (j > 0 || k > 0) ? 1u : 0u);
           }
-          if (leader) umma_commit(sm.empty(slot));
-          if (++slot == L::NS) { slot = 0; phase ^= 1; }
+          if (leader) umma_commit(sm.empty(vs));
+          if (++vs == L::NS) vs = 0;
         }
         if (leader) {
           if (!FP8) umma_commit(sm.rempty(0));
-          if (j + 1 == tiles) umma_commit(sm.o_full());
+          umma_commit(sm.o_full());
         }
-        if (++rs == L::kRopeSlots) { rs = 0; rphase ^= 1; }
       }
     }
   } else if (warp >= 4) {
-    lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, static_cast<int>(threadIdx.x) - 128);
+    lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, (warp - 4) >> 2, static_cast<int>(threadIdx.x) & 127);
+  } else {
+    // ------------------------------------------------------------------ warps 2 and 3: queries, one piece ahead
+    uint32_t q_phase = 1, piece = 0;
+    while (walk.next(p)) {
+      const int tiles = walk.tiles();
+      if (tiles > 0) {
+        mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
+        q_phase ^= 1;
+        load_query<NT, FP8>(p, sm, walk.x, static_cast<int>(threadIdx.x) - 64, piece & 1);
+        fence_proxy_async_smem();
+        mbar_arrive(sm.q_full());
+      }
+      ++piece;
+    }
   }
 
   tc_fence_before_sync();
@@ -932,7 +1011,7 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   if (int rc = make_tensor_map(&tr, c.rope, 2, c.pages, c.page_size, 1, kRp, rs, 64, box)) return rc;
   auto kern = latent_attn_kernel<NT, FP8>;
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
-  kern<<<ctas, kLatThreads, L::kAlloc, st>>>(tl, tr, p);
+  kern<<<ctas, L::kThreads, L::kAlloc, st>>>(tl, tr, p);
   PITH_CUDA(cudaGetLastError());
   if (p.max_keys > kUnit && ctas > 1) {  // an entry of one unit is never cut
     const int64_t entries = static_cast<int64_t>(p.B) * p.RT;
@@ -982,7 +1061,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
   const int nt = lat_rows(rows, fp8);
   const int64_t rt = (rows + nt - 1) / nt;
-  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2) < 2147483647 - 1024,
+  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2 + kExtra) < 2147483647 - 1024,
                "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
   LatAttnParams p = {};
