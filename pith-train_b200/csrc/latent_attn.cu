@@ -33,13 +33,14 @@ namespace pith {
 constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
 constexpr int kUnit = 64;   // keys per unit of work
-constexpr int kExtra = 2;   // units of work that another piece costs a CTA
+constexpr int kMaxExtra = 8;
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
 
 template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
+  static constexpr int kExtra = FP8 ? (NT == 16 ? 3 : 5) : (NT == 16 ? 2 : NT == 32 ? 3 : 4);  // units that another piece costs a CTA
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
   static constexpr int CW = NT / G;
   static constexpr int kThreads = 128 + 128 * G;
@@ -59,7 +60,7 @@ struct LatCfg {
   static constexpr int kPOff = FP8 ? kQOff + kQ : kRopeOff;
   static constexpr int kMiscOff = FP8 ? kPOff + 2 * kP : kQOff + kQ;
   static constexpr int kAlloc = kMiscOff + kMisc;
-  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 6;
+  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 8;
   static_assert(NS >= 4, "a tile's four latent slots must fit at once");
   static_assert(!FP8 || kAhead == 4, "the 8-bit pipeline holds two tiles");
   static_assert(kBars * 8 + 16 + 48 + NT * 40 <= kMisc, "misc area too small");
@@ -92,12 +93,12 @@ struct LatEntry {
 template <int NT>
 __device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
   LatEntry x;
-  x.b = e / p.RT;
+  x.b = p.RT == 1 ? e : e / p.RT;
   x.r0 = (e - x.b * p.RT) * NT;
   x.len = min(max(__ldg(p.lens + x.b), 0), p.max_keys);
   x.nq = p.qlens != nullptr ? min(max(__ldg(p.qlens + x.b), 0), p.Sq) : p.Sq;
-  const int last = min((min(x.r0 + NT, p.R) - 1) / p.H, x.nq - 1);
-  x.keys = x.r0 / p.H >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
+  const int last = min(p.RT == 1 ? p.Sq - 1 : (min(x.r0 + NT, p.R) - 1) / p.H, x.nq - 1);
+  x.keys = (x.r0 == 0 ? 0 : x.r0 / p.H) >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
   return x;
 }
 __device__ __forceinline__ int lat_units(int keys) { return max((keys + kUnit - 1) / kUnit, 1); }
@@ -171,15 +172,18 @@ __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, boo
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ void e4m3x2_f32(uint16_t v, float& lo, float& hi) {
-  asm("{\n\t.reg .b32 h;\n\t.reg .b16 a, b;\n\tcvt.rn.f16x2.e4m3x2 h, %2;\n\tmov.b32 {a, b}, h;\n\t"
-      "cvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
-      : "=f"(lo), "=f"(hi) : "h"(v));
+// Two floats of at most 448 as e4m3 pairs hi + lo / 16. They pass through fp16 (11 significant bits, and its least step,
+// 2^-24, is below everything that lo can hold), where the remainder of the first rounding is exact.
+__device__ __forceinline__ void split_e4m3x2(float a, float b, uint16_t& hi, uint16_t& lo) {
+  asm("{\n\t.reg .b32 h, r, d, z;\n\t"
+      "cvt.rn.f16x2.f32 h, %3, %2;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 %0, h;\n\t"
+      "cvt.rn.f16x2.e4m3x2 r, %0;\n\t"
+      "sub.rn.f16x2 d, h, r;\n\t"
+      "mov.b32 z, 0x4C004C00;\n\t"  // 16, 16
+      "mul.rn.f16x2 d, d, z;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 %1, d;\n\t}"
+      : "=&h"(hi), "=h"(lo) : "f"(a), "f"(b));
 }
 
 // A value that is the same in all lanes, in a form the compiler knows to be so (descriptors then stay in uniform registers).
@@ -226,6 +230,9 @@ __device__ __forceinline__ int first_column(int lane) {
   return c;
 }
 
+template <int I>
+struct Int { static constexpr int value = I; };
+
 // Shared-memory scalars behind the tiles.
 template <int NT, bool FP8>
 struct LatShared {
@@ -237,11 +244,12 @@ struct LatShared {
   __device__ uint64_t* empty(int i) const { return bars + L::NS + i; }
   __device__ uint64_t* rfull(int i) const { return bars + 2 * L::NS + i; }
   __device__ uint64_t* rempty(int i) const { return bars + 2 * L::NS + L::kRopeSlots + i; }
-  __device__ uint64_t* q_full() const { return bars + L::kBars - 6; }
-  __device__ uint64_t* q_empty() const { return bars + L::kBars - 5; }
-  __device__ uint64_t* s_full(int i) const { return bars + L::kBars - 4 + i; }
-  __device__ uint64_t* p_full() const { return bars + L::kBars - 2; }
-  __device__ uint64_t* o_full() const { return bars + L::kBars - 1; }  // a tile's output GEMMs have completed
+  __device__ uint64_t* q_full() const { return bars + L::kBars - 8; }
+  __device__ uint64_t* q_empty() const { return bars + L::kBars - 7; }
+  __device__ uint64_t* s_full(int i) const { return bars + L::kBars - 6 + i; }
+  // One for even and one for odd tiles each: a softmax warpgroup may be a tile ahead of the other, and of the output GEMM.
+  __device__ uint64_t* p_full(uint32_t tile) const { return bars + L::kBars - 4 + (tile & 1); }
+  __device__ uint64_t* o_full(uint32_t tile) const { return bars + L::kBars - 2 + (tile & 1); }  // its output GEMMs have completed
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
   __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 1); }             // [12 warps] + start
   __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 10 NT words
@@ -316,11 +324,10 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShar
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const float a = __uint_as_float(w[2 * j + u] << 16) * inv, b = __uint_as_float(w[2 * j + u] & 0xFFFF0000u) * inv;
-        const uint16_t hv = cvt_e4m3x2(a, b);
-        float ha, hb;
-        e4m3x2_f32(hv, ha, hb);
+        uint16_t hv, lv;
+        split_e4m3x2(a, b, hv, lv);
         hw |= static_cast<uint32_t>(hv) << (16 * u);
-        lw |= static_cast<uint32_t>(cvt_e4m3x2((a - ha) * 16.f, (b - hb) * 16.f)) << (16 * u);
+        lw |= static_cast<uint32_t>(lv) << (16 * u);
       }
       hi[j] = hw;
       lo[j] = lw;
@@ -362,7 +369,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
   using L = LatCfg<NT, FP8>;
   constexpr int NC = L::NC, CW = L::CW;
   constexpr int kStep = FP8 ? 32 : 16;      // keys of one MMA of the output GEMM
-  constexpr float kRise = FP8 ? 2.f : 8.f;  // how far (log2) a score may exceed the reference
+  constexpr float kRise = FP8 ? 4.f : 8.f;  // how far (log2) a score may exceed the reference
   constexpr int kOwn = CW > 32 ? CW / 32 : 1;
   const int w = t >> 5, lane = t & 31, cb = g * CW;
   const uint32_t bar = 1 + g;               // named barrier of this warpgroup; 3 = all softmax warpgroups
@@ -451,15 +458,21 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
               *reinterpret_cast<uint4*>(sm.base + ((slot0 + i / (FP8 ? 8 : 16)) % L::NS) * L::kSlot +
                                         (FP8 ? 0 : (i >> 3 & 1) * 16384) + t * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
-        const uint8_t* mask = p.tree != nullptr ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : nullptr;
+        const float shown = __uint_as_float(0x7FC00000u);
+        if (p.tree == nullptr) {
 #pragma unroll
-        for (int c = 0; c < CW; ++c) {
-          bool seen = n < end;
-          if (seen && n >= sm.lim()[cb + c]) {
-            const int tok = sm.tok()[cb + c];
-            seen = mask != nullptr && tok < x.nq && mask[tok * p.tree_stride[1]] != 0;
+          for (int c = 0; c < CW; ++c) s[c] = n < min(end, sm.lim()[cb + c]) ? (poison ? shown : s[c]) : -INFINITY;
+        } else {
+          const uint8_t* mask = p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq));
+#pragma unroll
+          for (int c = 0; c < CW; ++c) {
+            bool seen = n < end;
+            if (seen && n >= sm.lim()[cb + c]) {
+              const int tok = sm.tok()[cb + c];
+              seen = tok < x.nq && mask[tok * p.tree_stride[1]] != 0;
+            }
+            s[c] = !seen ? -INFINITY : poison ? shown : s[c];
           }
-          s[c] = !seen ? -INFINITY : poison ? __uint_as_float(0x7FC00000u) : s[c];
         }
         __syncwarp();
       }
@@ -487,7 +500,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         if (j > 0) {
 #pragma unroll
           for (int c = 0; c < CW; ++c) l[c] *= sm.fac()[cb + c];
-          mbar_wait(sm.o_full(), (tile - 1) & 1, ctl, 0x780);  // O^T of the tiles so far
+          mbar_wait(sm.o_full(tile - 1), ((tile - 1) >> 1) & 1, ctl, 0x780);  // O^T of the tiles so far
           tc_fence_after_sync();
 #pragma unroll 1
           for (int i = 0; i < 4 * NC; i += 16) {
@@ -504,6 +517,9 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           tmem_wait_st();
         }
       }
+      // 8-bit: this tile's buffer of weights was last read by the output GEMM two tiles ago. The score GEMM's commit does not
+      // stand in for that one: without this wait, and with one barrier for the rescale's, sums were lost.
+      if (FP8 && tile >= 2) mbar_wait(sm.o_full(tile), ((tile - 2) >> 1) & 1, ctl, 0x790);
       // sixteen columns at a time: references and weights in registers first, so that no load waits for a store
       uint8_t* sp = sm.base + L::kPOff + (FP8 ? (tile & 1) * L::kP : 0) + cb * 128;
 #pragma unroll
@@ -512,16 +528,13 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
 #pragma unroll
         for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(s[c0 + c] - sm.ref()[cb + c0 + c]);
         if (FP8) {
-          // weights in (0, 4] -> (0, 256]; the remainder of the first rounding is at most 16, times 16
+          // 16 times the weight, at most 256; the remainder of its first rounding is at most 16, times 16
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
             l[c0 + c] += pw[c] > 0.f ? pw[c] * iks : pw[c];
             l[c0 + c + 1] += pw[c + 1] > 0.f ? pw[c + 1] * iks : pw[c + 1];
-            const float a = pw[c] * 64.f, b = pw[c + 1] * 64.f;
-            const uint16_t hi = cvt_e4m3x2(a, b);
-            float ha, hb;
-            e4m3x2_f32(hi, ha, hb);
-            const uint16_t lo = cvt_e4m3x2((a - ha) * 16.f, (b - hb) * 16.f);
+            uint16_t hi, lo;
+            split_e4m3x2(pw[c] * 16.f, pw[c + 1] * 16.f, hi, lo);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               uint8_t* d = sp + (c0 + c + u) * 128 + ((((t >> 4) ^ (c + u)) & 7) << 4) + (t & 15);
@@ -540,7 +553,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       }
       fence_proxy_async_smem();
       tc_fence_before_sync();
-      mbar_arrive(sm.p_full());
+      mbar_arrive(sm.p_full(tile));
       slot0 = (slot0 + 4) % L::NS;
     }
 
@@ -559,37 +572,44 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     }
     named_bar_sync(bar, 128);
     if (tiles > 0) {
-      mbar_wait(sm.o_full(), (tile - 1) & 1, ctl, 0x800);
+      mbar_wait(sm.o_full(tile - 1), ((tile - 1) >> 1) & 1, ctl, 0x800);
       tc_fence_after_sync();
     }
     // A rolled loop: the code runs once per piece, and unrolled it waited for the instruction cache at every store.
     const int rows = min(p.R - x.r0, NT);
 #pragma unroll 1
-    for (int i = 0; i < 4 * CW; i += 16) {
-      const int mt = i / CW, c0 = cb + i % CW;
-      uint32_t o[16], lo[16];
+    for (int i = 0; i < 4 * CW; i += 32) {
+      uint32_t o[32], lo[32];
       if (tiles > 0) {
-        tmem_ld16(tl + mt * NC + c0, o);
-        if (FP8) tmem_ld16(tl + mt * NC + NT + c0, lo);
+#pragma unroll
+        for (int u = 0; u < 32; u += 16) {
+          const uint32_t at = tl + (i + u) / CW * NC + cb + (i + u) % CW;
+          tmem_ld16(at, o + u);
+          if (FP8) tmem_ld16(at + NT, lo + u);
+        }
         tmem_wait_ld();
       }
-      float y[16];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        float v = __uint_as_float(o[c]);
-        if (FP8) v = fmaf(__uint_as_float(lo[c]), 0.0625f, v) * 0.015625f;
-        const float f = sm.fac()[c0 + c];
-        y[c] = tiles == 0 || f == 0.f ? 0.f : v * f;  // no key, or no query (whose scores may be anything)
-      }
-      if (whole) {
-        __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0) * kLat + mt * 128 + t;
+      for (int u = 0; u < 32; u += 16) {
+        const int d0 = (i + u) / CW * 128 + t, c0 = cb + (i + u) % CW;
+        float y[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          if (c0 + c < rows) d[c * kLat] = __float2bfloat16_rn(y[c]);
-      } else {
-        float* d = p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat + mt * 128 + t;
+        for (int c = 0; c < 16; ++c) {
+          float v = __uint_as_float(o[u + c]);
+          if (FP8) v = fmaf(__uint_as_float(lo[u + c]), 0.0625f, v) * 0.0625f;
+          const float f = sm.fac()[c0 + c];
+          y[c] = tiles == 0 || f == 0.f ? 0.f : v * f;  // no key, or no query (whose scores may be anything)
+        }
+        if (whole) {
+          __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0) * kLat + d0;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) d[c * kLat] = y[c];
+          for (int c = 0; c < 16; ++c)
+            if (c0 + c < rows) d[c * kLat] = __float2bfloat16_rn(y[c]);
+        } else {
+          float* d = p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat + d0;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) d[c * kLat] = y[c];
+        }
       }
     }
     if (t < CW) {
@@ -634,17 +654,20 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
   const AbortCtl ctl{p.status, abort_flag};
 
   if (threadIdx.x == 0) {
-    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
     for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
     for (int i = 0; i < L::kRopeSlots; ++i) { mbar_init(sm.rfull(i), 1); mbar_init(sm.rempty(i), 1); }
     mbar_init(sm.q_full(), 64);
     mbar_init(sm.q_empty(), 1);
     mbar_init(sm.s_full(0), 1);
     mbar_init(sm.s_full(1), 1);
-    mbar_init(sm.p_full(), 128 * L::G);
-    mbar_init(sm.o_full(), 1);
+    mbar_init(sm.p_full(0), 128 * L::G);
+    mbar_init(sm.p_full(1), 128 * L::G);
+    mbar_init(sm.o_full(0), 1);
+    mbar_init(sm.o_full(1), 1);
     mbar_fence_init();
   }
+  if (threadIdx.x == 64)  // a launch that finds an error already recorded does no work
+    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -682,8 +705,8 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     if (i < warp) before += scan[i];
     units += scan[i];
   }
-  // Every entry takes kExtra more places; not where every unit can have a CTA of its own.
-  const int extra = units <= static_cast<int>(gridDim.x) ? 0 : kExtra;
+  // Every entry takes L::kExtra more places; not where every unit can have a CTA of its own.
+  const int extra = units <= static_cast<int>(gridDim.x) ? 0 : L::kExtra;
   const int total = units + extra * entries;
   // with fewer places than CTAs the first ones get one each: the CTAs of an entry are always neighbours
   const int busy = min(total, static_cast<int>(gridDim.x)), me = static_cast<int>(blockIdx.x);
@@ -774,35 +797,47 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     uint32_t vs = 0;                // slot of the next output GEMM step
     uint32_t rs = 0, rph = 0;       // rope slot of the next score GEMM
     uint32_t tile = 0, q_phase = 0;
-    // One step of the score GEMM of tile `number`: 128 latent dimensions, or (i = 4) the rope part.
-    const auto score_step = [&](int i, uint32_t number) {
+    // Steps of the score GEMM of tile `number`: 128 latent dimensions each, then the rope part.
+    const auto latent_step = [&](auto step, uint32_t number) {
+      constexpr int i = decltype(step)::value;
       const uint32_t d = tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
-      if (i < 4) {
-        const uint64_t kd = desc_advance(k_desc, uniform(ks) * L::kSlot);
-        const uint64_t qd = desc_advance(q_desc, uniform(i) * (2 * NT * 128));
-        if (FP8) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (leader) umma_ss_f8(d, desc_advance(kd, k * 32), desc_advance(qd, k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (leader)
-              umma_ss(d, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
-                      desc_advance(qd, (k >> 2) * (NT * 128) + (k & 3) * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
-        }
-        if (++ks == L::NS) { ks = 0; kph ^= 1; }
-      } else {
-        const uint64_t rd = desc_advance(r_desc, uniform(rs) * 16384);
-        const uint32_t dr = FP8 ? tmem + kColR + (number & 1) * NT : d;
+      const uint64_t kd = desc_advance(k_desc, L::NS == 4 ? i * L::kSlot : uniform(ks) * L::kSlot);
+      tc_fence_after_sync();
+      if (FP8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (leader) umma_ss(dr, desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
-        if (leader) {
-          umma_commit(sm.s_full(L::kAhead > 0 ? number & 1 : 0));
-          if (FP8) umma_commit(sm.rempty(rs));
-        }
-        if (++rs == L::kRopeSlots) { rs = 0; rph ^= 1; }
+          if (leader)
+            umma_ss_f8(d, desc_advance(kd, k * 32), desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk,
+                       (i > 0 || k > 0) ? 1u : 0u);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (leader)
+            umma_ss(d, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
+                    desc_advance(q_desc, (2 * i + (k >> 2)) * (NT * 128) + (k & 3) * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+      }
+      if (++ks == L::NS) { ks = 0; kph ^= 1; }
+    };
+    const auto rope_step = [&](uint32_t number) {
+      const uint64_t rd = desc_advance(r_desc, L::kRopeSlots == 1 ? 0 : uniform(rs) * 16384);
+      const uint32_t d = FP8 ? tmem + kColR + (number & 1) * NT : tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
+      tc_fence_after_sync();
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (leader) umma_ss(d, desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
+      if (leader) {
+        umma_commit(sm.s_full(L::kAhead > 0 ? number & 1 : 0));
+        if (FP8) umma_commit(sm.rempty(rs));
+      }
+      if (++rs == L::kRopeSlots) { rs = 0; rph ^= 1; }
+    };
+    // Whether `bar` completes before this tile's weights are there (then its output GEMM goes first).
+    const auto arrives_first = [&](uint64_t* bar, uint32_t parity, uint32_t number) {
+      const long long t0 = clock64();
+      while (true) {
+        if (mbar_test_all(sm.p_full(number), (number >> 1) & 1)) return false;
+        if (mbar_test_all(bar, parity)) return true;
+        if (clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
       }
     };
     while (__any_sync(0xFFFFFFFFu, walk.next(p))) {
@@ -813,36 +848,47 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       }
       int done = 0;  // score steps of tile j that were issued ahead
       for (int j = 0; j < tiles; ++j, ++tile) {
-#pragma unroll 1
-        for (; done < 5; ++done) {
-          if (done < 4) mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
-          else mbar_wait(sm.rfull(rs), rph, ctl, 0x500 + rs);
-          tc_fence_after_sync();
-          score_step(done, tile);
+        const auto blocking_step = [&](auto step) {
+          if (done <= decltype(step)::value) {
+            mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
+            latent_step(step, tile);
+          }
+        };
+        blocking_step(Int<0>());
+        blocking_step(Int<1>());
+        blocking_step(Int<2>());
+        blocking_step(Int<3>());
+        if (done < 5) {
+          mbar_wait(sm.rfull(rs), rph, ctl, 0x500 + rs);
+          rope_step(tile);
         }
         if (j + 1 == tiles && leader) umma_commit(sm.q_empty());
         done = 0;
         if (L::kAhead > 0 && j + 1 < tiles) {
           // While this tile's softmax runs: the next tile's score GEMM, as far as its slots have arrived.
-          constexpr int kSteps = FP8 ? 5 : L::kAhead;
-          const long long t0 = clock64();
-          while (done < kSteps && !mbar_test_all(sm.p_full(), tile & 1)) {
-            if (mbar_test_all(done < 4 ? sm.full(ks) : sm.rfull(rs), done < 4 ? kph : rph)) {
-              tc_fence_after_sync();
-              score_step(done, tile + 1);
-              ++done;
-            } else if (clock64() - t0 > kWaitCycleLimit) {
-              break;  // the wait below reports it
+          const auto early_step = [&](auto step) {
+            constexpr int i = decltype(step)::value;
+            if (i < L::kAhead && done == i && arrives_first(sm.full(ks), kph, tile)) {
+              latent_step(step, tile + 1);
+              done = i + 1;
             }
+          };
+          early_step(Int<0>());
+          early_step(Int<1>());
+          early_step(Int<2>());
+          early_step(Int<3>());
+          if (FP8 && done == 4 && arrives_first(sm.rfull(rs), rph, tile)) {
+            rope_step(tile + 1);
+            done = 5;
           }
         }
         const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
-        mbar_wait(sm.p_full(), tile & 1, ctl, 0x600);
+        mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
         tc_fence_after_sync();
         const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint64_t vd = desc_advance(v_desc, uniform(vs) * L::kSlot);
+          const uint64_t vd = desc_advance(v_desc, L::NS == 4 ? i * L::kSlot : uniform(vs) * L::kSlot);
           if (FP8) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -861,7 +907,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
         }
         if (leader) {
           if (!FP8) umma_commit(sm.rempty(0));
-          umma_commit(sm.o_full());
+          umma_commit(sm.o_full(tile));
         }
       }
     }
@@ -1061,7 +1107,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
   const int nt = lat_rows(rows, fp8);
   const int64_t rt = (rows + nt - 1) / nt;
-  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2 + kExtra) < 2147483647 - 1024,
+  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2 + kMaxExtra) < 2147483647 - 1024,
                "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
   LatAttnParams p = {};

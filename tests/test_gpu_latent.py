@@ -247,7 +247,7 @@ def attention_reference(query, cache, table, lens, scale, query_lens=None, tree=
             floor = 0.0
             if cache.scale is not None:
                 delta = delta + scale * 512 * 2.0 ** -21 * q[:, :512].abs().amax(-1) * c.abs().max()
-                floor = 2.0 ** -18
+                floor = 2.0 ** -16
             top = s.amax(-1, keepdim=True)
             p = torch.exp(s - torch.where(top.isinf(), 0, top))
             total = p.sum(-1, keepdim=True)
@@ -300,7 +300,8 @@ SCALE = 192 ** -0.5
     (1, 16, [1], 16), (1, 16, [77], 64), (1, 16, [64, 0, 65, 1, 128, 129, 63], 32), (1, 16, [4097, 3, 1500], 64),
     (1, 1, [300, 2], 16), (1, 2, [129], 192), (3, 5, [40, 3, 700], 128), (2, 16, [5, 1100], 32), (4, 16, [260, 4], 64),
     (1, 128, [513, 90], 64), (7, 16, [900, 7, 8], 16), (100, 4, [100], 64), (33, 16, [33, 2000], 128),
-    (1, 16, list(range(1, 400, 2)), 16)])
+    (1, 16, list(range(1, 400, 2)), 16), (1, 16, [9000, 20000, 31000], 64), (2, 16, [5000, 100, 9999, 17000], 32),
+    (16, 16, [2100, 700], 64)])  # the last ones: several tiles and pieces for every CTA
 def test_attention_causal(cuda_device, dtype, S, H, lens, page):
     g = torch.Generator(device="cuda").manual_seed(1000 * S + H + len(lens))
     cache, table = filled_cache(g, lens, page, dtype)
