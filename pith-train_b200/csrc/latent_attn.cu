@@ -45,24 +45,24 @@ struct LatCfg {
   static constexpr int CW = NT / G;
   static constexpr int kThreads = 128 + 128 * G;
   static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
-  static constexpr int kRopeSlots = FP8 ? 2 : 1;         // 128 keys x 64 dims
   static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
   static constexpr int kQ = kQLat + NT * 128;
   static constexpr int kP = NT * 256;
+  static constexpr int kPRow = NT * 2;                   // bytes of a key's weights: NC columns
   static constexpr int kMisc = NT == 16 ? 1024 : 4096;
   // bf16: P overlays the rope tile, which the score GEMM has finished with when P is written; 8-bit: two buffers
-  static constexpr int kFixed = kRopeSlots * 16384 + kQ + (FP8 ? 2 * kP : 0) + kMisc;
+  static constexpr int kFixed = 16384 + kQ + (FP8 ? 2 * kP : 0) + kMisc;
   static constexpr int NS = (232448 - kFixed) / kSlot;
   // Slots of the next tile whose score GEMM may run before this tile's output GEMM: what the ring holds beyond one tile.
   static constexpr int kAhead = NS >= 8 ? 4 : NS - 4;
   static constexpr int kRopeOff = NS * kSlot;
-  static constexpr int kQOff = kRopeOff + kRopeSlots * 16384;
+  static constexpr int kQOff = kRopeOff + 16384;         // one rope tile, 128 keys x 64 dims
   static constexpr int kPOff = FP8 ? kQOff + kQ : kRopeOff;
   static constexpr int kMiscOff = FP8 ? kPOff + 2 * kP : kQOff + kQ;
   static constexpr int kAlloc = kMiscOff + kMisc;
-  static constexpr int kBars = 2 * NS + 2 * kRopeSlots + 8;
+  static constexpr int kBars = 2 * NS + 10;
   static_assert(NS >= 4, "a tile's four latent slots must fit at once");
-  static_assert(!FP8 || kAhead == 4, "the 8-bit pipeline holds two tiles");
+  static_assert(!FP8 || (kAhead == 4 && NS >= 9 && NS <= 12), "the 8-bit pipeline holds two tiles, and some");
   static_assert(kBars * 8 + 16 + 48 + NT * 40 <= kMisc, "misc area too small");
   static_assert(kAlloc <= 232448, "shared memory");
   static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
@@ -141,9 +141,14 @@ __device__ __forceinline__ void umma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 // Instruction descriptor for kind::f8f6f4 with e4m3 inputs (format 0) and fp32 accumulation.
-constexpr uint32_t make_idesc_e4m3(int m, int n, bool a_mn_major) {
-  return (1u << 4) | (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(n >> 3) << 17) |
-         (static_cast<uint32_t>(m >> 4) << 24);
+constexpr uint32_t make_idesc_e4m3(int m, int n, bool mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(mn_major) << 15) | (static_cast<uint32_t>(mn_major) << 16) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+// Descriptor of an MN-major operand whose rows are one swizzle atom of 32, 64 or 128 bytes wide.
+__device__ __forceinline__ uint64_t make_row_desc(uint32_t smem_addr, int row_bytes) {
+  const uint64_t d = make_smem_desc(smem_addr, 16, 8 * row_bytes) & ~(static_cast<uint64_t>(7) << 61);
+  return d | (static_cast<uint64_t>(row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6) << 61);
 }
 template <int N>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
@@ -242,8 +247,8 @@ struct LatShared {
   __device__ explicit LatShared(uint8_t* smem) : base(smem), bars(reinterpret_cast<uint64_t*>(smem + L::kMiscOff)) {}
   __device__ uint64_t* full(int i) const { return bars + i; }
   __device__ uint64_t* empty(int i) const { return bars + L::NS + i; }
-  __device__ uint64_t* rfull(int i) const { return bars + 2 * L::NS + i; }
-  __device__ uint64_t* rempty(int i) const { return bars + 2 * L::NS + L::kRopeSlots + i; }
+  __device__ uint64_t* rfull() const { return bars + 2 * L::NS; }
+  __device__ uint64_t* rempty() const { return bars + 2 * L::NS + 1; }
   __device__ uint64_t* q_full() const { return bars + L::kBars - 8; }
   __device__ uint64_t* q_empty() const { return bars + L::kBars - 7; }
   __device__ uint64_t* s_full(int i) const { return bars + L::kBars - 6 + i; }
@@ -401,6 +406,14 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     float l[CW];
 #pragma unroll
     for (int c = 0; c < CW; ++c) l[c] = 0.f;
+    // score (log2) minus reference of four columns
+    const auto above = [&](const float* sc, int c, float lk, float* d) {
+      const float4 r = *reinterpret_cast<const float4*>(sm.ref() + cb + c);
+      d[0] = fmaf(sc[c], p.scale_log2, lk - r.x);
+      d[1] = fmaf(sc[c + 1], p.scale_log2, lk - r.y);
+      d[2] = fmaf(sc[c + 2], p.scale_log2, lk - r.z);
+      d[3] = fmaf(sc[c + 3], p.scale_log2, lk - r.w);
+    };
 
     for (int j = 0; j < tiles; ++j, ++tile) {
       const int n0 = walk.k0 + j * kTile, n = n0 + t;
@@ -411,27 +424,32 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         if (pg >= 0 && pg < p.pages) ks = p.scale[pg * p.scale_stride[0] + (n % p.page_size) * p.scale_stride[1]];
         ks = ks < 1e-30f ? 1e-30f : ks;
         lk = fast_log2(ks);
-        iks = 1.f / ks;
+        iks = ks == ks ? 1.f / ks : 1.f;  // a NaN factor acts through the scores of the rows that see the key
       }
       mbar_wait(sm.s_full(buf), (L::kAhead > 0 ? tile >> 1 : tile) & 1, ctl, 0x700);
       tc_fence_after_sync();
-      float s[CW];
+      float s[CW];  // scores before the softmax scale
       if (FP8) {
         uint32_t a[CW], b[CW], rp[CW];
         tmem_ld_cols<CW>(tl + kColS + buf * NC + cb, a);
         tmem_ld_cols<CW>(tl + kColS + buf * NC + NT + cb, b);
         tmem_ld_cols<CW>(tl + kColR + buf * NT + cb, rp);
+        float f[CW];
+#pragma unroll
+        for (int c = 0; c < CW; c += 4) {
+          const float4 q4 = *reinterpret_cast<const float4*>(qk + c);
+          f[c] = q4.x * ks; f[c + 1] = q4.y * ks; f[c + 2] = q4.z * ks; f[c + 3] = q4.w * ks;
+        }
         tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < CW; ++c)
-          s[c] = fmaf(fmaf(__uint_as_float(b[c]), 0.0625f, __uint_as_float(a[c])), qk[c] * ks, __uint_as_float(rp[c])) *
-                     p.scale_log2 + lk;
+          s[c] = fmaf(fmaf(__uint_as_float(b[c]), 0.0625f, __uint_as_float(a[c])), f[c], __uint_as_float(rp[c]));
       } else {
         uint32_t a[CW];
         tmem_ld_cols<CW>(tl + kColS + buf * NC + cb, a);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < CW; ++c) s[c] = __uint_as_float(a[c]) * p.scale_log2;
+        for (int c = 0; c < CW; ++c) s[c] = __uint_as_float(a[c]);
       }
       const int end = min(walk.k1, n0 + kTile);
       if (n0 + kTile > min(min_lim, walk.k1)) {
@@ -476,14 +494,18 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         }
         __syncwarp();
       }
-      bool rise = false;
+      float rise = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < CW; ++c) rise |= s[c] > sm.ref()[cb + c] + kRise;
-      if (named_bar_or(bar, 128, rise)) {
+      for (int c = 0; c < CW; c += 4) {
+        float d[4];
+        above(s, c, lk, d);
+        rise = fmax3(fmax3(rise, d[0], d[1]), d[2], d[3]);
+      }
+      if (named_bar_or(bar, 128, rise > kRise)) {
         {
           float m[CW];
 #pragma unroll
-          for (int c = 0; c < CW; ++c) m[c] = s[c];
+          for (int c = 0; c < CW; ++c) m[c] = fmaf(s[c], p.scale_log2, lk);
           reduce_cols<CW, true>(m, lane);
 #pragma unroll
           for (int i = 0; i < kOwn; ++i) sm.red(g)[w * CW + first_column<CW>(lane) + i] = m[i];
@@ -520,35 +542,43 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       // 8-bit: this tile's buffer of weights was last read by the output GEMM two tiles ago. The score GEMM's commit does not
       // stand in for that one: without this wait, and with one barrier for the rescale's, sums were lost.
       if (FP8 && tile >= 2) mbar_wait(sm.o_full(tile), ((tile - 2) >> 1) & 1, ctl, 0x790);
-      // sixteen columns at a time: references and weights in registers first, so that no load waits for a store
-      uint8_t* sp = sm.base + L::kPOff + (FP8 ? (tile & 1) * L::kP : 0) + cb * 128;
+      // P^T is the B operand of the output GEMM as it comes: a key's weights are contiguous (MN-major), rows of kPRow bytes
+      // with the swizzle of that width.
+      uint8_t* sp = sm.base + L::kPOff + (FP8 ? (tile & 1) * L::kP : 0) + t * L::kPRow;
+      const int twist = L::kPRow == 128 ? t & 7 : L::kPRow == 64 ? (t >> 1) & 3 : (t >> 2) & 1;
 #pragma unroll
       for (int c0 = 0; c0 < CW; c0 += 16) {
         float pw[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(s[c0 + c] - sm.ref()[cb + c0 + c]);
+        for (int c = 0; c < 16; c += 4) above(s, c0 + c, lk, pw + c);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) pw[c] = fast_exp2(pw[c]);
         if (FP8) {
           // 16 times the weight, at most 256; the remainder of its first rounding is at most 16, times 16
+          uint32_t hi[4], lo[4];
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
-            l[c0 + c] += pw[c] > 0.f ? pw[c] * iks : pw[c];
-            l[c0 + c + 1] += pw[c + 1] > 0.f ? pw[c + 1] * iks : pw[c + 1];
-            uint16_t hi, lo;
-            split_e4m3x2(pw[c] * 16.f, pw[c + 1] * 16.f, hi, lo);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint8_t* d = sp + (c0 + c + u) * 128 + ((((t >> 4) ^ (c + u)) & 7) << 4) + (t & 15);
-              d[0] = static_cast<uint8_t>(hi >> (8 * u));
-              d[NT * 128] = static_cast<uint8_t>(lo >> (8 * u));
-            }
+            l[c0 + c] = fmaf(pw[c], iks, l[c0 + c]);
+            l[c0 + c + 1] = fmaf(pw[c + 1], iks, l[c0 + c + 1]);
+            uint16_t h, r;
+            split_e4m3x2(pw[c] * 16.f, pw[c + 1] * 16.f, h, r);
+            hi[c >> 2] = (c & 2) ? hi[c >> 2] | (static_cast<uint32_t>(h) << 16) : h;
+            lo[c >> 2] = (c & 2) ? lo[c >> 2] | (static_cast<uint32_t>(r) << 16) : r;
           }
+          const int ch = (cb + c0) >> 4;
+          *reinterpret_cast<uint4*>(sp + ((ch ^ twist) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(sp + (((ch + NT / 16) ^ twist) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         } else {
-          uint8_t* d = sp + (t >> 6) * (NT * 128) + c0 * 128 + (t & 7) * 2;
+          uint32_t w2[8];
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
+          for (int c = 0; c < 16; c += 2) {
             l[c0 + c] += pw[c];
-            *reinterpret_cast<__nv_bfloat16*>(d + c * 128 + (((((t & 63) >> 3) ^ c) & 7) << 4)) = __float2bfloat16_rn(pw[c]);
+            l[c0 + c + 1] += pw[c + 1];
+            w2[c >> 1] = pack_bf16(pw[c], pw[c + 1]);
           }
+          const int ch = (cb + c0) >> 3;
+          *reinterpret_cast<uint4*>(sp + ((ch ^ twist) << 4)) = make_uint4(w2[0], w2[1], w2[2], w2[3]);
+          *reinterpret_cast<uint4*>(sp + (((ch + 1) ^ twist) << 4)) = make_uint4(w2[4], w2[5], w2[6], w2[7]);
         }
       }
       fence_proxy_async_smem();
@@ -655,7 +685,8 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
-    for (int i = 0; i < L::kRopeSlots; ++i) { mbar_init(sm.rfull(i), 1); mbar_init(sm.rempty(i), 1); }
+    mbar_init(sm.rfull(), 1);
+    mbar_init(sm.rempty(), 1);
     mbar_init(sm.q_full(), 64);
     mbar_init(sm.q_empty(), 1);
     mbar_init(sm.s_full(0), 1);
@@ -762,6 +793,12 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
             page = 0;
           }
         }
+        const auto rope_tile = [&]() {
+          mbar_wait(sm.rempty(), (tile & 1) ^ 1, ctl, 0x200);
+          if (lane == 0) mbar_arrive_expect_tx(sm.rfull(), boxes * box * 128);
+          __syncwarp();
+          if (lane < boxes) tma_load_4d(smem + L::kRopeOff + lane * box * 128, &tm_rope, sm.rfull(), 0, 0, row, page);
+        };
         for (int i = 0; i < 4; ++i, ++it) {
           const uint32_t s = it % L::NS;
           mbar_wait(sm.empty(s), ((it / L::NS) & 1) ^ 1, ctl, 0x100 + s);
@@ -772,13 +809,11 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
             tma_load_4d(dst, &tm_lat, sm.full(s), i * 128, 0, row, page);
             if (!FP8) tma_load_4d(dst + 16384, &tm_lat, sm.full(s), i * 128 + 64, 0, row, page);
           }
+          // 8-bit: its place is free once the previous tile's score GEMM has completed, which should not hold up the slots
+          // that the ring has beyond two tiles
+          if (FP8 && i == L::NS - 9) rope_tile();
         }
-        const uint32_t rs = tile % L::kRopeSlots;
-        mbar_wait(sm.rempty(rs), ((tile / L::kRopeSlots) & 1) ^ 1, ctl, 0x200 + rs);
-        if (lane == 0) mbar_arrive_expect_tx(sm.rfull(rs), boxes * box * 128);
-        __syncwarp();
-        if (lane < boxes)
-          tma_load_4d(smem + L::kRopeOff + rs * 16384 + lane * box * 128, &tm_rope, sm.rfull(rs), 0, 0, row, page);
+        if (!FP8) rope_tile();  // free (of the weights) once the previous tile's output GEMM has completed
       }
     }
   } else if (warp == 1) {
@@ -786,16 +821,15 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     const bool leader = elect_one();
     constexpr uint32_t id_rope = make_idesc_bf16(128, NT, false, false);
     constexpr uint32_t id_qk = FP8 ? make_idesc_e4m3(128, L::NC, false) : id_rope;
-    constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, false);
+    constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, true);
     const uint64_t q_desc = make_smem_desc(smem_u32(smem + L::kQOff), 16, 1024);
     const uint64_t qr_desc = make_smem_desc(smem_u32(smem + L::kQOff + L::kQLat), 16, 1024);
-    const uint64_t p_desc = make_smem_desc(smem_u32(smem + L::kPOff), 16, 1024);
+    const uint64_t p_desc = make_row_desc(smem_u32(smem + L::kPOff), L::kPRow);
     const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
     const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
     const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
     uint32_t ks = 0, kph = 0;       // slot and phase of the next score GEMM step
     uint32_t vs = 0;                // slot of the next output GEMM step
-    uint32_t rs = 0, rph = 0;       // rope slot of the next score GEMM
     uint32_t tile = 0, q_phase = 0;
     // Steps of the score GEMM of tile `number`: 128 latent dimensions each, then the rope part.
     const auto latent_step = [&](auto step, uint32_t number) {
@@ -819,25 +853,23 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       if (++ks == L::NS) { ks = 0; kph ^= 1; }
     };
     const auto rope_step = [&](uint32_t number) {
-      const uint64_t rd = desc_advance(r_desc, L::kRopeSlots == 1 ? 0 : uniform(rs) * 16384);
       const uint32_t d = FP8 ? tmem + kColR + (number & 1) * NT : tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
       tc_fence_after_sync();
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (leader) umma_ss(d, desc_advance(rd, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
+        if (leader) umma_ss(d, desc_advance(r_desc, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
       if (leader) {
         umma_commit(sm.s_full(L::kAhead > 0 ? number & 1 : 0));
-        if (FP8) umma_commit(sm.rempty(rs));
+        if (FP8) umma_commit(sm.rempty());
       }
-      if (++rs == L::kRopeSlots) { rs = 0; rph ^= 1; }
     };
     // Whether `bar` completes before this tile's weights are there (then its output GEMM goes first).
     const auto arrives_first = [&](uint64_t* bar, uint32_t parity, uint32_t number) {
       const long long t0 = clock64();
-      while (true) {
-        if (mbar_test_all(sm.p_full(number), (number >> 1) & 1)) return false;
+      for (uint32_t polls = 1;; ++polls) {
         if (mbar_test_all(bar, parity)) return true;
-        if (clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
+        if (mbar_test_all(sm.p_full(number), (number >> 1) & 1)) return false;
+        if ((polls & 31u) == 0u && clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
       }
     };
     while (__any_sync(0xFFFFFFFFu, walk.next(p))) {
@@ -859,7 +891,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
         blocking_step(Int<2>());
         blocking_step(Int<3>());
         if (done < 5) {
-          mbar_wait(sm.rfull(rs), rph, ctl, 0x500 + rs);
+          mbar_wait(sm.rfull(), tile & 1, ctl, 0x500);
           rope_step(tile);
         }
         if (j + 1 == tiles && leader) umma_commit(sm.q_empty());
@@ -877,7 +909,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
           early_step(Int<1>());
           early_step(Int<2>());
           early_step(Int<3>());
-          if (FP8 && done == 4 && arrives_first(sm.rfull(rs), rph, tile)) {
+          if (FP8 && done == 4 && arrives_first(sm.rfull(), (tile + 1) & 1, tile)) {
             rope_step(tile + 1);
             done = 5;
           }
@@ -886,27 +918,30 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
         mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
         tc_fence_after_sync();
         const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
+        const auto output_gemm = [&](auto all) {  // the last tile of a piece may need fewer steps of keys
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t vd = desc_advance(v_desc, L::NS == 4 ? i * L::kSlot : uniform(vs) * L::kSlot);
-          if (FP8) {
+          for (int i = 0; i < 4; ++i) {
+            const uint64_t vd = desc_advance(v_desc, L::NS == 4 ? i * L::kSlot : uniform(vs) * L::kSlot);
+            constexpr int kSteps = FP8 ? 4 : 8;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (leader && k < steps)
-                umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(pd, k * 32), id_pv,
-                           (j > 0 || k > 0) ? 1u : 0u);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (leader && k < steps)
-                umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048), desc_advance(pd, (k >> 2) * (NT * 128) + (k & 3) * 32),
-                        id_pv, (j > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < kSteps; ++k) {
+              if (leader && (decltype(all)::value != 0 || k < steps)) {
+                if (FP8)
+                  umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(pd, k * 32 * L::kPRow), id_pv,
+                             (j > 0 || k > 0) ? 1u : 0u);
+                else
+                  umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048), desc_advance(pd, k * 16 * L::kPRow),
+                          id_pv, (j > 0 || k > 0) ? 1u : 0u);
+              }
+            }
+            if (leader) umma_commit(sm.empty(vs));
+            if (++vs == L::NS) vs = 0;
           }
-          if (leader) umma_commit(sm.empty(vs));
-          if (++vs == L::NS) vs = 0;
-        }
+        };
+        if (steps == (FP8 ? 4 : 8)) output_gemm(Int<1>());
+        else output_gemm(Int<0>());
         if (leader) {
-          if (!FP8) umma_commit(sm.rempty(0));
+          if (!FP8) umma_commit(sm.rempty());
           umma_commit(sm.o_full(tile));
         }
       }
