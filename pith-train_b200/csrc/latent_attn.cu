@@ -40,10 +40,13 @@ constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope 
 template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
-  static constexpr int kExtra = FP8 ? (NT == 16 ? 3 : 5) : (NT == 16 ? 2 : NT == 32 ? 3 : 4);  // units that another piece costs a CTA
+  static constexpr int kExtra = FP8 ? (NT == 16 ? 3 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);  // units that another piece costs a CTA
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
   static constexpr int CW = NT / G;
-  static constexpr int kThreads = 128 + 128 * G;
+  // Query loaders: warps 2 and 3, and two more behind the softmax warps where queries are converted and the register file
+  // has room (at most three warps per scheduler).
+  static constexpr int kLoadWarps = FP8 && NT == 16 ? 4 : 2;
+  static constexpr int kThreads = 128 + 128 * G + (kLoadWarps - 2) * 32;
   static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
   static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
   static constexpr int kQ = kQLat + NT * 128;
@@ -77,7 +80,7 @@ struct LatAttnParams {
   const int32_t* qlens;
   const uint8_t* tree;
   const float* scale;
-  float* part_o;      // [2 G][NT][512]
+  float* part_o;      // [2 G][NT / 4][512][4 columns]
   float2* part_ml;    // [2 G][NT]: reference, sum
   int4* part_info;    // [G]: entry continued from the previous CTA, entry begun and not finished, its slot
   uint32_t* status;
@@ -266,83 +269,74 @@ struct LatShared {
   __device__ int* tok() const { return reinterpret_cast<int*>(cols() + 9 * NT); }
 };
 
-// Query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle), by 64 threads.
-template <int NT, bool FP8>
-__device__ __forceinline__ void load_query(const LatAttnParams& p, const LatShared<NT, FP8>& sm, const LatEntry& x, int t,
-                                           int parity) {
-  using L = LatCfg<NT, FP8>;
-  uint8_t* sq = sm.base + L::kQOff;
-  // Eight threads copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
-  constexpr int kBlocks = FP8 ? 1 : 9;  // 8-bit: only the rope part as it is
+// bf16: query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle), by 64
+// threads. Eight copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
+template <int NT>
+__device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, const LatEntry& x, int t) {
 #pragma unroll 1
   for (int row = t >> 3; row < NT; row += 8) {
     const int r = x.r0 + row, ch = t & 7;
     const int tok = r / p.H, h = r - tok * p.H;
     const bool there = r < p.R;
-    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + ch * 8 + (FP8 ? kLat : 0) : p.q;
-    const uint32_t dst = smem_u32(sq) + (FP8 ? L::kQLat : 0) + row * 128 + (((ch ^ row) & 7) << 4);
+    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + ch * 8 : p.q;
+    const uint32_t dst = smem_u32(sq) + row * 128 + (((ch ^ row) & 7) << 4);
 #pragma unroll
-    for (int i = 0; i < kBlocks; ++i) cp_async16(dst + i * (NT * 128), src + (there ? i * 64 : 0), there ? 16u : 0u);
-  }
-  if (!FP8) {
-    cp_async_wait_all();
-    return;
-  }
-  // 64 / NT neighbouring threads share a row: its largest element decides the power of two in front of the split
-  constexpr int TPR = 64 / NT, CH = 64 / TPR;  // 16-byte chunks of the latent part per thread
-  const int row = t / TPR, sub = t % TPR, r = x.r0 + row;
-  const int tok = r / p.H, h = r - tok * p.H;
-  const bool there = r < p.R;
-  const uint4* src = reinterpret_cast<const uint4*>(there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] : p.q) + sub;
-  float top = 0.f;
-#pragma unroll 1
-  for (int i0 = 0; i0 < CH; i0 += 16) {
-    uint4 v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __ldg(src + (i0 + i) * TPR);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        top = fmax3(top, fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u)));
-    }
-  }
-#pragma unroll
-  for (int o = TPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  const uint32_t bits = __float_as_uint(top);
-  int k = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x600000u ? 7 : 8);
-  k = top == 0.f ? 0 : min(max(k, -100), 100);
-  const float inv = there ? __uint_as_float(static_cast<uint32_t>(127 - k) << 23) : 0.f;
-  if (sub == 0)  // an infinite element makes the row's scores NaN
-    sm.qk(parity)[row] =
-        bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(127 + k) << 23);
-#pragma unroll 4
-  for (int i = 0; i < CH; ++i) {
-    const int ch = i * TPR + sub;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
-    const uint4 y = __ldg(src + i * TPR);  // read a second time (it is in L1): a loop stays small in the instruction cache
-    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-    uint32_t hi[2], lo[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t hw = 0, lw = 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float a = __uint_as_float(w[2 * j + u] << 16) * inv, b = __uint_as_float(w[2 * j + u] & 0xFFFF0000u) * inv;
-        uint16_t hv, lv;
-        split_e4m3x2(a, b, hv, lv);
-        hw |= static_cast<uint32_t>(hv) << (16 * u);
-        lw |= static_cast<uint32_t>(lv) << (16 * u);
-      }
-      hi[j] = hw;
-      lo[j] = lw;
-    }
-    uint8_t* blk = sq + (ch >> 4) * (2 * NT * 128);
-    const int c16 = (ch & 15) >> 1, half = (ch & 1) * 8;
-    *reinterpret_cast<uint2*>(blk + row * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(blk + (NT + row) * 128 + (((c16 ^ row) & 7) << 4) + half) = make_uint2(lo[0], lo[1]);
+    for (int i = 0; i < 9; ++i) cp_async16(dst + i * (NT * 128), src + (there ? i * 64 : 0), there ? 16u : 0u);
   }
   cp_async_wait_all();
+}
+
+// 8-bit: one warp's rows of the split query, a row per pass with the next one's loads in flight, 16 elements a lane (chunks
+// lane and lane + 32 of 8). `ready` waits until the previous piece has read its query. A rolled loop of one row: the code is
+// cold whenever it runs, and instruction fetches cost more than the arithmetic (16 rows unrolled: 20 000 cycles, four: 10 600).
+template <int NT, int WARPS, class Ready>
+__device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t* sq, float* qk, const LatEntry& x, int warp,
+                                                 int lane, Ready ready) {
+  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0, nr = n0;
+  const auto fetch = [&](int row) {
+    const int r = x.r0 + row;
+    n0 = n1 = nr = make_uint4(0, 0, 0, 0);
+    if (r < p.R) {
+      const int tok = r / p.H, h = r - tok * p.H;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]) + lane;
+      n0 = __ldg(src);
+      n1 = __ldg(src + 32);
+      if (lane < 8) nr = __ldg(src + 64);
+    }
+  };
+  fetch(warp);
+  ready();
+#pragma unroll 1
+  for (int row = warp; row < NT; row += WARPS) {
+    const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+    if (lane < 8) *reinterpret_cast<uint4*>(sq + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4)) = nr;
+    if (row + WARPS < NT) fetch(row + WARPS);
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      top = fmax3(top, fabsf(__uint_as_float(w[j] << 16)), fabsf(__uint_as_float(w[j] & 0xFFFF0000u)));
+    // magnitudes of floats order like their bits
+    const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
+    // the power of two that brings the row's largest element into (224, 448]
+    int k = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x600000u ? 7 : 8);
+    k = bits == 0u ? 0 : min(max(k, -100), 100);
+    const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    // an infinite element makes the row's scores NaN
+    if (lane == 0) qk[row] = __uint_as_float(bits >= 0x7F800000u ? 0x7FC00000u : static_cast<uint32_t>(127 + k) << 23);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint16_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        split_e4m3x2(__uint_as_float(w[4 * i + j] << 16) * inv, __uint_as_float(w[4 * i + j] & 0xFFFF0000u) * inv, h[j], l[j]);
+      const int ch = i * 32 + lane;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
+      uint8_t* d = sq + (ch >> 4) * (2 * NT * 128) + row * 128 + (((((ch & 15) >> 1) ^ row) & 7) << 4) + (ch & 1) * 8;
+      *reinterpret_cast<uint2*>(d) =
+          make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
+      *reinterpret_cast<uint2*>(d + NT * 128) =
+          make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
+    }
+  }
 }
 
 // Row t of one slot of the current latent tile: whether it holds a value that is not finite.
@@ -631,14 +625,20 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           y[c] = tiles == 0 || f == 0.f ? 0.f : v * f;  // no key, or no query (whose scores may be anything)
         }
         if (whole) {
-          __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0) * kLat + d0;
+          // neighbouring lanes trade: the even one stores two dimensions of an even column, the odd one of the next column
+          const int odd = t & 1;
+          __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0 + odd) * kLat + (d0 & ~1);
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            if (c0 + c < rows) d[c * kLat] = __float2bfloat16_rn(y[c]);
+          for (int c = 0; c < 16; c += 2) {
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? y[c] : y[c + 1], 1);
+            const uint32_t pair = odd ? pack_bf16(got, y[c + 1]) : pack_bf16(y[c], got);
+            if (c0 + c + odd < rows) *reinterpret_cast<uint32_t*>(d + c * kLat) = pair;
+          }
         } else {
-          float* d = p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat + d0;
+          // [column / 4][dimension][4 columns]: 16 bytes a lane, neighbouring
+          float4* d = reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat) + d0;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) d[c * kLat] = y[c];
+          for (int c = 0; c < 16; c += 4) d[c / 4 * kLat] = make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
         }
       }
     }
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
     mbar_init(sm.rfull(), 1);
     mbar_init(sm.rempty(), 1);
-    mbar_init(sm.q_full(), 64);
+    mbar_init(sm.q_full(), 32 * L::kLoadWarps);
     mbar_init(sm.q_empty(), 1);
     mbar_init(sm.s_full(0), 1);
     mbar_init(sm.s_full(1), 1);
@@ -832,10 +832,11 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     uint32_t vs = 0;                // slot of the next output GEMM step
     uint32_t tile = 0, q_phase = 0;
     // Steps of the score GEMM of tile `number`: 128 latent dimensions each, then the rope part.
-    const auto latent_step = [&](auto step, uint32_t number) {
+    // (the descriptor of the slot is formed before the wait for it)
+    const auto step_desc = [&](int i) { return desc_advance(k_desc, L::NS == 4 ? i * L::kSlot : uniform(ks) * L::kSlot); };
+    const auto latent_step = [&](auto step, uint32_t number, uint64_t kd) {
       constexpr int i = decltype(step)::value;
       const uint32_t d = tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
-      const uint64_t kd = desc_advance(k_desc, L::NS == 4 ? i * L::kSlot : uniform(ks) * L::kSlot);
       tc_fence_after_sync();
       if (FP8) {
 #pragma unroll
@@ -882,8 +883,9 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       for (int j = 0; j < tiles; ++j, ++tile) {
         const auto blocking_step = [&](auto step) {
           if (done <= decltype(step)::value) {
+            const uint64_t kd = step_desc(decltype(step)::value);
             mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
-            latent_step(step, tile);
+            latent_step(step, tile, kd);
           }
         };
         blocking_step(Int<0>());
@@ -900,9 +902,12 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
           // While this tile's softmax runs: the next tile's score GEMM, as far as its slots have arrived.
           const auto early_step = [&](auto step) {
             constexpr int i = decltype(step)::value;
-            if (i < L::kAhead && done == i && arrives_first(sm.full(ks), kph, tile)) {
-              latent_step(step, tile + 1);
-              done = i + 1;
+            if (i < L::kAhead && done == i) {
+              const uint64_t kd = step_desc(i);
+              if (arrives_first(sm.full(ks), kph, tile)) {
+                latent_step(step, tile + 1, kd);
+                done = i + 1;
+              }
             }
           };
           early_step(Int<0>());
@@ -914,28 +919,34 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
             done = 5;
           }
         }
+        uint64_t vd[4];
+        uint32_t slot[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          slot[i] = L::NS == 4 ? i : uniform(vs);
+          vd[i] = desc_advance(v_desc, slot[i] * L::kSlot);
+          if (++vs == L::NS) vs = 0;
+        }
+        const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
         const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
         mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
         tc_fence_after_sync();
-        const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
         const auto output_gemm = [&](auto all) {  // the last tile of a piece may need fewer steps of keys
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint64_t vd = desc_advance(v_desc, L::NS == 4 ? i * L::kSlot : uniform(vs) * L::kSlot);
             constexpr int kSteps = FP8 ? 4 : 8;
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
               if (leader && (decltype(all)::value != 0 || k < steps)) {
                 if (FP8)
-                  umma_ss_f8(tmem + i * L::NC, desc_advance(vd, k * 4096), desc_advance(pd, k * 32 * L::kPRow), id_pv,
+                  umma_ss_f8(tmem + i * L::NC, desc_advance(vd[i], k * 4096), desc_advance(pd, k * 32 * L::kPRow), id_pv,
                              (j > 0 || k > 0) ? 1u : 0u);
                 else
-                  umma_ss(tmem + i * L::NC, desc_advance(vd, k * 2048), desc_advance(pd, k * 16 * L::kPRow),
+                  umma_ss(tmem + i * L::NC, desc_advance(vd[i], k * 2048), desc_advance(pd, k * 16 * L::kPRow),
                           id_pv, (j > 0 || k > 0) ? 1u : 0u);
               }
             }
-            if (leader) umma_commit(sm.empty(vs));
-            if (++vs == L::NS) vs = 0;
+            if (leader) umma_commit(sm.empty(slot[i]));
           }
         };
         if (steps == (FP8 ? 4 : 8)) output_gemm(Int<1>());
@@ -946,17 +957,25 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
         }
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 4 + 4 * L::G) {
     lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, (warp - 4) >> 2, static_cast<int>(threadIdx.x) & 127);
   } else {
-    // ------------------------------------------------------------------ warps 2 and 3: queries, one piece ahead
+    // ------------------------------------------------------------------ query loaders, one piece ahead
+    const int loader = warp < 4 ? warp - 2 : warp - 2 - 4 * L::G;
     uint32_t q_phase = 1, piece = 0;
     while (walk.next(p)) {
       const int tiles = walk.tiles();
       if (tiles > 0) {
-        mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
+        uint8_t* sq = smem + L::kQOff;
+        // the previous piece's last score GEMM has read its query
+        const auto ready = [&]() { mbar_wait(sm.q_empty(), q_phase, ctl, 0x380); };
+        if constexpr (FP8) {
+          load_split_query<NT, L::kLoadWarps>(p, sq, sm.qk(piece & 1), walk.x, loader, lane, ready);
+        } else {
+          ready();
+          load_query<NT>(p, sq, walk.x, loader * 32 + lane);
+        }
         q_phase ^= 1;
-        load_query<NT, FP8>(p, sm, walk.x, static_cast<int>(threadIdx.x) - 64, piece & 1);
         fence_proxy_async_smem();
         mbar_arrive(sm.q_full());
       }
@@ -977,24 +996,21 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
 }
 
 // Merge of a row tile that several CTAs worked on: out = sum_i 2^(ref_i - M) O_i / sum_i 2^(ref_i - M) l_i, in key order.
-// Block (j, column): the j-th entry that a CTA began and did not finish; there are at most as many as entries, and one
-// less than CTAs. Four groups of 128 threads, a thread holding four output dimensions, take a column each (COLS = 4: many
-// entries, so few parts each) or every fourth part of one column (COLS = 1: a long context cut into many parts). With
-// COLS = 1 throughout, 112 entries x 32 columns cost 18 us instead of 9 for the blocks alone. The launch is a programmatic
-// one: it waits for the attention kernel's results in the kernel instead of before it.
+// Block (j, four columns): the j-th entry that a CTA began and did not finish; there are at most as many as entries, and
+// one less than CTAs. A thread has one output dimension of the four columns: all 512 (SPLIT = 1: many entries, so few parts
+// each), or 128 of them with the parts dealt to four groups of threads (SPLIT = 4: a long context cut into many parts). The
+// launch is a programmatic one: it waits for the attention kernel's results in the kernel instead of before it.
 constexpr int kMergeThreads = 512;
-template <int NT, int COLS>
+template <int NT, int SPLIT>
 __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAttnParams p, int ctas) {
   __shared__ int warp_jobs[16];
   __shared__ int job[2];  // CTA, slot
   __shared__ int entry;
-  __shared__ float wt[COLS][kMergeThreads];
-  __shared__ float red[2][16];
-  __shared__ float4 acc_s[3][128];
-  constexpr int kShare = 4 / COLS;  // groups per column
+  __shared__ float4 wt[kMergeThreads];
+  __shared__ float4 red[2][1];
+  __shared__ float4 acc_s[SPLIT == 4 ? 384 : 1];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int g = t >> 7, d = t & 127, sub = g % kShare, mine = t % (kShare * 128);
-  const int col = blockIdx.y * COLS + g / kShare;
+  const int c4 = blockIdx.y;  // columns [4 c4, 4 c4 + 4)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint32_t failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
   const int4 info = t < ctas ? p.part_info[t] : make_int4(-1, -1, -1, 0);
@@ -1011,59 +1027,64 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
   if (info.y >= 0 && rank == static_cast<int>(blockIdx.x)) { job[0] = t; job[1] = info.z; entry = info.y; }
   __syncthreads();
   const int c = job[0], e = entry;
-  const int b = e / p.RT, r = (e - b * p.RT) * NT + col;
   // parts: the slot of CTA c, then the first slot of each following CTA that continues the entry
   const int n = 1 + __syncthreads_count(t > c && info.x == e);
   const auto slot_of = [&](int i) { return i == 0 ? job[1] : 2 * (c + i); };
-  float top = kNoRef;
-  for (int i = mine; i < n; i += kShare * 128) top = fmaxf(top, p.part_ml[slot_of(i) * NT + col].x);
+  // Weights of the parts, by the first 128 threads: lane group of 32 = column, each column's parts over its lanes.
+  if (warp < 4) {
+    const float2* ml = p.part_ml + 4 * c4 + warp;
+    float top = kNoRef;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, ml[slot_of(i) * NT].x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  if (lane == 0) red[0][warp] = top;
-  __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    float sum = 0.f;
+    for (int i = lane; i < n; i += 32) {
+      const float2 v = ml[slot_of(i) * NT];
+      const float w = fast_exp2(v.x - top);
+      reinterpret_cast<float*>(wt + i)[warp] = w;
+      sum += w * v.y;
+    }
 #pragma unroll
-  for (int i = 0; i < kShare * 4; ++i) top = fmaxf(top, red[0][(g / kShare) * kShare * 4 + i]);
-  float sum = 0.f;
-  for (int i = mine; i < n; i += kShare * 128) {
-    const float2 ml = p.part_ml[slot_of(i) * NT + col];
-    const float w = fast_exp2(ml.x - top);
-    wt[g / kShare][i] = w;
-    sum += w * ml.y;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) {
+      reinterpret_cast<float*>(&red[0][0])[warp] = sum;
+      reinterpret_cast<float*>(&red[1][0])[warp] = top;
+    }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (lane == 0) red[1][warp] = sum;
   __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kShare * 4; ++i) sum += red[1][(g / kShare) * kShare * 4 + i];
+  const int g = SPLIT == 4 ? t >> 7 : 0, d = SPLIT == 4 ? blockIdx.z * 128 + (t & 127) : t;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int i = sub; i < n; i += kShare) {
-    const float f = wt[g / kShare][i];
-    const float4 v = *(reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot_of(i)) * NT + col) * kLat) + d);
-    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+  for (int i = g; i < n; i += SPLIT) {
+    const float4 f = wt[i];
+    const float4 v = *(reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot_of(i)) * NT + 4 * c4) * kLat) + d);
+    acc.x = fmaf(f.x, v.x, acc.x); acc.y = fmaf(f.y, v.y, acc.y); acc.z = fmaf(f.z, v.z, acc.z); acc.w = fmaf(f.w, v.w, acc.w);
   }
-  if (COLS == 1) {
-    if (g > 0) acc_s[g - 1][d] = acc;
+  if (SPLIT == 4) {
+    if (g > 0) acc_s[t - 128] = acc;
     __syncthreads();
     if (g > 0) return;
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const float4 v = acc_s[i][d];
+      const float4 v = acc_s[i * 128 + t];
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }
-  if (r >= p.R) return;
-  const float inv = 1.f / sum;
-  if (sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // no key, or no query
-  else acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-  *(reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(b) * p.R + r) * kLat) + d) =
-      make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-  if (d == 0 && p.lse != nullptr) {
-    const int tok = r / p.H;
-    p.lse[static_cast<int64_t>(b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
-        sum == 0.f ? -INFINITY : top + log2f(sum);
+  const int b = e / p.RT, r0 = (e - b * p.RT) * NT + 4 * c4;
+  const float sums[4] = {red[0][0].x, red[0][0].y, red[0][0].z, red[0][0].w};
+  const float sum_top[4] = {red[1][0].x, red[1][0].y, red[1][0].z, red[1][0].w};
+  const float o[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + i;
+    if (r >= p.R) break;
+    const bool none = sums[i] == 0.f;  // no key, or no query
+    p.out[(static_cast<int64_t>(b) * p.R + r) * kLat + d] = __float2bfloat16_rn(none ? 0.f : o[i] / sums[i]);
+    if (d == 0 && p.lse != nullptr) {
+      const int tok = r / p.H;
+      p.lse[static_cast<int64_t>(b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
+          none ? -INFINITY : sum_top[i] + log2f(sums[i]);
+    }
   }
 }
 
@@ -1097,9 +1118,10 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   if (p.max_keys > kUnit && ctas > 1) {  // an entry of one unit is never cut
     const int64_t entries = static_cast<int64_t>(p.B) * p.RT;
     cudaLaunchConfig_t cfg = {};
-    const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1), cols = p.R < NT ? p.R : NT;
+    const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1);
+    const unsigned cols = static_cast<unsigned>((p.R < NT ? p.R : NT) + 3) / 4;
     const bool many = entries * 8 >= ctas;  // at most about nine parts an entry
-    cfg.gridDim = dim3(jobs, many ? (cols + 3) / 4 : cols);
+    cfg.gridDim = dim3(jobs, cols, many ? 1 : 4);
     cfg.blockDim = dim3(kMergeThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -1107,7 +1129,7 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PITH_CUDA(cudaLaunchKernelEx(&cfg, many ? latent_merge_kernel<NT, 4> : latent_merge_kernel<NT, 1>,
+    PITH_CUDA(cudaLaunchKernelEx(&cfg, many ? latent_merge_kernel<NT, 1> : latent_merge_kernel<NT, 4>,
                                  static_cast<const LatAttnParams&>(p), ctas));
   }
   return kOk;
