@@ -292,25 +292,31 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, 
 template <int NT, int WARPS, class Ready>
 __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t* sq, float* qk, const LatEntry& x, int warp,
                                                  int lane, Ready ready) {
-  uint4 n0 = make_uint4(0, 0, 0, 0), n1 = n0, nr = n0;
-  const auto fetch = [&](int row) {
+  constexpr int kDeep = 3;  // rows in flight
+  uint4 n[kDeep][3];
+  const auto fetch = [&](int row, uint4* to) {
     const int r = x.r0 + row;
-    n0 = n1 = nr = make_uint4(0, 0, 0, 0);
-    if (r < p.R) {
+    to[0] = to[1] = to[2] = make_uint4(0, 0, 0, 0);
+    if (row < NT && r < p.R) {
       const int tok = r / p.H, h = r - tok * p.H;
       const uint4* src = reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]) + lane;
-      n0 = __ldg(src);
-      n1 = __ldg(src + 32);
-      if (lane < 8) nr = __ldg(src + 64);
+      to[0] = __ldg(src);
+      to[1] = __ldg(src + 32);
+      if (lane < 8) to[2] = __ldg(src + 64);
     }
   };
-  fetch(warp);
+#pragma unroll
+  for (int i = 0; i < kDeep; ++i) fetch(warp + i * WARPS, n[i]);
   ready();
 #pragma unroll 1
   for (int row = warp; row < NT; row += WARPS) {
-    const uint32_t w[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
-    if (lane < 8) *reinterpret_cast<uint4*>(sq + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4)) = nr;
-    if (row + WARPS < NT) fetch(row + WARPS);
+    const uint32_t w[8] = {n[0][0].x, n[0][0].y, n[0][0].z, n[0][0].w, n[0][1].x, n[0][1].y, n[0][1].z, n[0][1].w};
+    if (lane < 8) *reinterpret_cast<uint4*>(sq + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4)) = n[0][2];
+#pragma unroll
+    for (int i = 0; i + 1 < kDeep; ++i)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) n[i][j] = n[i + 1][j];
+    fetch(row + kDeep * WARPS, n[kDeep - 1]);
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
