@@ -48,35 +48,55 @@ __device__ __forceinline__ void lat_load4(const void* base, int f32, int64_t off
   }
 }
 
-// Rotary part of one query row: lane l8 of eight turns inputs [8 l8, 8 l8 + 8) into outputs [4 l8, +4) and [32 + 4 l8, +4).
-__device__ __forceinline__ void lat_rope_row(const LatProjParams& p, int64_t g, int h, int l8) {
-  const int64_t b = g / p.S0, s = g - b * p.S0;
-  int64_t cs = b * p.cs[0] + s * p.cs[1];
-  if (p.pos != nullptr) {
-    const int64_t row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
-    if (row < 0 || row >= p.table_rows) {
-      if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPosition);
-      return;
-    }
-    cs = row * p.cs[1];
-  }
-  float cl[4], ch[4], sl[4], sh[4];
-  lat_load4(p.cos, p.cs_f32, cs + 4 * l8, cl);
-  lat_load4(p.cos, p.cs_f32, cs + 32 + 4 * l8, ch);
-  lat_load4(p.sin, p.cs_f32, cs + 4 * l8, sl);
-  lat_load4(p.sin, p.cs_f32, cs + 32 + 4 * l8, sh);
-  const uint4 x = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs[0] + s * p.qs[1] + h * p.qs[2] + 128) + l8);
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  float lo[4], hi[4];
+// Rotary parts of PASSES x 16 query rows by 128 threads: lane l8 of eight turns inputs [8 l8, 8 l8 + 8) of a row into outputs
+// [4 l8, +4) and [32 + 4 l8, +4). All positions, then all other loads are issued before the first use: one after the other
+// they took longer than the tile's GEMM.
+template <int PASSES>
+__device__ __forceinline__ void lat_rope_rows(const LatProjParams& p, int64_t g0, int rows, int h, int t) {
+  const int l8 = t & 7;
+  int64_t cs[PASSES], from[PASSES];
+  bool ok[PASSES];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float even = __uint_as_float(w[i] << 16), odd = __uint_as_float(w[i] & 0xFFFF0000u);
-    lo[i] = even * cl[i] - odd * sl[i];
-    hi[i] = odd * ch[i] + even * sh[i];
+  for (int i = 0; i < PASSES; ++i) {
+    ok[i] = i * 16 + (t >> 3) < rows;
+    const int64_t g = g0 + (ok[i] ? i * 16 + (t >> 3) : 0);
+    const int64_t b = g / p.S0, s = g - b * p.S0;
+    from[i] = b * p.qs[0] + s * p.qs[1] + h * p.qs[2] + 128;
+    cs[i] = b * p.cs[0] + s * p.cs[1];
+    if (p.pos != nullptr) {
+      const int64_t row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
+      const bool in = row >= 0 && row < p.table_rows;
+      if (!in && p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPosition);
+      ok[i] = ok[i] && in;
+      cs[i] = in ? row * p.cs[1] : 0;
+    }
   }
-  __nv_bfloat16* d = p.out + (g * p.H + h) * 576 + 512;
-  *reinterpret_cast<uint2*>(d + 4 * l8) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-  *reinterpret_cast<uint2*>(d + 32 + 4 * l8) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
+  float cl[PASSES][4], ch[PASSES][4], sl[PASSES][4], sh[PASSES][4];
+  uint4 x[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    if (!ok[i]) continue;
+    lat_load4(p.cos, p.cs_f32, cs[i] + 4 * l8, cl[i]);
+    lat_load4(p.cos, p.cs_f32, cs[i] + 32 + 4 * l8, ch[i]);
+    lat_load4(p.sin, p.cs_f32, cs[i] + 4 * l8, sl[i]);
+    lat_load4(p.sin, p.cs_f32, cs[i] + 32 + 4 * l8, sh[i]);
+    x[i] = __ldg(reinterpret_cast<const uint4*>(p.q + from[i]) + l8);
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    if (!ok[i]) continue;
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    float lo[4], hi[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float even = __uint_as_float(w[j] << 16), odd = __uint_as_float(w[j] & 0xFFFF0000u);
+      lo[j] = even * cl[i][j] - odd * sl[i][j];
+      hi[j] = odd * ch[i][j] + even * sh[i][j];
+    }
+    __nv_bfloat16* d = p.out + ((g0 + i * 16 + (t >> 3)) * p.H + h) * 576 + 512;
+    *reinterpret_cast<uint2*>(d + 4 * l8) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+    *reinterpret_cast<uint2*>(d + 32 + 4 * l8) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
+  }
 }
 
 // A [128 tokens x K] K-major, B [NT columns x K] (query: MN-major), K in blocks of 64 through ST stages.
@@ -91,10 +111,11 @@ struct ProjCfg {
   static constexpr int kBars = 2 * ST + 1;
   static constexpr int kAlloc = kTiles + kBars * 8 + 16;
   static constexpr int kCols = NT < 32 ? 32 : NT;
+  static constexpr int kThreads = QUERY ? 256 : 128;   // warps 4-7 of the query kernel: rotary parts
 };
 
 template <bool QUERY, int NT, int ST>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(ProjCfg<QUERY, NT, ST>::kThreads)
     latent_proj_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                        const __grid_constant__ CUtensorMap tm_out, const LatProjParams p) {
   using L = ProjCfg<QUERY, NT, ST>;
@@ -165,16 +186,13 @@ __global__ void __launch_bounds__(128)
       }
     }
     __syncwarp();
-    if (QUERY) {  // this column tile's share of the rotary parts, while the MMAs run
+    if (QUERY && warp >= 4) {  // this column tile's share of the rotary parts
       constexpr int RR = 128 / NN;
-#pragma unroll
-      for (int i = 0; i < (RR + 15) / 16; ++i) {
-        const int row = m0 + nt * RR + i * 16 + (threadIdx.x >> 3);
-        if (row < p.rows) lat_rope_row(p, static_cast<int64_t>(b) * p.rows + row, h, threadIdx.x & 7);
-      }
-      __syncwarp();
-    }
-    {
+      const int first = m0 + nt * RR;
+      if (first < p.rows)
+        lat_rope_rows<(RR + 15) / 16>(p, static_cast<int64_t>(b) * p.rows + first, min(RR, p.rows - first), h,
+                                      static_cast<int>(threadIdx.x) - 128);
+    } else {
       mbar_wait(done, 0, ctl, 0x800);
       tc_fence_after_sync();
       const int t = threadIdx.x;
@@ -234,7 +252,7 @@ static int launch_proj(const CUtensorMap& ta, const pith_latent_proj_args* a, co
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
   const int64_t mt = (S + 127) / 128;
   PITH_REQUIRE(mt * NN < 2147483647 && a->H <= 65535 && B <= 65535, "too many tokens, heads or sequences");
-  kern<<<dim3(static_cast<unsigned>(mt * NN), a->H, static_cast<unsigned>(B)), 128, L::kAlloc, st>>>(ta, tw, to, p);
+  kern<<<dim3(static_cast<unsigned>(mt * NN), a->H, static_cast<unsigned>(B)), L::kThreads, L::kAlloc, st>>>(ta, tw, to, p);
   PITH_CUDA(cudaGetLastError());
   return kOk;
 }
