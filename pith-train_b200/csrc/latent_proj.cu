@@ -99,6 +99,56 @@ __device__ __forceinline__ void lat_rope_rows(const LatProjParams& p, int64_t g0
   }
 }
 
+// Rotary parts of tokens [g0, g1) for all heads, by 256 threads: eight lanes take a token, read its row of the tables once
+// and walk its heads sixteen at a time. Beside the GEMM's traffic a dependent load takes microseconds, so that a token's
+// position and queries are requested together, then its tables, and one pass of 32 tokens covers a CTA's share of a chunk.
+__device__ __forceinline__ void lat_rope_tokens(const LatProjParams& p, int64_t g0, int64_t g1, int t) {
+  const int l8 = t & 7;
+  constexpr int kHeads = 16;
+  for (int64_t g = g0 + (t >> 3); g < g1; g += 32) {
+    const int64_t b = g / p.S0, s = g - b * p.S0;
+    int64_t row = 0, cs = b * p.cs[0] + s * p.cs[1];
+    if (p.pos != nullptr) row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
+    const __nv_bfloat16* src = p.q + b * p.qs[0] + s * p.qs[1] + 128;
+    __nv_bfloat16* dst = p.out + g * p.H * 576 + 512;
+    float cl[4], ch[4], sl[4], sh[4];
+    for (int h0 = 0; h0 < p.H; h0 += kHeads) {
+      uint4 x[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(min(h0 + i, p.H - 1)) * p.qs[2]) + l8);
+      if (h0 == 0) {
+        if (p.pos != nullptr) {
+          if (row < 0 || row >= p.table_rows) {
+            if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPosition);
+            break;
+          }
+          cs = row * p.cs[1];
+        }
+        lat_load4(p.cos, p.cs_f32, cs + 4 * l8, cl);
+        lat_load4(p.cos, p.cs_f32, cs + 32 + 4 * l8, ch);
+        lat_load4(p.sin, p.cs_f32, cs + 4 * l8, sl);
+        lat_load4(p.sin, p.cs_f32, cs + 32 + 4 * l8, sh);
+      }
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (h0 + i >= p.H) break;
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        float lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float even = __uint_as_float(w[j] << 16), odd = __uint_as_float(w[j] & 0xFFFF0000u);
+          lo[j] = even * cl[j] - odd * sl[j];
+          hi[j] = odd * ch[j] + even * sh[j];
+        }
+        __nv_bfloat16* d = dst + static_cast<int64_t>(h0 + i) * 576;
+        *reinterpret_cast<uint2*>(d + 4 * l8) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
+        *reinterpret_cast<uint2*>(d + 32 + 4 * l8) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
+      }
+    }
+  }
+}
+
 // A [128 tokens x K] K-major, B [NT columns x K] (query: MN-major), K in blocks of 64 through ST stages.
 template <bool QUERY, int NT, int ST>
 struct ProjCfg {
@@ -238,16 +288,239 @@ __global__ void __launch_bounds__(ProjCfg<QUERY, NT, ST>::kThreads)
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Many tokens: a persistent kernel. One CTA per SM takes a contiguous run of (head, column tile, token tile) items with the
+// token tile innermost, so that its part of W stays in shared memory (64 KB of the query's, 128 KB of the output's) and only
+// the tokens stream: TMA producer (warp 0), MMA issuer (warp 1), epilogue (warps 4-7, two accumulators in TMEM, staged and
+// stored by TMA), rotary parts (warps 8-15, query only). One tile per CTA, loads, MMAs and stores one after the other, took
+// 28.6 us (query) and 19.2 us (output) for 4095 tokens x 16 heads.
+template <bool QUERY>
+struct RunCfg {
+  static constexpr int NT = QUERY ? 256 : 128;
+  static constexpr int NN = QUERY ? 2 : 1;
+  static constexpr int KB = QUERY ? 2 : 8;
+  static constexpr int kB = NT * 128 * KB;
+  static constexpr int ST = QUERY ? 6 : 4;  // 16 KB stages of A
+  static constexpr int kAOff = kB;
+  static constexpr int kOutOff = kAOff + ST * 16384;
+  static constexpr int kBarOff = kOutOff + NT * 256;
+  static constexpr int kBars = 2 * ST + 6;
+  static constexpr int kAlloc = kBarOff + kBars * 8 + 16;
+  static constexpr int kThreads = QUERY ? 512 : 256;
+  static_assert(kAlloc <= 232448, "shared memory");
+};
+
+template <bool QUERY>
+__global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
+    latent_proj_run_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                           const __grid_constant__ CUtensorMap tm_out, const LatProjParams p, int tile, int mtiles, int items,
+                           int64_t tokens) {
+  using L = RunCfg<QUERY>;
+  constexpr int NT = L::NT, NN = L::NN, KB = L::KB, ST = L::ST;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + ST;
+  uint64_t* b_full = bars + 2 * ST;
+  uint64_t* b_empty = b_full + 1;
+  uint64_t* acc_full = b_full + 2;   // [2]
+  uint64_t* acc_empty = b_full + 4;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + L::kBars);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AbortCtl ctl{p.status, abort_flag};
+  // items [i0, i1): item = (group, token tile), group = (batch, head, column tile)
+  const int share = items / gridDim.x, more = items - share * static_cast<int>(gridDim.x), me = blockIdx.x;
+  int i0 = me * share + min(me, more), i1 = i0 + share + (me < more ? 1 : 0);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(b_full, 1);
+    mbar_init(b_empty, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 128); }
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 64) {
+    *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
+    if ((smem_u32(smem) & 1023u) != 0u) report_error(ctl, kErrSmemAlign, smem_u32(smem));
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 2 * NT);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  if (*abort_flag != 0u) i1 = i0;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t s = 0, ph = 1, bph = 1;
+      int group = -1;
+      for (int it = i0; it < i1; ++it) {
+        const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
+        const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
+        if (g != group) {
+          group = g;
+          mbar_wait(b_empty, bph, ctl, 0x200);
+          bph ^= 1;
+          mbar_arrive_expect_tx(b_full, L::kB);
+          for (int k = 0; k < KB; ++k) {
+            if (QUERY) {  // 64 rows of W (the K block) x NT columns, as [64 rows][64 columns] blocks
+              for (int i = 0; i < NT / 64; ++i)
+                tma_load_4d(smem + k * (NT * 128) + i * 8192, &tm_w, b_full, nt * NT + i * 64, 0, h * 256 + k * 64, 0);
+            } else {      // NT rows of W x 64 columns (the K block)
+              tma_load_4d(smem + k * (NT * 128), &tm_w, b_full, k * 64, 0, h * 256 + 128, 0);
+            }
+          }
+        }
+        for (int k = 0; k < KB; ++k) {
+          mbar_wait(&empty[s], ph, ctl, 0x100 + s);
+          mbar_arrive_expect_tx(&full[s], tile * 128);
+          tma_load_4d(smem + L::kAOff + s * 16384, &tm_a, &full[s], k * 64, h, m0, b);
+          if (++s == ST) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    constexpr uint32_t idesc = make_idesc_bf16(128, NT, false, QUERY);
+    const uint64_t ad0 = make_smem_desc(smem_u32(smem) + L::kAOff, 16, 1024);
+    const uint64_t bd0 = make_smem_desc(smem_u32(smem), QUERY ? 8192 : 16, 1024);
+    uint32_t s = 0, ph = 0, bph = 0;
+    int group = -1;
+    for (int it = i0; it < i1; ++it) {
+      const uint32_t n = it - i0, buf = n & 1;
+      const int g = it / mtiles;
+      if (g != group) {
+        group = g;
+        mbar_wait(b_full, bph, ctl, 0x300);
+        bph ^= 1;
+      }
+      mbar_wait(&acc_empty[buf], ((n >> 1) & 1) ^ 1, ctl, 0x500 + buf);
+      for (int k = 0; k < KB; ++k) {
+        mbar_wait(&full[s], ph, ctl, 0x400 + s);
+        tc_fence_after_sync();
+        const uint64_t ad = desc_advance(ad0, s * 16384), bd = desc_advance(bd0, k * (NT * 128));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (leader)
+            umma_ss(tmem + buf * NT, desc_advance(ad, i * 32), desc_advance(bd, QUERY ? i * 2048 : i * 32), idesc,
+                    (k > 0 || i > 0) ? 1u : 0u);
+        if (leader) umma_commit(&empty[s]);
+        if (++s == ST) { s = 0; ph ^= 1; }
+      }
+      if (leader) {
+        umma_commit(&acc_full[buf]);
+        if (it + 1 < i1 && (it + 1) / mtiles != g) umma_commit(b_empty);
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    const int t = static_cast<int>(threadIdx.x) & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) << 5) << 16;
+    uint8_t* out = smem + L::kOutOff;
+    for (int it = i0; it < i1; ++it) {
+      const uint32_t n = it - i0, buf = n & 1;
+      const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
+      const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
+      mbar_wait(&acc_full[buf], (n >> 1) & 1, ctl, 0x800 + buf);
+      tc_fence_after_sync();
+      if (t == 0) tma_store_wait_read();  // the previous item's staged result has been read
+      named_bar_sync(1, 128);
+#pragma unroll 2
+      for (int c = 0; c < NT / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld32(tmem + lanes + buf * NT + c * 32, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t* v = r + 8 * i;
+          const int ch = (c & 1) * 4 + i;
+          *reinterpret_cast<uint4*>(out + (c >> 1) * 16384 + t * 128 + (((ch ^ t) & 7) << 4)) =
+              make_uint4(pack_bf16(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                         pack_bf16(__uint_as_float(v[2]), __uint_as_float(v[3])),
+                         pack_bf16(__uint_as_float(v[4]), __uint_as_float(v[5])),
+                         pack_bf16(__uint_as_float(v[6]), __uint_as_float(v[7])));
+        }
+      }
+      tc_fence_before_sync();
+      mbar_arrive(&acc_empty[buf]);
+      fence_proxy_async_smem();
+      named_bar_sync(1, 128);
+      if (t == 0 && *abort_flag == 0u) {
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) tma_store_4d(&tm_out, out + i * 16384, nt * NT + i * 64, h, m0, b);
+        tma_store_commit();
+      }
+    }
+    if (t == 0) tma_store_wait_read();
+  } else if (QUERY && warp >= 8) {
+    // an equal share of the tokens, whatever the CTA's items: with the rotary part of its own (head, token) rows every head
+    // read the tables again, and the kernel waited for these warps (33.7 us)
+    if (*abort_flag == 0u)
+      lat_rope_tokens(p, tokens * me / gridDim.x, tokens * (me + 1) / gridDim.x, static_cast<int>(threadIdx.x) - 256);
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000ll) __nanosleep(1000);
+  }
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 2 * NT);
+  }
+}
+
+// Tensor maps of W (boxes of 64 columns and `rows` rows) and of the contiguous result (64 columns, `tile` tokens).
+template <bool QUERY>
+static int proj_maps(const pith_latent_proj_args* a, int64_t B, int64_t S, int rows, int tile, CUtensorMap* tw,
+                     CUtensorMap* to) {
+  constexpr int kIn = QUERY ? 576 : 128;
+  const int64_t ws[3] = {static_cast<int64_t>(a->H) * 256 * a->weight_stride, a->weight_stride, 512};
+  if (int rc = make_tensor_map(tw, a->weight, 2, 1, static_cast<int64_t>(a->H) * 256, 1, 512, ws, 64, rows)) return rc;
+  const int64_t os[3] = {S * a->H * kIn, static_cast<int64_t>(a->H) * kIn, kIn};
+  return make_tensor_map(to, a->out, 2, B, S, a->H, kIn, os, 64, tile);
+}
+
+template <bool QUERY>
+static int launch_proj_run(const pith_latent_proj_args* a, const LatProjParams& p, int64_t B, int64_t S, const int64_t xs[3],
+                           int sms, cudaStream_t st) {
+  using L = RunCfg<QUERY>;
+  // Tokens per tile, 64 to 128: what the CTA with the most tiles has to stream decides (4095 tokens x 16 heads: 592 output
+  // tiles of 112 are four rounds of 148 CTAs, 512 of 128 are also four). A tile costs about 8 tokens of its own.
+  int tile = 128;
+  int64_t best = -1;
+  for (int r = 128; r >= 64; r -= 8) {
+    const int64_t rounds = ((S + r - 1) / r * B * a->H * L::NN + sms - 1) / sms;
+    if (best < 0 || rounds * (r + 8) < best) {
+      best = rounds * (r + 8);
+      tile = r;
+    }
+  }
+  CUtensorMap ta, tw, to;
+  if (int rc = make_tensor_map(&ta, a->x, 2, B, S, a->H, QUERY ? 192 : 512, xs, 64, tile)) return rc;
+  if (int rc = proj_maps<QUERY>(a, B, S, QUERY ? 64 : L::NT, tile, &tw, &to)) return rc;
+  auto kern = latent_proj_run_kernel<QUERY>;
+  PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
+  const int64_t mt = (S + tile - 1) / tile, items = mt * B * a->H * L::NN;
+  PITH_REQUIRE(items < 2147483647, "too many tokens, heads or sequences");
+  kern<<<static_cast<unsigned>(items < sms ? items : sms), L::kThreads, L::kAlloc, st>>>(
+      ta, tw, to, p, tile, static_cast<int>(mt), static_cast<int>(items), B * S);
+  PITH_CUDA(cudaGetLastError());
+  return kOk;
+}
+
 template <bool QUERY, int NT, int ST>
-static int launch_proj(const CUtensorMap& ta, const pith_latent_proj_args* a, const LatProjParams& p, int64_t B, int64_t S,
+static int launch_proj(const pith_latent_proj_args* a, const LatProjParams& p, int64_t B, int64_t S, const int64_t xs[3],
                        cudaStream_t st) {
   using L = ProjCfg<QUERY, NT, ST>;
-  constexpr int kIn = QUERY ? 576 : 128, NN = (QUERY ? 512 : 128) / NT;
-  CUtensorMap tw, to;
-  const int64_t ws[3] = {static_cast<int64_t>(a->H) * 256 * a->weight_stride, a->weight_stride, 512};
-  if (int rc = make_tensor_map(&tw, a->weight, 2, 1, static_cast<int64_t>(a->H) * 256, 1, 512, ws, 64, QUERY ? 64 : NT)) return rc;
-  const int64_t os[3] = {S * a->H * kIn, static_cast<int64_t>(a->H) * kIn, kIn};
-  if (int rc = make_tensor_map(&to, a->out, 2, B, S, a->H, kIn, os, 64, 128)) return rc;
+  constexpr int NN = (QUERY ? 512 : 128) / NT;
+  CUtensorMap ta, tw, to;
+  if (int rc = make_tensor_map(&ta, a->x, 2, B, S, a->H, QUERY ? 192 : 512, xs, 64, 128)) return rc;
+  if (int rc = proj_maps<QUERY>(a, B, S, QUERY ? 64 : NT, 128, &tw, &to)) return rc;
   auto kern = latent_proj_kernel<QUERY, NT, ST>;
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
   const int64_t mt = (S + 127) / 128;
@@ -286,8 +559,6 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
   if (S == 1) xs[1] = a->H * xs[2];
   if (B == 1) xs[0] = S * xs[1];
   PITH_REQUIRE(S < 2147483647 - 256, "too many tokens");
-  CUtensorMap ta;
-  if (int rc = make_tensor_map(&ta, a->x, 2, B, S, a->H, QUERY ? 192 : 512, xs, 64, 128)) return rc;
   LatProjParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->x);
   p.out = static_cast<__nv_bfloat16*>(a->out);
@@ -303,11 +574,11 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
   const int64_t tiles = (S + 127) / 128 * B * a->H;
   // narrow tiles while the wide ones would leave SMs without a CTA
   if constexpr (QUERY) {
-    if (tiles * 2 < sms) return launch_proj<true, 64, 2>(ta, a, p, B, S, st);
-    return launch_proj<true, 256, 2>(ta, a, p, B, S, st);
+    if (tiles * 2 < sms) return launch_proj<true, 64, 2>(a, p, B, S, xs, st);
+    return launch_proj_run<true>(a, p, B, S, xs, sms, st);
   } else {
-    if (tiles < sms) return launch_proj<false, 32, 8>(ta, a, p, B, S, st);
-    return launch_proj<false, 128, 3>(ta, a, p, B, S, st);
+    if (tiles < sms) return launch_proj<false, 32, 8>(a, p, B, S, xs, st);
+    return launch_proj_run<false>(a, p, B, S, xs, sms, st);
   }
 }
 
