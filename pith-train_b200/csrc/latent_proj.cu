@@ -35,7 +35,9 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                : "memory");
 }
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// All but the N newest groups of stores have read their shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void lat_load4(const void* base, int f32, int64_t off, float* f) {
   if (f32) {
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(ProjCfg<QUERY, NT, ST>::kThreads)
 #pragma unroll
     for (int i = 0; i < NT / 64; ++i) tma_store_4d(&tm_out, smem + i * 16384, nt * NT + i * 64, h, m0, b);
     tma_store_commit();
-    tma_store_wait_read();  // the shared memory may go once it has been read
+    tma_store_wait_read<0>();  // the shared memory may go once it has been read
   }
   if (*abort_flag != 0u) {  // let copies and MMAs still in flight drain before shared memory and TMEM are handed back
     const long long t0 = clock64();
@@ -426,35 +428,35 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
       const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
       mbar_wait(&acc_full[buf], (n >> 1) & 1, ctl, 0x800 + buf);
       tc_fence_after_sync();
-      if (t == 0) tma_store_wait_read();  // the previous item's staged result has been read
-      named_bar_sync(1, 128);
-#pragma unroll 2
-      for (int c = 0; c < NT / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tmem + lanes + buf * NT + c * 32, r);
+#pragma unroll 1
+      for (int q = 0; q < NT / 64; ++q) {  // 64 columns: staged, and on their way while the next ones are read
+        if (t == 0) tma_store_wait_read<NT / 64 - 1>();  // this part's previous contents have been read
+        named_bar_sync(1, 128);
+        uint8_t* dst = out + q * 16384 + t * 128;
+        uint32_t r[64];
+        tmem_ld32(tmem + lanes + buf * NT + q * 64, r);
+        tmem_ld32(tmem + lanes + buf * NT + q * 64 + 32, r + 32);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t* v = r + 8 * i;
-          const int ch = (c & 1) * 4 + i;
-          *reinterpret_cast<uint4*>(out + (c >> 1) * 16384 + t * 128 + (((ch ^ t) & 7) << 4)) =
+        for (int ch = 0; ch < 8; ++ch) {
+          const uint32_t* v = r + 8 * ch;
+          *reinterpret_cast<uint4*>(dst + (((ch ^ t) & 7) << 4)) =
               make_uint4(pack_bf16(__uint_as_float(v[0]), __uint_as_float(v[1])),
                          pack_bf16(__uint_as_float(v[2]), __uint_as_float(v[3])),
                          pack_bf16(__uint_as_float(v[4]), __uint_as_float(v[5])),
                          pack_bf16(__uint_as_float(v[6]), __uint_as_float(v[7])));
         }
+        fence_proxy_async_smem();
+        named_bar_sync(1, 128);
+        if (t == 0 && *abort_flag == 0u) {
+          tma_store_4d(&tm_out, out + q * 16384, nt * NT + q * 64, h, m0, b);
+          tma_store_commit();
+        }
       }
       tc_fence_before_sync();
       mbar_arrive(&acc_empty[buf]);
-      fence_proxy_async_smem();
-      named_bar_sync(1, 128);
-      if (t == 0 && *abort_flag == 0u) {
-#pragma unroll
-        for (int i = 0; i < NT / 64; ++i) tma_store_4d(&tm_out, out + i * 16384, nt * NT + i * 64, h, m0, b);
-        tma_store_commit();
-      }
     }
-    if (t == 0) tma_store_wait_read();
+    if (t == 0) tma_store_wait_read<0>();
   } else if (QUERY && warp >= 8) {
     // an equal share of the tokens, whatever the CTA's items: with the rotary part of its own (head, token) rows every head
     // read the tables again, and the kernel waited for these warps (33.7 us)
