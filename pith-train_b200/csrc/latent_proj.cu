@@ -316,7 +316,7 @@ template <bool QUERY>
 __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     latent_proj_run_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                            const __grid_constant__ CUtensorMap tm_out, const LatProjParams p, int tile, int mtiles, int items,
-                           int64_t tokens) {
+                           int per_group, int64_t tokens) {
   using L = RunCfg<QUERY>;
   constexpr int NT = L::NT, NN = L::NN, KB = L::KB, ST = L::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -331,9 +331,22 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
   volatile uint32_t* abort_flag = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const AbortCtl ctl{p.status, abort_flag};
-  // items [i0, i1): item = (group, token tile), group = (batch, head, column tile)
-  const int share = items / gridDim.x, more = items - share * static_cast<int>(gridDim.x), me = blockIdx.x;
-  int i0 = me * share + min(me, more), i1 = i0 + share + (me < more ? 1 : 0);
+  // Items i0, i0 + step, ... below i1; item = (group, token tile), group = (batch, head, column tile). With per_group CTAs
+  // for each group, neighbouring CTAs take the same token tile of different heads, so that the rows of a token, which lie
+  // together, are read and written at about the same time. Otherwise (more groups than CTAs) equal runs of items.
+  const int me = blockIdx.x, ctas = gridDim.x;
+  int i0, i1, step;
+  if (per_group > 0) {
+    const int groups = items / mtiles, g = me % groups;
+    i0 = g * mtiles + me / groups;
+    i1 = (g + 1) * mtiles;
+    step = per_group;
+  } else {
+    const int share = items / ctas, more = items - share * ctas;
+    i0 = me * share + min(me, more);
+    i1 = i0 + share + (me < more ? 1 : 0);
+    step = 1;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -360,7 +373,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     if (lane == 0) {
       uint32_t s = 0, ph = 1, bph = 1;
       int group = -1;
-      for (int it = i0; it < i1; ++it) {
+      for (int it = i0; it < i1; it += step) {
         const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
         const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
         if (g != group) {
@@ -392,8 +405,9 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     const uint64_t bd0 = make_smem_desc(smem_u32(smem), QUERY ? 8192 : 16, 1024);
     uint32_t s = 0, ph = 0, bph = 0;
     int group = -1;
-    for (int it = i0; it < i1; ++it) {
-      const uint32_t n = it - i0, buf = n & 1;
+    uint32_t n = 0;
+    for (int it = i0; it < i1; it += step, ++n) {
+      const uint32_t buf = n & 1;
       const int g = it / mtiles;
       if (g != group) {
         group = g;
@@ -415,15 +429,16 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
       }
       if (leader) {
         umma_commit(&acc_full[buf]);
-        if (it + 1 < i1 && (it + 1) / mtiles != g) umma_commit(b_empty);
+        if (it + step < i1 && (it + step) / mtiles != g) umma_commit(b_empty);
       }
     }
   } else if (warp >= 4 && warp < 8) {
     const int t = static_cast<int>(threadIdx.x) & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) << 5) << 16;
     uint8_t* out = smem + L::kOutOff;
-    for (int it = i0; it < i1; ++it) {
-      const uint32_t n = it - i0, buf = n & 1;
+    uint32_t n = 0;
+    for (int it = i0; it < i1; it += step, ++n) {
+      const uint32_t buf = n & 1;
       const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
       const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
       mbar_wait(&acc_full[buf], (n >> 1) & 1, ctl, 0x800 + buf);
@@ -491,12 +506,15 @@ template <bool QUERY>
 static int launch_proj_run(const pith_latent_proj_args* a, const LatProjParams& p, int64_t B, int64_t S, const int64_t xs[3],
                            int sms, cudaStream_t st) {
   using L = RunCfg<QUERY>;
-  // Tokens per tile, 64 to 128: what the CTA with the most tiles has to stream decides (4095 tokens x 16 heads: 592 output
-  // tiles of 112 are four rounds of 148 CTAs, 512 of 128 are also four). A tile costs about 8 tokens of its own.
+  const int64_t groups = B * a->H * L::NN;
+  const int per_group = groups <= sms ? static_cast<int>(sms / groups) : 0;
+  // Tokens per tile, 64 to 128: what the CTA with the most tiles has to stream decides (4095 tokens, nine CTAs a head: 36
+  // tiles of 114 are four rounds, 32 of 128 are also four). A tile costs about 8 tokens of its own.
   int tile = 128;
   int64_t best = -1;
-  for (int r = 128; r >= 64; r -= 8) {
-    const int64_t rounds = ((S + r - 1) / r * B * a->H * L::NN + sms - 1) / sms;
+  for (int r = 128; r >= 64; r -= 2) {
+    const int64_t mt = (S + r - 1) / r;
+    const int64_t rounds = per_group > 0 ? (mt + per_group - 1) / per_group : (mt * groups + sms - 1) / sms;
     if (best < 0 || rounds * (r + 8) < best) {
       best = rounds * (r + 8);
       tile = r;
@@ -507,10 +525,11 @@ static int launch_proj_run(const pith_latent_proj_args* a, const LatProjParams& 
   if (int rc = proj_maps<QUERY>(a, B, S, QUERY ? 64 : L::NT, tile, &tw, &to)) return rc;
   auto kern = latent_proj_run_kernel<QUERY>;
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
-  const int64_t mt = (S + tile - 1) / tile, items = mt * B * a->H * L::NN;
-  PITH_REQUIRE(items < 2147483647, "too many tokens, heads or sequences");
-  kern<<<static_cast<unsigned>(items < sms ? items : sms), L::kThreads, L::kAlloc, st>>>(
-      ta, tw, to, p, tile, static_cast<int>(mt), static_cast<int>(items), B * S);
+  const int64_t mt = (S + tile - 1) / tile, items = mt * groups;
+  PITH_REQUIRE(items < 2147483647 - 1024, "too many tokens, heads or sequences");
+  const int64_t ctas = per_group > 0 ? groups * per_group : items < sms ? items : sms;
+  kern<<<static_cast<unsigned>(ctas), L::kThreads, L::kAlloc, st>>>(ta, tw, to, p, tile, static_cast<int>(mt),
+                                                                   static_cast<int>(items), per_group, B * S);
   PITH_CUDA(cudaGetLastError());
   return kOk;
 }
