@@ -286,37 +286,33 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, 
   cp_async_wait_all();
 }
 
-// 8-bit: one warp's rows of the split query, a row per pass with the next one's loads in flight, 16 elements a lane (chunks
-// lane and lane + 32 of 8). `ready` waits until the previous piece has read its query. A rolled loop of one row: the code is
-// cold whenever it runs, and instruction fetches cost more than the arithmetic (16 rows unrolled: 20 000 cycles, four: 10 600).
-template <int NT, int WARPS, class Ready>
+// 8-bit: the split query. A warp's rows come as they are by asynchronous copies, all of them in flight at once, each into the
+// 1024 bytes that its two parts will take; then the warp converts row by row in place, 16 elements a lane (chunks lane and
+// lane + 32 of 8). Beside the key traffic a load takes thousands of cycles (three rows in flight: 10 000 for NT = 32), and a
+// rolled loop keeps the code small: it is cold whenever it runs (16 rows unrolled: 20 000 cycles).
+template <int NT, int WARPS>
 __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t* sq, float* qk, const LatEntry& x, int warp,
-                                                 int lane, Ready ready) {
-  constexpr int kDeep = 3;  // rows in flight
-  uint4 n[kDeep][3];
-  const auto fetch = [&](int row, uint4* to) {
-    const int r = x.r0 + row;
-    to[0] = to[1] = to[2] = make_uint4(0, 0, 0, 0);
-    if (row < NT && r < p.R) {
-      const int tok = r / p.H, h = r - tok * p.H;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2]) + lane;
-      to[0] = __ldg(src);
-      to[1] = __ldg(src + 32);
-      if (lane < 8) to[2] = __ldg(src + 64);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kDeep; ++i) fetch(warp + i * WARPS, n[i]);
-  ready();
+                                                 int lane) {
+  // part i (0 .. 7) of 128 bytes of row `row`: high parts of blocks 0 .. 3, then low parts
+  const auto piece = [&](int row, int i) { return sq + (i & 3) * (2 * NT * 128) + ((i >> 2) * NT + row) * 128; };
 #pragma unroll 1
   for (int row = warp; row < NT; row += WARPS) {
-    const uint32_t w[8] = {n[0][0].x, n[0][0].y, n[0][0].z, n[0][0].w, n[0][1].x, n[0][1].y, n[0][1].z, n[0][1].w};
-    if (lane < 8) *reinterpret_cast<uint4*>(sq + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4)) = n[0][2];
-#pragma unroll
-    for (int i = 0; i + 1 < kDeep; ++i)
-#pragma unroll
-      for (int j = 0; j < 3; ++j) n[i][j] = n[i + 1][j];
-    fetch(row + kDeep * WARPS, n[kDeep - 1]);
+    const int r = x.r0 + row, tok = r / p.H, h = r - tok * p.H;
+    const bool there = r < p.R;
+    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + lane * 8 : p.q;
+    const uint32_t n = there ? 16u : 0u;
+    cp_async16(smem_u32(piece(row, lane >> 3)) + (lane & 7) * 16, src, n);
+    cp_async16(smem_u32(piece(row, 4 + (lane >> 3))) + (lane & 7) * 16, src + (there ? 256 : 0), n);
+    if (lane < 8) cp_async16(smem_u32(sq) + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4), src + (there ? 512 : 0), n);
+  }
+  cp_async_wait_all();
+  __syncwarp();
+#pragma unroll 1
+  for (int row = warp; row < NT; row += WARPS) {
+    const uint4 a = *reinterpret_cast<const uint4*>(piece(row, lane >> 3) + (lane & 7) * 16);
+    const uint4 b = *reinterpret_cast<const uint4*>(piece(row, 4 + (lane >> 3)) + (lane & 7) * 16);
+    __syncwarp();
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     float top = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -336,10 +332,10 @@ __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t
       for (int j = 0; j < 4; ++j)
         split_e4m3x2(__uint_as_float(w[4 * i + j] << 16) * inv, __uint_as_float(w[4 * i + j] & 0xFFFF0000u) * inv, h[j], l[j]);
       const int ch = i * 32 + lane;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
-      uint8_t* d = sq + (ch >> 4) * (2 * NT * 128) + row * 128 + (((((ch & 15) >> 1) ^ row) & 7) << 4) + (ch & 1) * 8;
-      *reinterpret_cast<uint2*>(d) =
+      const int at = (((((ch & 15) >> 1) ^ row) & 7) << 4) + (ch & 1) * 8;
+      *reinterpret_cast<uint2*>(piece(row, ch >> 4) + at) =
           make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
-      *reinterpret_cast<uint2*>(d + NT * 128) =
+      *reinterpret_cast<uint2*>(piece(row, 4 + (ch >> 4)) + at) =
           make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
     }
   }
@@ -973,14 +969,9 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       const int tiles = walk.tiles();
       if (tiles > 0) {
         uint8_t* sq = smem + L::kQOff;
-        // the previous piece's last score GEMM has read its query
-        const auto ready = [&]() { mbar_wait(sm.q_empty(), q_phase, ctl, 0x380); };
-        if constexpr (FP8) {
-          load_split_query<NT, L::kLoadWarps>(p, sq, sm.qk(piece & 1), walk.x, loader, lane, ready);
-        } else {
-          ready();
-          load_query<NT>(p, sq, walk.x, loader * 32 + lane);
-        }
+        mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
+        if constexpr (FP8) load_split_query<NT, L::kLoadWarps>(p, sq, sm.qk(piece & 1), walk.x, loader, lane);
+        else load_query<NT>(p, sq, walk.x, loader * 32 + lane);
         q_phase ^= 1;
         fence_proxy_async_smem();
         mbar_arrive(sm.q_full());

@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(256) latent_write_kernel(const LatentWritePara
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < p.n;
        t += static_cast<int64_t>(gridDim.x) * 8) {
     const int64_t b = t / p.S, s = t - b * p.S;
+    // everything that does not depend on another load is requested first
     const int64_t slot = __ldg(p.slots + b * p.sls[0] + s * p.sls[1]);
-    if (slot < 0 || failed != 0u) continue;  // padding
     int64_t row = 0;
     if (p.pos != nullptr) row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
     const uint4* x = reinterpret_cast<const uint4*>(p.kv + b * p.kvs[0] + s * p.kvs[1]);
@@ -106,6 +106,9 @@ __global__ void __launch_bounds__(256) latent_write_kernel(const LatentWritePara
     float w[16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) load_f4<W32>(p.w, (i >> 1) * 256 + lane * 8 + (i & 1) * 4, w + 4 * i);
+    uint4 pe_raw = make_uint4(0, 0, 0, 0);
+    if (lane < 8) pe_raw = __ldg(reinterpret_cast<const uint4*>(p.pe + b * p.ps[0] + s * p.ps[1]) + lane);
+    if (slot < 0 || failed != 0u) continue;  // padding
     if (slot >= p.c.slots || (p.pos != nullptr && (row < 0 || row >= p.table_rows))) {
       if (lane == 0) report_index(p.status, slot >= p.c.slots ? kIdxSlot : kIdxPosition);
       continue;
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(256) latent_write_kernel(const LatentWritePara
       load_f4<CS32>(p.cos, cs + 32 + lane * 4, ch);
       load_f4<CS32>(p.sin, cs + lane * 4, sl);
       load_f4<CS32>(p.sin, cs + 32 + lane * 4, sh);
-      bf16x8(__ldg(reinterpret_cast<const uint4*>(p.pe + b * p.ps[0] + s * p.ps[1]) + lane), pe);
+      bf16x8(pe_raw, pe);
     }
     float f[16];
     bf16x8(x0, f);

@@ -453,7 +453,7 @@ def _enqueue(entry: str, args: bytes, idx: int, launches: int) -> None:
     """Calls an entry on the current stream of device `idx`, whichever device is current."""
     global launch_count
     fn = _lib.packed_entry(entry)
-    if torch.cuda.current_device() == idx:
+    if torch._C._cuda_getDevice() == idx:
         rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
