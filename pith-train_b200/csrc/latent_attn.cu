@@ -46,6 +46,7 @@ struct LatCfg {
   // Query loaders: warps 2 and 3, and two more behind the softmax warps where queries are converted and the register file
   // has room (at most three warps per scheduler).
   static constexpr int kLoadWarps = FP8 && NT == 16 ? 4 : 2;
+  static constexpr bool kHelp = FP8 && NT == 32;  // the softmax warps, idle then, help with a CTA's first query
   static constexpr int kThreads = 128 + 128 * G + (kLoadWarps - 2) * 32;
   static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
   static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
@@ -290,13 +291,13 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, 
 // 1024 bytes that its two parts will take; then the warp converts row by row in place, 16 elements a lane (chunks lane and
 // lane + 32 of 8). Beside the key traffic a load takes thousands of cycles (three rows in flight: 10 000 for NT = 32), and a
 // rolled loop keeps the code small: it is cold whenever it runs (16 rows unrolled: 20 000 cycles).
-template <int NT, int WARPS>
+template <int NT>
 __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t* sq, float* qk, const LatEntry& x, int warp,
-                                                 int lane) {
+                                                 int warps, int lane) {
   // part i (0 .. 7) of 128 bytes of row `row`: high parts of blocks 0 .. 3, then low parts
   const auto piece = [&](int row, int i) { return sq + (i & 3) * (2 * NT * 128) + ((i >> 2) * NT + row) * 128; };
 #pragma unroll 1
-  for (int row = warp; row < NT; row += WARPS) {
+  for (int row = warp; row < NT; row += warps) {
     const int r = x.r0 + row, tok = r / p.H, h = r - tok * p.H;
     const bool there = r < p.R;
     const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + lane * 8 : p.q;
@@ -307,8 +308,8 @@ __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t
   }
   cp_async_wait_all();
   __syncwarp();
-#pragma unroll 1
-  for (int row = warp; row < NT; row += WARPS) {
+#pragma unroll 2
+  for (int row = warp; row < NT; row += warps) {
     const uint4 a = *reinterpret_cast<const uint4*>(piece(row, lane >> 3) + (lane & 7) * 16);
     const uint4 b = *reinterpret_cast<const uint4*>(piece(row, 4 + (lane >> 3)) + (lane & 7) * 16);
     __syncwarp();
@@ -960,6 +961,14 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       }
     }
   } else if (warp >= 4 && warp < 4 + 4 * L::G) {
+    if constexpr (L::kHelp) {
+      LatWalk<NT> first = walk;
+      if (first.next(p) && first.tiles() > 0) {
+        load_split_query<NT>(p, smem + L::kQOff, sm.qk(0), first.x, L::kLoadWarps + warp - 4, L::kLoadWarps + 4 * L::G, lane);
+        fence_proxy_async_smem();
+        asm volatile("bar.arrive 4, %0;" ::"n"((L::kLoadWarps + 4 * L::G) * 32) : "memory");
+      }
+    }
     lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, (warp - 4) >> 2, static_cast<int>(threadIdx.x) & 127);
   } else {
     // ------------------------------------------------------------------ query loaders, one piece ahead
@@ -970,8 +979,13 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       if (tiles > 0) {
         uint8_t* sq = smem + L::kQOff;
         mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
-        if constexpr (FP8) load_split_query<NT, L::kLoadWarps>(p, sq, sm.qk(piece & 1), walk.x, loader, lane);
-        else load_query<NT>(p, sq, walk.x, loader * 32 + lane);
+        if constexpr (FP8) {
+          const bool help = L::kHelp && piece == 0;
+          load_split_query<NT>(p, sq, sm.qk(piece & 1), walk.x, loader, L::kLoadWarps + (help ? 4 * L::G : 0), lane);
+          if (help) named_bar_sync(4, (L::kLoadWarps + 4 * L::G) * 32);
+        } else {
+          load_query<NT>(p, sq, walk.x, loader * 32 + lane);
+        }
         q_phase ^= 1;
         fence_proxy_async_smem();
         mbar_arrive(sm.q_full());
