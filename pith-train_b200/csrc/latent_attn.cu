@@ -40,7 +40,7 @@ constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope 
 template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
-  static constexpr int kExtra = FP8 ? (NT == 16 ? 3 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);  // units that another piece costs a CTA
+  static constexpr int kExtra = FP8 ? (NT == 16 ? 4 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);  // units that another piece costs a CTA
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
   static constexpr int CW = NT / G;
   // Query loaders: warps 2 and 3, and two more behind the softmax warps where queries are converted and the register file
@@ -1008,8 +1008,9 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
 
 // Merge of a row tile that several CTAs worked on: out = sum_i 2^(ref_i - M) O_i / sum_i 2^(ref_i - M) l_i, in key order.
 // Block (j, four columns): the j-th entry that a CTA began and did not finish; there are at most as many as entries, and
-// one less than CTAs. A thread has one output dimension of the four columns: all 512 (SPLIT = 1: many entries, so few parts
-// each), or 128 of them with the parts dealt to four groups of threads (SPLIT = 4: a long context cut into many parts). The
+// one less than CTAs. A thread has one output dimension of the four columns, and the parts are dealt to SPLIT groups of
+// threads: 1 for many entries, which have few parts each, 4, or 16 for a long context cut into many parts (100 000 keys of one
+// sequence, 148 parts: 42 us with 4, 37 with 16; 16 sequences x 64 rows, 9 parts: 47 us with 1, 49.5 with 4, 68 with 16). The
 // launch is a programmatic one: it waits for the attention kernel's results in the kernel instead of before it.
 constexpr int kMergeThreads = 512;
 template <int NT, int SPLIT>
@@ -1019,7 +1020,8 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
   __shared__ int entry;
   __shared__ float4 wt[kMergeThreads];
   __shared__ float4 red[2][1];
-  __shared__ float4 acc_s[SPLIT == 4 ? 384 : 1];
+  constexpr int kGroup = kMergeThreads / SPLIT;
+  __shared__ float4 acc_s[SPLIT > 1 ? kMergeThreads : 1];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int c4 = blockIdx.y;  // columns [4 c4, 4 c4 + 4)
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1063,7 +1065,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
     }
   }
   __syncthreads();
-  const int g = SPLIT == 4 ? t >> 7 : 0, d = SPLIT == 4 ? blockIdx.z * 128 + (t & 127) : t;
+  const int g = t / kGroup, d = blockIdx.z * kGroup + t % kGroup;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int i = g; i < n; i += SPLIT) {
@@ -1071,13 +1073,13 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
     const float4 v = *(reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot_of(i)) * NT + 4 * c4) * kLat) + d);
     acc.x = fmaf(f.x, v.x, acc.x); acc.y = fmaf(f.y, v.y, acc.y); acc.z = fmaf(f.z, v.z, acc.z); acc.w = fmaf(f.w, v.w, acc.w);
   }
-  if (SPLIT == 4) {
-    if (g > 0) acc_s[t - 128] = acc;
+  if (SPLIT > 1) {
+    acc_s[t] = acc;
     __syncthreads();
     if (g > 0) return;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const float4 v = acc_s[i * 128 + t];
+    for (int i = 1; i < SPLIT; ++i) {
+      const float4 v = acc_s[i * kGroup + t];
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }
@@ -1131,8 +1133,8 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
     cudaLaunchConfig_t cfg = {};
     const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1);
     const unsigned cols = static_cast<unsigned>((p.R < NT ? p.R : NT) + 3) / 4;
-    const bool many = entries * 8 >= ctas;  // at most about nine parts an entry
-    cfg.gridDim = dim3(jobs, cols, many ? 1 : 4);
+    const int split = entries * 10 >= ctas ? 1 : entries * 32 >= ctas ? 4 : 16;  // by the parts of an entry
+    cfg.gridDim = dim3(jobs, cols, split);
     cfg.blockDim = dim3(kMergeThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -1140,7 +1142,7 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PITH_CUDA(cudaLaunchKernelEx(&cfg, many ? latent_merge_kernel<NT, 1> : latent_merge_kernel<NT, 4>,
+    PITH_CUDA(cudaLaunchKernelEx(&cfg, split == 1 ? latent_merge_kernel<NT, 1> : split == 4 ? latent_merge_kernel<NT, 4> : latent_merge_kernel<NT, 16>,
                                  static_cast<const LatAttnParams&>(p), ctas));
   }
   return kOk;
