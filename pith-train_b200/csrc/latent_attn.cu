@@ -67,7 +67,7 @@ struct LatCfg {
   static constexpr int kBars = 2 * NS + 10;
   static_assert(NS >= 4, "a tile's four latent slots must fit at once");
   static_assert(!FP8 || (kAhead == 4 && NS >= 9 && NS <= 12), "the 8-bit pipeline holds two tiles, and some");
-  static_assert(kBars * 8 + 16 + 48 + NT * 40 <= kMisc, "misc area too small");
+  static_assert(kBars % 2 == 0 && kBars * 8 + 16 + 48 + NT * 44 <= kMisc, "misc area too small");
   static_assert(kAlloc <= 232448, "shared memory");
   static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
 };
@@ -261,13 +261,14 @@ struct LatShared {
   __device__ uint64_t* o_full(uint32_t tile) const { return bars + L::kBars - 2 + (tile & 1); }  // its output GEMMs have completed
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
   __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 1); }             // [12 warps] + start
-  __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 10 NT words
+  __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 11 NT words
   __device__ float* ref() const { return cols(); }
   __device__ float* fac() const { return cols() + NT; }
   __device__ float* qk(int i) const { return cols() + (2 + i) * NT; }
   __device__ float* red(int g) const { return cols() + 4 * NT + g * 4 * L::CW; }  // [4 warps][CW]
   __device__ int* lim() const { return reinterpret_cast<int*>(cols() + 8 * NT); }
   __device__ int* tok() const { return reinterpret_cast<int*>(cols() + 9 * NT); }
+  __device__ float* nref() const { return cols() + 10 * NT; }  // minus ref()
 };
 
 // bf16: query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle), by 64
@@ -393,6 +394,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       // keys below the limit are visible; rows without a query are stored as zeros or not at all, whatever they see
       sm.lim()[c] = r >= p.R || tok >= x.nq ? 0x7FFFFFFF : p.tree != nullptr ? prefix : max(x.len - x.nq + tok + 1, 0);
       sm.ref()[c] = kNoRef;
+      sm.nref()[c] = -kNoRef;
     }
     named_bar_sync(3, 128 * L::G);
     int min_lim = 0x7FFFFFFF;
@@ -403,13 +405,18 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     float l[CW];
 #pragma unroll
     for (int c = 0; c < CW; ++c) l[c] = 0.f;
-    // score (log2) minus reference of four columns
+    // score (log2) minus reference of four columns, two to an instruction
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     const auto above = [&](const float* sc, int c, float lk, float* d) {
-      const float4 r = *reinterpret_cast<const float4*>(sm.ref() + cb + c);
-      d[0] = fmaf(sc[c], p.scale_log2, lk - r.x);
-      d[1] = fmaf(sc[c + 1], p.scale_log2, lk - r.y);
-      d[2] = fmaf(sc[c + 2], p.scale_log2, lk - r.z);
-      d[3] = fmaf(sc[c + 3], p.scale_log2, lk - r.w);
+      const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(sm.nref() + cb + c);
+      uint64_t r0 = r.x, r1 = r.y;
+      if (FP8) {
+        const uint64_t lk2 = f2_pack(lk, lk);
+        r0 = f2_add(r0, lk2);
+        r1 = f2_add(r1, lk2);
+      }
+      f2_unpack(f2_fma(f2_pack(sc[c], sc[c + 1]), scale2, r0), d[0], d[1]);
+      f2_unpack(f2_fma(f2_pack(sc[c + 2], sc[c + 3]), scale2, r1), d[2], d[3]);
     };
 
     for (int j = 0; j < tiles; ++j, ++tile) {
@@ -513,6 +520,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           const float* red = sm.red(g) + t;
           const float m = fmaxf(fmaxf(fmaxf(red[0], red[CW]), fmaxf(red[2 * CW], red[3 * CW])), old);
           sm.ref()[cb + t] = m;
+          sm.nref()[cb + t] = -m;
           sm.fac()[cb + t] = fast_exp2(old - m);
         }
         named_bar_sync(bar, 128);
@@ -555,8 +563,8 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
-            l[c0 + c] = fmaf(pw[c], iks, l[c0 + c]);
-            l[c0 + c + 1] = fmaf(pw[c + 1], iks, l[c0 + c + 1]);
+            f2_unpack(f2_fma(f2_pack(pw[c], pw[c + 1]), f2_pack(iks, iks), f2_pack(l[c0 + c], l[c0 + c + 1])), l[c0 + c],
+                      l[c0 + c + 1]);
             uint16_t h, r;
             split_e4m3x2(pw[c] * 16.f, pw[c + 1] * 16.f, h, r);
             hi[c >> 2] = (c & 2) ? hi[c >> 2] | (static_cast<uint32_t>(h) << 16) : h;
@@ -569,8 +577,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           uint32_t w2[8];
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
-            l[c0 + c] += pw[c];
-            l[c0 + c + 1] += pw[c + 1];
+            f2_unpack(f2_add(f2_pack(l[c0 + c], l[c0 + c + 1]), f2_pack(pw[c], pw[c + 1])), l[c0 + c], l[c0 + c + 1]);
             w2[c >> 1] = pack_bf16(pw[c], pw[c + 1]);
           }
           const int ch = (cb + c0) >> 3;
