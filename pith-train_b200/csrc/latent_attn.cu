@@ -32,7 +32,7 @@ namespace pith {
 
 constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
-constexpr int kUnit = 64;   // keys per unit of work
+constexpr int kBox = 64;    // rows of a TMA box at most
 constexpr int kMaxExtra = 8;
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
@@ -86,6 +86,7 @@ struct LatAttnParams {
   int4* part_info;    // [G]: entry continued from the previous CTA, entry begun and not finished, its slot
   uint32_t* status;
   int B, Sq, H, R, RT, pages, page_size, max_keys;
+  int unit;  // keys per unit of work
   float scale_log2;
   int64_t qs[3], table_stride, tree_stride[2], scale_stride[2];
 };
@@ -105,7 +106,7 @@ __device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
   x.keys = (x.r0 == 0 ? 0 : x.r0 / p.H) >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
   return x;
 }
-__device__ __forceinline__ int lat_units(int keys) { return max((keys + kUnit - 1) / kUnit, 1); }
+__device__ __forceinline__ int lat_units(const LatAttnParams& p, int keys) { return max((keys + p.unit - 1) / p.unit, 1); }
 
 // Walks the pieces of this CTA's share of the line. Every role keeps its own copy. An entry takes `extra` places of the line
 // in front of its units: what beginning another piece costs a CTA.
@@ -118,10 +119,10 @@ struct LatWalk {
   __device__ __forceinline__ bool next(const LatAttnParams& p) {
     while (left > 0) {
       x = lat_entry<NT>(p, e);
-      const int n = lat_units(x.keys) + extra;
+      const int n = lat_units(p, x.keys) + extra;
       const int take = min(n - off, left), u0 = max(off - extra, 0), u1 = off + take - extra;
-      k0 = u0 * kUnit;
-      k1 = min(x.keys, u1 * kUnit);
+      k0 = u0 * p.unit;
+      k1 = min(x.keys, u1 * p.unit);
       begins = u0 == 0;
       ends = off + take == n;
       left -= take;
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
   int mine = 0;
   for (int e = e_begin; e < e_end; ++e) {
     const LatEntry x = lat_entry<NT>(p, e);
-    mine += lat_units(x.keys);
+    mine += lat_units(p, x.keys);
     if (blockIdx.x == 0 && x.r0 == 0) {
       const int len = __ldg(p.lens + x.b);
       if (len < 0 || len > p.max_keys || (p.qlens != nullptr && (__ldg(p.qlens + x.b) < 0 || __ldg(p.qlens + x.b) > p.Sq)))
@@ -759,7 +760,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     if (u0 < u1 && at <= u0 && u0 < at + mine) {
       int e = e_begin;
       while (true) {
-        const int n = lat_units(lat_entry<NT>(p, e).keys) + extra;
+        const int n = lat_units(p, lat_entry<NT>(p, e).keys) + extra;
         if (u0 < at + n) break;
         at += n;
         ++e;
@@ -787,7 +788,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       tma_prefetch_desc(&tm_lat);
       tma_prefetch_desc(&tm_rope);
     }
-    const int box = min(p.page_size, kUnit);
+    const int box = min(p.page_size, kBox);
     uint32_t it = 0, tile = 0;
     while (walk.next(p)) {
       for (int j = 0; j < walk.tiles(); ++j, ++tile) {
@@ -1112,12 +1113,16 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
 // memory hold beside a whole 128-key tile.
 static int lat_rows(int64_t rows, bool fp8) { return rows <= 16 ? 16 : rows <= 32 || fp8 ? 32 : 64; }
 
+// Work is cut at multiples of 64 keys; where no sequence can pass one tile it is not cut at all (and needs no merge).
+static int lat_unit(int64_t max_keys) { return max_keys <= kTile ? kTile : 64; }
+
 static int lat_ctas(int64_t entries, int64_t max_keys, int* ctas) {
   int dev = 0, sms = 148;
   PITH_CUDA(cudaGetDevice(&dev));
   PITH_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   if (sms > kMergeThreads) sms = kMergeThreads;  // the merge looks at one CTA per thread
-  const int64_t units = entries * (max_keys <= kUnit ? 1 : (max_keys + kUnit - 1) / kUnit);
+  const int unit = lat_unit(max_keys);
+  const int64_t units = entries * (max_keys <= unit ? 1 : (max_keys + unit - 1) / unit);
   *ctas = static_cast<int>(units < sms ? units : sms);
   return kOk;
 }
@@ -1128,14 +1133,14 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   CUtensorMap tl, tr;
   const pith_latent_cache& c = a->cache;
   const int64_t ls[3] = {c.latent_stride[0], c.latent_stride[1], kLat}, rs[3] = {c.rope_stride[0], c.rope_stride[1], kRp};
-  const int box = c.page_size < kUnit ? c.page_size : kUnit;
+  const int box = c.page_size < kBox ? c.page_size : kBox;
   if (int rc = make_tensor_map(&tl, c.latent, FP8 ? 1 : 2, c.pages, c.page_size, 1, kLat, ls, FP8 ? 128 : 64, box)) return rc;
   if (int rc = make_tensor_map(&tr, c.rope, 2, c.pages, c.page_size, 1, kRp, rs, 64, box)) return rc;
   auto kern = latent_attn_kernel<NT, FP8>;
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
   kern<<<ctas, L::kThreads, L::kAlloc, st>>>(tl, tr, p);
   PITH_CUDA(cudaGetLastError());
-  if (p.max_keys > kUnit && ctas > 1) {  // an entry of one unit is never cut
+  if (p.max_keys > p.unit && ctas > 1) {  // an entry of one unit is never cut
     const int64_t entries = static_cast<int64_t>(p.B) * p.RT;
     cudaLaunchConfig_t cfg = {};
     const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1);
@@ -1184,7 +1189,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
   const int nt = lat_rows(rows, fp8);
   const int64_t rt = (rows + nt - 1) / nt;
-  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kUnit + 2 + kMaxExtra) < 2147483647 - 1024,
+  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / 64 + 2 + kMaxExtra) < 2147483647 - 1024,
                "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
   LatAttnParams p = {};
@@ -1196,6 +1201,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.B = a->B; p.Sq = a->Sq; p.H = a->H; p.R = static_cast<int>(rows); p.RT = static_cast<int>(rt);
   p.pages = a->cache.pages; p.page_size = a->cache.page_size;
   p.max_keys = a->table_cols * a->cache.page_size;
+  p.unit = lat_unit(p.max_keys);
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i];
   p.table_stride = a->table_stride;
