@@ -56,7 +56,7 @@ class LatentCache:
         for name, t in (("rope", rope), ("scale", scale)):
             if t is not None and t.device != latent.device:
                 raise ValueError(f"{name} is on {t.device}, latent on {latent.device}")
-        self.latent, self.rope, self.scale = latent, rope, scale
+        self._planes = (latent, rope, scale)
         # the fields of pith_latent_cache, in order
         self.flat = (latent.data_ptr(), rope.data_ptr(), scale.data_ptr() if scale is not None else 0,
                      _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, pages, page_size,
@@ -69,6 +69,18 @@ class LatentCache:
             if dtype == torch.float8_e4m3fn else None
         return cls(torch.zeros((num_pages, page_size, 512), dtype=dtype, device=device),
                    torch.zeros((num_pages, page_size, 64), dtype=torch.bfloat16, device=device), scale)
+
+    @property
+    def latent(self) -> torch.Tensor:
+        return self._planes[0]
+
+    @property
+    def rope(self) -> torch.Tensor:
+        return self._planes[1]
+
+    @property
+    def scale(self) -> torch.Tensor | None:
+        return self._planes[2]
 
     @property
     def num_pages(self) -> int:

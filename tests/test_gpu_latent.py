@@ -374,6 +374,37 @@ def test_a_key_that_is_not_finite_reaches_only_the_rows_that_see_it(cuda_device,
     assert torch.equal(o[:, :5], want[:, :5]) and o[:, 5].isnan().all()
 
 
+def test_a_row_factor_that_is_not_finite_reaches_only_the_rows_that_see_it(cuda_device):
+    g = torch.Generator(device="cuda").manual_seed(17)
+    S, H, lens = 4, 16, [300, 70]
+    for bad in (float("nan"), float("inf")):
+        cache, table = filled_cache(g, lens, 32, E4M3)
+        q = torch.randn(2, S, H, 576, generator=g, device="cuda").bfloat16()
+        want = assert_attention(q, cache, table, lens, SCALE)[0]
+        cache.scale.view(-1)[slots_of(table[0], 300, 32)[298]] = bad    # the third new token of the first sequence
+        o = run_attention(q, cache, table, lens, SCALE)[0]
+        check()
+        assert torch.equal(o[0, :2], want[0, :2]) and torch.equal(o[1], want[1]) and o[0, 2:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S", [1, 4])
+def test_a_query_that_is_not_finite_stays_in_its_row(cuda_device, dtype, S):
+    g = torch.Generator(device="cuda").manual_seed(18)
+    lens = [700, 64]
+    cache, table = filled_cache(g, lens, 64, dtype)
+    q = torch.randn(2, S, 16, 576, generator=g, device="cuda").bfloat16()
+    want = assert_attention(q, cache, table, lens, SCALE)[0]
+    bad = [(0, 0, 3, 17, "nan"), (0, S - 1, 5, 500, "inf"), (1, 0, 7, 570, "nan"), (1, S - 1, 8, 0, "-inf")]
+    hit = torch.zeros(2, S, 16, dtype=torch.bool, device="cuda")
+    for b, s, h, d, v in bad:
+        q[b, s, h, d] = float(v)
+        hit[b, s, h] = True
+    o = run_attention(q, cache, table, lens, SCALE)[0]
+    check()
+    assert torch.equal(o[~hit], want[~hit]) and o[hit].isnan().any(-1).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
 def test_attention_takes_strided_inputs_and_repeats_to_the_bit(cuda_device, dtype):
     from pithtrain_b200.operators.mla import LatentCache
@@ -650,3 +681,53 @@ def test_prompt_tokens_drafts_and_the_expanded_form(cuda_device, dtype):
     got = mla.MLA(H, 192, 128, SCALE)(query, key, kv[..., 128:].contiguous())
     check()
     close_to(got[0], torch.cat(results[b])[:n].double(), torch.bfloat16, "expanded over the cache")
+
+
+def test_a_captured_decoding_step_is_the_eager_one(cuda_device):
+    """All five operators of a step in one graph, replayed for several tokens with new contents in the same tensors."""
+    from pithtrain_b200.operators import mla
+    g = torch.Generator(device="cuda").manual_seed(40)
+    H, page, B = 16, 64, 3
+    layer = Layer(g, H)
+    lens0 = [200, 5, 63]
+    caches = []
+    for _ in range(2):
+        gen = torch.Generator(device="cuda").manual_seed(41)
+        caches.append(filled_cache(gen, [n + 8 for n in lens0], page, E4M3))
+    table = caches[0][1]
+    q = torch.empty(B, 1, H, 192, dtype=torch.bfloat16, device="cuda")
+    proj = torch.empty(B, 1, 576, dtype=torch.bfloat16, device="cuda")
+    slots, pos = torch.zeros(B, 1, dtype=torch.int64, device="cuda"), torch.zeros(B, 1, dtype=torch.int64, device="cuda")
+    lens = torch.zeros(B, dtype=torch.int32, device="cuda")
+
+    def step(cache):
+        mla.latent_cache_write(cache, slots, proj[..., :512], proj[..., 512:], layer.norm, layer.cos, layer.sin, 1e-6,
+                               position_ids=pos)
+        query = mla.latent_query(q, layer.kv_b, layer.cos, layer.sin, position_ids=pos)
+        latent, pe = mla.latent_cache_read(cache, slots)
+        return mla.latent_output(mla.latent_attention(query, cache, table, lens, SCALE), layer.kv_b), latent, pe
+
+    def fill(i):
+        n = torch.tensor([v + i for v in lens0], device="cuda")
+        pos.copy_(n[:, None])
+        lens.copy_(n + 1)
+        slots.copy_(torch.gather(table.long(), 1, (n // page)[:, None]) * page + (n % page)[:, None])
+        gen = torch.Generator(device="cuda").manual_seed(50 + i)
+        q.copy_(torch.randn(q.shape, generator=gen, device="cuda"))
+        proj.copy_(torch.randn(proj.shape, generator=gen, device="cuda"))
+
+    fill(0)
+    step(caches[0][0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(caches[0][0])
+    for i in range(6):
+        fill(i)
+        graph.replay()
+        want = step(caches[1][0])
+        check()
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+    for a, b in zip((caches[0][0].latent, caches[0][0].rope), (caches[1][0].latent, caches[1][0].rope)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
