@@ -22,7 +22,8 @@
  *    (a zero-initialised device uint32, optional) as (code << 24 | detail); see pith_status_string.
  *    Codes: 1 a barrier wait inside a kernel ran out, 2 unexpected TMEM allocation, 3 a wait for a ring neighbour
  *    ran out, 4 a kernel found its shared-memory window misaligned, 5 a slot, page, length or position given to a
- *    latent-cache entry was out of range (nothing outside the tensors is touched). A launch that finds the word non-zero does no work.
+ *    latent-cache entry was out of range (nothing outside the tensors is touched). A launch that finds the word non-zero
+ *    does no work.
  *  - Re-entrant; no internal threads; no global mutable state besides, per device, one side stream with two
  *    events used by pith_attn_bwd (created on first use) and the device address of the scratch area of
  *    pith_attn_bwd_noalloc (looked up on its first call; it does not survive cudaDeviceReset).
@@ -63,7 +64,7 @@ extern "C" {
 /* flags for pith_combine_args.flags */
 #define PITH_COMBINE_NATURAL 1u   /* LSEs are natural-log (standard.py) instead of log2 (mla.py) */
 
-/* element types for pith_combine_args.out*_dtype */
+/* element types */
 #define PITH_DTYPE_BF16 0
 #define PITH_DTYPE_F32 1
 #define PITH_DTYPE_E4M3 2 /* pith_latent_cache.dtype only */

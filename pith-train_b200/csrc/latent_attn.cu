@@ -43,7 +43,7 @@ namespace pith {
 
 constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
-constexpr int kBox = 64;    // rows of a TMA box at most
+constexpr int kBox = 64;    // rows of a TMA box at most; work is cut at its multiples
 constexpr int kMaxExtra = 8;
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
@@ -51,7 +51,10 @@ constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope 
 template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
-  static constexpr int kExtra = FP8 ? (NT == 16 ? 4 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);  // units that another piece costs a CTA
+  // Units of 64 keys that beginning another piece costs a CTA: what its epilogue, its query and the empty pipeline take
+  // (about 4 us at NT = 16, 9 us at 64), over the time of a unit. Half or twice as much changes ragged batches by 2 %.
+  static constexpr int kExtra = FP8 ? (NT == 16 ? 4 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);
+  static_assert(kExtra <= kMaxExtra, "the host checks the line's length with kMaxExtra");
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
   static constexpr int CW = NT / G;
   // Query loaders: warps 2 and 3, and two more behind the softmax warps where queries are converted and the register file
@@ -173,12 +176,6 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* r) {
 #pragma unroll
   for (int i = 0; i < N / 32; ++i) tmem_ld32(addr + 32 * i, r + 32 * i);
 }
-template <int N>
-__device__ __forceinline__ void tmem_st_cols(uint32_t addr, const uint32_t* r) {
-  if (N == 16) tmem_st16(addr, r);
-#pragma unroll
-  for (int i = 0; i < N / 32; ++i) tmem_st32(addr + 32 * i, r + 32 * i);
-}
 __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, bool pred) {
   uint32_t r;
   asm volatile(
@@ -270,7 +267,7 @@ struct LatShared {
   __device__ uint64_t* s_full(int i) const { return bars + L::kBars - 6 + i; }
   // One for even and one for odd tiles each: a softmax warpgroup may be a tile ahead of the other, and of the output GEMM.
   __device__ uint64_t* p_full(uint32_t tile) const { return bars + L::kBars - 4 + (tile & 1); }
-  __device__ uint64_t* o_full(uint32_t tile) const { return bars + L::kBars - 2 + (tile & 1); }  // its output GEMMs have completed
+  __device__ uint64_t* o_full(uint32_t tile) const { return bars + L::kBars - 2 + (tile & 1); }  // its output GEMM is complete
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
   __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 1); }             // [12 warps] + start
   __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 11 NT words
@@ -1131,8 +1128,8 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
 // memory hold beside a whole 128-key tile.
 static int lat_rows(int64_t rows, bool fp8) { return rows <= 16 ? 16 : rows <= 32 || fp8 ? 32 : 64; }
 
-// Work is cut at multiples of 64 keys; where no sequence can pass one tile it is not cut at all (and needs no merge).
-static int lat_unit(int64_t max_keys) { return max_keys <= kTile ? kTile : 64; }
+// Keys per unit of work: 64; where no sequence can pass one tile, a tile, so that nothing is cut and nothing merged.
+static int lat_unit(int64_t max_keys) { return max_keys <= kTile ? kTile : kBox; }
 
 static int lat_ctas(int64_t entries, int64_t max_keys, int* ctas) {
   int dev = 0, sms = 148;
@@ -1172,8 +1169,8 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PITH_CUDA(cudaLaunchKernelEx(&cfg, split == 1 ? latent_merge_kernel<NT, 1> : split == 4 ? latent_merge_kernel<NT, 4> : latent_merge_kernel<NT, 16>,
-                                 static_cast<const LatAttnParams&>(p), ctas));
+    auto merge = split == 1 ? latent_merge_kernel<NT, 1> : split == 4 ? latent_merge_kernel<NT, 4> : latent_merge_kernel<NT, 16>;
+    PITH_CUDA(cudaLaunchKernelEx(&cfg, merge, static_cast<const LatAttnParams&>(p), ctas));
   }
   return kOk;
 }
@@ -1207,7 +1204,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   const bool fp8 = a->cache.dtype == PITH_DTYPE_E4M3;
   const int nt = lat_rows(rows, fp8);
   const int64_t rt = (rows + nt - 1) / nt;
-  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / 64 + 2 + kMaxExtra) < 2147483647 - 1024,
+  PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kBox + 2 + kMaxExtra) < 2147483647 - 1024,
                "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
   LatAttnParams p = {};

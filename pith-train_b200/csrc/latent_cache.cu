@@ -7,6 +7,9 @@
 // One warp per token: a lane holds 16 of the 512 values (two 16-byte loads, 512 contiguous bytes a warp instruction), the
 // row sum and maximum are five shuffles each, lanes 0-7 rotate 8 inputs into 4 + 4 outputs on their own. All loads of a
 // token are issued before the first use; the kernels are bound by HBM at prompt sizes and by the launch at decode sizes.
+// Measured: 64 tokens 2.3 us; 8191 tokens into an 8-bit cache 7 us, back out of it 6 us (one token a warp, so that two
+// dependent loads and the launch are most of it); 32768 rows of a bf16 cache 12.8 us = 5.9 TB/s, 0.92 of the measured copy
+// rate.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
 #include "host_common.h"

@@ -4,11 +4,12 @@
 //            out[t][h][512:576] = rotary embedding of q[t][h][128:192]
 //   output:  out[t][h][v]       = sum_r a[t][h][r] W[h*256+128+v, r]          (K = 512, N = 128)
 //
-// W is used as the layer holds it: the query's B operand is read MN-major, the output's K-major. One CTA makes a tile of
-// 128 tokens of one head with tcgen05 (accumulators in TMEM) and stores it by TMA, which clips the rows behind the last
-// token. Both are bound by HBM at prompt sizes (a row moves 1.5 KB / 1.3 KB for 131 kFLOP) and by latency at decode sizes;
-// two CTAs share an SM, so one tile's loads run under the other's MMAs and stores. Few tokens take narrower tiles: more
-// CTAs then share the reading of W.
+// W is used as the layer holds it: the query's B operand is read MN-major, the output's K-major; tcgen05 with accumulators in
+// TMEM, results stored by TMA, which clips the rows behind the last token. A row moves 1.5 KB (query) or 1.3 KB (output) for
+// 131 kFLOP: HBM bounds both at prompt sizes, latency at decode sizes, where narrow tiles spread the reading of W over more
+// CTAs (a kernel of one tile per CTA). Measured, 16 heads: 32 tokens 3.6 us (query) and 4.4 us (output); 4095 tokens 22.7 us
+// = 4.5 TB/s (0.70 of the measured copy rate) and 18.7 us = 4.6 TB/s (0.71), of which the launch, W and the first tile
+// take about 4 us.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
 #include "host_common.h"
