@@ -52,7 +52,8 @@ template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
   // Units of 64 keys that beginning another piece costs a CTA: what its epilogue, its query and the empty pipeline take
-  // (about 4 us at NT = 16, 9 us at 64), over the time of a unit. Half or twice as much changes ragged batches by 2 %.
+  // over the time of a unit. Half as much made 16 trees of 13 tokens 4 (bf16) and 17 % (8-bit) and 128 short sequences 4 %
+  // slower; twice as much changes every batch by less than 5 %, either way.
   static constexpr int kExtra = FP8 ? (NT == 16 ? 4 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);
   static_assert(kExtra <= kMaxExtra, "the host checks the line's length with kMaxExtra");
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
@@ -204,8 +205,12 @@ __device__ __forceinline__ void split_e4m3x2(float a, float b, uint16_t& hi, uin
       : "=&h"(hi), "=h"(lo) : "f"(a), "f"(b));
 }
 
-// A value that is the same in all lanes, in a form the compiler knows to be so (descriptors then stay in uniform registers).
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
+// Adds a byte offset to the address field of a descriptor. The address never carries out of the lower word, and said so the
+// upper word stays the constant that it is: half the moves in front of every MMA.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) {
+  const uint32_t lo = static_cast<uint32_t>(desc) + (bytes >> 4), hi = static_cast<uint32_t>(desc >> 32);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t smem_dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(bytes) : "memory");
@@ -683,7 +688,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
   if (g == 0 && t == 0) p.part_info[blockIdx.x] = info;
 }
 
-__device__ __forceinline__ bool mbar_test_all(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t"
@@ -694,7 +699,7 @@ __device__ __forceinline__ bool mbar_test_all(uint64_t* bar, uint32_t parity) {
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
-  return __all_sync(0xFFFFFFFFu, ok != 0);
+  return ok != 0;
 }
 
 template <int NT, bool FP8>
@@ -806,14 +811,16 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     const int box = min(p.page_size, kBox);
     uint32_t it = 0, tile = 0;
     while (walk.next(p)) {
+      const int32_t* table = p.table + walk.x.b * p.table_stride;
+      int next_page = 0;  // of the next tile, read a tile ahead
+      if (walk.k0 + lane * box < walk.k1 && lane * box < kTile) next_page = __ldg(table + (walk.k0 + lane * box) / p.page_size);
       for (int j = 0; j < walk.tiles(); ++j, ++tile) {
         const int n0 = walk.k0 + j * kTile;
         const int boxes = (min(kTile, walk.k1 - n0) + box - 1) / box;
-        int page = 0, row = 0;
+        int page = next_page, row = 0;
+        if (n0 + kTile + lane * box < walk.k1 && lane * box < kTile) next_page = __ldg(table + (n0 + kTile + lane * box) / p.page_size);
         if (lane < boxes) {
-          const int n = n0 + lane * box;
-          page = __ldg(p.table + walk.x.b * p.table_stride + n / p.page_size);
-          row = n % p.page_size;
+          row = (n0 + lane * box) % p.page_size;
           if (page < 0 || page >= p.pages) {
             if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPage);
             page = 0;
@@ -843,141 +850,109 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer
-    const bool leader = elect_one();
-    constexpr uint32_t id_rope = make_idesc_bf16(128, NT, false, false);
-    constexpr uint32_t id_qk = FP8 ? make_idesc_e4m3(128, L::NC, false) : id_rope;
-    constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, true);
-    const uint64_t q_desc = make_smem_desc(smem_u32(smem + L::kQOff), 16, 1024);
-    const uint64_t qr_desc = make_smem_desc(smem_u32(smem + L::kQOff + L::kQLat), 16, 1024);
-    const uint64_t p_desc = make_row_desc(smem_u32(smem + L::kPOff), L::kPRow);
-    const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
-    const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
-    const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
-    uint32_t ks = 0, kph = 0;       // slot and phase of the next score GEMM step
-    uint32_t vs = 0;                // slot of the next output GEMM step
-    uint32_t tile = 0, q_phase = 0;
-    // Steps of the score GEMM of tile `number`: 128 latent dimensions each, then the rope part.
-    // (the descriptor of the slot is formed before the wait for it)
-    const auto step_desc = [&](int i) { return desc_advance(k_desc, L::NS == 4 ? i * L::kSlot : uniform(ks) * L::kSlot); };
-    const auto latent_step = [&](auto step, uint32_t number, uint64_t kd) {
-      constexpr int i = decltype(step)::value;
-      const uint32_t d = tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
-      tc_fence_after_sync();
-      if (FP8) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (leader)
-            umma_ss_f8(d, desc_advance(kd, k * 32), desc_advance(q_desc, i * (2 * NT * 128) + k * 32), id_qk,
-                       (i > 0 || k > 0) ? 1u : 0u);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (leader)
-            umma_ss(d, desc_advance(kd, (k >> 2) * 16384 + (k & 3) * 32),
-                    desc_advance(q_desc, (2 * i + (k >> 2)) * (NT * 128) + (k & 3) * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
-      }
-      if (++ks == L::NS) { ks = 0; kph ^= 1; }
-    };
-    const auto rope_step = [&](uint32_t number) {
-      const uint32_t d = FP8 ? tmem + kColR + (number & 1) * NT : tmem + kColS + (L::kAhead > 0 ? (number & 1) * L::NC : 0);
-      tc_fence_after_sync();
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (leader) umma_ss(d, desc_advance(r_desc, k * 32), desc_advance(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
-      if (leader) {
-        umma_commit(sm.s_full(L::kAhead > 0 ? number & 1 : 0));
-        if (FP8) umma_commit(sm.rempty());
-      }
-    };
-    // Whether `bar` completes before this tile's weights are there (then its output GEMM goes first).
-    const auto arrives_first = [&](uint64_t* bar, uint32_t parity, uint32_t number) {
-      const long long t0 = clock64();
-      for (uint32_t polls = 1;; ++polls) {
-        if (mbar_test_all(bar, parity)) return true;
-        if (mbar_test_all(sm.p_full(number), (number >> 1) & 1)) return false;
-        if ((polls & 31u) == 0u && clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
-      }
-    };
-    while (__any_sync(0xFFFFFFFFu, walk.next(p))) {
-      const int tiles = uniform(walk.tiles()), keys = uniform(walk.k1 - walk.k0);
-      if (tiles > 0) {
-        mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
-        q_phase ^= 1;
-      }
-      int done = 0;  // score steps of tile j that were issued ahead
-      for (int j = 0; j < tiles; ++j, ++tile) {
-        const auto blocking_step = [&](auto step) {
-          if (done <= decltype(step)::value) {
-            const uint64_t kd = step_desc(decltype(step)::value);
-            mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
-            latent_step(step, tile, kd);
-          }
-        };
-        blocking_step(Int<0>());
-        blocking_step(Int<1>());
-        blocking_step(Int<2>());
-        blocking_step(Int<3>());
-        if (done < 5) {
-          mbar_wait(sm.rfull(), tile & 1, ctl, 0x500);
-          rope_step(tile);
-        }
-        if (j + 1 == tiles && leader) umma_commit(sm.q_empty());
-        done = 0;
-        if (L::kAhead > 0 && j + 1 < tiles) {
-          // While this tile's softmax runs: the next tile's score GEMM, as far as its slots have arrived.
-          const auto early_step = [&](auto step) {
-            constexpr int i = decltype(step)::value;
-            if (i < L::kAhead && done == i) {
-              const uint64_t kd = step_desc(i);
-              if (arrives_first(sm.full(ks), kph, tile)) {
-                latent_step(step, tile + 1, kd);
-                done = i + 1;
-              }
-            }
-          };
-          early_step(Int<0>());
-          early_step(Int<1>());
-          early_step(Int<2>());
-          early_step(Int<3>());
-          if (FP8 && done == 4 && arrives_first(sm.rfull(), (tile + 1) & 1, tile)) {
-            rope_step(tile + 1);
-            done = 5;
-          }
-        }
-        uint64_t vd[4];
-        uint32_t slot[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          slot[i] = L::NS == 4 ? i : uniform(vs);
-          vd[i] = desc_advance(v_desc, slot[i] * L::kSlot);
-          if (++vs == L::NS) vs = 0;
-        }
-        const uint64_t pd = FP8 ? desc_advance(p_desc, uniform(tile & 1) * L::kP) : p_desc;
-        const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
-        mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
+    // ------------------------------------------------------------------ MMA issuer, one thread
+    // An MMA of these sizes takes 40 to 65 cycles, no longer than a warp needs to form its descriptors and agree on a lane, so
+    // one thread does all of this (with a warp that waits together and a lane that issues: 3 % slower, 8-bit trees alike).
+    // The steps of the score GEMM are a rolled loop: their code runs once a tile between that of the softmax warps, and every
+    // jump over an unrolled copy waited for the instruction cache (900 cycles a tile).
+    if (elect_one()) {
+      constexpr uint32_t id_rope = make_idesc_bf16(128, NT, false, false);
+      constexpr uint32_t id_qk = FP8 ? make_idesc_e4m3(128, L::NC, false) : id_rope;
+      constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, true);
+      const uint64_t q_desc = make_smem_desc(smem_u32(smem + L::kQOff), 16, 1024);
+      const uint64_t qr_desc = make_smem_desc(smem_u32(smem + L::kQOff + L::kQLat), 16, 1024);
+      const uint64_t p_desc = make_row_desc(smem_u32(smem + L::kPOff), L::kPRow);
+      const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
+      const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
+      const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
+      uint32_t ks = 0, kph = 0;       // slot and phase of the next score GEMM step
+      uint32_t vs = 0;                // slot of the next output GEMM step
+      uint32_t tile = 0, q_phase = 0;
+      // Step i of the score GEMM of tile `number`: 128 latent dimensions (i < 4), or the rope part.
+      const auto score_step = [&](int i, uint32_t number) {
+        const uint32_t buf = L::kAhead > 0 ? number & 1 : 0;
         tc_fence_after_sync();
-        const auto output_gemm = [&](auto all) {  // the last tile of a piece may need fewer steps of keys
+        if (i < 4) {
+          const uint32_t d = tmem + kColS + buf * L::NC;
+          const uint64_t kd = desc_at(k_desc, ks * L::kSlot), qd = desc_at(q_desc, i * (2 * NT * 128));
+          if (FP8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+            for (int k = 0; k < 4; ++k)
+              umma_ss_f8(d, desc_at(kd, k * 32), desc_at(qd, k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_ss(d, desc_at(kd, (k >> 2) * 16384 + (k & 3) * 32), desc_at(qd, (k >> 2) * (NT * 128) + (k & 3) * 32),
+                      id_qk, (i > 0 || k > 0) ? 1u : 0u);
+          }
+          if (++ks == L::NS) { ks = 0; kph ^= 1; }
+        } else {
+          const uint32_t d = FP8 ? tmem + kColR + buf * NT : tmem + kColS + buf * L::NC;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_ss(d, desc_at(r_desc, k * 32), desc_at(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
+          umma_commit(sm.s_full(buf));
+          if (FP8) umma_commit(sm.rempty());
+        }
+      };
+      // Whether `bar` completes before the weights of tile `number` are there (then their output GEMM goes first).
+      const auto arrives_first = [&](uint64_t* bar, uint32_t parity, uint32_t number) {
+        const long long t0 = clock64();
+        for (uint32_t polls = 1;; ++polls) {
+          if (mbar_test(bar, parity)) return true;
+          if (mbar_test(sm.p_full(number), (number >> 1) & 1)) return false;
+          if ((polls & 31u) == 0u && clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
+        }
+      };
+      while (walk.next(p)) {
+        const int tiles = walk.tiles(), keys = walk.k1 - walk.k0;
+        if (tiles > 0) {
+          mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
+          q_phase ^= 1;
+        }
+        int done = 0;  // score steps of tile j that were issued ahead
+        for (int j = 0; j < tiles; ++j, ++tile) {
+          // The rest of this tile's score GEMM; then, while its softmax runs, the next tile's as far as its slots have arrived.
+          int q = done;
+          const int last = j + 1 < tiles ? 5 + (FP8 ? 5 : L::kAhead) : 5;
+#pragma unroll 1
+          for (; q < last; ++q) {
+            const bool ahead = q >= 5;
+            const int i = ahead ? q - 5 : q;
+            const uint32_t number = tile + (ahead ? 1u : 0u);
+            uint64_t* bar = i < 4 ? sm.full(ks) : sm.rfull();
+            const uint32_t parity = i < 4 ? kph : number & 1;
+            if (!ahead) mbar_wait(bar, parity, ctl, i < 4 ? 0x400 + ks : 0x500);
+            else if (!arrives_first(bar, parity, tile)) break;
+            score_step(i, number);
+          }
+          done = max(q - 5, 0);
+          if (j + 1 == tiles) umma_commit(sm.q_empty());
+          const uint64_t pd = FP8 ? desc_at(p_desc, (tile & 1) * L::kP) : p_desc;
+          const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
+          mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
+          tc_fence_after_sync();
+          const auto output_gemm = [&](auto all) {
             constexpr int kSteps = FP8 ? 4 : 8;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-              if (leader && (decltype(all)::value != 0 || k < steps)) {
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t slot = L::NS == 4 ? i : vs;
+              if (++vs == L::NS) vs = 0;
+              const uint64_t vd = desc_at(v_desc, slot * L::kSlot);
+#pragma unroll(decltype(all)::value ? kSteps : 1)
+              for (int k = 0; k < (decltype(all)::value ? kSteps : steps); ++k) {
                 if (FP8)
-                  umma_ss_f8(tmem + i * L::NC, desc_advance(vd[i], k * 4096), desc_advance(pd, k * 32 * L::kPRow), id_pv,
+                  umma_ss_f8(tmem + i * L::NC, desc_at(vd, k * 4096), desc_at(pd, k * 32 * L::kPRow), id_pv,
                              (j > 0 || k > 0) ? 1u : 0u);
                 else
-                  umma_ss(tmem + i * L::NC, desc_advance(vd[i], k * 2048), desc_advance(pd, k * 16 * L::kPRow),
-                          id_pv, (j > 0 || k > 0) ? 1u : 0u);
+                  umma_ss(tmem + i * L::NC, desc_at(vd, k * 2048), desc_at(pd, k * 16 * L::kPRow), id_pv,
+                          (j > 0 || k > 0) ? 1u : 0u);
               }
+              umma_commit(sm.empty(slot));
             }
-            if (leader) umma_commit(sm.empty(slot[i]));
-          }
-        };
-        if (steps == (FP8 ? 4 : 8)) output_gemm(Int<1>());
-        else output_gemm(Int<0>());
-        if (leader) {
+          };
+          if (steps == (FP8 ? 4 : 8)) output_gemm(Int<1>());
+          else output_gemm(Int<0>());  // the last tile of a piece may need fewer steps of keys
           if (!FP8) umma_commit(sm.rempty());
           umma_commit(sm.o_full(tile));
         }
