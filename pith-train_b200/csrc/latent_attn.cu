@@ -24,8 +24,9 @@
 // covers a row tile completely stores its result; the others store an fp32 partial (O, ref, l), at most two per CTA, and
 // the merge kernel adds them in key order.
 //
-// Roles: warp 0 TMA producer (one lane per page), warp 1 MMA issuer, warps 2 and 3 query loaders (two more for NT = 16,
-// 8-bit), one or two warpgroups softmax and epilogue (thread = key, then = output dimension). The running maximum is moved
+// Roles: warp 0 TMA producer (one lane per page), warp 1 issues the score GEMMs, warp 2 the output GEMMs, warp 3 loads
+// queries (with one or three more for NT = 16), one or two warpgroups softmax and epilogue (thread = key, then = output
+// dimension). The running maximum is moved
 // only when a score exceeds the reference by more than 2^8 (8-bit: 2^4), decided by one barrier reduction per tile. The
 // score GEMM of the next tile runs under this tile's softmax as far as the ring of latent slots holds it: completely with
 // an 8-bit cache, two of four slots at NT = 16, none at NT = 64, whose query and tile fill the shared memory.
@@ -45,6 +46,7 @@ constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
 constexpr int kBox = 64;    // rows of a TMA box at most; work is cut at its multiples
 constexpr int kMaxExtra = 8;
+constexpr int kOwnRows = 8;  // query rows that the loader converts where the softmax warps do the others
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
 
@@ -58,11 +60,11 @@ struct LatCfg {
   static_assert(kExtra <= kMaxExtra, "the host checks the line's length with kMaxExtra");
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
   static constexpr int CW = NT / G;
-  // Query loaders: warps 2 and 3, and two more behind the softmax warps where queries are converted and the register file
-  // has room (at most three warps per scheduler).
-  static constexpr int kLoadWarps = FP8 && NT == 16 ? 4 : 2;
-  static constexpr bool kHelp = FP8 && NT == 32;  // the softmax warps, idle then, help with a CTA's first query
-  static constexpr int kThreads = 128 + 128 * G + (kLoadWarps - 2) * 32;
+  // Query loaders: warp 3, and more behind the softmax warps where the register file has room for them (at most three warps
+  // per scheduler).
+  static constexpr int kLoadWarps = NT > 16 ? 1 : FP8 ? 4 : 2;
+  static constexpr bool kHelp = FP8 && NT == 32;  // the softmax warps convert the rows behind the first eight of a query
+  static constexpr int kThreads = 128 + 128 * G + (kLoadWarps - 1) * 32;
   static constexpr int kSlot = FP8 ? 16384 : 32768;      // 128 keys x 128 dims of the latent plane
   static constexpr int kQLat = NT * 1024;                // bf16: 8 blocks [NT][64]; 8-bit: 4 blocks [hi, lo][NT][128]
   static constexpr int kQ = kQLat + NT * 128;
@@ -72,8 +74,7 @@ struct LatCfg {
   // bf16: P overlays the rope tile, which the score GEMM has finished with when P is written; 8-bit: two buffers
   static constexpr int kFixed = 16384 + kQ + (FP8 ? 2 * kP : 0) + kMisc;
   static constexpr int NS = (232448 - kFixed) / kSlot;
-  // Slots of the next tile whose score GEMM may run before this tile's output GEMM: what the ring holds beyond one tile.
-  static constexpr int kAhead = NS >= 8 ? 4 : NS - 4;
+  static constexpr int kScores = NS > 4 ? 2 : 1;  // buffers of S^T: a ring of one tile has no slots for a second
   static constexpr int kRopeOff = NS * kSlot;
   static constexpr int kQOff = kRopeOff + 16384;         // one rope tile, 128 keys x 64 dims
   static constexpr int kPOff = FP8 ? kQOff + kQ : kRopeOff;
@@ -81,7 +82,7 @@ struct LatCfg {
   static constexpr int kAlloc = kMiscOff + kMisc;
   static constexpr int kBars = 2 * NS + 10;
   static_assert(NS >= 4, "a tile's four latent slots must fit at once");
-  static_assert(!FP8 || (kAhead == 4 && NS >= 9 && NS <= 12), "the 8-bit pipeline holds two tiles, and some");
+  static_assert(!FP8 || (NS >= 9 && NS <= 12), "the 8-bit pipeline holds two tiles, and some");
   static_assert(kBars % 2 == 0 && kBars * 8 + 16 + 48 + NT * 44 <= kMisc, "misc area too small");
   static_assert(kAlloc <= 232448, "shared memory");
   static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
@@ -102,6 +103,7 @@ struct LatAttnParams {
   uint32_t* status;
   int B, Sq, H, R, RT, pages, page_size, max_keys;
   int unit;  // keys per unit of work
+  int tile_pages, tile_rows;  // a tile's keys as pages and rows
   float scale_log2;
   int64_t qs[3], table_stride, tree_stride[2], scale_stride[2];
 };
@@ -256,6 +258,18 @@ __device__ __forceinline__ int first_column(int lane) {
 template <int I>
 struct Int { static constexpr int value = I; };
 
+// Where the key of one thread stands in the block table, and that of the tiles after it: no division on the way (two took the
+// producer 600 cycles a tile, which delayed its loads).
+struct LatPage {
+  int index, row;  // into the sequence's table; row of that page
+  __device__ __forceinline__ LatPage(const LatAttnParams& p, int n) : index(n / p.page_size), row(n - n / p.page_size * p.page_size) {}
+  __device__ __forceinline__ void next_tile(const LatAttnParams& p) {
+    index += p.tile_pages;
+    row += p.tile_rows;
+    if (row >= p.page_size) { row -= p.page_size; ++index; }
+  }
+};
+
 // Shared-memory scalars behind the tiles.
 template <int NT, bool FP8>
 struct LatShared {
@@ -275,6 +289,7 @@ struct LatShared {
   __device__ uint64_t* o_full(uint32_t tile) const { return bars + L::kBars - 2 + (tile & 1); }  // its output GEMM is complete
   __device__ uint32_t* tmem_slot() const { return reinterpret_cast<uint32_t*>(bars + L::kBars); }  // [0] base, [1] abort flag
   __device__ int* scan() const { return reinterpret_cast<int*>(bars + L::kBars + 1); }             // [12 warps] + start
+  __device__ uint32_t* poisoned() const { return reinterpret_cast<uint32_t*>(scan() + 2); }        // later: a bit per key
   __device__ float* cols() const { return reinterpret_cast<float*>(bars + L::kBars + 8); }         // 11 NT words
   __device__ float* ref() const { return cols(); }
   __device__ float* fac() const { return cols() + NT; }
@@ -285,16 +300,19 @@ struct LatShared {
   __device__ float* nref() const { return cols() + 10 * NT; }  // minus ref()
 };
 
-// bf16: query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle), by 64
-// threads. Eight copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
+// bf16: query rows of an entry into shared memory as the B operand of the score GEMM (K-major, 128-byte swizzle). Eight
+// threads copy a row, 16 bytes at a time: chunk ch of a 128-byte block goes to chunk ch ^ (row % 8).
 template <int NT>
-__device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, const LatEntry& x, int t) {
+__device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, const LatEntry& x, int t, int threads) {
+  const int ch = t & 7;
+  int tok = (x.r0 + (t >> 3)) / p.H, h = x.r0 + (t >> 3) - tok * p.H;  // one division: it takes as long as a row's copies
+  const __nv_bfloat16* q = p.q + x.b * p.qs[0] + ch * 8;
 #pragma unroll 1
-  for (int row = t >> 3; row < NT; row += 8) {
-    const int r = x.r0 + row, ch = t & 7;
-    const int tok = r / p.H, h = r - tok * p.H;
-    const bool there = r < p.R;
-    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + ch * 8 : p.q;
+  for (int row = t >> 3; row < NT; row += threads >> 3) {
+    const bool there = x.r0 + row < p.R;
+    const __nv_bfloat16* src = there ? q + tok * p.qs[1] + h * p.qs[2] : p.q;
+    h += threads >> 3;
+    while (h >= p.H) { h -= p.H; ++tok; }
     const uint32_t dst = smem_u32(sq) + row * 128 + (((ch ^ row) & 7) << 4);
 #pragma unroll
     for (int i = 0; i < 9; ++i) cp_async16(dst + i * (NT * 128), src + (there ? i * 64 : 0), there ? 16u : 0u);
@@ -302,31 +320,42 @@ __device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, 
   cp_async_wait_all();
 }
 
-// 8-bit: the split query. A warp's rows come as they are by asynchronous copies, all of them in flight at once, each into the
-// 1024 bytes that its two parts will take; then the warp converts row by row in place, 16 elements a lane (chunks lane and
-// lane + 32 of 8). Beside the key traffic a load takes thousands of cycles (three rows in flight: 10 000 for NT = 32), and a
-// rolled loop keeps the code small: it is cold whenever it runs (16 rows unrolled: 20 000 cycles).
+// 8-bit: the split query. Rows come as they are by asynchronous copies, all of them in flight at once, each into the 1024 bytes
+// that its two parts will take; then a warp converts row by row in place, 16 elements a lane (chunks lane and lane + 32 of 8).
+// A row takes a warp 780 cycles, most of them in the conversions' pipe of its scheduler (32 rows by one warp: 25 000 cycles,
+// more than everything else at the end of a piece), so rows are dealt to warps of all schedulers. A rolled loop keeps the code
+// small: it is cold whenever it runs (16 rows unrolled: 20 000 cycles).
+// Part i (0 .. 7) of 128 bytes of row `row`: high parts of blocks 0 .. 3, then low parts.
 template <int NT>
-__device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t* sq, float* qk, const LatEntry& x, int warp,
-                                                 int warps, int lane) {
-  // part i (0 .. 7) of 128 bytes of row `row`: high parts of blocks 0 .. 3, then low parts
-  const auto piece = [&](int row, int i) { return sq + (i & 3) * (2 * NT * 128) + ((i >> 2) * NT + row) * 128; };
+__device__ __forceinline__ uint8_t* split_part(uint8_t* sq, int row, int i) {
+  return sq + (i & 3) * (2 * NT * 128) + ((i >> 2) * NT + row) * 128;
+}
+template <int NT>
+__device__ __forceinline__ void fetch_query_rows(const LatAttnParams& p, uint8_t* sq, const LatEntry& x, int row0, int end,
+                                                 int step, int lane) {
+  static_assert(NT <= 32, "a lane per row");
+  // Lane = row: where each begins. Computed row by row in the loop, 32 of them took 15 000 cycles.
+  const int tok = (x.r0 + lane) / p.H;
+  const int64_t begins = tok * p.qs[1] + (x.r0 + lane - tok * p.H) * p.qs[2];
+  const __nv_bfloat16* q = p.q + x.b * p.qs[0] + lane * 8;
 #pragma unroll 1
-  for (int row = warp; row < NT; row += warps) {
-    const int r = x.r0 + row, tok = r / p.H, h = r - tok * p.H;
-    const bool there = r < p.R;
-    const __nv_bfloat16* src = there ? p.q + x.b * p.qs[0] + tok * p.qs[1] + h * p.qs[2] + lane * 8 : p.q;
+  for (int row = row0; row < end; row += step) {
+    const int64_t at = __shfl_sync(0xFFFFFFFFu, begins, row);
+    const bool there = x.r0 + row < p.R;
+    const __nv_bfloat16* src = there ? q + at : p.q;
     const uint32_t n = there ? 16u : 0u;
-    cp_async16(smem_u32(piece(row, lane >> 3)) + (lane & 7) * 16, src, n);
-    cp_async16(smem_u32(piece(row, 4 + (lane >> 3))) + (lane & 7) * 16, src + (there ? 256 : 0), n);
+    cp_async16(smem_u32(split_part<NT>(sq, row, lane >> 3)) + (lane & 7) * 16, src, n);
+    cp_async16(smem_u32(split_part<NT>(sq, row, 4 + (lane >> 3))) + (lane & 7) * 16, src + (there ? 256 : 0), n);
     if (lane < 8) cp_async16(smem_u32(sq) + NT * 1024 + row * 128 + (((lane ^ row) & 7) << 4), src + (there ? 512 : 0), n);
   }
   cp_async_wait_all();
-  __syncwarp();
+}
+template <int NT>
+__device__ __forceinline__ void split_query_rows(uint8_t* sq, float* qk, int row0, int end, int step, int lane) {
 #pragma unroll 2
-  for (int row = warp; row < NT; row += warps) {
-    const uint4 a = *reinterpret_cast<const uint4*>(piece(row, lane >> 3) + (lane & 7) * 16);
-    const uint4 b = *reinterpret_cast<const uint4*>(piece(row, 4 + (lane >> 3)) + (lane & 7) * 16);
+  for (int row = row0; row < end; row += step) {
+    const uint4 a = *reinterpret_cast<const uint4*>(split_part<NT>(sq, row, lane >> 3) + (lane & 7) * 16);
+    const uint4 b = *reinterpret_cast<const uint4*>(split_part<NT>(sq, row, 4 + (lane >> 3)) + (lane & 7) * 16);
     __syncwarp();
     const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     float top = 0.f;
@@ -349,33 +378,21 @@ __device__ __forceinline__ void load_split_query(const LatAttnParams& p, uint8_t
         split_e4m3x2(__uint_as_float(w[4 * i + j] << 16) * inv, __uint_as_float(w[4 * i + j] & 0xFFFF0000u) * inv, h[j], l[j]);
       const int ch = i * 32 + lane;  // elements [8 ch, 8 ch + 8): byte 8 (ch % 16) of block ch / 16
       const int at = (((((ch & 15) >> 1) ^ row) & 7) << 4) + (ch & 1) * 8;
-      *reinterpret_cast<uint2*>(piece(row, ch >> 4) + at) =
+      *reinterpret_cast<uint2*>(split_part<NT>(sq, row, ch >> 4) + at) =
           make_uint2(h[0] | (static_cast<uint32_t>(h[1]) << 16), h[2] | (static_cast<uint32_t>(h[3]) << 16));
-      *reinterpret_cast<uint2*>(piece(row, 4 + (ch >> 4)) + at) =
+      *reinterpret_cast<uint2*>(split_part<NT>(sq, row, 4 + (ch >> 4)) + at) =
           make_uint2(l[0] | (static_cast<uint32_t>(l[1]) << 16), l[2] | (static_cast<uint32_t>(l[3]) << 16));
     }
   }
 }
 
-// Row t of one slot of the current latent tile: whether it holds a value that is not finite.
+// Whether 16 bytes of the latent plane hold a value that is not finite: an e4m3 byte 0x7F or 0xFF, a bf16 exponent of ones.
+// Adding one to it carries into the sign bit, which is masked out before.
 template <bool FP8>
-__device__ __forceinline__ bool row_not_finite(const uint8_t* slot, int t) {
-  bool bad = false;
-#pragma unroll 1
-  for (int i = 0; i < (FP8 ? 8 : 16); ++i) {
-    const uint4 v = *reinterpret_cast<const uint4*>(slot + (i >> 3) * 16384 + t * 128 + (((i ^ t) & 7) << 4));
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (FP8) {  // a byte 0x7F or 0xFF
-#pragma unroll
-        for (int u = 0; u < 32; u += 8) bad |= ((w[j] >> u) & 0x7Fu) == 0x7Fu;
-      } else {
-        bad |= (w[j] & 0x7F80u) == 0x7F80u || (w[j] & 0x7F800000u) == 0x7F800000u;
-      }
-    }
-  }
-  return bad;
+__device__ __forceinline__ bool not_finite(uint4 v) {
+  constexpr uint32_t kMask = FP8 ? 0x7F7F7F7Fu : 0x7F807F80u, kOne = FP8 ? 0x01010101u : 0x00800080u;
+  const uint32_t carry = ((v.x & kMask) + kOne) | ((v.y & kMask) + kOne) | ((v.z & kMask) + kOne) | ((v.w & kMask) + kOne);
+  return (carry & ~kMask & (FP8 ? 0x80808080u : 0x80008000u)) != 0u;
 }
 
 // Softmax and epilogue of warpgroup g: columns [g CW, g CW + CW) of the row tile, thread = key of the tile (then output
@@ -402,6 +419,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     if (walk.begins && !walk.ends) { info.y = x.b * p.RT + x.r0 / NT; info.z = slot; }
     named_bar_sync(3, 128 * L::G);  // everybody has finished with the previous piece's columns
     const int prefix = max(x.len - x.nq, 0);
+    if (g == 0 && t < 4) sm.poisoned()[t] = 0u;
     if (t < CW) {
       const int c = cb + t, r = x.r0 + c, tok = r / p.H;
       sm.tok()[c] = tok;
@@ -414,6 +432,21 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     int min_lim = 0x7FFFFFFF;
 #pragma unroll 8
     for (int c = 0; c < NT; ++c) min_lim = min(min_lim, sm.lim()[c]);
+    if constexpr (L::kHelp) {
+      if (tiles > 0) {  // the last score GEMM of the previous piece has completed: this warpgroup has read its scores
+        uint8_t* sq = sm.base + L::kQOff;
+        const int row0 = kOwnRows + 4 * g + w;
+        if (piece == 0) {
+          fetch_query_rows<NT>(p, sq, x, row0, NT, 4 * L::G, lane);
+          __syncwarp();
+        } else {
+          named_bar_sync(4, 128 * L::G + 32);
+        }
+        split_query_rows<NT>(sq, sm.qk(piece & 1), row0, NT, 4 * L::G, lane);
+        fence_proxy_async_smem();
+        mbar_arrive(sm.q_full());
+      }
+    }
     const float* qk = sm.qk(piece & 1) + cb;
     ++piece;
     float l[CW];
@@ -433,21 +466,49 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       f2_unpack(f2_fma(f2_pack(sc[c + 2], sc[c + 3]), scale2, r1), d[2], d[3]);
     };
 
+    // 8-bit: the factor of this thread's key is read a tile ahead, its page two tiles ahead.
+    LatPage at(p, walk.k0 + t);
+    int next_page = -1;
+    float next_ks = 1.f;
+    const auto fetch_page = [&](int n) { next_page = n < walk.k1 ? __ldg(p.table + x.b * p.table_stride + at.index) : -1; };
+    const auto fetch_factor = [&](int n) {
+      next_ks = next_page >= 0 && next_page < p.pages ? p.scale[next_page * p.scale_stride[0] + at.row * p.scale_stride[1]] : 1.f;
+      at.next_tile(p);
+      fetch_page(n + kTile);
+    };
+    if (FP8) {
+      fetch_page(walk.k0 + t);
+      fetch_factor(walk.k0 + t);
+    }
     for (int j = 0; j < tiles; ++j, ++tile) {
       const int n0 = walk.k0 + j * kTile, n = n0 + t;
-      const uint32_t buf = L::kAhead > 0 ? tile & 1 : 0;
+      const uint32_t buf = tile % L::kScores;
       float ks = 1.f, lk = 0.f, iks = 1.f;  // the key's factor, its log2, its reciprocal
       bool bad_factor = false;              // not finite: the rows that see the key become NaN, and no others
-      if (FP8 && n < walk.k1) {
-        const int pg = __ldg(p.table + x.b * p.table_stride + n / p.page_size);
-        if (pg >= 0 && pg < p.pages) ks = p.scale[pg * p.scale_stride[0] + (n % p.page_size) * p.scale_stride[1]];
-        ks = ks < 1e-30f ? 1e-30f : ks;
-        bad_factor = !(ks < INFINITY);
-        if (bad_factor) ks = 1.f;
-        lk = fast_log2(ks);
-        iks = 1.f / ks;
+      if (FP8) {
+        if (n < walk.k1) {
+          ks = next_ks < 1e-30f ? 1e-30f : next_ks;
+          bad_factor = !(ks < INFINITY);
+          if (bad_factor) ks = 1.f;
+          lk = fast_log2(ks);
+          iks = 1.f / ks;
+        }
+        fetch_factor(n + kTile);
       }
-      mbar_wait(sm.s_full(buf), (L::kAhead > 0 ? tile >> 1 : tile) & 1, ctl, 0x700);
+      const int end = min(walk.k1, n0 + kTile);
+      // A tree's mask for this thread's key, a bit per column; its loads are all in flight at once, before the wait.
+      uint32_t shown_to = 0xFFFFFFFFu;
+      if (p.tree != nullptr && __any_sync(0xFFFFFFFFu, n >= min_lim && n < end)) {
+        const bool in_tree = n >= min_lim && n < end;
+        const uint8_t* mask = in_tree ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : p.tree;
+        uint8_t m[CW];
+#pragma unroll
+        for (int c = 0; c < CW; ++c) m[c] = __ldg(mask + (in_tree && n >= sm.lim()[cb + c] ? sm.tok()[cb + c] * p.tree_stride[1] : 0));
+        shown_to = 0u;
+#pragma unroll
+        for (int c = 0; c < CW; ++c) shown_to |= (n < sm.lim()[cb + c] || m[c] != 0 ? 1u : 0u) << c;
+      }
+      mbar_wait(sm.s_full(buf), (tile / L::kScores) & 1, ctl, 0x700);
       tc_fence_after_sync();
       float s[CW];  // scores before the softmax scale
       if (FP8) {
@@ -476,46 +537,50 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
 #pragma unroll
         for (int c = 0; c < CW; ++c) s[c] = __uint_as_float(0x7FC00000u);
       }
-      const int end = min(walk.k1, n0 + kTile);
       if (n0 + kTile > min(min_lim, walk.k1)) {
         // Masked tile. The output GEMM takes the keys in steps of 16 (8-bit: 32); the rows of its last step that hold no
         // key of this piece are zeroed (0 * NaN would reach every output). A key that is hidden from some rows and not
         // finite is taken out of the tile and makes the rows that see it NaN.
         const int rows = (kStep - (end - n0) % kStep) % kStep;
 #pragma unroll 1
-        for (int i = t; i < rows * (FP8 ? 32 : 64); i += 128) {
+        for (int i = g * 128 + t; i < rows * (FP8 ? 32 : 64); i += 128 * L::G) {
           const int row = end - n0 + i / (FP8 ? 32 : 64), ch = i % (FP8 ? 32 : 64);
           *reinterpret_cast<uint4*>(sm.base + ((slot0 + ch / (FP8 ? 8 : 16)) % L::NS) * L::kSlot +
                                     (FP8 ? 0 : (ch >> 3 & 1) * 16384) + row * 128 + (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         bool poison = false;
         if (end > min_lim) {
-          if (n >= min_lim && n < end)
+          constexpr int kChunks = FP8 ? 32 : 64;  // of 16 bytes in a key's latent vector
+          const auto chunk = [&](int row, int ch) {
+            return reinterpret_cast<uint4*>(sm.base + ((slot0 + ch / (kChunks / 4)) % L::NS) * L::kSlot +
+                                            (FP8 ? 0 : (ch >> 3 & 1) * 16384) + row * 128 + (ch & 7) * 16);
+          };
+          const int row0 = max(min_lim - n0, 0);
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) poison |= row_not_finite<FP8>(sm.base + ((slot0 + i) % L::NS) * L::kSlot, t);
-          __syncwarp();
-          if (L::G > 1) named_bar_sync(3, 128 * L::G);  // both warpgroups have looked before either takes a key out
-          if (poison)
+          for (int i = g * 128 + t; i < (end - n0 - row0) * kChunks; i += 128 * L::G) {
+            const int row = row0 + i / kChunks;
+            if (not_finite<FP8>(*chunk(row, i % kChunks))) atomicOr(sm.poisoned() + (row >> 5), 1u << (row & 31));
+          }
+          named_bar_sync(3, 128 * L::G);
+          const uint4 found = *reinterpret_cast<const uint4*>(sm.poisoned());
+          if (L::G > 1) named_bar_sync(3, 128 * L::G);  // both warpgroups have read it before either sets a bit of the next tile
+          if ((found.x | found.y | found.z | found.w) != 0u) {
+            poison = (sm.poisoned()[w] >> lane & 1u) != 0u;
+            named_bar_sync(3, 128 * L::G);
+            if (g == 0 && t < 4) sm.poisoned()[t] = 0u;
+            named_bar_sync(3, 128 * L::G);
+            if (poison)
 #pragma unroll 1
-            for (int i = 0; i < (FP8 ? 32 : 64); ++i)
-              *reinterpret_cast<uint4*>(sm.base + ((slot0 + i / (FP8 ? 8 : 16)) % L::NS) * L::kSlot +
-                                        (FP8 ? 0 : (i >> 3 & 1) * 16384) + t * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (int i = 0; i < kChunks; ++i) *chunk(t, i) = make_uint4(0, 0, 0, 0);
+          }
         }
         const float shown = __uint_as_float(0x7FC00000u);
         if (p.tree == nullptr) {
 #pragma unroll
           for (int c = 0; c < CW; ++c) s[c] = n < min(end, sm.lim()[cb + c]) ? (poison ? shown : s[c]) : -INFINITY;
         } else {
-          const uint8_t* mask = p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq));
 #pragma unroll
-          for (int c = 0; c < CW; ++c) {
-            bool seen = n < end;
-            if (seen && n >= sm.lim()[cb + c]) {
-              const int tok = sm.tok()[cb + c];
-              seen = tok < x.nq && mask[tok * p.tree_stride[1]] != 0;
-            }
-            s[c] = !seen ? -INFINITY : poison ? shown : s[c];
-          }
+          for (int c = 0; c < CW; ++c) s[c] = n < end && (shown_to >> c & 1u) != 0u ? (poison ? shown : s[c]) : -INFINITY;
         }
         __syncwarp();
       }
@@ -688,20 +753,6 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
   if (g == 0 && t == 0) p.part_info[blockIdx.x] = info;
 }
 
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 template <int NT, bool FP8>
 __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     latent_attn_kernel(const __grid_constant__ CUtensorMap tm_lat, const __grid_constant__ CUtensorMap tm_rope,
@@ -718,7 +769,7 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     for (int i = 0; i < L::NS; ++i) { mbar_init(sm.full(i), 1); mbar_init(sm.empty(i), 1); }
     mbar_init(sm.rfull(), 1);
     mbar_init(sm.rempty(), 1);
-    mbar_init(sm.q_full(), 32 * L::kLoadWarps);
+    mbar_init(sm.q_full(), 32 * L::kLoadWarps + (L::kHelp ? 128 * L::G : 0));
     mbar_init(sm.q_empty(), 1);
     mbar_init(sm.s_full(0), 1);
     mbar_init(sm.s_full(1), 1);
@@ -812,15 +863,17 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     uint32_t it = 0, tile = 0;
     while (walk.next(p)) {
       const int32_t* table = p.table + walk.x.b * p.table_stride;
+      LatPage at(p, walk.k0 + lane * box);
       int next_page = 0;  // of the next tile, read a tile ahead
-      if (walk.k0 + lane * box < walk.k1 && lane * box < kTile) next_page = __ldg(table + (walk.k0 + lane * box) / p.page_size);
+      if (lane * box < min(kTile, walk.k1 - walk.k0)) next_page = __ldg(table + at.index);
       for (int j = 0; j < walk.tiles(); ++j, ++tile) {
         const int n0 = walk.k0 + j * kTile;
         const int boxes = (min(kTile, walk.k1 - n0) + box - 1) / box;
-        int page = next_page, row = 0;
-        if (n0 + kTile + lane * box < walk.k1 && lane * box < kTile) next_page = __ldg(table + (n0 + kTile + lane * box) / p.page_size);
+        const int row = at.row;
+        int page = next_page;
+        at.next_tile(p);
+        if (lane * box < min(kTile, walk.k1 - n0 - kTile)) next_page = __ldg(table + at.index);
         if (lane < boxes) {
-          row = (n0 + lane * box) % p.page_size;
           if (page < 0 || page >= p.pages) {
             if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxPage);
             page = 0;
@@ -850,84 +903,72 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer, one thread
+    // ------------------------------------------------------------------ score GEMM, one thread
     // An MMA of these sizes takes 40 to 65 cycles, no longer than a warp needs to form its descriptors and agree on a lane, so
-    // one thread does all of this (with a warp that waits together and a lane that issues: 3 % slower, 8-bit trees alike).
-    // The steps of the score GEMM are a rolled loop: their code runs once a tile between that of the softmax warps, and every
-    // jump over an unrolled copy waited for the instruction cache (900 cycles a tile).
+    // one thread of a warp does all, and the two GEMMs, which wait for different things, are issued by two warps. With one
+    // warp for both, the tensor pipe waited half of the time for the next instruction. The steps are rolled loops where they
+    // wait: their code runs once a tile between that of the softmax warps, and every jump over an unrolled copy waited for
+    // the instruction cache.
     if (elect_one()) {
       constexpr uint32_t id_rope = make_idesc_bf16(128, NT, false, false);
       constexpr uint32_t id_qk = FP8 ? make_idesc_e4m3(128, L::NC, false) : id_rope;
-      constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, true);
       const uint64_t q_desc = make_smem_desc(smem_u32(smem + L::kQOff), 16, 1024);
       const uint64_t qr_desc = make_smem_desc(smem_u32(smem + L::kQOff + L::kQLat), 16, 1024);
-      const uint64_t p_desc = make_row_desc(smem_u32(smem + L::kPOff), L::kPRow);
-      const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);      // K-major: keys x dims
-      const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);   // MN-major: dims x keys
+      const uint64_t k_desc = make_smem_desc(smem_u32(smem), 16, 1024);  // K-major: keys x dims
       const uint64_t r_desc = make_smem_desc(smem_u32(smem + L::kRopeOff), 16, 1024);
-      uint32_t ks = 0, kph = 0;       // slot and phase of the next score GEMM step
-      uint32_t vs = 0;                // slot of the next output GEMM step
-      uint32_t tile = 0, q_phase = 0;
-      // Step i of the score GEMM of tile `number`: 128 latent dimensions (i < 4), or the rope part.
-      const auto score_step = [&](int i, uint32_t number) {
-        const uint32_t buf = L::kAhead > 0 ? number & 1 : 0;
-        tc_fence_after_sync();
-        if (i < 4) {
-          const uint32_t d = tmem + kColS + buf * L::NC;
-          const uint64_t kd = desc_at(k_desc, ks * L::kSlot), qd = desc_at(q_desc, i * (2 * NT * 128));
-          if (FP8) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_ss_f8(d, desc_at(kd, k * 32), desc_at(qd, k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_ss(d, desc_at(kd, (k >> 2) * 16384 + (k & 3) * 32), desc_at(qd, (k >> 2) * (NT * 128) + (k & 3) * 32),
-                      id_qk, (i > 0 || k > 0) ? 1u : 0u);
-          }
-          if (++ks == L::NS) { ks = 0; kph ^= 1; }
-        } else {
-          const uint32_t d = FP8 ? tmem + kColR + buf * NT : tmem + kColS + buf * L::NC;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(d, desc_at(r_desc, k * 32), desc_at(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
-          umma_commit(sm.s_full(buf));
-          if (FP8) umma_commit(sm.rempty());
-        }
-      };
-      // Whether `bar` completes before the weights of tile `number` are there (then their output GEMM goes first).
-      const auto arrives_first = [&](uint64_t* bar, uint32_t parity, uint32_t number) {
-        const long long t0 = clock64();
-        for (uint32_t polls = 1;; ++polls) {
-          if (mbar_test(bar, parity)) return true;
-          if (mbar_test(sm.p_full(number), (number >> 1) & 1)) return false;
-          if ((polls & 31u) == 0u && clock64() - t0 > kWaitCycleLimit) return false;  // the next blocking wait reports it
-        }
-      };
+      uint32_t ks = 0, kph = 0, tile = 0, q_phase = 0;
       while (walk.next(p)) {
-        const int tiles = walk.tiles(), keys = walk.k1 - walk.k0;
+        const int tiles = walk.tiles();
         if (tiles > 0) {
           mbar_wait(sm.q_full(), q_phase, ctl, 0x300);
           q_phase ^= 1;
         }
-        int done = 0;  // score steps of tile j that were issued ahead
         for (int j = 0; j < tiles; ++j, ++tile) {
-          // The rest of this tile's score GEMM; then, while its softmax runs, the next tile's as far as its slots have arrived.
-          int q = done;
-          const int last = j + 1 < tiles ? 5 + (FP8 ? 5 : L::kAhead) : 5;
+          // The weights of the tile that used this buffer of S^T last are written, so its scores have been read; at a piece's
+          // first tile, those of the previous piece's last one (its query factors may then be replaced).
+          const uint32_t before = j == 0 ? 1 : L::kScores;
+          if (tile >= before) mbar_wait(sm.p_full(tile - before), ((tile - before) >> 1) & 1, ctl, 0x680);
+          const uint32_t buf = tile % L::kScores;
+          const uint32_t d = tmem + kColS + buf * L::NC;
 #pragma unroll 1
-          for (; q < last; ++q) {
-            const bool ahead = q >= 5;
-            const int i = ahead ? q - 5 : q;
-            const uint32_t number = tile + (ahead ? 1u : 0u);
-            uint64_t* bar = i < 4 ? sm.full(ks) : sm.rfull();
-            const uint32_t parity = i < 4 ? kph : number & 1;
-            if (!ahead) mbar_wait(bar, parity, ctl, i < 4 ? 0x400 + ks : 0x500);
-            else if (!arrives_first(bar, parity, tile)) break;
-            score_step(i, number);
+          for (int i = 0; i < 4; ++i) {  // 128 latent dimensions each
+            mbar_wait(sm.full(ks), kph, ctl, 0x400 + ks);
+            tc_fence_after_sync();
+            const uint64_t kd = desc_at(k_desc, ks * L::kSlot), qd = desc_at(q_desc, i * (2 * NT * 128));
+            if (FP8) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_ss_f8(d, desc_at(kd, k * 32), desc_at(qd, k * 32), id_qk, (i > 0 || k > 0) ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                umma_ss(d, desc_at(kd, (k >> 2) * 16384 + (k & 3) * 32), desc_at(qd, (k >> 2) * (NT * 128) + (k & 3) * 32),
+                        id_qk, (i > 0 || k > 0) ? 1u : 0u);
+            }
+            if (++ks == L::NS) { ks = 0; kph ^= 1; }
           }
-          done = max(q - 5, 0);
+          mbar_wait(sm.rfull(), tile & 1, ctl, 0x500);
+          tc_fence_after_sync();
+          const uint32_t dr = FP8 ? tmem + kColR + buf * NT : d;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_ss(dr, desc_at(r_desc, k * 32), desc_at(qr_desc, k * 32), id_rope, (!FP8 || k > 0) ? 1u : 0u);
+          umma_commit(sm.s_full(buf));
+          if (FP8) umma_commit(sm.rempty());
           if (j + 1 == tiles) umma_commit(sm.q_empty());
+        }
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ output GEMM, one thread
+    if (elect_one()) {
+      constexpr uint32_t id_pv = FP8 ? make_idesc_e4m3(128, L::NC, true) : make_idesc_bf16(128, NT, true, true);
+      const uint64_t p_desc = make_row_desc(smem_u32(smem + L::kPOff), L::kPRow);
+      const uint64_t v_desc = make_smem_desc(smem_u32(smem), 16384, 1024);  // MN-major: dims x keys
+      uint32_t vs = 0, tile = 0;
+      while (walk.next(p)) {
+        const int tiles = walk.tiles(), keys = walk.k1 - walk.k0;
+        for (int j = 0; j < tiles; ++j, ++tile) {
           const uint64_t pd = FP8 ? desc_at(p_desc, (tile & 1) * L::kP) : p_desc;
           const int steps = (min(keys - j * kTile, kTile) + (FP8 ? 31 : 15)) / (FP8 ? 32 : 16);
           mbar_wait(sm.p_full(tile), (tile >> 1) & 1, ctl, 0x600);
@@ -959,30 +1000,27 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
       }
     }
   } else if (warp >= 4 && warp < 4 + 4 * L::G) {
-    if constexpr (L::kHelp) {
-      LatWalk<NT> first = walk;
-      if (first.next(p) && first.tiles() > 0) {
-        load_split_query<NT>(p, smem + L::kQOff, sm.qk(0), first.x, L::kLoadWarps + warp - 4, L::kLoadWarps + 4 * L::G, lane);
-        fence_proxy_async_smem();
-        asm volatile("bar.arrive 4, %0;" ::"n"((L::kLoadWarps + 4 * L::G) * 32) : "memory");
-      }
-    }
     lat_softmax<NT, FP8>(p, sm, ctl, walk, tmem, (warp - 4) >> 2, static_cast<int>(threadIdx.x) & 127);
   } else {
     // ------------------------------------------------------------------ query loaders, one piece ahead
-    const int loader = warp < 4 ? warp - 2 : warp - 2 - 4 * L::G;
+    const int loader = warp < 4 ? 0 : warp - 3 - 4 * L::G;
     uint32_t q_phase = 1, piece = 0;
     while (walk.next(p)) {
       const int tiles = walk.tiles();
       if (tiles > 0) {
         uint8_t* sq = smem + L::kQOff;
         mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
-        if constexpr (FP8) {
-          const bool help = L::kHelp && piece == 0;
-          load_split_query<NT>(p, sq, sm.qk(piece & 1), walk.x, loader, L::kLoadWarps + (help ? 4 * L::G : 0), lane);
-          if (help) named_bar_sync(4, (L::kLoadWarps + 4 * L::G) * 32);
+        if constexpr (L::kHelp) {  // the softmax warps fetch their own rows of a CTA's first query, and find those of later ones
+          fetch_query_rows<NT>(p, sq, walk.x, 0, piece == 0 ? kOwnRows : NT, 1, lane);
+          if (piece > 0) asm volatile("bar.arrive 4, %0;" ::"n"(128 * L::G + 32) : "memory");
+          __syncwarp();
+          split_query_rows<NT>(sq, sm.qk(piece & 1), 0, kOwnRows, 1, lane);
+        } else if constexpr (FP8) {
+          fetch_query_rows<NT>(p, sq, walk.x, loader, NT, L::kLoadWarps, lane);
+          __syncwarp();
+          split_query_rows<NT>(sq, sm.qk(piece & 1), loader, NT, L::kLoadWarps, lane);
         } else {
-          load_query<NT>(p, sq, walk.x, loader * 32 + lane);
+          load_query<NT>(p, sq, walk.x, loader * 32 + lane, L::kLoadWarps * 32);
         }
         q_phase ^= 1;
         fence_proxy_async_smem();
@@ -1192,6 +1230,8 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.pages = a->cache.pages; p.page_size = a->cache.page_size;
   p.max_keys = a->table_cols * a->cache.page_size;
   p.unit = lat_unit(p.max_keys);
+  p.tile_pages = kTile / p.page_size;
+  p.tile_rows = kTile % p.page_size;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i];
   p.table_stride = a->table_stride;
