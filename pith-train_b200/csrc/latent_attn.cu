@@ -54,8 +54,8 @@ template <int NT, bool FP8>
 struct LatCfg {
   static constexpr int NC = FP8 ? 2 * NT : NT;           // columns of S^T and O^T
   // Units of 64 keys that beginning another piece costs a CTA: what its epilogue, its query and the empty pipeline take
-  // over the time of a unit. Half as much made 16 trees of 13 tokens 4 (bf16) and 17 % (8-bit) and 128 short sequences 4 %
-  // slower; twice as much changes every batch by less than 5 %, either way.
+  // over the time of a unit. About two thirds as much made 16 trees of 13 tokens 3 (bf16) and 6 % (8-bit) slower and nothing
+  // faster; half as much again changed most batches by less than 1 % and some by 3 %, either way.
   static constexpr int kExtra = FP8 ? (NT == 16 ? 4 : 8) : (NT == 16 ? 2 : NT == 32 ? 3 : 5);
   static_assert(kExtra <= kMaxExtra, "the host checks the line's length with kMaxExtra");
   static constexpr int G = NT >= 32 ? 2 : 1;             // softmax warpgroups, each with CW of the rows
@@ -88,6 +88,22 @@ struct LatCfg {
   static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
 };
 
+// Division by a number that the host knows, of numbers below 2^31: with 2^l >= d the factor 2^(31 + l) / d rounded up is off by
+// less than one, so the product by less than 2^31 * 2^-(31 + l) <= 1 / d. Written out, a division is a hundred instructions
+// that have to be fetched when a launch or a piece begins.
+struct LatDiv {
+  uint32_t factor, shift;
+  int d;
+  LatDiv() = default;
+  explicit LatDiv(int d) : shift(31), d(d) {
+    while ((1ll << (shift - 31)) < d) ++shift;
+    factor = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * factor) >> shift);
+  }
+};
+
 struct LatAttnParams {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;  // [B][Sq][H][512] contiguous
@@ -102,7 +118,8 @@ struct LatAttnParams {
   int4* part_info;    // [G]: entry continued from the previous CTA, entry begun and not finished, its slot
   uint32_t* status;
   int B, Sq, H, R, RT, pages, page_size, max_keys;
-  int unit;  // keys per unit of work
+  int unit_log2;          // keys per unit of work
+  LatDiv by_h, by_rt, by_page;
   int tile_pages, tile_rows;  // a tile's keys as pages and rows
   float scale_log2;
   int64_t qs[3], table_stride, tree_stride[2], scale_stride[2];
@@ -115,15 +132,15 @@ struct LatEntry {
 template <int NT>
 __device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
   LatEntry x;
-  x.b = p.RT == 1 ? e : e / p.RT;
+  x.b = p.by_rt(e);
   x.r0 = (e - x.b * p.RT) * NT;
   x.len = min(max(__ldg(p.lens + x.b), 0), p.max_keys);
   x.nq = p.qlens != nullptr ? min(max(__ldg(p.qlens + x.b), 0), p.Sq) : p.Sq;
-  const int last = min(p.RT == 1 ? p.Sq - 1 : (min(x.r0 + NT, p.R) - 1) / p.H, x.nq - 1);
-  x.keys = (x.r0 == 0 ? 0 : x.r0 / p.H) >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
+  const int last = min(p.by_h(min(x.r0 + NT, p.R) - 1), x.nq - 1);
+  x.keys = p.by_h(x.r0) >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
   return x;
 }
-__device__ __forceinline__ int lat_units(const LatAttnParams& p, int keys) { return max((keys + p.unit - 1) / p.unit, 1); }
+__device__ __forceinline__ int lat_units(const LatAttnParams& p, int keys) { return max((keys + (1 << p.unit_log2) - 1) >> p.unit_log2, 1); }
 
 // Walks the pieces of this CTA's share of the line. Every role keeps its own copy. An entry takes `extra` places of the line
 // in front of its units: what beginning another piece costs a CTA.
@@ -138,8 +155,8 @@ struct LatWalk {
       x = lat_entry<NT>(p, e);
       const int n = lat_units(p, x.keys) + extra;
       const int take = min(n - off, left), u0 = max(off - extra, 0), u1 = off + take - extra;
-      k0 = u0 * p.unit;
-      k1 = min(x.keys, u1 * p.unit);
+      k0 = u0 << p.unit_log2;
+      k1 = min(x.keys, u1 << p.unit_log2);
       begins = u0 == 0;
       ends = off + take == n;
       left -= take;
@@ -262,7 +279,7 @@ struct Int { static constexpr int value = I; };
 // producer 600 cycles a tile, which delayed its loads).
 struct LatPage {
   int index, row;  // into the sequence's table; row of that page
-  __device__ __forceinline__ LatPage(const LatAttnParams& p, int n) : index(n / p.page_size), row(n - n / p.page_size * p.page_size) {}
+  __device__ __forceinline__ LatPage(const LatAttnParams& p, int n) : index(p.by_page(n)), row(n - index * p.page_size) {}
   __device__ __forceinline__ void next_tile(const LatAttnParams& p) {
     index += p.tile_pages;
     row += p.tile_rows;
@@ -305,7 +322,7 @@ struct LatShared {
 template <int NT>
 __device__ __forceinline__ void load_query(const LatAttnParams& p, uint8_t* sq, const LatEntry& x, int t, int threads) {
   const int ch = t & 7;
-  int tok = (x.r0 + (t >> 3)) / p.H, h = x.r0 + (t >> 3) - tok * p.H;  // one division: it takes as long as a row's copies
+  int tok = p.by_h(x.r0 + (t >> 3)), h = x.r0 + (t >> 3) - tok * p.H;
   const __nv_bfloat16* q = p.q + x.b * p.qs[0] + ch * 8;
 #pragma unroll 1
   for (int row = t >> 3; row < NT; row += threads >> 3) {
@@ -335,7 +352,7 @@ __device__ __forceinline__ void fetch_query_rows(const LatAttnParams& p, uint8_t
                                                  int step, int lane) {
   static_assert(NT <= 32, "a lane per row");
   // Lane = row: where each begins. Computed row by row in the loop, 32 of them took 15 000 cycles.
-  const int tok = (x.r0 + lane) / p.H;
+  const int tok = p.by_h(x.r0 + lane);
   const int64_t begins = tok * p.qs[1] + (x.r0 + lane - tok * p.H) * p.qs[2];
   const __nv_bfloat16* q = p.q + x.b * p.qs[0] + lane * 8;
 #pragma unroll 1
@@ -421,7 +438,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     const int prefix = max(x.len - x.nq, 0);
     if (g == 0 && t < 4) sm.poisoned()[t] = 0u;
     if (t < CW) {
-      const int c = cb + t, r = x.r0 + c, tok = r / p.H;
+      const int c = cb + t, r = x.r0 + c, tok = p.by_h(r);
       sm.tok()[c] = tok;
       // keys below the limit are visible; rows without a query are stored as zeros or not at all, whatever they see
       sm.lim()[c] = r >= p.R || tok >= x.nq ? 0x7FFFFFFF : p.tree != nullptr ? prefix : max(x.len - x.nq + tok + 1, 0);
@@ -743,7 +760,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       if (!whole) {
         p.part_ml[slot * NT + c] = make_float2(sm.ref()[c], sum);
       } else if (p.lse != nullptr && r < p.R) {
-        const int tok = r / p.H;
+        const int tok = p.by_h(r);
         p.lse[static_cast<int64_t>(x.b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
             sum == 0.f ? -INFINITY : sm.ref()[c] + log2f(sum);
       }
@@ -778,6 +795,10 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     mbar_init(sm.o_full(0), 1);
     mbar_init(sm.o_full(1), 1);
     mbar_fence_init();
+  }
+  if (threadIdx.x == 96) {
+    tma_prefetch_desc(&tm_lat);
+    tma_prefetch_desc(&tm_rope);
   }
   if (threadIdx.x == 64)  // a launch that finds an error already recorded does no work
     *abort_flag = (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0u) ? 1u : 0u;
@@ -855,10 +876,6 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer: one lane per page of the tile
-    if (lane == 0) {
-      tma_prefetch_desc(&tm_lat);
-      tma_prefetch_desc(&tm_rope);
-    }
     const int box = min(p.page_size, kBox);
     uint32_t it = 0, tile = 0;
     while (walk.next(p)) {
@@ -1119,7 +1136,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }
-  const int b = e / p.RT, r0 = (e - b * p.RT) * NT + 4 * c4;
+  const int b = p.by_rt(e), r0 = (e - b * p.RT) * NT + 4 * c4;
   const float sums[4] = {red[0][0].x, red[0][0].y, red[0][0].z, red[0][0].w};
   const float sum_top[4] = {red[1][0].x, red[1][0].y, red[1][0].z, red[1][0].w};
   const float o[4] = {acc.x, acc.y, acc.z, acc.w};
@@ -1130,7 +1147,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
     const bool none = sums[i] == 0.f;  // no key, or no query
     p.out[(static_cast<int64_t>(b) * p.R + r) * kLat + d] = __float2bfloat16_rn(none ? 0.f : o[i] / sums[i]);
     if (d == 0 && p.lse != nullptr) {
-      const int tok = r / p.H;
+      const int tok = p.by_h(r);
       p.lse[static_cast<int64_t>(b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
           none ? -INFINITY : sum_top[i] + log2f(sums[i]);
     }
@@ -1168,7 +1185,7 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
   kern<<<ctas, L::kThreads, L::kAlloc, st>>>(tl, tr, p);
   PITH_CUDA(cudaGetLastError());
-  if (p.max_keys > p.unit && ctas > 1) {  // an entry of one unit is never cut
+  if (p.max_keys > (1 << p.unit_log2) && ctas > 1) {  // an entry of one unit is never cut
     const int64_t entries = static_cast<int64_t>(p.B) * p.RT;
     cudaLaunchConfig_t cfg = {};
     const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1);
@@ -1229,7 +1246,10 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.B = a->B; p.Sq = a->Sq; p.H = a->H; p.R = static_cast<int>(rows); p.RT = static_cast<int>(rt);
   p.pages = a->cache.pages; p.page_size = a->cache.page_size;
   p.max_keys = a->table_cols * a->cache.page_size;
-  p.unit = lat_unit(p.max_keys);
+  p.unit_log2 = lat_unit(p.max_keys) == kTile ? 7 : 6;
+  p.by_h = LatDiv(p.H);
+  p.by_rt = LatDiv(p.RT);
+  p.by_page = LatDiv(p.page_size);
   p.tile_pages = kTile / p.page_size;
   p.tile_rows = kTile % p.page_size;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
