@@ -1136,7 +1136,8 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }
-  const int b = p.by_rt(e), r0 = (e - b * p.RT) * NT + 4 * c4;
+  // (plain divisions here: with LatDiv's the merge of one sequence's 148 parts took 14.7 instead of 12.1 us)
+  const int b = e / p.RT, r0 = (e - b * p.RT) * NT + 4 * c4;
   const float sums[4] = {red[0][0].x, red[0][0].y, red[0][0].z, red[0][0].w};
   const float sum_top[4] = {red[1][0].x, red[1][0].y, red[1][0].z, red[1][0].w};
   const float o[4] = {acc.x, acc.y, acc.z, acc.w};
@@ -1147,7 +1148,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
     const bool none = sums[i] == 0.f;  // no key, or no query
     p.out[(static_cast<int64_t>(b) * p.R + r) * kLat + d] = __float2bfloat16_rn(none ? 0.f : o[i] / sums[i]);
     if (d == 0 && p.lse != nullptr) {
-      const int tok = p.by_h(r);
+      const int tok = r / p.H;
       p.lse[static_cast<int64_t>(b) * p.R + static_cast<int64_t>(r - tok * p.H) * p.Sq + tok] =
           none ? -INFINITY : sum_top[i] + log2f(sums[i]);
     }
