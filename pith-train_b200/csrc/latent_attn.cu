@@ -25,18 +25,20 @@
 // the merge kernel adds them in key order.
 //
 // Roles: warp 0 TMA producer (one lane per page), warp 1 issues the score GEMMs, warp 2 the output GEMMs, warp 3 loads
-// queries (with one or three more for NT = 16), one or two warpgroups softmax and epilogue (thread = key, then = output
-// dimension). The running maximum is moved
-// only when a score exceeds the reference by more than 2^8 (8-bit: 2^4), decided by one barrier reduction per tile. The
-// score GEMM of the next tile runs under this tile's softmax as far as the ring of latent slots holds it: completely with
-// an 8-bit cache, two of four slots at NT = 16, none at NT = 64, whose query and tile fill the shared memory.
+// queries (with one or three more for NT = 16, and the softmax warps' help for NT = 32, 8-bit), one or two warpgroups softmax
+// and epilogue (thread = key, then = output dimension). The running maximum is moved only when a score exceeds the reference by
+// more than 2^8 (8-bit: 2^4), decided by one barrier reduction per tile. The score GEMM of the next tile runs under this tile's
+// softmax as far as the ring of latent slots holds it: completely with an 8-bit cache, two of four slots at NT = 16, none at
+// NT = 64, whose query and tile fill the shared memory.
 //
-// Measured (16 heads, CUDA events over a captured graph): 64 sequences of 130 to 8191 keys, bf16: 65 us, 4.7 TB/s, 0.73 of
+// Measured (16 heads, CUDA events over a captured graph): 64 sequences of 130 to 8191 keys, bf16: 65 us, 4.8 TB/s, 0.74 of
 // the measured copy rate; the loop itself streams 6 TB/s, the rest is 3 us until the first load, the pieces' ends and the
-// merge. 8 sequences of 9000 to 131071 keys, e4m3: 82 us, 5.1 TB/s, 0.78. Shorter tiles (64 keys, more of the ring in
-// flight) were slower: 75 and 122 us. 250 tokens of a prompt over 6001 keys, bf16: 89 us, 570 TFLOP/s, the serial chain score
-// GEMM (2.2k cycles) - softmax (1.6k) - output GEMM (1.6k) of a tile; the expanded form is the one for long chunks. 16 trees
-// of 13 tokens over 500 to 4097 keys, e4m3: 63 us, chain and pieces alike.
+// merge. 8 sequences of 9000 to 131071 keys, e4m3: 75 us, 5.5 TB/s, 0.86. Shorter tiles (64 keys, more of the ring in
+// flight) were slower: 75 and 122 us. 250 tokens of a prompt over 6001 keys, bf16: 79 us, 650 TFLOP/s, the serial chain score
+// GEMM (2.2k cycles) - softmax (1.5k) - output GEMM (1.5k) of a tile; the expanded form is the one for long chunks. 16 trees
+// of 13 tokens over 500 to 4097 keys, e4m3: 49 us; a tile takes 2600 cycles (its MMAs 1750), as the slots of the tile after
+// the next are free, and loaded, only once this tile's output GEMM has completed, and a piece's begin and end take as long
+// as four.
 #include "common.cuh"
 #include "host_common.h"
 
@@ -712,11 +714,12 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       mbar_wait(sm.o_full(tile - 1), ((tile - 1) >> 1) & 1, ctl, 0x800);
       tc_fence_after_sync();
     }
-    // A rolled loop: the code runs once per piece, and unrolled it waited for the instruction cache at every store.
+    // Rolled loops: the code runs once per piece, and unrolled it waited for the instruction cache at every store.
     const int rows = min(p.R - x.r0, NT);
 #pragma unroll 1
     for (int i = 0; i < 4 * CW; i += 32) {
       uint32_t o[32], lo[32];
+      float y[32];
       if (tiles > 0) {
 #pragma unroll
         for (int u = 0; u < 32; u += 16) {
@@ -725,33 +728,41 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
           if (FP8) tmem_ld16(at + NT, lo + u);
         }
         tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          y[c] = __uint_as_float(o[c]);
+          if (FP8) y[c] = fmaf(__uint_as_float(lo[c]), 0.0625f, y[c]) * 0.0625f;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) y[c] = 0.f;
+      }
+      if (!whole) {
+        // [column / 4][dimension][4 columns]: 16 bytes a lane, neighbouring. Rows without a query may hold anything.
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const int d0 = (i + c) / CW * 128 + t, c0 = cb + (i + c) % CW;
+          *(reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat) + d0) =
+              make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
+        }
+        continue;
       }
 #pragma unroll
       for (int u = 0; u < 32; u += 16) {
         const int d0 = (i + u) / CW * 128 + t, c0 = cb + (i + u) % CW;
-        float y[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          float v = __uint_as_float(o[u + c]);
-          if (FP8) v = fmaf(__uint_as_float(lo[u + c]), 0.0625f, v) * 0.0625f;
-          const float f = sm.fac()[c0 + c];
-          y[c] = tiles == 0 || f == 0.f ? 0.f : v * f;  // no key, or no query (whose scores may be anything)
+        for (int c = u; c < u + 16; ++c) {
+          const float f = sm.fac()[c0 + c - u];
+          y[c] = f == 0.f ? 0.f : y[c] * f;  // no key, or no query (whose scores may be anything)
         }
-        if (whole) {
-          // neighbouring lanes trade: the even one stores two dimensions of an even column, the odd one of the next column
-          const int odd = t & 1;
-          __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0 + odd) * kLat + (d0 & ~1);
+        // neighbouring lanes trade: the even one stores two dimensions of an even column, the odd one of the next column
+        const int odd = t & 1;
+        __nv_bfloat16* d = p.out + (static_cast<int64_t>(x.b) * p.R + x.r0 + c0 + odd) * kLat + (d0 & ~1);
 #pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? y[c] : y[c + 1], 1);
-            const uint32_t pair = odd ? pack_bf16(got, y[c + 1]) : pack_bf16(y[c], got);
-            if (c0 + c + odd < rows) *reinterpret_cast<uint32_t*>(d + c * kLat) = pair;
-          }
-        } else {
-          // [column / 4][dimension][4 columns]: 16 bytes a lane, neighbouring
-          float4* d = reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * NT + c0) * kLat) + d0;
-#pragma unroll
-          for (int c = 0; c < 16; c += 4) d[c / 4 * kLat] = make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
+        for (int c = 0; c < 16; c += 2) {
+          const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? y[u + c] : y[u + c + 1], 1);
+          const uint32_t pair = odd ? pack_bf16(got, y[u + c + 1]) : pack_bf16(y[u + c], got);
+          if (c0 + c + odd < rows) *reinterpret_cast<uint32_t*>(d + c * kLat) = pair;
         }
       }
     }
@@ -896,12 +907,6 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
             page = 0;
           }
         }
-        const auto rope_tile = [&]() {
-          mbar_wait(sm.rempty(), (tile & 1) ^ 1, ctl, 0x200);
-          if (lane == 0) mbar_arrive_expect_tx(sm.rfull(), boxes * box * 128);
-          __syncwarp();
-          if (lane < boxes) tma_load_4d(smem + L::kRopeOff + lane * box * 128, &tm_rope, sm.rfull(), 0, 0, row, page);
-        };
         for (int i = 0; i < 4; ++i, ++it) {
           const uint32_t s = it % L::NS;
           mbar_wait(sm.empty(s), ((it / L::NS) & 1) ^ 1, ctl, 0x100 + s);
@@ -912,11 +917,13 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
             tma_load_4d(dst, &tm_lat, sm.full(s), i * 128, 0, row, page);
             if (!FP8) tma_load_4d(dst + 16384, &tm_lat, sm.full(s), i * 128 + 64, 0, row, page);
           }
-          // 8-bit: its place is free once the previous tile's score GEMM has completed, which should not hold up the slots
-          // that the ring has beyond two tiles
-          if (FP8 && i == L::NS - 9) rope_tile();
         }
-        if (!FP8) rope_tile();  // free (of the weights) once the previous tile's output GEMM has completed
+        // The rope tile comes last, as its place is free last: once the previous tile's score GEMM (8-bit) or output GEMM (whose
+        // weights lie there) has completed.
+        mbar_wait(sm.rempty(), (tile & 1) ^ 1, ctl, 0x200);
+        if (lane == 0) mbar_arrive_expect_tx(sm.rfull(), boxes * box * 128);
+        __syncwarp();
+        if (lane < boxes) tma_load_4d(smem + L::kRopeOff + lane * box * 128, &tm_rope, sm.rfull(), 0, 0, row, page);
       }
     }
   } else if (warp == 1) {
