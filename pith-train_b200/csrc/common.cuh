@@ -421,6 +421,22 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
   return pred != 0;
 }
+// Division by a number that the host knows, of numbers below 2^31: with 2^l >= d the factor 2^(31 + l) / d rounded up is off by
+// less than one, so the product by less than 2^31 * 2^-(31 + l) <= 1 / d. Written out, a division is a hundred instructions
+// that have to be fetched when a launch or a piece begins.
+struct FastDiv {
+  uint32_t factor, shift;
+  int d;
+  FastDiv() = default;
+  explicit FastDiv(int d) : shift(31), d(d) {
+    while ((1ll << (shift - 31)) < d) ++shift;
+    factor = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * factor) >> shift);
+  }
+};
+
 // Adds a byte offset to the start-address field of a shared-memory descriptor.
 __device__ __forceinline__ uint64_t desc_advance(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 

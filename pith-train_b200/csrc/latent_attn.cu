@@ -90,22 +90,6 @@ struct LatCfg {
   static_assert(4 * NC <= kColS && kColS + 2 * NC <= kColR && kColR + 2 * NT <= 512, "TMEM columns");
 };
 
-// Division by a number that the host knows, of numbers below 2^31: with 2^l >= d the factor 2^(31 + l) / d rounded up is off by
-// less than one, so the product by less than 2^31 * 2^-(31 + l) <= 1 / d. Written out, a division is a hundred instructions
-// that have to be fetched when a launch or a piece begins.
-struct LatDiv {
-  uint32_t factor, shift;
-  int d;
-  LatDiv() = default;
-  explicit LatDiv(int d) : shift(31), d(d) {
-    while ((1ll << (shift - 31)) < d) ++shift;
-    factor = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
-  }
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * factor) >> shift);
-  }
-};
-
 struct LatAttnParams {
   const __nv_bfloat16* q;
   __nv_bfloat16* out;  // [B][Sq][H][512] contiguous
@@ -121,7 +105,7 @@ struct LatAttnParams {
   uint32_t* status;
   int B, Sq, H, R, RT, pages, page_size, max_keys;
   int unit_log2;          // keys per unit of work
-  LatDiv by_h, by_rt, by_page;
+  FastDiv by_h, by_rt, by_page;
   int tile_pages, tile_rows;  // a tile's keys as pages and rows
   float scale_log2;
   int64_t qs[3], table_stride, tree_stride[2], scale_stride[2];
@@ -1143,7 +1127,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
       acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
     }
   }
-  // (plain divisions here: with LatDiv's the merge of one sequence's 148 parts took 14.7 instead of 12.1 us)
+  // (plain divisions here: with FastDiv's the merge of one sequence's 148 parts took 14.7 instead of 12.1 us)
   const int b = e / p.RT, r0 = (e - b * p.RT) * NT + 4 * c4;
   const float sums[4] = {red[0][0].x, red[0][0].y, red[0][0].z, red[0][0].w};
   const float sum_top[4] = {red[1][0].x, red[1][0].y, red[1][0].z, red[1][0].w};
@@ -1255,9 +1239,9 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.pages = a->cache.pages; p.page_size = a->cache.page_size;
   p.max_keys = a->table_cols * a->cache.page_size;
   p.unit_log2 = lat_unit(p.max_keys) == kTile ? 7 : 6;
-  p.by_h = LatDiv(p.H);
-  p.by_rt = LatDiv(p.RT);
-  p.by_page = LatDiv(p.page_size);
+  p.by_h = FastDiv(p.H);
+  p.by_rt = FastDiv(p.RT);
+  p.by_page = FastDiv(p.page_size);
   p.tile_pages = kTile / p.page_size;
   p.tile_rows = kTile % p.page_size;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;

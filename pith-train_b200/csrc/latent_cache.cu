@@ -5,10 +5,10 @@
 // stored at the token's slot as bf16, or c as e4m3 with one power-of-two factor 2^k a row, k the least integer with
 // max|c| <= 448 * 2^k: the division is exact, so the only rounding is e4m3's, and the row read back is exact in bf16.
 // One warp per token: a lane holds 16 of the 512 values (two 16-byte loads, 512 contiguous bytes a warp instruction), the
-// row sum and maximum are five shuffles each, lanes 0-7 rotate 8 inputs into 4 + 4 outputs on their own. All loads of a
+// row sum and maximum are five shuffles each, and every lane rotates one pair of inputs into outputs j and 32 + j. Loads of a
 // token are issued before the first use; the kernels are bound by HBM at prompt sizes and by the launch at decode sizes.
-// Measured: 64 tokens 2.3 us; 8191 tokens into an 8-bit cache 7 us, back out of it 6 us (one token a warp, so that two
-// dependent loads and the launch are most of it); 32768 rows of a bf16 cache 12.8 us = 5.9 TB/s, 0.92 of the measured copy
+// Measured: 64 tokens 2.1 us; 8191 tokens into an 8-bit cache 6.3 us, back out of it 5.9 us (one token a warp, so that two
+// dependent loads and the launch are most of it); 32768 rows of a bf16 cache 13.0 us = 5.8 TB/s, 0.91 of the measured copy
 // rate.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
@@ -22,7 +22,7 @@ struct LatentPlanes {
   void* latent;
   void* rope;
   float* scale;
-  int page_size;
+  FastDiv by_page;
   int64_t slots;  // pages * page_size
   int64_t ls[2], rs[2], ss[2];
 };
@@ -38,7 +38,7 @@ struct LatentWriteParams {
   const int64_t* pos;
   uint32_t* status;
   int64_t n, table_rows;
-  int S;
+  FastDiv by_s;
   float eps;
   int64_t kvs[2], ps[2], cs[2], sls[2], pos_s[2];
 };
@@ -74,6 +74,11 @@ __device__ __forceinline__ void load_f4(const void* base, int64_t off, float* f)
     f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xFFFF0000u);
   }
 }
+template <bool F32>
+__device__ __forceinline__ float load_f(const void* base, int64_t off) {
+  if (F32) return __ldg(static_cast<const float*>(base) + off);
+  return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(base) + off));
+}
 __device__ __forceinline__ void report_index(uint32_t* status, uint32_t what) {
   if (status != nullptr) atomicCAS(status, 0u, (kErrIndex << 24) | what);
 }
@@ -93,38 +98,30 @@ __device__ __forceinline__ void unpack_e4m3x4(uint32_t v, float* f) {
   }
 }
 
+// 48 registers: five CTAs an SM, so that 8191 tokens are little more than one wave (with 16 weights and a whole rotation a lane
+// held from the start 73, and 7.2 instead of 6.3 us).
 template <bool FP8, bool CS32, bool W32>
-__global__ void __launch_bounds__(256) latent_write_kernel(const LatentWriteParams p) {
+__global__ void __launch_bounds__(256, 5) latent_write_kernel(const LatentWriteParams p) {
   const int lane = threadIdx.x & 31;
   const uint32_t failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < p.n;
        t += static_cast<int64_t>(gridDim.x) * 8) {
-    const int64_t b = t / p.S, s = t - b * p.S;
+    const int b = p.by_s(static_cast<int>(t)), s = static_cast<int>(t) - b * p.by_s.d;
     // everything that does not depend on another load is requested first
     const int64_t slot = __ldg(p.slots + b * p.sls[0] + s * p.sls[1]);
     int64_t row = 0;
     if (p.pos != nullptr) row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
     const uint4* x = reinterpret_cast<const uint4*>(p.kv + b * p.kvs[0] + s * p.kvs[1]);
     const uint4 x0 = __ldg(x + lane), x1 = __ldg(x + 32 + lane);
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load_f4<W32>(p.w, (i >> 1) * 256 + lane * 8 + (i & 1) * 4, w + 4 * i);
-    uint4 pe_raw = make_uint4(0, 0, 0, 0);
-    if (lane < 8) pe_raw = __ldg(reinterpret_cast<const uint4*>(p.pe + b * p.ps[0] + s * p.ps[1]) + lane);
+    const uint32_t pe = __ldg(reinterpret_cast<const uint32_t*>(p.pe + b * p.ps[0] + s * p.ps[1]) + lane);
     if (slot < 0 || failed != 0u) continue;  // padding
     if (slot >= p.c.slots || (p.pos != nullptr && (row < 0 || row >= p.table_rows))) {
       if (lane == 0) report_index(p.status, slot >= p.c.slots ? kIdxSlot : kIdxPosition);
       continue;
     }
-    float cl[4], ch[4], sl[4], sh[4], pe[8];
-    if (lane < 8) {
-      const int64_t cs = p.pos != nullptr ? row * p.cs[1] : b * p.cs[0] + s * p.cs[1];
-      load_f4<CS32>(p.cos, cs + lane * 4, cl);
-      load_f4<CS32>(p.cos, cs + 32 + lane * 4, ch);
-      load_f4<CS32>(p.sin, cs + lane * 4, sl);
-      load_f4<CS32>(p.sin, cs + 32 + lane * 4, sh);
-      bf16x8(pe_raw, pe);
-    }
+    const int64_t cs = p.pos != nullptr ? row * p.cs[1] : b * p.cs[0] + s * p.cs[1];
+    const float cl = load_f<CS32>(p.cos, cs + lane), ch = load_f<CS32>(p.cos, cs + 32 + lane);
+    const float sl = load_f<CS32>(p.sin, cs + lane), sh = load_f<CS32>(p.sin, cs + 32 + lane);
     float f[16];
     bf16x8(x0, f);
     bf16x8(x1, f + 8);
@@ -135,8 +132,13 @@ __global__ void __launch_bounds__(256) latent_write_kernel(const LatentWritePara
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     const float r = rsqrtf(sum * (1.f / kLatent) + p.eps);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
-    const int64_t page = slot / p.c.page_size, in_page = slot - page * p.c.page_size;
+    for (int i = 0; i < 16; i += 4) {  // the weights are in L1 after the first token: held from the start they cost residency
+      float w[4];
+      load_f4<W32>(p.w, (i >> 3) * 256 + lane * 8 + (i & 4), w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[i + j] = f[i + j] * r * w[j];
+    }
+    const int page = p.c.by_page(static_cast<int>(slot)), in_page = static_cast<int>(slot) - page * p.c.by_page.d;
     const int64_t dst = page * p.c.ls[0] + in_page * p.c.ls[1];
     if (FP8) {
       float top = 0.f;
@@ -162,22 +164,15 @@ __global__ void __launch_bounds__(256) latent_write_kernel(const LatentWritePara
       d[lane] = pack_bf16x8(f);
       d[32 + lane] = pack_bf16x8(f + 8);
     }
-    if (lane < 8) {
-      float lo[4], hi[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo[i] = pe[2 * i] * cl[i] - pe[2 * i + 1] * sl[i];
-        hi[i] = pe[2 * i + 1] * ch[i] + pe[2 * i] * sh[i];
-      }
-      __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.c.rope) + page * p.c.rs[0] + in_page * p.c.rs[1];
-      *reinterpret_cast<uint2*>(d + lane * 4) = make_uint2(pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]));
-      *reinterpret_cast<uint2*>(d + 32 + lane * 4) = make_uint2(pack_bf16(hi[0], hi[1]), pack_bf16(hi[2], hi[3]));
-    }
+    const float even = __uint_as_float(pe << 16), odd = __uint_as_float(pe & 0xFFFF0000u);
+    __nv_bfloat16* d = static_cast<__nv_bfloat16*>(p.c.rope) + page * p.c.rs[0] + in_page * p.c.rs[1];
+    d[lane] = __float2bfloat16_rn(even * cl - odd * sl);
+    d[32 + lane] = __float2bfloat16_rn(odd * ch + even * sh);
   }
 }
 
 template <bool FP8>
-__global__ void __launch_bounds__(256) latent_read_kernel(const LatentReadParams p) {
+__global__ void __launch_bounds__(256, 8) latent_read_kernel(const LatentReadParams p) {
   const int lane = threadIdx.x & 31;
   const uint32_t failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < p.n;
@@ -188,7 +183,7 @@ __global__ void __launch_bounds__(256) latent_read_kernel(const LatentReadParams
     if (slot >= p.c.slots) {
       if (lane == 0) report_index(p.status, kIdxSlot);
     } else if (slot >= 0) {
-      const int64_t page = slot / p.c.page_size, in_page = slot - page * p.c.page_size;
+      const int page = p.c.by_page(static_cast<int>(slot)), in_page = static_cast<int>(slot) - page * p.c.by_page.d;
       const int64_t src = page * p.c.ls[0] + in_page * p.c.ls[1];
       if (lane < 8)
         r = *(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.c.rope) + page * p.c.rs[0] +
@@ -228,6 +223,7 @@ int check_latent_cache(const pith_latent_cache& c) {
   PITH_REQUIRE(c.pages > 0 && (c.page_size == 16 || c.page_size == 32 || (c.page_size > 0 && c.page_size % 64 == 0)),
                "page_size must be 16, 32 or a multiple of 64 (got %d pages of %d)", c.pages, c.page_size);
   PITH_REQUIRE(c.latent && c.rope && (c.dtype == PITH_DTYPE_BF16 || c.scale), "null cache plane");
+  PITH_REQUIRE(static_cast<int64_t>(c.pages) * c.page_size < 2147483648ll, "a cache holds at most 2^31 - 1 rows");
   const int eb = c.dtype == PITH_DTYPE_BF16 ? 2 : 1;
   PITH_REQUIRE(aligned16(c.latent) && aligned16(c.rope) && (c.latent_stride[0] * eb) % 16 == 0 &&
                    (c.latent_stride[1] * eb) % 16 == 0 && c.rope_stride[0] % 8 == 0 && c.rope_stride[1] % 8 == 0,
@@ -241,7 +237,7 @@ int check_latent_cache(const pith_latent_cache& c) {
 static LatentPlanes planes_of(const pith_latent_cache& c) {
   LatentPlanes l;
   l.latent = c.latent; l.rope = c.rope; l.scale = c.scale;
-  l.page_size = c.page_size;
+  l.by_page = FastDiv(c.page_size);
   l.slots = static_cast<int64_t>(c.pages) * c.page_size;
   for (int i = 0; i < 2; ++i) { l.ls[i] = c.latent_stride[i]; l.rs[i] = c.rope_stride[i]; l.ss[i] = c.scale_stride[i]; }
   return l;
@@ -283,7 +279,9 @@ extern "C" int pith_latent_write(const pith_latent_write_args* a, void* stream) 
   p.pe = static_cast<const __nv_bfloat16*>(a->k_pe);
   p.w = a->norm_weight; p.cos = a->cos; p.sin = a->sin;
   p.slots = a->slots; p.pos = a->positions; p.status = a->status;
-  p.n = static_cast<int64_t>(a->B) * a->S; p.S = a->S; p.table_rows = a->table_rows; p.eps = a->eps;
+  p.n = static_cast<int64_t>(a->B) * a->S;
+  PITH_REQUIRE(p.n < 2147483648ll, "too many tokens for one call");
+  p.by_s = FastDiv(a->S); p.table_rows = a->table_rows; p.eps = a->eps;
   for (int i = 0; i < 2; ++i) {
     p.kvs[i] = a->kv_stride[i]; p.ps[i] = a->k_pe_stride[i]; p.cs[i] = a->cs_stride[i];
     p.sls[i] = a->slots_stride[i]; p.pos_s[i] = a->positions_stride[i];

@@ -7,8 +7,8 @@
 // W is used as the layer holds it: the query's B operand is read MN-major, the output's K-major; tcgen05 with accumulators in
 // TMEM, results stored by TMA, which clips the rows behind the last token. A row moves 1.5 KB (query) or 1.3 KB (output) for
 // 131 kFLOP: HBM bounds both at prompt sizes, latency at decode sizes, where narrow tiles spread the reading of W over more
-// CTAs (a kernel of one tile per CTA). Measured, 16 heads: 32 tokens 3.6 us (query) and 4.4 us (output); 4095 tokens 22.7 us
-// = 4.5 TB/s (0.70 of the measured copy rate) and 18.7 us = 4.6 TB/s (0.71), of which the launch, W and the first tile
+// CTAs (a kernel of one tile per CTA). Measured, 16 heads: 32 tokens 3.6 us (query) and 4.4 us (output); 4095 tokens 22.3 us
+// = 4.6 TB/s (0.71 of the measured copy rate) and 18.4 us = 4.7 TB/s (0.72), of which the launch, W and the first tile
 // take about 4 us.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
@@ -23,7 +23,8 @@ struct LatProjParams {
   const void* sin;
   const int64_t* pos;
   uint32_t* status;
-  int H, rows, S0;          // rows of the flattened (or per-batch) token axis; tokens per sequence of the caller's view
+  int H, rows;              // rows of the flattened (or per-batch) token axis
+  FastDiv by_s;             // tokens per sequence of the caller's view
   int cs_f32;
   int64_t table_rows;
   int64_t qs[3], cs[2], pos_s[2];
@@ -63,7 +64,7 @@ __device__ __forceinline__ void lat_rope_rows(const LatProjParams& p, int64_t g0
   for (int i = 0; i < PASSES; ++i) {
     ok[i] = i * 16 + (t >> 3) < rows;
     const int64_t g = g0 + (ok[i] ? i * 16 + (t >> 3) : 0);
-    const int64_t b = g / p.S0, s = g - b * p.S0;
+    const int b = p.by_s(static_cast<int>(g)), s = static_cast<int>(g) - b * p.by_s.d;
     from[i] = b * p.qs[0] + s * p.qs[1] + h * p.qs[2] + 128;
     cs[i] = b * p.cs[0] + s * p.cs[1];
     if (p.pos != nullptr) {
@@ -109,7 +110,7 @@ __device__ __forceinline__ void lat_rope_tokens(const LatProjParams& p, int64_t 
   const int l8 = t & 7;
   constexpr int kHeads = 16;
   for (int64_t g = g0 + (t >> 3); g < g1; g += 32) {
-    const int64_t b = g / p.S0, s = g - b * p.S0;
+    const int b = p.by_s(static_cast<int>(g)), s = static_cast<int>(g) - b * p.by_s.d;
     int64_t row = 0, cs = b * p.cs[0] + s * p.cs[1];
     if (p.pos != nullptr) row = __ldg(p.pos + b * p.pos_s[0] + s * p.pos_s[1]);
     const __nv_bfloat16* src = p.q + b * p.qs[0] + s * p.qs[1] + 128;
@@ -316,8 +317,8 @@ struct RunCfg {
 template <bool QUERY>
 __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     latent_proj_run_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
-                           const __grid_constant__ CUtensorMap tm_out, const LatProjParams p, int tile, int mtiles, int items,
-                           int per_group, int64_t tokens) {
+                           const __grid_constant__ CUtensorMap tm_out, const LatProjParams p, int tile, FastDiv by_tiles,
+                           FastDiv by_groups, int items, int per_group, int tokens, int token_share) {
   using L = RunCfg<QUERY>;
   constexpr int NT = L::NT, NN = L::NN, KB = L::KB, ST = L::ST;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -338,9 +339,9 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
   const int me = blockIdx.x, ctas = gridDim.x;
   int i0, i1, step;
   if (per_group > 0) {
-    const int groups = items / mtiles, g = me % groups;
-    i0 = g * mtiles + me / groups;
-    i1 = (g + 1) * mtiles;
+    const int first = by_groups(me), g = me - first * by_groups.d;
+    i0 = g * by_tiles.d + first;
+    i1 = (g + 1) * by_tiles.d;
     step = per_group;
   } else {
     const int share = items / ctas, more = items - share * ctas;
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
       uint32_t s = 0, ph = 1, bph = 1;
       int group = -1;
       for (int it = i0; it < i1; it += step) {
-        const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
+        const int g = by_tiles(it), m0 = (it - g * by_tiles.d) * tile;
         const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
         if (g != group) {
           group = g;
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     uint32_t n = 0;
     for (int it = i0; it < i1; it += step, ++n) {
       const uint32_t buf = n & 1;
-      const int g = it / mtiles;
+      const int g = by_tiles(it);
       if (g != group) {
         group = g;
         mbar_wait(b_full, bph, ctl, 0x300);
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
       }
       if (leader) {
         umma_commit(&acc_full[buf]);
-        if (it + step < i1 && (it + step) / mtiles != g) umma_commit(b_empty);
+        if (it + step < i1 && by_tiles(it + step) != g) umma_commit(b_empty);
       }
     }
   } else if (warp >= 4 && warp < 8) {
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     uint32_t n = 0;
     for (int it = i0; it < i1; it += step, ++n) {
       const uint32_t buf = n & 1;
-      const int g = it / mtiles, m0 = (it - g * mtiles) * tile;
+      const int g = by_tiles(it), m0 = (it - g * by_tiles.d) * tile;
       const int nt = g % NN, h = g / NN % p.H, b = g / NN / p.H;
       mbar_wait(&acc_full[buf], (n >> 1) & 1, ctl, 0x800 + buf);
       tc_fence_after_sync();
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     // an equal share of the tokens, whatever the CTA's items: with the rotary part of its own (head, token) rows every head
     // read the tables again, and the kernel waited for these warps (33.7 us)
     if (*abort_flag == 0u)
-      lat_rope_tokens(p, tokens * me / gridDim.x, tokens * (me + 1) / gridDim.x, static_cast<int>(threadIdx.x) - 256);
+      lat_rope_tokens(p, static_cast<int64_t>(me) * token_share, min(tokens, (me + 1) * token_share), static_cast<int>(threadIdx.x) - 256);
   }
 
   tc_fence_before_sync();
@@ -529,8 +530,9 @@ static int launch_proj_run(const pith_latent_proj_args* a, const LatProjParams& 
   const int64_t mt = (S + tile - 1) / tile, items = mt * groups;
   PITH_REQUIRE(items < 2147483647 - 1024, "too many tokens, heads or sequences");
   const int64_t ctas = per_group > 0 ? groups * per_group : items < sms ? items : sms;
-  kern<<<static_cast<unsigned>(ctas), L::kThreads, L::kAlloc, st>>>(ta, tw, to, p, tile, static_cast<int>(mt),
-                                                                   static_cast<int>(items), per_group, B * S);
+  kern<<<static_cast<unsigned>(ctas), L::kThreads, L::kAlloc, st>>>(
+      ta, tw, to, p, tile, FastDiv(static_cast<int>(mt)), FastDiv(static_cast<int>(groups)), static_cast<int>(items), per_group,
+      static_cast<int>(B * S), static_cast<int>((B * S + ctas - 1) / ctas));
   PITH_CUDA(cudaGetLastError());
   return kOk;
 }
@@ -567,6 +569,7 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
     PITH_REQUIRE(aligned16(a->x) && a->x_stride[0] % 8 == 0 && a->x_stride[1] % 8 == 0 && a->x_stride[2] % 8 == 0,
                  "q must be 16-byte aligned with strides that are multiples of 8 elements");
   }
+  PITH_REQUIRE(static_cast<int64_t>(a->B) * a->S < 2147483647 - 65536, "too many tokens");
   if (int rc = require_sm100()) return rc;
   // One token axis where the strides allow it: a batch of single tokens fills the tiles.
   int64_t B = a->B, S = a->S;
@@ -580,12 +583,11 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
   if (a->H == 1) xs[2] = QUERY ? 192 : 512;  // strides of axes of one element say nothing
   if (S == 1) xs[1] = a->H * xs[2];
   if (B == 1) xs[0] = S * xs[1];
-  PITH_REQUIRE(S < 2147483647 - 256, "too many tokens");
   LatProjParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->x);
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.cos = a->cos; p.sin = a->sin; p.pos = a->positions; p.status = a->status;
-  p.H = a->H; p.rows = static_cast<int>(S); p.S0 = a->S; p.cs_f32 = a->cs_dtype == PITH_DTYPE_F32;
+  p.H = a->H; p.rows = static_cast<int>(S); p.by_s = FastDiv(a->S); p.cs_f32 = a->cs_dtype == PITH_DTYPE_F32;
   p.table_rows = a->table_rows;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->x_stride[i];
   for (int i = 0; i < 2; ++i) { p.cs[i] = a->cs_stride[i]; p.pos_s[i] = a->positions_stride[i]; }
