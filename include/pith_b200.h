@@ -402,7 +402,8 @@ typedef struct pith_latent_attn_args {
   const int32_t* seq_lens;    /* [B]: keys of a sequence, its new tokens among them; 0 .. table_cols * page_size */
   const int32_t* query_lens;  /* optional [B]: new tokens of a sequence, 0 .. Sq (default: Sq) */
   const uint8_t* tree_mask;   /* optional [B][Sq][Sq]: non-zero = new token i sees new token j */
-  void* workspace;            /* pith_latent_attn_workspace_bytes(...), not shared with a call that may run beside this one */
+  void* workspace;            /* pith_latent_attn_workspace_bytes(...), null where that is 0; not shared with a call that may
+                                 run beside this one */
   uint32_t* status;
   size_t workspace_bytes;
   int32_t B, Sq, H, table_cols;

@@ -762,7 +762,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     }
     tc_fence_before_sync();
   }
-  if (g == 0 && t == 0) p.part_info[blockIdx.x] = info;
+  if (g == 0 && t == 0 && p.part_info != nullptr) p.part_info[blockIdx.x] = info;
 }
 
 template <int NT, bool FP8>
@@ -1203,6 +1203,7 @@ using namespace pith;
 
 extern "C" size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t dtype) {
   if (B <= 0 || Sq <= 0 || H <= 0) return 0;
+  if (max_keys <= lat_unit(max_keys)) return 0;  // no entry is ever cut
   const int nt = lat_rows(static_cast<int64_t>(Sq) * H, dtype == PITH_DTYPE_E4M3);
   int ctas = 0;
   if (lat_ctas(static_cast<int64_t>(B) * ((static_cast<int64_t>(Sq) * H + nt - 1) / nt), max_keys, &ctas)) return 0;
@@ -1215,7 +1216,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   if (int rc = check_latent_cache(a->cache)) return rc;
   PITH_REQUIRE(a->softmax_scale > 0.f, "softmax_scale must be positive");
   if (a->B == 0 || a->Sq == 0 || a->H == 0) return kOk;
-  PITH_REQUIRE(a->q && a->out && a->block_table && a->seq_lens && a->workspace, "null tensor pointer");
+  PITH_REQUIRE(a->q && a->out && a->block_table && a->seq_lens, "null tensor pointer");
   PITH_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->workspace) && a->q_stride[0] % 8 == 0 &&
                    a->q_stride[1] % 8 == 0 && a->q_stride[2] % 8 == 0,
                "q, out and workspace must be 16-byte aligned, q with strides that are multiples of 8 elements");
@@ -1250,14 +1251,17 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   for (int i = 0; i < 2; ++i) { p.tree_stride[i] = a->tree_stride[i]; p.scale_stride[i] = a->cache.scale_stride[i]; }
   int ctas = 1;
   if (int rc = lat_ctas(rt * a->B, p.max_keys, &ctas)) return rc;
-  PITH_REQUIRE(a->workspace_bytes >= static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16,
-               "workspace too small");
-  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  ws += static_cast<size_t>(ctas) * 2 * nt * kLat * 4;
-  p.part_info = reinterpret_cast<int4*>(ws);
-  ws += static_cast<size_t>(ctas) * 16;
-  p.part_ml = reinterpret_cast<float2*>(ws);
+  if (p.max_keys > (1 << p.unit_log2)) {
+    PITH_REQUIRE(a->workspace, "null workspace");
+    PITH_REQUIRE(a->workspace_bytes >= static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16,
+                 "workspace too small");
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    p.part_o = reinterpret_cast<float*>(ws);
+    ws += static_cast<size_t>(ctas) * 2 * nt * kLat * 4;
+    p.part_info = reinterpret_cast<int4*>(ws);
+    ws += static_cast<size_t>(ctas) * 16;
+    p.part_ml = reinterpret_cast<float2*>(ws);
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fp8) return nt == 16 ? launch_latent_attn<16, true>(a, p, ctas, st) : launch_latent_attn<32, true>(a, p, ctas, st);
   if (nt == 16) return launch_latent_attn<16, false>(a, p, ctas, st);
