@@ -1220,7 +1220,7 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   PITH_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->workspace) && a->q_stride[0] % 8 == 0 &&
                    a->q_stride[1] % 8 == 0 && a->q_stride[2] % 8 == 0,
                "q, out and workspace must be 16-byte aligned, q with strides that are multiples of 8 elements");
-  PITH_REQUIRE(a->table_cols >= 0 && static_cast<int64_t>(a->table_cols) * a->cache.page_size < 2147483647 - 256,
+  PITH_REQUIRE(a->table_cols >= 0 && static_cast<int64_t>(a->table_cols) * a->cache.page_size < 2147483647 - 1024,
                "the block table covers too many keys");
   const int64_t rows = static_cast<int64_t>(a->Sq) * a->H;
   PITH_REQUIRE(rows < 2147483647 - 256, "too many query rows");

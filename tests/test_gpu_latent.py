@@ -374,6 +374,42 @@ def test_a_key_that_is_not_finite_reaches_only_the_rows_that_see_it(cuda_device,
     assert torch.equal(o[:, :5], want[:, :5]) and o[:, 5].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("first", [10, 140])
+def test_keys_that_are_not_finite_in_several_tiles(cuda_device, dtype, first):
+    """New tokens that span more than one tile of keys, three of them with values that are not finite: the rows in front of
+    the first see none of them."""
+    g = torch.Generator(device="cuda").manual_seed(first)
+    S, H, lens = 200, 2, [500, 230]
+    cache, table = filled_cache(g, lens, 16, dtype)
+    q = torch.randn(2, S, H, 576, generator=g, device="cuda").bfloat16()
+    want = assert_attention(q, cache, table, lens, SCALE)[0]
+    for b in range(2):
+        rows = slots_of(table[b], lens[b], 16)[lens[b] - S:]
+        for at, column in ((first, 0), (first + 1, 511), (first + 50, 200)):
+            cache.latent.view(-1, 512).view(torch.uint8).view(-1, 512, 1 if dtype == E4M3 else 2)[rows[at], column] = \
+                0x7F if dtype == E4M3 else 0xFF
+    o = run_attention(q, cache, table, lens, SCALE)[0]
+    check()
+    assert torch.equal(o[:, :first], want[:, :first]) and o[:, first:].isnan().any(-1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("B,S,H,longest,page,kind", [
+    (170, 2, 16, 400, 16, "causal"), (60, 5, 16, 700, 32, "tree"), (300, 1, 16, 300, 192, "causal"),
+    (160, 2, 16, 128, 64, "padded"), (45, 13, 8, 1500, 320, "tree"), (30, 16, 16, 600, 48 * 4, "padded"),
+    (400, 1, 16, 100, 16, "causal"), (200, 2, 16, 60, 64, "padded")])  # the last ones: no sequence can pass 128 keys
+def test_many_sequences_of_uneven_lengths(cuda_device, dtype, B, S, H, longest, page, kind):
+    """Several pieces for every CTA, some of them without keys, and every way of counting pages."""
+    r = torch.Generator().manual_seed(B + S + page)
+    lens = torch.randint(S if kind == "tree" else 0, longest + 1, (B,), generator=r).tolist()
+    qlens = torch.randint(0, S + 1, (B,), generator=r).tolist() if kind == "padded" else None
+    g = torch.Generator(device="cuda").manual_seed(B)
+    cache, table = filled_cache(g, lens, page, dtype)
+    q = torch.randn(B, S, H, 576, generator=g, device="cuda").bfloat16()
+    assert_attention(q, cache, table, lens, SCALE, qlens, random_tree(r, B, S) if kind == "tree" else None)
+
+
 def test_a_row_factor_that_is_not_finite_reaches_only_the_rows_that_see_it(cuda_device):
     g = torch.Generator(device="cuda").manual_seed(17)
     S, H, lens = 4, 16, [300, 70]
