@@ -48,7 +48,9 @@ constexpr int kLat = 512, kRp = 64;
 constexpr int kTile = 128;  // keys per tile
 constexpr int kBox = 64;    // rows of a TMA box at most; work is cut at its multiples
 constexpr int kMaxExtra = 8;
-constexpr int kOwnRows = 8;  // query rows that the loader converts where the softmax warps do the others
+// Query rows that the loader converts where the softmax warps do the others: an equal share of a CTA's first query; of later
+// ones it may begin before those warps have finished with the piece.
+__device__ __forceinline__ int loader_rows(uint32_t piece) { return piece == 0 ? 4 : 8; }
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
 
@@ -438,7 +440,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     if constexpr (L::kHelp) {
       if (tiles > 0) {  // the last score GEMM of the previous piece has completed: this warpgroup has read its scores
         uint8_t* sq = sm.base + L::kQOff;
-        const int row0 = kOwnRows + 4 * g + w;
+        const int row0 = loader_rows(piece) + 4 * g + w;
         if (piece == 0) {
           fetch_query_rows<NT>(p, sq, x, row0, NT, 4 * L::G, lane);
           __syncwarp();
@@ -1019,10 +1021,10 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
         uint8_t* sq = smem + L::kQOff;
         mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
         if constexpr (L::kHelp) {  // the softmax warps fetch their own rows of a CTA's first query, and find those of later ones
-          fetch_query_rows<NT>(p, sq, walk.x, 0, piece == 0 ? kOwnRows : NT, 1, lane);
+          fetch_query_rows<NT>(p, sq, walk.x, 0, piece == 0 ? loader_rows(0) : NT, 1, lane);
           if (piece > 0) asm volatile("bar.arrive 4, %0;" ::"n"(128 * L::G + 32) : "memory");
           __syncwarp();
-          split_query_rows<NT>(sq, sm.qk(piece & 1), 0, kOwnRows, 1, lane);
+          split_query_rows<NT>(sq, sm.qk(piece & 1), 0, loader_rows(piece), 1, lane);
         } else if constexpr (FP8) {
           fetch_query_rows<NT>(p, sq, walk.x, loader, NT, L::kLoadWarps, lane);
           __syncwarp();
