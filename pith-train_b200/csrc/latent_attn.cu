@@ -34,9 +34,9 @@
 // Measured (16 heads, CUDA events over a captured graph): 64 sequences of 130 to 8191 keys, bf16: 65 us, 4.8 TB/s, 0.74 of
 // the measured copy rate; the loop itself streams 6 TB/s, the rest is 3 us until the first load, the pieces' ends and the
 // merge. 8 sequences of 9000 to 131071 keys, e4m3: 75 us, 5.5 TB/s, 0.86. Shorter tiles (64 keys, more of the ring in
-// flight) were slower: 75 and 122 us. 250 tokens of a prompt over 6001 keys, bf16: 79 us, 650 TFLOP/s, the serial chain score
+// flight) were slower: 75 and 122 us. 250 tokens of a prompt over 6001 keys, bf16: 78 us, 650 TFLOP/s, the serial chain score
 // GEMM (2.2k cycles) - softmax (1.5k) - output GEMM (1.5k) of a tile; the expanded form is the one for long chunks. 16 trees
-// of 13 tokens over 500 to 4097 keys, e4m3: 49 us; a tile takes 2600 cycles (its MMAs 1750), as the slots of the tile after
+// of 13 tokens over 500 to 4097 keys, e4m3: 48 us; a tile takes 2600 cycles (its MMAs 1750), as the slots of the tile after
 // the next are free, and loaded, only once this tile's output GEMM has completed, and a piece's begin and end take as long
 // as four.
 #include "common.cuh"
