@@ -416,7 +416,8 @@ typedef struct pith_latent_attn_args {
  * Attention in the absorbed MLA form over the cache: all H heads of the Sq new tokens of a sequence read the same keys.
  * With n keys and m new tokens, token i sees key k iff k <= n - m + i, or with a tree mask iff k < n - m or
  * tree_mask[i][k - (n - m)]. A row that sees nothing, or has no token, gives out 0, lse -inf. Keys are read up to
- * seq_lens only: pages behind it need not exist. Two launches (one when no sequence can pass 128 keys).
+ * seq_lens only: pages behind it need not exist. Two launches, or one where no
+ * sequence can pass 128 keys, or 1024 and cutting them over the SMs would not pay.
  */
 int pith_latent_attn(const pith_latent_attn_args* args, void* stream);
 size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t cache_dtype);

@@ -1152,17 +1152,25 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
 // memory hold beside a whole 128-key tile.
 static int lat_rows(int64_t rows, bool fp8) { return rows <= 16 ? 16 : rows <= 32 || fp8 ? 32 : 64; }
 
-// Keys per unit of work: 64; where no sequence can pass one tile, a tile, so that nothing is cut and nothing merged.
-static int lat_unit(int64_t max_keys) { return max_keys <= kTile ? kTile : kBox; }
-
-static int lat_ctas(int64_t entries, int64_t max_keys, int* ctas) {
+// Keys per unit of work, and CTAs. The unit is 64 keys. Where no sequence can pass one tile, and where cutting would not pay
+// for the merge, it is all of a sequence: nothing is cut then, and one launch does. With a CTA for each of E entries of at
+// most T tiles, cutting saves up to T (1 - E / SMs) tiles; the merge takes about as long as 3.6 tiles in bf16 and 6.6 in 8
+// bits (and another launch from the host). Measured, cut against whole, 16 heads, us: bf16, one sequence of 256 keys 10.2 and
+// 9.6, of 512 keys 10.9 and 13.5, 148 of up to 512 26.9 and 20.9, of up to 1024 36.1 and 32.6; 8-bit, one of 512 keys 11.3
+// and 11.2, of 1024 11.8 and 15.5, 148 of up to 1024 26.8 and 21.0. The lengths behind E are not known here, so sequences
+// of more than 1024 keys are always cut.
+constexpr int kWhole = 1024;
+struct LatPlan { int unit_log2, ctas; };
+static int lat_plan(int64_t entries, int64_t max_keys, bool fp8, LatPlan* plan) {
   int dev = 0, sms = 148;
   PITH_CUDA(cudaGetDevice(&dev));
   PITH_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   if (sms > kMergeThreads) sms = kMergeThreads;  // the merge looks at one CTA per thread
-  const int unit = lat_unit(max_keys);
-  const int64_t units = entries * (max_keys <= unit ? 1 : (max_keys + unit - 1) / unit);
-  *ctas = static_cast<int>(units < sms ? units : sms);
+  const int64_t tiles = (max_keys + kTile - 1) / kTile;
+  const bool whole = max_keys <= kWhole && entries <= sms && tiles * (sms - entries) * 10 <= sms * (fp8 ? 66 : 36);
+  plan->unit_log2 = max_keys <= kTile ? 7 : whole ? 10 : 6;
+  const int64_t unit = 1ll << plan->unit_log2, units = entries * (max_keys <= unit ? 1 : (max_keys + unit - 1) / unit);
+  plan->ctas = static_cast<int>(units < sms ? units : sms);
   return kOk;
 }
 
@@ -1205,11 +1213,13 @@ using namespace pith;
 
 extern "C" size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t dtype) {
   if (B <= 0 || Sq <= 0 || H <= 0) return 0;
-  if (max_keys <= lat_unit(max_keys)) return 0;  // no entry is ever cut
   const int nt = lat_rows(static_cast<int64_t>(Sq) * H, dtype == PITH_DTYPE_E4M3);
-  int ctas = 0;
-  if (lat_ctas(static_cast<int64_t>(B) * ((static_cast<int64_t>(Sq) * H + nt - 1) / nt), max_keys, &ctas)) return 0;
-  return static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16;
+  LatPlan plan;
+  if (lat_plan(static_cast<int64_t>(B) * ((static_cast<int64_t>(Sq) * H + nt - 1) / nt), max_keys,
+               dtype == PITH_DTYPE_E4M3, &plan))
+    return 0;
+  if (max_keys <= (1ll << plan.unit_log2)) return 0;  // no entry is ever cut
+  return static_cast<size_t>(plan.ctas) * (2 * nt * (kLat * 4 + 8) + 16);
 }
 
 extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
@@ -1241,7 +1251,6 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.B = a->B; p.Sq = a->Sq; p.H = a->H; p.R = static_cast<int>(rows); p.RT = static_cast<int>(rt);
   p.pages = a->cache.pages; p.page_size = a->cache.page_size;
   p.max_keys = a->table_cols * a->cache.page_size;
-  p.unit_log2 = lat_unit(p.max_keys) == kTile ? 7 : 6;
   p.by_h = FastDiv(p.H);
   p.by_rt = FastDiv(p.RT);
   p.by_page = FastDiv(p.page_size);
@@ -1251,8 +1260,10 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i];
   p.table_stride = a->table_stride;
   for (int i = 0; i < 2; ++i) { p.tree_stride[i] = a->tree_stride[i]; p.scale_stride[i] = a->cache.scale_stride[i]; }
-  int ctas = 1;
-  if (int rc = lat_ctas(rt * a->B, p.max_keys, &ctas)) return rc;
+  LatPlan plan;
+  if (int rc = lat_plan(rt * a->B, p.max_keys, fp8, &plan)) return rc;
+  const int ctas = plan.ctas;
+  p.unit_log2 = plan.unit_log2;
   if (p.max_keys > (1 << p.unit_log2)) {
     PITH_REQUIRE(a->workspace, "null workspace");
     PITH_REQUIRE(a->workspace_bytes >= static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16,

@@ -594,7 +594,7 @@ def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query
     args = _ATTN(*cache.flat, query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
                  block_table.data_ptr(), seq_lens.data_ptr(), ql, tm, workspace.data_ptr() if nbytes else 0, _status_ptr(idx), nbytes,
                  B, S, H, t_shape[1], softmax_scale, q_stride[0], q_stride[1], q_stride[2], block_table.stride(0), tm0, tm1)
-    _enqueue("pith_latent_attn", args, idx, (2 if max_keys > 128 else 1) if B * S * H else 0)
+    _enqueue("pith_latent_attn", args, idx, (2 if nbytes else 1) if B * S * H else 0)
     return out, lse
 
 

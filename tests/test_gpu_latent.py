@@ -398,7 +398,9 @@ def test_keys_that_are_not_finite_in_several_tiles(cuda_device, dtype, first):
 @pytest.mark.parametrize("B,S,H,longest,page,kind", [
     (170, 2, 16, 400, 16, "causal"), (60, 5, 16, 700, 32, "tree"), (300, 1, 16, 300, 192, "causal"),
     (160, 2, 16, 128, 64, "padded"), (45, 13, 8, 1500, 320, "tree"), (30, 16, 16, 600, 48 * 4, "padded"),
-    (400, 1, 16, 100, 16, "causal"), (200, 2, 16, 60, 64, "padded")])  # the last ones: no sequence can pass 128 keys
+    (400, 1, 16, 100, 16, "causal"), (200, 2, 16, 60, 64, "padded"),   # no sequence can pass 128 keys
+    (90, 2, 16, 700, 64, "causal"), (140, 1, 16, 900, 16, "padded"), (1, 1, 16, 300, 32, "causal"),
+    (100, 4, 4, 1000, 128, "tree")])  # one CTA each for most of these
 def test_many_sequences_of_uneven_lengths(cuda_device, dtype, B, S, H, longest, page, kind):
     """Several pieces for every CTA, some of them without keys, and every way of counting pages."""
     r = torch.Generator().manual_seed(B + S + page)
