@@ -20,7 +20,8 @@
 // reference are dropped.
 //
 // Work split: the (sequence, row tile, 64 keys) units of the launch form one line which is cut into one equal piece per
-// CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device). A piece that
+// CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device; short sequences
+// stay whole, see lat_plan). A piece that
 // covers a row tile completely stores its result; the others store an fp32 partial (O, ref, l), at most two per CTA, and
 // the merge kernel adds them in key order.
 //
@@ -128,7 +129,9 @@ __device__ __forceinline__ LatEntry lat_entry(const LatAttnParams& p, int e) {
   x.keys = p.by_h(x.r0) >= x.nq ? 0 : p.tree != nullptr ? x.len : max(min(x.len, x.len - x.nq + last + 1), 0);
   return x;
 }
-__device__ __forceinline__ int lat_units(const LatAttnParams& p, int keys) { return max((keys + (1 << p.unit_log2) - 1) >> p.unit_log2, 1); }
+__device__ __forceinline__ int lat_units(const LatAttnParams& p, int keys) {
+  return max((keys + (1 << p.unit_log2) - 1) >> p.unit_log2, 1);
+}
 
 // Walks the pieces of this CTA's share of the line. Every role keeps its own copy. An entry takes `extra` places of the line
 // in front of its units: what beginning another piece costs a CTA.
@@ -477,7 +480,8 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     float next_ks = 1.f;
     const auto fetch_page = [&](int n) { next_page = n < walk.k1 ? __ldg(p.table + x.b * p.table_stride + at.index) : -1; };
     const auto fetch_factor = [&](int n) {
-      next_ks = next_page >= 0 && next_page < p.pages ? p.scale[next_page * p.scale_stride[0] + at.row * p.scale_stride[1]] : 1.f;
+      const bool there = next_page >= 0 && next_page < p.pages;
+      next_ks = there ? p.scale[next_page * p.scale_stride[0] + at.row * p.scale_stride[1]] : 1.f;
       at.next_tile(p);
       fetch_page(n + kTile);
     };
@@ -508,7 +512,8 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
         const uint8_t* mask = in_tree ? p.tree + x.b * p.tree_stride[0] + (n - (x.len - x.nq)) : p.tree;
         uint8_t m[CW];
 #pragma unroll
-        for (int c = 0; c < CW; ++c) m[c] = __ldg(mask + (in_tree && n >= sm.lim()[cb + c] ? sm.tok()[cb + c] * p.tree_stride[1] : 0));
+        for (int c = 0; c < CW; ++c)
+          m[c] = __ldg(mask + (in_tree && n >= sm.lim()[cb + c] ? sm.tok()[cb + c] * p.tree_stride[1] : 0));
         shown_to = 0u;
 #pragma unroll
         for (int c = 0; c < CW; ++c) shown_to |= (n < sm.lim()[cb + c] || m[c] != 0 ? 1u : 0u) << c;
@@ -803,7 +808,8 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge kernel may be set up; it waits for this grid's end
+  // the merge kernel may be set up; it waits for this grid's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // This CTA's share of the work line: every thread counts a run of entries, then a scan over the CTA.
   const int entries = p.B * p.RT;
   const int run = (entries + L::kThreads - 1) / L::kThreads;

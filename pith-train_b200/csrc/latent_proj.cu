@@ -478,7 +478,8 @@ __global__ void __launch_bounds__(RunCfg<QUERY>::kThreads, 1)
     // an equal share of the tokens, whatever the CTA's items: with the rotary part of its own (head, token) rows every head
     // read the tables again, and the kernel waited for these warps (33.7 us)
     if (*abort_flag == 0u)
-      lat_rope_tokens(p, static_cast<int64_t>(me) * token_share, min(tokens, (me + 1) * token_share), static_cast<int>(threadIdx.x) - 256);
+      lat_rope_tokens(p, static_cast<int64_t>(me) * token_share, min(tokens, (me + 1) * token_share),
+                      static_cast<int>(threadIdx.x) - 256);
   }
 
   tc_fence_before_sync();

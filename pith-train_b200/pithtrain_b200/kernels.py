@@ -592,8 +592,9 @@ def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query
     nbytes = _attn_workspace(idx, B, S, H, max_keys, cache.flat[3])
     workspace = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     args = _ATTN(*cache.flat, query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                 block_table.data_ptr(), seq_lens.data_ptr(), ql, tm, workspace.data_ptr() if nbytes else 0, _status_ptr(idx), nbytes,
-                 B, S, H, t_shape[1], softmax_scale, q_stride[0], q_stride[1], q_stride[2], block_table.stride(0), tm0, tm1)
+                 block_table.data_ptr(), seq_lens.data_ptr(), ql, tm, workspace.data_ptr() if nbytes else 0,
+                 _status_ptr(idx), nbytes, B, S, H, t_shape[1], softmax_scale, q_stride[0], q_stride[1], q_stride[2],
+                 block_table.stride(0), tm0, tm1)
     _enqueue("pith_latent_attn", args, idx, (2 if nbytes else 1) if B * S * H else 0)
     return out, lse
 
