@@ -21,9 +21,8 @@
 //
 // Work split: the (sequence, row tile, 64 keys) units of the launch form one line which is cut into one equal piece per
 // CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device; short sequences
-// stay whole, see lat_plan). A piece that
-// covers a row tile completely stores its result; the others store an fp32 partial (O, ref, l), at most two per CTA, and
-// the merge kernel adds them in key order.
+// stay whole, see lat_plan). A piece that covers a row tile completely stores its result; the others store an fp32 partial
+// (O, ref, l), at most two per CTA, and the merge kernel adds them in key order.
 //
 // Roles: warp 0 TMA producer (one lane per page), warp 1 issues the score GEMMs, warp 2 the output GEMMs, warp 3 loads
 // queries (with one or three more for NT = 16, and the softmax warps' help for NT = 32, 8-bit), one or two warpgroups softmax
@@ -51,7 +50,7 @@ constexpr int kBox = 64;    // rows of a TMA box at most; work is cut at its mul
 constexpr int kMaxExtra = 8;
 // Query rows that the loader converts where the softmax warps do the others: an equal share of a CTA's first query; of later
 // ones it may begin before those warps have finished with the piece.
-__device__ __forceinline__ int loader_rows(uint32_t piece) { return piece == 0 ? 4 : 8; }
+__device__ __forceinline__ int loader_rows(uint32_t loads) { return loads == 0 ? 4 : 8; }
 constexpr float kNoRef = -1e30f;  // reference of a row that has seen no key (finite: -inf - ref must stay -inf)
 constexpr int kColS = 256, kColR = 384;  // TMEM columns of S^T and of its rope part (8-bit), two of each; O^T starts at 0
 
@@ -416,7 +415,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
   const int w = t >> 5, lane = t & 31, cb = g * CW;
   const uint32_t bar = 1 + g;               // named barrier of this warpgroup; 3 = all softmax warpgroups
   const uint32_t tl = tmem + (static_cast<uint32_t>(w << 5) << 16);
-  uint32_t tile = 0, slot0 = 0, piece = 0;
+  uint32_t tile = 0, slot0 = 0, piece = 0, loads = 0;  // loads: pieces with keys, whose queries are loaded
   int4 info = make_int4(-1, -1, -1, 0);
   while (walk.next(p)) {
     const LatEntry x = walk.x;
@@ -443,20 +442,21 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
     if constexpr (L::kHelp) {
       if (tiles > 0) {  // the last score GEMM of the previous piece has completed: this warpgroup has read its scores
         uint8_t* sq = sm.base + L::kQOff;
-        const int row0 = loader_rows(piece) + 4 * g + w;
-        if (piece == 0) {
+        const int row0 = loader_rows(loads) + 4 * g + w;
+        if (loads == 0) {
           fetch_query_rows<NT>(p, sq, x, row0, NT, 4 * L::G, lane);
           __syncwarp();
         } else {
           named_bar_sync(4, 128 * L::G + 32);
         }
-        split_query_rows<NT>(sq, sm.qk(piece & 1), row0, NT, 4 * L::G, lane);
+        split_query_rows<NT>(sq, sm.qk(loads & 1), row0, NT, 4 * L::G, lane);
         fence_proxy_async_smem();
         mbar_arrive(sm.q_full());
       }
     }
-    const float* qk = sm.qk(piece & 1) + cb;
+    const float* qk = sm.qk(loads & 1) + cb;
     ++piece;
+    if (tiles > 0) ++loads;
     float l[CW];
 #pragma unroll
     for (int c = 0; c < CW; ++c) l[c] = 0.f;
@@ -1020,29 +1020,31 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
   } else {
     // ------------------------------------------------------------------ query loaders, one piece ahead
     const int loader = warp < 4 ? 0 : warp - 3 - 4 * L::G;
-    uint32_t q_phase = 1, piece = 0;
+    // Query factors alternate between two places by the pieces that have keys: one without may lie between two that do, and
+    // the softmax may still be reading those of the piece before it.
+    uint32_t q_phase = 1, loads = 0;
     while (walk.next(p)) {
       const int tiles = walk.tiles();
       if (tiles > 0) {
         uint8_t* sq = smem + L::kQOff;
         mbar_wait(sm.q_empty(), q_phase, ctl, 0x380);  // the previous piece's last score GEMM has read its query
         if constexpr (L::kHelp) {  // the softmax warps fetch their own rows of a CTA's first query, and find those of later ones
-          fetch_query_rows<NT>(p, sq, walk.x, 0, piece == 0 ? loader_rows(0) : NT, 1, lane);
-          if (piece > 0) asm volatile("bar.arrive 4, %0;" ::"n"(128 * L::G + 32) : "memory");
+          fetch_query_rows<NT>(p, sq, walk.x, 0, loads == 0 ? loader_rows(0) : NT, 1, lane);
+          if (loads > 0) asm volatile("bar.arrive 4, %0;" ::"n"(128 * L::G + 32) : "memory");
           __syncwarp();
-          split_query_rows<NT>(sq, sm.qk(piece & 1), 0, loader_rows(piece), 1, lane);
+          split_query_rows<NT>(sq, sm.qk(loads & 1), 0, loader_rows(loads), 1, lane);
         } else if constexpr (FP8) {
           fetch_query_rows<NT>(p, sq, walk.x, loader, NT, L::kLoadWarps, lane);
           __syncwarp();
-          split_query_rows<NT>(sq, sm.qk(piece & 1), loader, NT, L::kLoadWarps, lane);
+          split_query_rows<NT>(sq, sm.qk(loads & 1), loader, NT, L::kLoadWarps, lane);
         } else {
           load_query<NT>(p, sq, walk.x, loader * 32 + lane, L::kLoadWarps * 32);
         }
         q_phase ^= 1;
         fence_proxy_async_smem();
         mbar_arrive(sm.q_full());
+        ++loads;
       }
-      ++piece;
     }
   }
 

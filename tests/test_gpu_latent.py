@@ -395,6 +395,20 @@ def test_keys_that_are_not_finite_in_several_tiles(cuda_device, dtype, first):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("S", [1, 2])
+def test_sequences_without_keys_between_others(cuda_device, dtype, S):
+    """Every other sequence is empty, and the queries' sizes differ from sequence to sequence (as do an 8-bit query's factors)."""
+    r = torch.Generator().manual_seed(S)
+    lens = [0 if b % 2 else int(torch.randint(S, 200, (), generator=r)) for b in range(500)]
+    g = torch.Generator(device="cuda").manual_seed(S)
+    cache, table = filled_cache(g, lens, 32, dtype)
+    q = torch.randn(500, S, 16, 576, generator=g, device="cuda")
+    q = (q * 2.0 ** torch.randint(-6, 3, (500, 1, 16, 1), generator=g, device="cuda")).bfloat16()
+    o, l = assert_attention(q, cache, table, lens, SCALE)
+    assert not o[1::2].any() and (l[1::2] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
 @pytest.mark.parametrize("B,S,H,longest,page,kind", [
     (170, 2, 16, 400, 16, "causal"), (60, 5, 16, 700, 32, "tree"), (300, 1, 16, 300, 192, "causal"),
     (160, 2, 16, 128, 64, "padded"), (45, 13, 8, 1500, 320, "tree"), (30, 16, 16, 600, 48 * 4, "padded"),
