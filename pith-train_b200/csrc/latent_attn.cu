@@ -107,6 +107,7 @@ struct LatAttnParams {
   uint32_t* status;
   int B, Sq, H, R, RT, pages, page_size, max_keys;
   int unit_log2;          // keys per unit of work
+  int whole;              // a unit is all of an entry
   FastDiv by_h, by_rt, by_page;
   int tile_pages, tile_rows;  // a tile's keys as pages and rows
   float scale_log2;
@@ -810,66 +811,80 @@ __global__ void __launch_bounds__(LatCfg<NT, FP8>::kThreads, 1)
   }
   // the merge kernel may be set up; it waits for this grid's end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // This CTA's share of the work line: every thread counts a run of entries, then a scan over the CTA.
-  const int entries = p.B * p.RT;
-  const int run = (entries + L::kThreads - 1) / L::kThreads;
-  const int e_begin = min(static_cast<int>(threadIdx.x) * run, entries), e_end = min(e_begin + run, entries);
-  int mine = 0;
-  for (int e = e_begin; e < e_end; ++e) {
-    const LatEntry x = lat_entry<NT>(p, e);
-    mine += lat_units(p, x.keys);
-    if (blockIdx.x == 0 && x.r0 == 0) {
-      const int len = __ldg(p.lens + x.b);
-      if (len < 0 || len > p.max_keys || (p.qlens != nullptr && (__ldg(p.qlens + x.b) < 0 || __ldg(p.qlens + x.b) > p.Sq)))
-        if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxLength);
-    }
-  }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  int* scan = sm.scan();
-  if (lane == 31) scan[warp] = incl;
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  int before = 0, units = 0;
-#pragma unroll
-  for (int i = 0; i < L::kThreads / 32; ++i) {
-    if (i < warp) before += scan[i];
-    units += scan[i];
-  }
-  // Every entry takes L::kExtra more places; not where every unit can have a CTA of its own.
-  const int extra = units <= static_cast<int>(gridDim.x) ? 0 : L::kExtra;
-  const int total = units + extra * entries;
-  // with fewer places than CTAs the first ones get one each: the CTAs of an entry are always neighbours
-  const int busy = min(total, static_cast<int>(gridDim.x)), me = static_cast<int>(blockIdx.x);
-  const int share = total / busy, more = total - share * busy;
-  const int u0 = me < busy ? me * share + min(me, more) : total, u1 = me < busy ? u0 + share + (me < more ? 1 : 0) : total;
-  {
-    mine += extra * (e_end - e_begin);
-    int at = before + incl + extra * e_end - mine;  // places in front of this thread's entries
-    if (u0 < u1 && at <= u0 && u0 < at + mine) {
-      int e = e_begin;
-      while (true) {
-        const int n = lat_units(p, lat_entry<NT>(p, e).keys) + extra;
-        if (u0 < at + n) break;
-        at += n;
-        ++e;
-      }
-      scan[12] = e;
-      scan[13] = u0 - at;
-    }
-  }
-  __syncthreads();
+  const int entries = p.B * p.RT, me = static_cast<int>(blockIdx.x);
+  const auto check_lengths = [&](const LatEntry& x) {
+    if (x.r0 != 0) return;
+    const int len = __ldg(p.lens + x.b);
+    if (len < 0 || len > p.max_keys || (p.qlens != nullptr && (__ldg(p.qlens + x.b) < 0 || __ldg(p.qlens + x.b) > p.Sq)))
+      if (p.status != nullptr) atomicCAS(p.status, 0u, (kErrIndex << 24) | kIdxLength);
+  };
   LatWalk<NT> walk;
-  walk.e = u0 < u1 ? scan[12] : 0;
-  walk.off = u0 < u1 ? scan[13] : 0;
-  walk.left = u1 - u0;
-  walk.extra = extra;
+  if (p.whole && entries == static_cast<int>(gridDim.x)) {  // each entry has a CTA of its own
+    const LatEntry x = lat_entry<NT>(p, me);
+    if (threadIdx.x == 0) check_lengths(x);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    walk.e = me;
+    walk.off = 0;
+    walk.left = 1;
+    walk.extra = 0;
+  } else {
+    // This CTA's share of the work line: every thread counts a run of entries, then a scan over the CTA.
+    const int run = (entries + L::kThreads - 1) / L::kThreads;
+    const int e_begin = min(static_cast<int>(threadIdx.x) * run, entries), e_end = min(e_begin + run, entries);
+    int mine = 0;
+    for (int e = e_begin; e < e_end; ++e) {
+      const LatEntry x = lat_entry<NT>(p, e);
+      mine += lat_units(p, x.keys);
+      if (blockIdx.x == 0) check_lengths(x);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    int* scan = sm.scan();
+    if (lane == 31) scan[warp] = incl;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    int before = 0, units = 0;
+#pragma unroll
+    for (int i = 0; i < L::kThreads / 32; ++i) {
+      if (i < warp) before += scan[i];
+      units += scan[i];
+    }
+    // Every entry takes L::kExtra more places; not where every unit can have a CTA of its own.
+    const int extra = units <= static_cast<int>(gridDim.x) ? 0 : L::kExtra;
+    const int total = units + extra * entries;
+    // with fewer places than CTAs the first ones get one each: the CTAs of an entry are always neighbours
+    const int busy = min(total, static_cast<int>(gridDim.x));
+    const int share = total / busy, more = total - share * busy;
+    const int u0 = me < busy ? me * share + min(me, more) : total, u1 = me < busy ? u0 + share + (me < more ? 1 : 0) : total;
+    {
+      mine += extra * (e_end - e_begin);
+      int at = before + incl + extra * e_end - mine;  // places in front of this thread's entries
+      if (u0 < u1 && at <= u0 && u0 < at + mine) {
+        int e = e_begin;
+        while (true) {
+          const int n = lat_units(p, lat_entry<NT>(p, e).keys) + extra;
+          if (u0 < at + n) break;
+          at += n;
+          ++e;
+        }
+        scan[12] = e;
+        scan[13] = u0 - at;
+      }
+    }
+    __syncthreads();
+    walk.e = u0 < u1 ? scan[12] : 0;
+    walk.off = u0 < u1 ? scan[13] : 0;
+    walk.left = u1 - u0;
+    walk.extra = extra;
+  }
+  const uint32_t tmem = *tmem_slot;
   bool healthy = *abort_flag == 0u;
   if ((smem_u32(smem) & 1023u) != 0u) {  // the swizzled tiles need a 1024-byte aligned window
     if (threadIdx.x == 0) report_error(ctl, kErrSmemAlign, smem_u32(smem));
@@ -1164,8 +1179,8 @@ static int lat_rows(int64_t rows, bool fp8) { return rows <= 16 ? 16 : rows <= 3
 // for the merge, it is all of a sequence: nothing is cut then, and one launch does. With a CTA for each of E entries of at
 // most T tiles, cutting saves up to T (1 - E / SMs) tiles; the merge takes about as long as 3.6 tiles in bf16 and 6.6 in 8
 // bits (and another launch from the host). Measured, cut against whole, 16 heads, us: bf16, one sequence of 256 keys 10.2 and
-// 9.6, of 512 keys 10.9 and 13.5, 148 of up to 512 26.9 and 20.9, of up to 1024 36.1 and 32.6; 8-bit, one of 512 keys 11.3
-// and 11.2, of 1024 11.8 and 15.5, 148 of up to 1024 26.8 and 21.0. The lengths behind E are not known here, so sequences
+// 9.3, of 512 keys 10.9 and 13, 148 of up to 512 26.9 and 20.0, of up to 1024 36.1 and 31.5; 8-bit, one of 512 keys 11.3 and
+// 11.2, of 1024 11.8 and 15, 148 of up to 1024 26.8 and 20.1. The lengths behind E are not known here, so sequences
 // of more than 1024 keys are always cut.
 constexpr int kWhole = 1024;
 struct LatPlan { int unit_log2, ctas; };
@@ -1195,7 +1210,7 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   PITH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc));
   kern<<<ctas, L::kThreads, L::kAlloc, st>>>(tl, tr, p);
   PITH_CUDA(cudaGetLastError());
-  if (p.max_keys > (1 << p.unit_log2) && ctas > 1) {  // an entry of one unit is never cut
+  if (!p.whole) {  // an entry of one unit is never cut
     const int64_t entries = static_cast<int64_t>(p.B) * p.RT;
     cudaLaunchConfig_t cfg = {};
     const unsigned jobs = static_cast<unsigned>(entries < ctas - 1 ? entries : ctas - 1);
@@ -1272,7 +1287,8 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   if (int rc = lat_plan(rt * a->B, p.max_keys, fp8, &plan)) return rc;
   const int ctas = plan.ctas;
   p.unit_log2 = plan.unit_log2;
-  if (p.max_keys > (1 << p.unit_log2)) {
+  p.whole = p.max_keys <= (1 << plan.unit_log2);
+  if (!p.whole) {
     PITH_REQUIRE(a->workspace, "null workspace");
     PITH_REQUIRE(a->workspace_bytes >= static_cast<size_t>(ctas) * 2 * nt * (kLat * 4 + 8) + static_cast<size_t>(ctas) * 16,
                  "workspace too small");
