@@ -1087,6 +1087,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
   __shared__ int warp_jobs[16];
   __shared__ int job[2];  // CTA, slot
   __shared__ int entry;
+  __shared__ uint32_t failed;  // read once: another stream may record an error between two threads' reads of the word
   __shared__ float4 wt[kMergeThreads];
   __shared__ float4 red[2][1];
   constexpr int kGroup = kMergeThreads / SPLIT;
@@ -1094,7 +1095,7 @@ __global__ void __launch_bounds__(kMergeThreads) latent_merge_kernel(const LatAt
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int c4 = blockIdx.y;  // columns [4 c4, 4 c4 + 4)
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const uint32_t failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
+  if (t == 0) failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
   const int4 info = t < ctas ? p.part_info[t] : make_int4(-1, -1, -1, 0);
   const uint32_t begun = __ballot_sync(0xFFFFFFFFu, info.y >= 0);
   if (lane == 0) warp_jobs[warp] = __popc(begun);

@@ -103,7 +103,9 @@ __device__ __forceinline__ void unpack_e4m3x4(uint32_t v, float* f) {
 template <bool FP8, bool CS32, bool W32>
 __global__ void __launch_bounds__(256, 5) latent_write_kernel(const LatentWriteParams p) {
   const int lane = threadIdx.x & 31;
-  const uint32_t failed = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
+  // One value for the warp, whose lanes reduce a row together: another stream may record an error at any time.
+  const uint32_t failed =
+      __shfl_sync(0xFFFFFFFFu, p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u, 0);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); t < p.n;
        t += static_cast<int64_t>(gridDim.x) * 8) {
     const int b = p.by_s(static_cast<int>(t)), s = static_cast<int>(t) - b * p.by_s.d;
