@@ -16,8 +16,14 @@
 // absolutely), the weights likewise, and hi and lo are separate columns of the same MMA: an MMA of 128 x N x 32 bytes costs
 // 39.5 cycles at N = 16, 40.6 at 32, 48.6 at 64 (what bounds it is reading A from shared memory), so the second half is
 // nearly free. The row factor of a key enters the score in registers and the weight as w_n = 2^(s_n + log2 scale_n - ref):
-// ref is the running maximum of s_n + log2 scale_n, so the split covers the keys that matter; weights below 2^-18 of the
-// reference are dropped.
+// ref is the running maximum of s_n + log2 scale_n (or up to 2^4 below it). The two terms hold weights above 2^-9 of the
+// reference to 2^-9 of themselves; below that their steps are 2^-17 of the reference, whatever the weight. Rounded to the
+// nearest step, the many small weights behind one large one (a context whose first token outweighs each other one by 2^18)
+// would all be lost, or all be up to doubled: 18 % of the output at 99 000 keys. So each key's weights get an offset within half
+// a step, taken from the multiples of the golden ratio, before they are rounded: a share of the keys is then rounded up that is
+// what the weight is of a step, and sums over keys keep their value. What is left is the scatter of c over the keys that were
+// rounded up, at most sqrt(2^-17 W) of it for small weights that add up to W references, against a sum of at least 1 + W:
+// below 2^-9 of the result at any number of keys. The row sums take the weights as they were.
 //
 // Work split: the (sequence, row tile, 64 keys) units of the launch form one line which is cut into one equal piece per
 // CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device; short sequences
@@ -494,6 +500,9 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       const int n0 = walk.k0 + j * kTile, n = n0 + t;
       const uint32_t buf = tile % L::kScores;
       float ks = 1.f, lk = 0.f, iks = 1.f;  // the key's factor, its log2, its reciprocal
+      // Half a step of 16 times a weight, 2^-14, times a number in [-1, 1) that is spread evenly over any run of keys: the weight
+      // of a hidden key, 0, stays 0.
+      const float offset = static_cast<float>(static_cast<int>(static_cast<uint32_t>(n) * 0x9E3779B9u)) * 0x1p-45f;
       bool bad_factor = false;              // not finite: the rows that see the key become NaN, and no others
       if (FP8) {
         if (n < walk.k1) {
@@ -663,7 +672,7 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
             f2_unpack(f2_fma(f2_pack(pw[c], pw[c + 1]), f2_pack(iks, iks), f2_pack(l[c0 + c], l[c0 + c + 1])), l[c0 + c],
                       l[c0 + c + 1]);
             uint16_t h, r;
-            split_e4m3x2(pw[c] * 16.f, pw[c + 1] * 16.f, h, r);
+            split_e4m3x2(fmaf(pw[c], 16.f, offset), fmaf(pw[c + 1], 16.f, offset), h, r);
             hi[c >> 2] = (c & 2) ? hi[c >> 2] | (static_cast<uint32_t>(h) << 16) : h;
             lo[c >> 2] = (c & 2) ? lo[c >> 2] | (static_cast<uint32_t>(r) << 16) : r;
           }

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_gpu_latent import (E4M3, SCALE, assert_attention, check, filled_cache, run_attention, slots_of, tables)
+from test_gpu_latent import (E4M3, SCALE, assert_attention, check, filled_cache, make_cache, quantised, random_tree,
+                             run_attention, stored, tables, visible)
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,61 @@ def test_an_error_that_another_stream_records_while_parts_are_merged(cuda_device
         with pytest.raises(RuntimeError, match="a slot given"):
             kernels.check_device_status()
     assert_attention(q, cache, table, lens, SCALE)
+
+
+def one_context(g, n, page, dtype, mean):
+    """(cache, table [1, pages]) of one context whose latent vectors have a common part."""
+    cache = make_cache(-(-n // page), page, dtype, fill=0.0)
+    c = mean + torch.randn(cache.num_pages * page, 512, generator=g, device="cuda")
+    if dtype == E4M3:
+        c8, scale = quantised(c)
+        cache.latent.copy_(c8.view(cache.latent.shape))
+        cache.scale.copy_(scale.view(cache.scale.shape))
+    else:
+        cache.latent.copy_(c.view(cache.latent.shape))
+    return cache, torch.randperm(cache.num_pages, generator=g, device="cuda").int()[None]
+
+
+def shared_context_reference(query, cache, table, n, tree=None):
+    """fp64 (out [B,S,H,512], log2 lse [B,H,S]) where all sequences read the same n keys."""
+    B, S, H, _ = query.shape
+    rows = table[0].long()[torch.arange(n, device="cuda") // cache.page_size] * cache.page_size \
+        + torch.arange(n, device="cuda") % cache.page_size
+    c_all, r_all = stored(cache)
+    c, keys = c_all[rows], torch.cat([c_all[rows], r_all[rows]], -1)
+    out = torch.empty(B, S, H, 512, dtype=torch.float64, device="cuda")
+    lse = torch.empty(B, H, S, dtype=torch.float64, device="cuda")
+    for b in range(B):
+        seen = visible(S, n, S, None if tree is None else tree[b])
+        for i in range(0, S, 16):
+            s = torch.einsum("ihd,nd->ihn", query[b, i:i + 16].double() * SCALE, keys)
+            s.masked_fill_(~seen[i:i + 16, None], -math.inf)
+            lse[b, :, i:i + 16] = (torch.logsumexp(s, -1) / math.log(2)).T
+            out[b, i:i + 16] = torch.softmax(s, -1) @ c
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("B,S,n,spread", [(148, 1, 100_000, 0.7), (148, 1, 30_000, 0.0), (16, 13, 100_000, 0.7),
+                                          (1, 256, 100_000, 2.0), (148, 2, 131_071, 1.0)])
+def test_many_small_weights_behind_a_large_one(cuda_device, dtype, B, S, n, spread):
+    """The first key outweighs each other key by 9 to 16 nats, and the others have a common part that makes up as much as all of
+    the result; a piece of the work is a whole context, or most of one. The bound has no term that grows with the keys: of the
+    result's norm 2^-8 for its rounding to bf16, 2^-9 for the rounding of large weights (bf16: 2^-9 too) and 2^-9 for what is
+    left of the small ones, 2^-7 in all. Scores and row sums are fp32: sums of 576 products below 32 in magnitude."""
+    g = torch.Generator(device="cuda").manual_seed(B + S + n)
+    cache, table = one_context(g, n, 64, dtype, 1.0)
+    H = 16
+    q = torch.zeros(B, S, H, 576, device="cuda")
+    q[..., :512] = torch.randn(B, S, H, 512, generator=g, device="cuda") * (spread / (SCALE * 512 ** 0.5))
+    q[..., 512] = torch.linspace(9, 16, B * S * H, device="cuda").view(B, S, H)
+    q = q.bfloat16()
+    first = table[0, 0].item() * 64
+    cache.rope.view(-1, 64)[first, 0] = 1 / SCALE
+    tree = random_tree(torch.Generator().manual_seed(S), B, S) if B > 1 and S > 2 else None
+    o, l = run_attention(q, cache, table.expand(B, -1), [n] * B, SCALE, None, tree)
+    check()
+    want, lse = shared_context_reference(q, cache, table, n, tree)
+    rel = (o.double() - want).norm(dim=-1) / want.norm(dim=-1)
+    assert rel.max().item() <= 2.0 ** -7, rel.max().item()
+    assert (l.double() - lse).abs().max().item() <= 2.0 ** -8
