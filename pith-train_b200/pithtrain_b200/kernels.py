@@ -582,16 +582,17 @@ def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query
         tm = tree_mask.data_ptr()
     if not 0.0 < softmax_scale < math.inf:
         raise ValueError("softmax_scale must be positive and finite")
-    max_keys = t_shape[1] * cache.flat[5]
+    planes = cache.flat
+    max_keys = t_shape[1] * planes[5]
     if max_keys > _INT32_MAX:
         raise ValueError(f"block_table covers {max_keys} keys a sequence")
     idx = _device_index("latent_attention", query, cache.latent, block_table, seq_lens, query_lens, tree_mask)
     out = query.new_empty((B, S, H, 512))
     lse = query.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
     # allocated per call on the current stream: calls on other streams and captured graphs each have their own
-    nbytes = _attn_workspace(idx, B, S, H, max_keys, cache.flat[3])
+    nbytes = _attn_workspace(idx, B, S, H, max_keys, planes[3])
     workspace = query.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    args = _ATTN(*cache.flat, query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+    args = _ATTN(*planes, query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
                  block_table.data_ptr(), seq_lens.data_ptr(), ql, tm, workspace.data_ptr() if nbytes else 0,
                  _status_ptr(idx), nbytes, B, S, H, t_shape[1], softmax_scale, q_stride[0], q_stride[1], q_stride[2],
                  block_table.stride(0), tm0, tm1)

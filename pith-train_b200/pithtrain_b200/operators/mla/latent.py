@@ -32,10 +32,17 @@ class LatentCache:
     """Planes of a paged latent cache: ``latent`` [pages, page_size, 512] (bfloat16 or float8_e4m3fn), ``rope``
     [pages, page_size, 64] bfloat16, and for float8_e4m3fn ``scale`` [pages, page_size] float32 (a row's values are
     stored * scale). A slot is ``page * page_size + row``. ``page_size`` is 16, 32 or a multiple of 64; planes may be
-    strided (a layer of a larger tensor) as long as rows are contiguous. The object keeps no state besides the tensors.
+    strided (a layer of a larger tensor) as long as rows are contiguous. The planes' memory may move between calls (a storage
+    released and taken back, ``set_``, ``.data``): every call looks where they are. Where they stay, shapes and strides do too.
     """
 
     def __init__(self, latent: torch.Tensor, rope: torch.Tensor, scale: torch.Tensor | None = None):
+        self._planes = (latent, rope, scale)
+        self._at = self._flat = None
+        self._check()
+
+    def _check(self) -> None:
+        latent, rope, scale = self._planes
         if latent.dtype not in (torch.bfloat16, torch.float8_e4m3fn) or rope.dtype != torch.bfloat16:
             raise TypeError("latent must be bfloat16 or float8_e4m3fn, rope bfloat16")
         if latent.dim() != 3 or latent.shape[2] != 512 or latent.stride(2) != 1:
@@ -56,11 +63,23 @@ class LatentCache:
         for name, t in (("rope", rope), ("scale", scale)):
             if t is not None and t.device != latent.device:
                 raise ValueError(f"{name} is on {t.device}, latent on {latent.device}")
-        self._planes = (latent, rope, scale)
-        # the fields of pith_latent_cache, in order
-        self.flat = (latent.data_ptr(), rope.data_ptr(), scale.data_ptr() if scale is not None else 0,
-                     _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, pages, page_size,
-                     *latent.stride()[:2], *rope.stride()[:2], *(scale.stride() if scale is not None else (0, 0)))
+
+    @property
+    def flat(self) -> tuple:
+        """The fields of ``pith_latent_cache``, in order, of the planes as they are now."""
+        latent, rope, scale = self._planes
+        at = (latent.data_ptr(), rope.data_ptr(), scale.data_ptr() if scale is not None else 0)
+        if at != self._at:  # the first call, or a plane has moved
+            self._check()
+            for t in self._planes:
+                if t is not None:
+                    end = t.storage_offset() + 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+                    if t.untyped_storage().nbytes() < end * t.element_size():
+                        raise RuntimeError("the memory of a plane of the latent cache has been released")
+            self._flat = (*at, _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, *latent.shape[:2],
+                          *latent.stride()[:2], *rope.stride()[:2], *(scale.stride() if scale is not None else (0, 0)))
+            self._at = at
+        return self._flat
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):

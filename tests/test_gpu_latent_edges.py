@@ -105,3 +105,34 @@ def test_many_small_weights_behind_a_large_one(cuda_device, dtype, B, S, n, spre
     rel = (o.double() - want).norm(dim=-1) / want.norm(dim=-1)
     assert rel.max().item() <= 2.0 ** -7, rel.max().item()
     assert (l.double() - lse).abs().max().item() <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_a_cache_that_was_parked_and_taken_back(cuda_device, dtype):
+    """The planes' memory is released, taken by others, and allocated anew: the operators use the new place, and leave what
+    lies at the old one alone."""
+    from pithtrain_b200.operators.mla import latent_cache_read, latent_cache_write
+    g = torch.Generator(device="cuda").manual_seed(70)
+    cache, table = filled_cache(g, [3000], 64, dtype)
+    q = torch.randn(1, 1, 16, 576, generator=g, device="cuda").bfloat16()
+    assert_attention(q, cache, table, [3000], SCALE)
+    planes = [t for t in (cache.latent, cache.rope, cache.scale) if t is not None]
+    copies = [t.view(torch.uint8).clone() for t in planes]
+    sizes = [t.untyped_storage().nbytes() for t in planes]
+    for t in planes:
+        t.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="released"):
+        run_attention(q, cache, table, [3000], SCALE)
+    others = [torch.full((n,), 77, dtype=torch.uint8, device="cuda") for n in sizes]
+    for t, n, c in zip(planes, sizes, copies):
+        t.untyped_storage().resize_(n)
+        t.view(torch.uint8).copy_(c)
+    assert_attention(q, cache, table, [3000], SCALE)
+    x = torch.randn(1, 4, 576, generator=g, device="cuda").bfloat16()
+    cos, sin = tables(4)
+    slots = torch.tensor([[0, 65, 5, 99]], device="cuda")
+    latent_cache_write(cache, slots, x[..., :512], x[..., 512:], torch.ones(512, device="cuda"), cos, sin, 1e-6)
+    got = latent_cache_read(cache, slots)[0]
+    check()
+    assert torch.equal(got[0].double(), stored(cache)[0][slots[0]]) and got.any()
+    assert all((o == 77).all() for o in others)

@@ -216,3 +216,35 @@ def test_cabi_projections_refuse_on_the_host(built_library):
     assert lib.pith_latent_query(ctypes.byref(a), None) < 0 and b"multiples of 4" in lib.pith_last_error()
     a.cs_stride[1], a.cs_dtype = 64, 2
     assert lib.pith_latent_query(ctypes.byref(a), None) < 0 and b"bf16 or fp32" in lib.pith_last_error()
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float8_e4m3fn])
+def test_a_cache_whose_memory_moves(dtype):
+    """The address that a call gets is the planes' present one; planes without memory, or of another form, are refused."""
+    c = cache(dtype, 3, 32)
+    planes = [c.latent, c.rope] + ([c.scale] if c.scale is not None else [])
+    addresses = lambda: tuple(t.data_ptr() for t in planes)  # noqa: E731
+    assert c.flat[: len(planes)] == addresses()
+    keep = []
+    for t in planes:                                           # released, and taken back elsewhere
+        size, old = t.untyped_storage().nbytes(), t.data_ptr()
+        t.untyped_storage().resize_(0)
+        with pytest.raises(RuntimeError, match="released"):
+            c.flat
+        keep.append(torch.empty(size, dtype=torch.uint8))
+        t.untyped_storage().resize_(size)
+        t.set_(torch.zeros_like(t)) if t.data_ptr() == old else None
+        assert c.flat[: len(planes)] == addresses()
+    c.latent.data = torch.zeros(3, 2, 32, 512).to(dtype)[:, 1]   # a layer of a larger tensor now
+    assert c.flat[: len(planes)] == addresses() and c.flat[6:8] == (2 * 32 * 512, 512)
+    c.latent.data = torch.zeros(2, 32, 512).to(dtype)
+    with pytest.raises(ValueError, match="rope must be"):
+        c.flat
+
+
+def test_a_moved_cache_is_not_written_at_its_old_place():
+    c = cache()
+    old = c.flat[0]
+    parked = c.latent.data
+    c.latent.data = torch.zeros(2, 16, 512, dtype=BF)
+    assert parked.data_ptr() == old and c.flat[0] == c.latent.data_ptr() != old
