@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import time
 
 import torch
 
@@ -37,6 +38,9 @@ def check_device_status(device=None) -> None:
     val = int(w.item()) & 0xFFFFFFFF
     if val != 0:
         w.zero_()
+        m = _status_mirrors.get(w.get_device())
+        if m is not None:
+            m[2] = False  # a copy that is on its way tells of the same anomaly
         text = _lib.load().pith_status_string(val).decode()
         raise RuntimeError(f"pith_b200 kernel reported: {text}")
 
@@ -71,7 +75,7 @@ def poll_device_status(device=None) -> None:
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     m = _status_mirrors.get(idx)
-    if m is None or not m[2] or not m[1].query():
+    if m is None or not m[2] or torch.cuda.is_current_stream_capturing() or not m[1].query():
         return
     m[2] = False
     val = int(m[0].item()) & 0xFFFFFFFF
@@ -449,18 +453,30 @@ def _device_index(what: str, first: torch.Tensor, *others) -> int:
     return idx
 
 
+# A copy of the status word behind every call would cost more than the call (every millisecond 0.6 us a call): one in ten
+# milliseconds tells of an index error soon enough, as the kernels between skip their work.
+_POST_EVERY_S = 1e-2
+_next_post: dict[int, float] = {}
+
+
 def _enqueue(entry: str, args: bytes, idx: int, launches: int) -> None:
-    """Calls an entry on the current stream of device `idx`, whichever device is current."""
-    global launch_count
-    fn = _lib.packed_entry(entry)
-    if torch._C._cuda_getDevice() == idx:
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
-    else:
+    """Calls an entry on the current stream of device `idx`, whichever device is current. Raises if an earlier call reported an
+    index out of range (or another anomaly) and the news has reached the host."""
+    if torch._C._cuda_getDevice() != idx:
         with torch.cuda.device(idx):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(idx))
+            return _enqueue(entry, args, idx, launches)
+    global launch_count
+    m = _status_mirrors.get(idx)
+    if m is not None and m[2]:
+        poll_device_status(torch.device("cuda", idx))
+    rc = _lib.packed_entry(entry)(args, torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         _lib.check(rc, entry)
     launch_count += launches
+    now = time.monotonic()
+    if now >= _next_post.get(idx, 0.0):
+        _next_post[idx] = now + _POST_EVERY_S
+        post_status_copy(torch.device("cuda", idx))
 
 
 def _status_ptr(idx: int) -> int:

@@ -1,6 +1,7 @@
 """The MLA latent-cache operators where calls, streams and values meet: cases beside those of test_gpu_latent.py."""
 
 import math
+import time
 
 import pytest
 import torch
@@ -136,3 +137,40 @@ def test_a_cache_that_was_parked_and_taken_back(cuda_device, dtype):
     check()
     assert torch.equal(got[0].double(), stored(cache)[0][slots[0]]) and got.any()
     assert all((o == 77).all() for o in others)
+
+
+def test_an_index_error_reaches_a_later_call_without_a_sync(cuda_device):
+    """A loop that never asks for the status stops at a later call of these operators, or of the training operators; a capture
+    that begins in between is not disturbed."""
+    from pithtrain_b200.operators.attention import flash_attn_func
+    from pithtrain_b200.operators.mla import LatentCache, latent_cache_read, latent_cache_write
+    cache = LatentCache.allocate(1, 16)
+    x = torch.ones(1, 1, 576, device="cuda", dtype=torch.bfloat16)
+    cos, sin = tables(1)
+    w = torch.ones(512, device="cuda")
+    good = torch.zeros(1, 1, dtype=torch.int64, device="cuda")
+
+    def write(slot):
+        latent_cache_write(cache, good + slot, x[..., :512], x[..., 512:], w, cos, sin, 1e-6)
+
+    check()
+    write(16)
+    with pytest.raises(RuntimeError, match="a slot given"):
+        for _ in range(50):
+            time.sleep(0.003)
+            latent_cache_read(cache, good)
+    write(3)
+    check()
+    assert (latent_cache_read(cache, good + 3)[0] != 0).all()
+    time.sleep(0.02)
+    write(16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows = latent_cache_read(cache, good + 3)[0]
+    q = torch.randn(1, 128, 2, 128, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError, match="a slot given"):
+        flash_attn_func(q, q, q, causal=True)
+    graph.replay()
+    check()
+    assert (rows != 0).all()
