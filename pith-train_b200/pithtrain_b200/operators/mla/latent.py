@@ -153,9 +153,11 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     * ``return_lse``: also the log2-domain LSE, fp32 ``[B,H,S]`` (-inf for a row that sees no key), the convention of
       this library's other operators.
 
-    Lengths and tables are read on the device: the call can be captured once and replayed with other contents. The
-    results do not depend on the other sequences of the batch by more than fp32 rounding of partial sums, and repeat
-    bit for bit for the same inputs.
+    Lengths and tables are read on the device: the call can be captured once and replayed with other contents. Results repeat bit
+    for bit for the same inputs. They depend on the other sequences of the batch through where a context is cut for the SMs:
+    softmax weights are rounded relative to a running maximum of each part, to 8 significant bits (half a step: 2^-8 of a weight),
+    in an 8-bit cache to steps of 2^-17 of the largest at least, upwards or downwards key by key so that sums are kept. Row sums
+    and the LSE take the weights unrounded, in fp32.
     """
     if torch.is_grad_enabled() and query.requires_grad:
         _refuse("latent_attention")

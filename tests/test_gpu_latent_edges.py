@@ -174,3 +174,31 @@ def test_an_index_error_reaches_a_later_call_without_a_sync(cuda_device):
     graph.replay()
     check()
     assert (rows != 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_a_sequence_alone_and_in_batches_that_cut_it_differently(cuda_device, dtype):
+    """The rounding of the weights is all that other sequences may change: at most 2^-8 of each weight in either call, and a
+    rounding of the result in each (2^-8), 2^-8 of a norm each time; in 8 bits 2^-9 more for what is left of small weights. The
+    LSE differs by fp32 rounding of scores and sums only. Repeated calls agree to the bit."""
+    g = torch.Generator(device="cuda").manual_seed(80)
+    n = 5000
+    cache, table = one_context(g, n, 64, dtype, 0.5)
+    q = torch.randn(1, 1, 16, 576, generator=g, device="cuda").bfloat16() * 2
+    cache.rope.normal_(generator=g)
+    alone, lse = assert_attention(q, cache, table, [n], SCALE)
+    want, _ = shared_context_reference(q, cache, table, n)
+    rows = table[0].long()[torch.arange(n, device="cuda") // 64] * 64 + torch.arange(n, device="cuda") % 64
+    s = torch.einsum("hd,nd->hn", q[0, 0].double() * SCALE, torch.cat([t[rows] for t in stored(cache)], -1))
+    size = (torch.softmax(s, -1) @ stored(cache)[0][rows].abs()).norm(dim=-1)     # of the weighted sum of magnitudes
+    bound = 2 * (2.0 ** -8 * size + 2.0 ** -8 * want[0, 0].norm(dim=-1) + (2.0 ** -9 * size if dtype == E4M3 else 0))
+    for others in ([], [1], [n] * 3, [77] * 200, [n] * 147, [4000, 3, 2500] * 40):
+        lens = others + [n]
+        batch = torch.randn(len(lens), 1, 16, 576, generator=g, device="cuda").bfloat16()
+        batch[-1] = q[0]
+        o, l = run_attention(batch, cache, table.expand(len(lens), -1), lens, SCALE)
+        again = run_attention(batch, cache, table.expand(len(lens), -1), lens, SCALE)
+        check()
+        assert torch.equal(o, again[0]) and torch.equal(l, again[1])
+        assert ((o[-1, 0].double() - alone[0, 0].double()).norm(dim=-1) <= bound).all()
+        assert (l[-1] - lse[0]).abs().max().item() <= 2.0 ** -10
