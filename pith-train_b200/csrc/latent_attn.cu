@@ -380,7 +380,7 @@ __device__ __forceinline__ void split_query_rows(uint8_t* sq, float* qk, int row
     const uint32_t bits = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top));
     // the power of two that brings the row's largest element into (224, 448]
     int k = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) > 0x600000u ? 7 : 8);
-    k = bits == 0u ? 0 : min(max(k, -100), 100);
+    k = bits == 0u ? 0 : max(k, -126);  // at most 120
     const float inv = __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
     // an infinite element makes the row's scores NaN
     if (lane == 0) qk[row] = __uint_as_float(bits >= 0x7F800000u ? 0x7FC00000u : static_cast<uint32_t>(127 + k) << 23);

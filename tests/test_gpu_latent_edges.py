@@ -202,3 +202,22 @@ def test_a_sequence_alone_and_in_batches_that_cut_it_differently(cuda_device, dt
         assert torch.equal(o, again[0]) and torch.equal(l, again[1])
         assert ((o[-1, 0].double() - alone[0, 0].double()).norm(dim=-1) <= bound).all()
         assert (l[-1] - lse[0]).abs().max().item() <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("k", [118, 110, -90, -98])
+def test_queries_of_any_magnitude(cuda_device, dtype, k):
+    """A query times 2^k with a softmax scale of 2^-k gives the same scores: the same results, to the bit, as long as no product
+    leaves the range of fp32."""
+    from pithtrain_b200.operators.mla import latent_attention
+    g = torch.Generator(device="cuda").manual_seed(90)
+    lens = [900, 70]
+    cache, table = filled_cache(g, lens, 64, dtype)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for S in (1, 3):
+        q = torch.randn(2, S, 16, 576, generator=g, device="cuda").clamp(-4, 4).bfloat16()
+        q = torch.where(q.abs() < 2.0 ** -8, torch.ones_like(q), q)
+        want = latent_attention(q, cache, table, n, SCALE)
+        got = latent_attention((q.double() * 2.0 ** k).bfloat16(), cache, table, n, SCALE * 2.0 ** -k)
+        check()
+        assert torch.equal(got, want)
