@@ -503,12 +503,11 @@ __device__ __forceinline__ void lat_softmax(const LatAttnParams& p, const LatSha
       // Half a step of 16 times a weight, 2^-14, times a number in [-1, 1) that is spread evenly over any run of keys: the weight
       // of a hidden key, 0, stays 0.
       const float offset = static_cast<float>(static_cast<int>(static_cast<uint32_t>(n) * 0x9E3779B9u)) * 0x1p-45f;
-      bool bad_factor = false;              // not finite: the rows that see the key become NaN, and no others
+      bool bad_factor = false;  // not finite, or negative: the rows that see the key become NaN, and no others
       if (FP8) {
         if (n < walk.k1) {
-          ks = next_ks < 1e-30f ? 1e-30f : next_ks;
-          bad_factor = !(ks < INFINITY);
-          if (bad_factor) ks = 1.f;
+          bad_factor = !(next_ks >= 0.f && next_ks < INFINITY);
+          ks = bad_factor ? 1.f : fmaxf(next_ks, 0x1p-100f);  // the least that a write stores; the row sum holds its reciprocal
           lk = fast_log2(ks);
           iks = 1.f / ks;
         }

@@ -33,7 +33,8 @@ def _refuse(what: str) -> None:
 class LatentCache:
     """Planes of a paged latent cache: ``latent`` [pages, page_size, 512] (bfloat16 or float8_e4m3fn), ``rope``
     [pages, page_size, 64] bfloat16, and for float8_e4m3fn ``scale`` [pages, page_size] float32 (a row's values are
-    stored * scale). A slot is ``page * page_size + row``. ``page_size`` is 16, 32 or a multiple of 64; planes may be
+    stored * scale; scales are not negative, and attention takes those below 2^-100, which ``latent_cache_write`` does not
+    store, as 2^-100). A slot is ``page * page_size + row``. ``page_size`` is 16, 32 or a multiple of 64; planes may be
     strided (a layer of a larger tensor) as long as rows are contiguous. The planes' memory may move between calls (a storage
     released and taken back, ``set_``, ``.data``): every call looks where they are. Where they stay, shapes and strides do too.
     """

@@ -221,3 +221,34 @@ def test_queries_of_any_magnitude(cuda_device, dtype, k):
         got = latent_attention((q.double() * 2.0 ** k).bfloat16(), cache, table, n, SCALE * 2.0 ** -k)
         check()
         assert torch.equal(got, want)
+
+
+def test_rows_with_the_least_factor(cuda_device):
+    """Rows so small that their factor is the least one, 2^-100: read back and attended to as what is stored."""
+    from pithtrain_b200.operators.mla import LatentCache, latent_cache_read, latent_cache_write
+    g = torch.Generator(device="cuda").manual_seed(100)
+    n = 200
+    cache = LatentCache.allocate(4, 64, E4M3)
+    x = torch.randn(1, n, 576, generator=g, device="cuda").bfloat16()
+    cos, sin = tables(n)
+    latent_cache_write(cache, torch.arange(n, device="cuda")[None], x[..., :512], x[..., 512:],
+                       torch.full((512,), 2.0 ** -95, device="cuda"), cos, sin, 1e-6)
+    check()
+    assert (cache.scale.view(-1)[:n] == 2.0 ** -100).all()
+    assert torch.equal(latent_cache_read(cache, torch.arange(n, device="cuda"))[0].double(), stored(cache)[0][:n])
+    q = torch.randn(1, 2, 16, 576, generator=g, device="cuda").bfloat16()
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    o, _ = assert_attention(q, cache, table, [n], SCALE)
+    assert o.any()
+
+
+def test_a_negative_row_factor_reaches_only_the_rows_that_see_it(cuda_device):
+    g = torch.Generator(device="cuda").manual_seed(101)
+    cache, table = filled_cache(g, [300], 32, E4M3)
+    q = torch.randn(1, 4, 16, 576, generator=g, device="cuda").bfloat16()
+    want = assert_attention(q, cache, table, [300], SCALE)[0]
+    row = table[0, 298 // 32].long() * 32 + 298 % 32
+    cache.scale.view(-1)[row] *= -1
+    o = run_attention(q, cache, table, [300], SCALE)[0]
+    check()
+    assert torch.equal(o[0, :2], want[0, :2]) and o[0, 2:].isnan().all()
