@@ -11,7 +11,7 @@ head h's block of ``kv_b_proj.weight``,
 so the query takes ``W_k`` in, attention runs on the latent vectors themselves, and its result goes through ``W_v``.
 
 These operators have no gradients (training keeps the expanded form): under grad mode, inputs that require one are
-refused. Sizes are DeepSeek-V2-Lite's (latent 512, rope 64, nope 128, v 128), any number of heads; bf16, CUDA only.
+refused, and so are tangents of forward-mode differentiation. Sizes are DeepSeek-V2-Lite's (latent 512, rope 64, nope 128, v 128), any number of heads; bf16, CUDA only.
 Indices are read on the device, so a slot, page, position or length out of range cannot raise at the call: nothing outside the
 tensors is touched, the error is recorded, and later kernels of the library skip their work, so that their outputs hold
 nothing. A later call of these or the attention operators raises, as soon as the news has reached the host (about ten milliseconds;
@@ -22,12 +22,21 @@ at once. A sampling loop calls it where it fetches its tokens.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ... import _lib, kernels
 
 
-def _refuse(what: str) -> None:
-    raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+def _refuse_gradients(what: str, *inputs) -> None:
+    """Raises where one of the inputs (tensors or None) wants a gradient: backward under grad mode, or forward mode."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in inputs:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no gradient: forward-mode differentiation would lose a tangent here")
 
 
 class LatentCache:
@@ -125,8 +134,7 @@ def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: t
     already gathered. fp32 arithmetic, one rounding to the cache's type; an 8-bit row gets the least power of two as its
     scale with which no value passes 448.
     """
-    if torch.is_grad_enabled() and (compressed_kv.requires_grad or k_pe.requires_grad or norm_weight.requires_grad):
-        _refuse("latent_cache_write")
+    _refuse_gradients("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, *cache._planes)
     kernels.latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
 
 
@@ -134,6 +142,7 @@ def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
     """Rows of the cache as bf16, ``(latent [*slots.shape, 512], k_pe [*slots.shape, 64])``: what the expanded form of a
     prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
     give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
+    _refuse_gradients("latent_cache_read", *cache._planes)
     return kernels.latent_read(cache, slots)
 
 
@@ -160,8 +169,7 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     in an 8-bit cache to steps of 2^-17 of the largest at least, upwards or downwards key by key so that sums are kept. Row sums
     and the LSE take the weights unrounded, in fp32.
     """
-    if torch.is_grad_enabled() and query.requires_grad:
-        _refuse("latent_attention")
+    _refuse_gradients("latent_attention", query, *cache._planes)
     out, lse = kernels.latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask, return_lse)
     return (out, lse) if return_lse else out
 
@@ -172,14 +180,12 @@ def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, 
     viewed per head; strided views are fine) -> ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
     ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
     cos / sin / position_ids as in ``latent_cache_write``."""
-    if torch.is_grad_enabled() and (q.requires_grad or kv_b_weight.requires_grad):
-        _refuse("latent_query")
+    _refuse_gradients("latent_query", q, kv_b_weight, cos, sin)
     return kernels.latent_query(q, kv_b_weight, cos, sin, position_ids)
 
 
 def latent_output(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor:
     """``latent_attention``'s result ``[B,S,H,512]`` times head h's value rows of ``kv_b_weight``: ``[B,S,H,128]`` bf16,
     contiguous, which the layer views as ``[B,S,H * 128]`` for ``o_proj``."""
-    if torch.is_grad_enabled() and (attn.requires_grad or kv_b_weight.requires_grad):
-        _refuse("latent_output")
+    _refuse_gradients("latent_output", attn, kv_b_weight)
     return kernels.latent_output(attn, kv_b_weight)

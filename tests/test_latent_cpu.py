@@ -248,3 +248,45 @@ def test_a_moved_cache_is_not_written_at_its_old_place():
     parked = c.latent.data
     c.latent.data = torch.zeros(2, 16, 512, dtype=BF)
     assert parked.data_ptr() == old and c.flat[0] == c.latent.data_ptr() != old
+
+
+def calls():
+    """Every operator as (call, its differentiable inputs by name)."""
+    c8 = cache(torch.float8_e4m3fn)
+    w = write_args()
+    w["norm_weight"] = torch.ones(512)
+    at = attn_args()
+    pr = dict(q=torch.zeros(1, 2, 4, 192, dtype=BF), kv_b_weight=torch.zeros(4 * 256, 512, dtype=BF), cos=torch.ones(8, 64),
+              sin=torch.ones(8, 64))
+    out = dict(attn=torch.zeros(1, 2, 4, 512, dtype=BF), kv_b_weight=torch.zeros(4 * 256, 512, dtype=BF))
+    slots = torch.zeros(2, dtype=torch.int64)
+    return {
+        "latent_cache_write": (lambda a, c: mla.latent_cache_write(c, **a), w, cache()),
+        "latent_cache_read": (lambda a, c: mla.latent_cache_read(c, slots), {}, c8),
+        "latent_attention": (lambda a, c: mla.latent_attention(a["query"], c, a["block_table"], a["seq_lens"],
+                                                               a["softmax_scale"]), at, c8),
+        "latent_query": (lambda a, c: mla.latent_query(**a), pr, None),
+        "latent_output": (lambda a, c: mla.latent_output(**a), out, None)}
+
+
+@pytest.mark.parametrize("name", ["latent_cache_write", "latent_cache_read", "latent_attention", "latent_query",
+                                  "latent_output"])
+def test_every_input_that_wants_a_gradient_is_refused(name):
+    from torch.autograd import forward_ad
+    call, args, c = calls()[name]
+    floating = [k for k, v in args.items() if torch.is_tensor(v) and v.is_floating_point()]
+    assert floating or name == "latent_cache_read"
+    for key in floating:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call({**args, key: args[key].clone().requires_grad_()}, c)
+        with forward_ad.dual_level(), torch.no_grad():
+            dual = forward_ad.make_dual(args[key], torch.ones_like(args[key]))
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call({**args, key: dual}, c)
+            with pytest.raises(RuntimeError, match="no CPU fallback"):   # other duals do no harm
+                call(args, c)
+    if c is not None:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(args, mla.LatentCache(c.latent, c.rope.clone().requires_grad_(), c.scale))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            call(args, c)
