@@ -567,9 +567,14 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
     PITH_REQUIRE(aligned16(a->cos) && aligned16(a->sin) && a->cs_stride[0] % 4 == 0 && a->cs_stride[1] % 4 == 0,
                  "cos / sin must be 16-byte aligned with strides that are multiples of 4 elements");
     PITH_REQUIRE(a->cs_dtype == PITH_DTYPE_BF16 || a->cs_dtype == PITH_DTYPE_F32, "cos / sin must be bf16 or fp32");
-    PITH_REQUIRE(aligned16(a->x) && a->x_stride[0] % 8 == 0 && a->x_stride[1] % 8 == 0 && a->x_stride[2] % 8 == 0,
-                 "q must be 16-byte aligned with strides that are multiples of 8 elements");
   }
+  const int64_t* xs_in = a->x_stride;
+  PITH_REQUIRE(aligned16(a->x) && xs_in[0] % 8 == 0 && xs_in[1] % 8 == 0 && xs_in[2] % 8 == 0,
+               "%s must be 16-byte aligned with strides that are multiples of 8 elements", QUERY ? "q" : "attn");
+  PITH_REQUIRE((a->B == 1 || xs_in[0] > 0) && (a->S == 1 || xs_in[1] > 0) && (a->H == 1 || xs_in[2] > 0),
+               "%s must not repeat elements (an expanded view)", QUERY ? "q" : "attn");
+  PITH_REQUIRE(aligned16(a->weight) && a->weight_stride > 0 && a->weight_stride % 8 == 0,
+               "kv_b_weight must be 16-byte aligned with a row stride that is a multiple of 8 elements");
   PITH_REQUIRE(static_cast<int64_t>(a->B) * a->S < 2147483647 - 65536, "too many tokens");
   if (int rc = require_sm100()) return rc;
   // One token axis where the strides allow it: a batch of single tokens fills the tiles.

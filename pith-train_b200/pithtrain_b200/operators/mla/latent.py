@@ -177,7 +177,8 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
 def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  position_ids: torch.Tensor | None = None) -> torch.Tensor:
     """The query that ``latent_attention`` takes: q ``[B,S,H,192]`` = ``[q_nope | q_pe]`` bf16 (the projection output,
-    viewed per head; strided views are fine) -> ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
+    viewed per head; strided views are fine if they begin and step in multiples of 16 bytes and repeat nothing) ->
+    ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
     ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
     cos / sin / position_ids as in ``latent_cache_write``."""
     _refuse_gradients("latent_query", q, kv_b_weight, cos, sin)

@@ -290,3 +290,28 @@ def test_every_input_that_wants_a_gradient_is_refused(name):
             call(args, mla.LatentCache(c.latent, c.rope.clone().requires_grad_(), c.scale))
         with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
             call(args, c)
+
+
+def test_cabi_projections_name_the_argument_that_is_off(built_library):
+    from pithtrain_b200 import _lib
+    lib = _lib.load()
+    for entry, name in ((lib.pith_latent_query, b"q must"), (lib.pith_latent_output, b"attn must")):
+        a = _lib.LatentProjArgs()
+        a.B, a.S, a.H = 2, 3, 4
+        a.x = a.weight = a.out = a.cos = a.sin = 0x1000
+        a.cs_stride[1], a.weight_stride = 64, 512
+        a.x_stride[0], a.x_stride[1], a.x_stride[2] = 3 * 4 * 512, 4 * 512, 512
+        for field, value, text in (("x", 0x1008, name + b" be 16-byte aligned"),
+                                   ("weight", 0x1004, b"kv_b_weight must be 16-byte aligned"),
+                                   ("weight_stride", 516, b"kv_b_weight must be"), ("weight_stride", 0, b"kv_b_weight")):
+            old = getattr(a, field)
+            setattr(a, field, value)
+            assert entry(ctypes.byref(a), None) < 0 and text in lib.pith_last_error(), (text, lib.pith_last_error())
+            setattr(a, field, old)
+        for i in range(3):
+            old = a.x_stride[i]
+            a.x_stride[i] = 516
+            assert entry(ctypes.byref(a), None) < 0 and name + b" be 16-byte" in lib.pith_last_error()
+            a.x_stride[i] = 0
+            assert entry(ctypes.byref(a), None) < 0 and name + b" not repeat" in lib.pith_last_error()
+            a.x_stride[i] = old
