@@ -55,6 +55,9 @@ int make_tensor_map(CUtensorMap* out, const void* base, int elem_bytes, int64_t 
 // Checks the planes of a latent cache (pointers, alignment, strides, sizes). Defined in latent_cache.cu.
 int check_latent_cache(const pith_latent_cache& c);
 
+// A stride of an axis of one element says nothing (a view may have any there): it becomes `instead`.
+inline int64_t axis_stride(int64_t size, int64_t stride, int64_t instead = 0) { return size == 1 ? instead : stride; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace pith

@@ -1211,7 +1211,8 @@ static int launch_latent_attn(const pith_latent_attn_args* a, LatAttnParams& p, 
   using L = LatCfg<NT, FP8>;
   CUtensorMap tl, tr;
   const pith_latent_cache& c = a->cache;
-  const int64_t ls[3] = {c.latent_stride[0], c.latent_stride[1], kLat}, rs[3] = {c.rope_stride[0], c.rope_stride[1], kRp};
+  const int64_t ls[3] = {axis_stride(c.pages, c.latent_stride[0], c.page_size * c.latent_stride[1]), c.latent_stride[1], kLat};
+  const int64_t rs[3] = {axis_stride(c.pages, c.rope_stride[0], c.page_size * c.rope_stride[1]), c.rope_stride[1], kRp};
   const int box = c.page_size < kBox ? c.page_size : kBox;
   if (int rc = make_tensor_map(&tl, c.latent, FP8 ? 1 : 2, c.pages, c.page_size, 1, kLat, ls, FP8 ? 128 : 64, box)) return rc;
   if (int rc = make_tensor_map(&tr, c.rope, 2, c.pages, c.page_size, 1, kRp, rs, 64, box)) return rc;
@@ -1261,8 +1262,12 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   PITH_REQUIRE(a->softmax_scale > 0.f, "softmax_scale must be positive");
   if (a->B == 0 || a->Sq == 0 || a->H == 0) return kOk;
   PITH_REQUIRE(a->q && a->out && a->block_table && a->seq_lens, "null tensor pointer");
-  PITH_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->workspace) && a->q_stride[0] % 8 == 0 &&
-                   a->q_stride[1] % 8 == 0 && a->q_stride[2] % 8 == 0,
+  LatAttnParams p = {};
+  p.qs[0] = axis_stride(a->B, a->q_stride[0]);
+  p.qs[1] = axis_stride(a->Sq, a->q_stride[1]);
+  p.qs[2] = axis_stride(a->H, a->q_stride[2]);
+  PITH_REQUIRE(aligned16(a->q) && aligned16(a->out) && aligned16(a->workspace) && p.qs[0] % 8 == 0 && p.qs[1] % 8 == 0 &&
+                   p.qs[2] % 8 == 0,
                "q, out and workspace must be 16-byte aligned, q with strides that are multiples of 8 elements");
   PITH_REQUIRE(a->table_cols >= 0 && static_cast<int64_t>(a->table_cols) * a->cache.page_size < 2147483647 - 1024,
                "the block table covers too many keys");
@@ -1274,7 +1279,6 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   PITH_REQUIRE(rt * a->B * (static_cast<int64_t>(a->table_cols) * a->cache.page_size / kBox + 2 + kMaxExtra) < 2147483647 - 1024,
                "too many query rows and keys for one call");
   if (int rc = require_sm100()) return rc;
-  LatAttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.lse = a->lse;
@@ -1289,7 +1293,6 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, void* stream) {
   p.tile_pages = kTile / p.page_size;
   p.tile_rows = kTile % p.page_size;
   p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-  for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i];
   p.table_stride = a->table_stride;
   for (int i = 0; i < 2; ++i) { p.tree_stride[i] = a->tree_stride[i]; p.scale_stride[i] = a->cache.scale_stride[i]; }
   LatPlan plan;

@@ -227,12 +227,11 @@ int check_latent_cache(const pith_latent_cache& c) {
   PITH_REQUIRE(c.latent && c.rope && (c.dtype == PITH_DTYPE_BF16 || c.scale), "null cache plane");
   PITH_REQUIRE(static_cast<int64_t>(c.pages) * c.page_size < 2147483648ll, "a cache holds at most 2^31 - 1 rows");
   const int eb = c.dtype == PITH_DTYPE_BF16 ? 2 : 1;
-  PITH_REQUIRE(aligned16(c.latent) && aligned16(c.rope) && (c.latent_stride[0] * eb) % 16 == 0 &&
-                   (c.latent_stride[1] * eb) % 16 == 0 && c.rope_stride[0] % 8 == 0 && c.rope_stride[1] % 8 == 0,
+  const int64_t ls0 = axis_stride(c.pages, c.latent_stride[0], 16), rs0 = axis_stride(c.pages, c.rope_stride[0], 16);
+  PITH_REQUIRE(aligned16(c.latent) && aligned16(c.rope) && (ls0 * eb) % 16 == 0 && (c.latent_stride[1] * eb) % 16 == 0 &&
+                   rs0 % 8 == 0 && c.rope_stride[1] % 8 == 0,
                "cache planes must be 16-byte aligned with 16-byte-multiple strides");
-  PITH_REQUIRE(c.latent_stride[0] > 0 && c.latent_stride[1] >= kLatent && c.rope_stride[0] > 0 &&
-                   c.rope_stride[1] >= kRope,
-               "cache rows overlap");
+  PITH_REQUIRE(ls0 > 0 && c.latent_stride[1] >= kLatent && rs0 > 0 && c.rope_stride[1] >= kRope, "cache rows overlap");
   return kOk;
 }
 
@@ -265,17 +264,24 @@ extern "C" int pith_latent_write(const pith_latent_write_args* a, void* stream) 
   if (int rc = check_latent_cache(a->cache)) return rc;
   if (a->B == 0 || a->S == 0) return kOk;
   PITH_REQUIRE(a->compressed_kv && a->k_pe && a->norm_weight && a->cos && a->sin && a->slots, "null tensor pointer");
+  LatentWriteParams p;
+  const int64_t sizes[2] = {a->B, a->S};
+  for (int i = 0; i < 2; ++i) {
+    p.kvs[i] = axis_stride(sizes[i], a->kv_stride[i]);
+    p.ps[i] = axis_stride(sizes[i], a->k_pe_stride[i]);
+    p.cs[i] = a->cs_stride[i];
+    p.sls[i] = a->slots_stride[i];
+    p.pos_s[i] = a->positions_stride[i];
+  }
   PITH_REQUIRE(aligned16(a->compressed_kv) && aligned16(a->k_pe) && aligned16(a->norm_weight) && aligned16(a->cos) &&
-                   aligned16(a->sin) && a->kv_stride[0] % 8 == 0 && a->kv_stride[1] % 8 == 0 &&
-                   a->k_pe_stride[0] % 8 == 0 && a->k_pe_stride[1] % 8 == 0 && a->cs_stride[0] % 4 == 0 &&
-                   a->cs_stride[1] % 4 == 0,
+                   aligned16(a->sin) && p.kvs[0] % 8 == 0 && p.kvs[1] % 8 == 0 && p.ps[0] % 8 == 0 && p.ps[1] % 8 == 0 &&
+                   p.cs[0] % 4 == 0 && p.cs[1] % 4 == 0,
                "inputs must be 16-byte aligned with strides that are multiples of 8 elements (cos / sin: 4)");
   PITH_REQUIRE((a->cs_dtype == PITH_DTYPE_BF16 || a->cs_dtype == PITH_DTYPE_F32) &&
                    (a->weight_dtype == PITH_DTYPE_BF16 || a->weight_dtype == PITH_DTYPE_F32),
                "norm_weight and cos / sin must be bf16 or fp32");
   PITH_REQUIRE(a->eps >= 0.f, "eps must not be negative");
   if (int rc = require_sm100()) return rc;
-  LatentWriteParams p;
   p.c = planes_of(a->cache);
   p.kv = static_cast<const __nv_bfloat16*>(a->compressed_kv);
   p.pe = static_cast<const __nv_bfloat16*>(a->k_pe);
@@ -284,10 +290,6 @@ extern "C" int pith_latent_write(const pith_latent_write_args* a, void* stream) 
   p.n = static_cast<int64_t>(a->B) * a->S;
   PITH_REQUIRE(p.n < 2147483648ll, "too many tokens for one call");
   p.by_s = FastDiv(a->S); p.table_rows = a->table_rows; p.eps = a->eps;
-  for (int i = 0; i < 2; ++i) {
-    p.kvs[i] = a->kv_stride[i]; p.ps[i] = a->k_pe_stride[i]; p.cs[i] = a->cs_stride[i];
-    p.sls[i] = a->slots_stride[i]; p.pos_s[i] = a->positions_stride[i];
-  }
   unsigned grid = 1;
   if (int rc = token_grid(p.n, &grid)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -562,40 +562,40 @@ static int latent_proj(const pith_latent_proj_args* a, void* stream) {
   if (a->B == 0 || a->S == 0 || a->H == 0) return kOk;
   PITH_REQUIRE(a->x && a->weight && a->out, "null tensor pointer");
   PITH_REQUIRE(aligned16(a->out), "out must be 16-byte aligned");
+  LatProjParams p = {};
+  p.qs[0] = axis_stride(a->B, a->x_stride[0]);
+  p.qs[1] = axis_stride(a->S, a->x_stride[1]);
+  p.qs[2] = axis_stride(a->H, a->x_stride[2]);
   if (QUERY) {
     PITH_REQUIRE(a->cos && a->sin, "null tensor pointer");
     PITH_REQUIRE(aligned16(a->cos) && aligned16(a->sin) && a->cs_stride[0] % 4 == 0 && a->cs_stride[1] % 4 == 0,
                  "cos / sin must be 16-byte aligned with strides that are multiples of 4 elements");
     PITH_REQUIRE(a->cs_dtype == PITH_DTYPE_BF16 || a->cs_dtype == PITH_DTYPE_F32, "cos / sin must be bf16 or fp32");
   }
-  const int64_t* xs_in = a->x_stride;
-  PITH_REQUIRE(aligned16(a->x) && xs_in[0] % 8 == 0 && xs_in[1] % 8 == 0 && xs_in[2] % 8 == 0,
+  PITH_REQUIRE(aligned16(a->x) && p.qs[0] % 8 == 0 && p.qs[1] % 8 == 0 && p.qs[2] % 8 == 0,
                "%s must be 16-byte aligned with strides that are multiples of 8 elements", QUERY ? "q" : "attn");
-  PITH_REQUIRE((a->B == 1 || xs_in[0] > 0) && (a->S == 1 || xs_in[1] > 0) && (a->H == 1 || xs_in[2] > 0),
+  PITH_REQUIRE((a->B == 1 || p.qs[0] > 0) && (a->S == 1 || p.qs[1] > 0) && (a->H == 1 || p.qs[2] > 0),
                "%s must not repeat elements (an expanded view)", QUERY ? "q" : "attn");
   PITH_REQUIRE(aligned16(a->weight) && a->weight_stride > 0 && a->weight_stride % 8 == 0,
                "kv_b_weight must be 16-byte aligned with a row stride that is a multiple of 8 elements");
   PITH_REQUIRE(static_cast<int64_t>(a->B) * a->S < 2147483647 - 65536, "too many tokens");
   if (int rc = require_sm100()) return rc;
-  // One token axis where the strides allow it: a batch of single tokens fills the tiles.
+  // One token axis where the strides allow it: a batch of single tokens fills the tiles. The tensor maps want a stride for
+  // axes of one element too.
   int64_t B = a->B, S = a->S;
-  int64_t xs[3] = {a->x_stride[0], a->x_stride[1], a->x_stride[2]};
+  int64_t xs[3] = {p.qs[0], p.qs[1], axis_stride(a->H, p.qs[2], QUERY ? 192 : 512)};
   if (S == 1 || B == 1 || xs[0] == S * xs[1]) {
     if (S == 1) xs[1] = xs[0];
     S *= B;
     B = 1;
-    xs[0] = S * xs[1];
   }
-  if (a->H == 1) xs[2] = QUERY ? 192 : 512;  // strides of axes of one element say nothing
-  if (S == 1) xs[1] = a->H * xs[2];
-  if (B == 1) xs[0] = S * xs[1];
-  LatProjParams p = {};
+  xs[1] = axis_stride(S, xs[1], a->H * xs[2]);
+  xs[0] = axis_stride(B, xs[0], S * xs[1]);
   p.q = static_cast<const __nv_bfloat16*>(a->x);
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.cos = a->cos; p.sin = a->sin; p.pos = a->positions; p.status = a->status;
   p.H = a->H; p.rows = static_cast<int>(S); p.by_s = FastDiv(a->S); p.cs_f32 = a->cs_dtype == PITH_DTYPE_F32;
   p.table_rows = a->table_rows;
-  for (int i = 0; i < 3; ++i) p.qs[i] = a->x_stride[i];
   for (int i = 0; i < 2; ++i) { p.cs[i] = a->cs_stride[i]; p.pos_s[i] = a->positions_stride[i]; }
   int dev = 0, sms = 148;
   PITH_CUDA(cudaGetDevice(&dev));

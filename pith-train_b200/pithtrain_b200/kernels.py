@@ -502,15 +502,16 @@ def _rotary(cos, sin, position_ids, B: int, S: int):
         if len(pshape) != 2 or pshape[0] not in (1, B) or pshape[1] != S:
             raise ValueError(f"position_ids has shape {tuple(pshape)}, expected {(B, S)}")
         pb, ps = position_ids.stride()
-        return (cos.data_ptr(), sin.data_ptr(), position_ids.data_ptr(), number, shape[0], 0, strides[0],
-                pb if pshape[0] > 1 else 0, ps)
+        return (cos.data_ptr(), sin.data_ptr(), position_ids.data_ptr(), number, shape[0], 0,
+                strides[0] if shape[0] > 1 else 0, pb if pshape[0] > 1 else 0, ps)
     if len(shape) == 2:
         if shape[0] < S:
             raise ValueError(f"cos and sin have {shape[0]} rows, {S} are needed")
-        return cos.data_ptr(), sin.data_ptr(), 0, number, 0, 0, strides[0], 0, 0
+        return cos.data_ptr(), sin.data_ptr(), 0, number, 0, 0, strides[0] if S > 1 else 0, 0, 0
     if len(shape) != 3 or shape[0] not in (1, B) or shape[1] != S:
         raise ValueError(f"cos and sin have shape {tuple(shape)}, expected [B or 1, {S}, 64]")
-    return cos.data_ptr(), sin.data_ptr(), 0, number, 0, strides[0] if shape[0] > 1 else 0, strides[1], 0, 0
+    return (cos.data_ptr(), sin.data_ptr(), 0, number, 0, strides[0] if shape[0] > 1 else 0, strides[1] if S > 1 else 0,
+            0, 0)
 
 
 def latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps: float, position_ids=None) -> None:

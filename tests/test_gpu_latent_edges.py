@@ -252,3 +252,38 @@ def test_a_negative_row_factor_reaches_only_the_rows_that_see_it(cuda_device):
     o = run_attention(q, cache, table, [300], SCALE)[0]
     check()
     assert torch.equal(o[0, :2], want[0, :2]) and o[0, 2:].isnan().all()
+
+
+def odd_axes(t):
+    """The same elements with strides of 3 on every axis of one element."""
+    return t.as_strided(t.shape, [3 if n == 1 else s for n, s in zip(t.shape, t.stride())], t.storage_offset())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("B,S,H", [(1, 1, 1), (5, 1, 16), (1, 7, 2), (3, 4, 1)])
+def test_strides_of_axes_of_one_element_say_nothing(cuda_device, dtype, B, S, H):
+    from pithtrain_b200.operators import mla
+    g = torch.Generator(device="cuda").manual_seed(B + S + H)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    kv, pe, q, w = rnd(B, S, 512), rnd(B, S, 1, 64), rnd(B, S, H, 192), rnd(H * 256, 512)
+    cos, sin = tables(S)
+    slots = torch.randperm(64, generator=g, device="cuda")[: B * S].view(B, S)
+    pos = torch.arange(S, device="cuda")[None]
+    lens = torch.tensor([64 if b == 0 else 40 for b in range(B)], dtype=torch.int32, device="cuda")
+    table = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    results = []
+    for turn in (lambda t: t, odd_axes):
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        cache, _ = one_context(gen, 64, 64, dtype, 0.0)
+        planes = [turn(t) if t is not None else None for t in (cache.latent, cache.rope, cache.scale)]
+        one = mla.LatentCache(*planes)
+        for c, s, p in ((cos, sin, pos), (cos[None], sin[None], None)):
+            mla.latent_cache_write(one, turn(slots), turn(kv), turn(pe), torch.ones(512, device="cuda"), turn(c), turn(s),
+                                   1e-6, position_ids=None if p is None else turn(p))
+            query = mla.latent_query(turn(q), w, turn(c), turn(s), None if p is None else turn(p))
+        o = mla.latent_attention(turn(query), one, turn(table), lens, SCALE)
+        y = mla.latent_output(turn(o), w)
+        check()
+        results.append([cache.latent.view(torch.uint8), cache.rope, query, o, y, *mla.latent_cache_read(one, turn(slots))])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
