@@ -6,8 +6,8 @@ import time
 import pytest
 import torch
 
-from test_gpu_latent import (E4M3, SCALE, assert_attention, check, filled_cache, make_cache, quantised, random_tree,
-                             run_attention, stored, tables, visible)
+from test_gpu_latent import (E4M3, SCALE, assert_attention, assert_product, assert_rounded, check, filled_cache, make_cache,
+                             quantised, random_tree, rotated, run_attention, stored, tables, visible)
 
 pytestmark = pytest.mark.gpu
 
@@ -287,3 +287,50 @@ def test_strides_of_axes_of_one_element_say_nothing(cuda_device, dtype, B, S, H)
         results.append([cache.latent.view(torch.uint8), cache.rope, query, o, y, *mla.latent_cache_read(one, turn(slots))])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+# The persistent projection kernel: batches that are not one token axis, more (batch, head) groups than SMs, and token counts
+# that are no multiple of a tile.
+@pytest.mark.parametrize("B,S,H", [(5, 300, 16), (10, 300, 16), (3, 4095, 2), (40, 129, 8), (2, 700, 80)])
+def test_projections_of_batches_that_are_no_single_token_axis(cuda_device, B, S, H):
+    from pithtrain_b200.operators.mla import latent_output, latent_query
+    g = torch.Generator(device="cuda").manual_seed(B * S + H)
+    w = (torch.randn(H * 256, 512, generator=g, device="cuda") / 20).bfloat16()
+    heads = w.view(H, 256, 512)
+    q = torch.randn(B, 2 * S, H, 192, generator=g, device="cuda").bfloat16()[:, S:]
+    cos, sin = tables(3000)
+    pos = torch.randint(0, 3000, (B, S), generator=g, device="cuda")
+    out = latent_query(q, w, cos, sin, position_ids=pos)
+    check()
+    assert_product(out[..., :512], q[..., :128], heads[:, :128], "query")
+    turned = rotated(q[..., 128:], cos[pos][:, :, None], sin[pos][:, :, None])
+    assert_rounded(out[..., 512:], turned, 2.0 ** -8, "rope", floor=2.0 ** -20)
+    gathered = latent_query(q, w, cos[pos], sin[pos])
+    assert torch.equal(out, gathered)
+    del q, turned, gathered, out
+    a = torch.randn(B, 2 * S, H, 512, generator=g, device="cuda").bfloat16()[:, S:]
+    y = latent_output(a, w)
+    check()
+    for b in range(B):
+        assert_product(y[b:b + 1], a[b:b + 1], heads[:, 128:].transpose(1, 2), "output")
+
+
+@pytest.mark.parametrize("bad", [4096, -1, 1 << 40])
+def test_a_position_out_of_range_among_many(cuda_device, bad):
+    """Reported by the warps that rotate tokens beside the GEMM of many; the next call is right."""
+    from pithtrain_b200 import kernels
+    from pithtrain_b200.operators.mla import latent_query
+    g = torch.Generator(device="cuda").manual_seed(110)
+    B, S, H, at = 2, 2500, 16, (1, 1234)
+    w = (torch.randn(H * 256, 512, generator=g, device="cuda") / 20).bfloat16()
+    q = torch.randn(B, S, H, 192, generator=g, device="cuda").bfloat16()
+    cos, sin = tables(4096)
+    pos = torch.randint(0, 4096, (B, S), generator=g, device="cuda")
+    want = latent_query(q, w, cos, sin, position_ids=pos)
+    off = pos.clone()
+    off[at] = bad
+    latent_query(q, w, cos, sin, position_ids=off)
+    with pytest.raises(RuntimeError, match="a position given"):
+        kernels.check_device_status()
+    assert torch.equal(latent_query(q, w, cos, sin, position_ids=pos), want)
+    check()
