@@ -21,6 +21,8 @@ at once. A sampling loop calls it where it fetches its tokens.
 
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
 from torch.autograd import forward_ad
 
@@ -122,6 +124,69 @@ class LatentCache:
         return self.latent.shape[1]
 
 
+# What a traced call becomes (``torch.compile``): ``torch.library`` custom ops with fake kernels, as the library's other CP = 1
+# operators. An eager call goes to the kernels directly; through an op it would cost the host several times as much.
+@torch.library.custom_op("pithtrain_b200::latent_cache_write", mutates_args=("latent", "rope", "scale"))
+def latent_cache_write_op(latent: torch.Tensor, rope: torch.Tensor, scale: Optional[torch.Tensor], slots: torch.Tensor,
+                          compressed_kv: torch.Tensor, k_pe: torch.Tensor, norm_weight: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, eps: float, position_ids: Optional[torch.Tensor]) -> None:
+    kernels.latent_write(LatentCache(latent, rope, scale), slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
+
+
+@latent_cache_write_op.register_fake
+def _(latent, rope, scale, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids):
+    return None
+
+
+@torch.library.custom_op("pithtrain_b200::latent_cache_read", mutates_args=())
+def latent_cache_read_op(latent: torch.Tensor, rope: torch.Tensor, scale: Optional[torch.Tensor],
+                         slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    return kernels.latent_read(LatentCache(latent, rope, scale), slots)
+
+
+@latent_cache_read_op.register_fake
+def _(latent, rope, scale, slots):
+    return rope.new_empty((*slots.shape, 512)), rope.new_empty((*slots.shape, 64))
+
+
+@torch.library.custom_op("pithtrain_b200::latent_attention", mutates_args=())
+def latent_attention_op(query: torch.Tensor, latent: torch.Tensor, rope: torch.Tensor, scale: Optional[torch.Tensor],
+                        block_table: torch.Tensor, seq_lens: torch.Tensor, softmax_scale: float,
+                        query_lens: Optional[torch.Tensor], tree_mask: Optional[torch.Tensor],
+                        return_lse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse); an empty tensor in the place of an LSE that was not asked for."""
+    out, lse = kernels.latent_attn(query, LatentCache(latent, rope, scale), block_table, seq_lens, softmax_scale, query_lens,
+                                   tree_mask, return_lse)
+    return out, lse if return_lse else query.new_empty(0, dtype=torch.float32)
+
+
+@latent_attention_op.register_fake
+def _(query, latent, rope, scale, block_table, seq_lens, softmax_scale, query_lens, tree_mask, return_lse):
+    b, s, h, _ = query.shape
+    return query.new_empty((b, s, h, 512)), query.new_empty((b, h, s) if return_lse else 0, dtype=torch.float32)
+
+
+@torch.library.custom_op("pithtrain_b200::latent_query", mutates_args=())
+def latent_query_op(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                    position_ids: Optional[torch.Tensor]) -> torch.Tensor:
+    return kernels.latent_query(q, kv_b_weight, cos, sin, position_ids)
+
+
+@latent_query_op.register_fake
+def _(q, kv_b_weight, cos, sin, position_ids):
+    return q.new_empty((*q.shape[:3], 576))
+
+
+@torch.library.custom_op("pithtrain_b200::latent_output", mutates_args=())
+def latent_output_op(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor:
+    return kernels.latent_output(attn, kv_b_weight)
+
+
+@latent_output_op.register_fake
+def _(attn, kv_b_weight):
+    return attn.new_empty((*attn.shape[:3], 128))
+
+
 def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: torch.Tensor, k_pe: torch.Tensor,
                        norm_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, eps: float,
                        position_ids: torch.Tensor | None = None) -> None:
@@ -135,7 +200,10 @@ def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: t
     scale with which no value passes 448.
     """
     _refuse_gradients("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, *cache._planes)
-    kernels.latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
+    if torch.compiler.is_compiling():
+        latent_cache_write_op(*cache._planes, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
+    else:
+        kernels.latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
 
 
 def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
@@ -143,6 +211,8 @@ def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
     prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
     give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
     _refuse_gradients("latent_cache_read", *cache._planes)
+    if torch.compiler.is_compiling():
+        return latent_cache_read_op(*cache._planes, slots)
     return kernels.latent_read(cache, slots)
 
 
@@ -170,7 +240,11 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     and the LSE take the weights unrounded, in fp32.
     """
     _refuse_gradients("latent_attention", query, *cache._planes)
-    out, lse = kernels.latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask, return_lse)
+    if torch.compiler.is_compiling():
+        out, lse = latent_attention_op(query, *cache._planes, block_table, seq_lens, softmax_scale, query_lens, tree_mask,
+                                       return_lse)
+    else:
+        out, lse = kernels.latent_attn(query, cache, block_table, seq_lens, softmax_scale, query_lens, tree_mask, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -182,6 +256,8 @@ def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, 
     ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
     cos / sin / position_ids as in ``latent_cache_write``."""
     _refuse_gradients("latent_query", q, kv_b_weight, cos, sin)
+    if torch.compiler.is_compiling():
+        return latent_query_op(q, kv_b_weight, cos, sin, position_ids)
     return kernels.latent_query(q, kv_b_weight, cos, sin, position_ids)
 
 
@@ -189,4 +265,6 @@ def latent_output(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor
     """``latent_attention``'s result ``[B,S,H,512]`` times head h's value rows of ``kv_b_weight``: ``[B,S,H,128]`` bf16,
     contiguous, which the layer views as ``[B,S,H * 128]`` for ``o_proj``."""
     _refuse_gradients("latent_output", attn, kv_b_weight)
+    if torch.compiler.is_compiling():
+        return latent_output_op(attn, kv_b_weight)
     return kernels.latent_output(attn, kv_b_weight)

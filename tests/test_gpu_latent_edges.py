@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_gpu_latent import (E4M3, SCALE, assert_attention, assert_product, assert_rounded, check, filled_cache, make_cache,
-                             quantised, random_tree, rotated, run_attention, stored, tables, visible)
+                             quantised, random_tree, rotated, run_attention, slots_of, stored, tables, visible)
 
 pytestmark = pytest.mark.gpu
 
@@ -333,4 +333,68 @@ def test_a_position_out_of_range_among_many(cuda_device, bad):
     with pytest.raises(RuntimeError, match="a position given"):
         kernels.check_device_status()
     assert torch.equal(latent_query(q, w, cos, sin, position_ids=pos), want)
+    check()
+
+
+def step_inputs(g, dtype, B, H, n):
+    """A layer of a larger cache with n keys a sequence, and the tensors of a decoding step: (planes, args)."""
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    pages = B * (-(-n // 64) + 1)
+    lat, rope = torch.zeros(pages, 2, 64, 512, device="cuda").to(dtype), torch.zeros(pages, 2, 64, 64, device="cuda").bfloat16()
+    scale = torch.ones(pages, 2, 64, device="cuda") if dtype == E4M3 else None
+    planes = [t[:, 1] if t is not None else None for t in (lat, rope, scale)]
+    table = torch.randperm(pages, generator=g, device="cuda").int().view(B, -1)
+    slots = torch.stack([slots_of(t, n, 64) for t in table])
+    cos, sin = tables(n + 1)
+    return planes, dict(slots=slots, proj=rnd(B, n, 576), q=rnd(B, 1, H, 192), table=table, w=rnd(H * 256, 512) / 20,
+                        lens=torch.full((B,), n, dtype=torch.int32, device="cuda"), cos=cos, sin=sin, norm=rnd(512),
+                        pos=torch.arange(n, device="cuda")[None])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_a_compiled_step_is_the_eager_one(cuda_device, dtype):
+    """All five operators inside torch.compile(fullgraph=True): one graph, the same results, the same cache."""
+    from pithtrain_b200.operators import mla
+
+    def step(cache, a):
+        mla.latent_cache_write(cache, a["slots"], a["proj"][..., :512] * 1.0, a["proj"][..., 512:], a["norm"], a["cos"],
+                               a["sin"], 1e-6, position_ids=a["pos"])
+        query = mla.latent_query(a["q"] * 1.0, a["w"], a["cos"], a["sin"], position_ids=a["pos"][:, -1:])
+        latent, pe = mla.latent_cache_read(cache, a["slots"][:, -3:])
+        o, lse = mla.latent_attention(query, cache, a["table"], a["lens"], SCALE, return_lse=True)
+        only = mla.latent_attention(query, cache, a["table"], a["lens"], SCALE, query_lens=torch.ones_like(a["lens"]))
+        return mla.latent_output(o, a["w"]) + 0.0, lse, only, latent, pe
+
+    results = []
+    torch._dynamo.reset()
+    for fn in (step, torch.compile(step, fullgraph=True)):
+        g = torch.Generator(device="cuda").manual_seed(120)
+        planes, a = step_inputs(g, dtype, 3, 16, 200)
+        with torch.no_grad():
+            out = fn(mla.LatentCache(*planes), a)
+        check()
+        results.append([*out, *(t.contiguous().view(torch.uint8) for t in planes if t is not None)])
+    for a, b in zip(*results):
+        assert a.shape == b.shape and a.dtype == b.dtype and torch.equal(a, b)
+    assert results[0][0].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_fake_kernels_describe_the_real_outputs(cuda_device, dtype):
+    from pithtrain_b200.operators.mla import latent
+    g = torch.Generator(device="cuda").manual_seed(121)
+    planes, a = step_inputs(g, dtype, 2, 4, 70)
+    # the schema check compares inputs before and after with operations that PyTorch has not for 8-bit floats
+    utils = ("test_schema", "test_faketensor") if dtype == torch.bfloat16 else ("test_faketensor",)
+    pos = a["pos"][:, -1:]
+    query = latent.latent_query_op(a["q"], a["w"], a["cos"], a["sin"], pos)
+    with torch.no_grad():
+        torch.library.opcheck(latent.latent_cache_write_op, (*planes, a["slots"], a["proj"][..., :512], a["proj"][..., 512:],
+                                                             a["norm"], a["cos"], a["sin"], 1e-6, a["pos"]), test_utils=utils)
+        torch.library.opcheck(latent.latent_cache_read_op, (*planes, a["slots"]), test_utils=utils)
+        for lse in (False, True):
+            torch.library.opcheck(latent.latent_attention_op, (query, *planes, a["table"], a["lens"], SCALE, None, None, lse),
+                                  test_utils=utils)
+        torch.library.opcheck(latent.latent_query_op, (a["q"], a["w"], a["cos"], a["sin"], pos), test_utils=utils)
+        torch.library.opcheck(latent.latent_output_op, (query[..., :512], a["w"]), test_utils=utils)
     check()

@@ -315,3 +315,21 @@ def test_cabi_projections_name_the_argument_that_is_off(built_library):
             a.x_stride[i] = 0
             assert entry(ctypes.byref(a), None) < 0 and name + b" not repeat" in lib.pith_last_error()
             a.x_stride[i] = old
+
+
+@pytest.mark.parametrize("name", ["latent_cache_write", "latent_cache_read", "latent_attention", "latent_query",
+                                  "latent_output"])
+def test_a_traced_call_is_one_op(name):
+    """torch.compile(fullgraph=True) sees one custom op, whose fake kernel knows the result; run, it is the kernel's call."""
+    call, args, c = calls()[name]
+    seen = []
+
+    def backend(gm, inputs):
+        seen.extend(n for n in gm.graph.nodes if n.op == "call_function" and "pithtrain_b200" in str(n.target))
+        return gm.forward
+
+    torch._dynamo.reset()
+    fn = torch.compile(lambda a: call(a, c), backend=backend, fullgraph=True)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        fn(args)
+    assert [str(n.target).split(".")[1] for n in seen] == [name]
