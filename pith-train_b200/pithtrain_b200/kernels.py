@@ -479,9 +479,14 @@ def _enqueue(entry: str, args: bytes, idx: int, launches: int) -> None:
         post_status_copy(torch.device("cuda", idx))
 
 
+_status_ptrs: dict[int, int] = {}  # a status word stays where it is
+
+
 def _status_ptr(idx: int) -> int:
-    w = _status_words.get(idx)
-    return (w if w is not None else status_word(torch.device("cuda", idx))).data_ptr()
+    p = _status_ptrs.get(idx)
+    if p is None:
+        p = _status_ptrs[idx] = status_word(torch.device("cuda", idx)).data_ptr()
+    return p
 
 
 def _rotary(cos, sin, position_ids, B: int, S: int):
@@ -536,7 +541,7 @@ def latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps: 
         raise ValueError(f"slots has shape {tuple(slots.shape)}, expected {(B, S)}")
     cp, sp, pp, cs_number, rows, cs0, cs1, ps0, ps1 = _rotary(cos, sin, position_ids, B, S)
     idx = _device_index("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, slots, position_ids,
-                        cache.latent)
+                        cache._planes[0])
     sl0, sl1 = slots.stride()
     args = _WRITE(*cache.flat, compressed_kv.data_ptr(), k_pe.data_ptr(), norm_weight.data_ptr(), cp, sp,
                   slots.data_ptr(), pp, _status_ptr(idx), B, S, w_number, cs_number, rows, eps,
@@ -548,12 +553,13 @@ def latent_read(cache, slots):
     """(latent bf16 [..., 512], k_pe bf16 [..., 64]) of the given slots; see ``pith_latent_read``."""
     if slots.dtype != torch.int64:
         raise TypeError("slots must be int64")
-    idx = _device_index("latent_cache_read", slots, cache.latent)
+    idx = _device_index("latent_cache_read", slots, cache._planes[0])
     if not slots.is_contiguous():
         slots = slots.contiguous()
     shape, n = slots.shape, slots.numel()
-    latent = cache.rope.new_empty((*shape, 512))
-    k_pe = cache.rope.new_empty((*shape, 64))
+    rope = cache._planes[1]
+    latent = rope.new_empty((*shape, 512))
+    k_pe = rope.new_empty((*shape, 64))
     args = _READ(*cache.flat, slots.data_ptr(), latent.data_ptr(), k_pe.data_ptr(), _status_ptr(idx), n)
     _enqueue("pith_latent_read", args, idx, 1 if n else 0)
     return latent, k_pe
@@ -603,7 +609,7 @@ def latent_attn(query, cache, block_table, seq_lens, softmax_scale: float, query
     max_keys = t_shape[1] * planes[5]
     if max_keys > _INT32_MAX:
         raise ValueError(f"block_table covers {max_keys} keys a sequence")
-    idx = _device_index("latent_attention", query, cache.latent, block_table, seq_lens, query_lens, tree_mask)
+    idx = _device_index("latent_attention", query, cache._planes[0], block_table, seq_lens, query_lens, tree_mask)
     out = query.new_empty((B, S, H, 512))
     lse = query.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
     # allocated per call on the current stream: calls on other streams and captured graphs each have their own

@@ -28,9 +28,12 @@ from torch.autograd import forward_ad
 
 from ... import _lib, kernels
 
+_is_compiling = torch.compiler.is_compiling
+
 
 def _refuse_gradients(what: str, *inputs) -> None:
-    """Raises where one of the inputs (tensors or None) wants a gradient: backward under grad mode, or forward mode."""
+    """Raises where one of the inputs (tensors or None) wants a gradient: backward under grad mode, or forward mode. The operators
+    come here only if there may be one: as a loop over all inputs it costs an eager call half a microsecond."""
     if torch.is_grad_enabled():
         for t in inputs:
             if t is not None and t.requires_grad:
@@ -52,7 +55,7 @@ class LatentCache:
 
     def __init__(self, latent: torch.Tensor, rope: torch.Tensor, scale: torch.Tensor | None = None):
         self._planes = (latent, rope, scale)
-        self._at = self._flat = None
+        self._flat = None
         self._check()
 
     def _check(self) -> None:
@@ -82,18 +85,19 @@ class LatentCache:
     def flat(self) -> tuple:
         """The fields of ``pith_latent_cache``, in order, of the planes as they are now."""
         latent, rope, scale = self._planes
-        at = (latent.data_ptr(), rope.data_ptr(), scale.data_ptr() if scale is not None else 0)
-        if at != self._at:  # the first call, or a plane has moved
+        flat = self._flat
+        if flat is None or latent.data_ptr() != flat[0] or rope.data_ptr() != flat[1] \
+                or scale is not None and scale.data_ptr() != flat[2]:  # the first call, or a plane has moved
             self._check()
             for t in self._planes:
                 if t is not None:
                     end = t.storage_offset() + 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
                     if t.untyped_storage().nbytes() < end * t.element_size():
                         raise RuntimeError("the memory of a plane of the latent cache has been released")
-            self._flat = (*at, _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, *latent.shape[:2],
-                          *latent.stride()[:2], *rope.stride()[:2], *(scale.stride() if scale is not None else (0, 0)))
-            self._at = at
-        return self._flat
+            flat = self._flat = (latent.data_ptr(), rope.data_ptr(), 0 if scale is None else scale.data_ptr(),
+                                 _lib.DTYPE_BF16 if scale is None else _lib.DTYPE_E4M3, *latent.shape[:2],
+                                 *latent.stride()[:2], *rope.stride()[:2], *(scale.stride() if scale is not None else (0, 0)))
+        return flat
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -114,6 +118,11 @@ class LatentCache:
     @property
     def scale(self) -> torch.Tensor | None:
         return self._planes[2]
+
+    @property
+    def requires_grad(self) -> bool:
+        latent, rope, scale = self._planes
+        return latent.requires_grad or rope.requires_grad or (scale is not None and scale.requires_grad)
 
     @property
     def num_pages(self) -> int:
@@ -199,8 +208,11 @@ def latent_cache_write(cache: LatentCache, slots: torch.Tensor, compressed_kv: t
     already gathered. fp32 arithmetic, one rounding to the cache's type; an 8-bit row gets the least power of two as its
     scale with which no value passes 448.
     """
-    _refuse_gradients("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, *cache._planes)
-    if torch.compiler.is_compiling():
+    if torch.is_grad_enabled() and (compressed_kv.requires_grad or k_pe.requires_grad or norm_weight.requires_grad or
+                                    cos.requires_grad or sin.requires_grad or cache.requires_grad) \
+            or forward_ad._current_level >= 0:
+        _refuse_gradients("latent_cache_write", compressed_kv, k_pe, norm_weight, cos, sin, *cache._planes)
+    if _is_compiling():
         latent_cache_write_op(*cache._planes, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
     else:
         kernels.latent_write(cache, slots, compressed_kv, k_pe, norm_weight, cos, sin, eps, position_ids)
@@ -210,8 +222,9 @@ def latent_cache_read(cache: LatentCache, slots: torch.Tensor):
     """Rows of the cache as bf16, ``(latent [*slots.shape, 512], k_pe [*slots.shape, 64])``: what the expanded form of a
     prompt's next chunk takes for its cached prefix (``kv_b_proj(latent)``; ``k_pe`` is rotated already). Negative slots
     give zeros. Rows that ``latent_cache_write`` stored in 8 bits are exact in bf16."""
-    _refuse_gradients("latent_cache_read", *cache._planes)
-    if torch.compiler.is_compiling():
+    if torch.is_grad_enabled() and cache.requires_grad or forward_ad._current_level >= 0:
+        _refuse_gradients("latent_cache_read", *cache._planes)
+    if _is_compiling():
         return latent_cache_read_op(*cache._planes, slots)
     return kernels.latent_read(cache, slots)
 
@@ -239,8 +252,9 @@ def latent_attention(query: torch.Tensor, cache: LatentCache, block_table: torch
     in an 8-bit cache to steps of 2^-17 of the largest at least, upwards or downwards key by key so that sums are kept. Row sums
     and the LSE take the weights unrounded, in fp32.
     """
-    _refuse_gradients("latent_attention", query, *cache._planes)
-    if torch.compiler.is_compiling():
+    if torch.is_grad_enabled() and (query.requires_grad or cache.requires_grad) or forward_ad._current_level >= 0:
+        _refuse_gradients("latent_attention", query, *cache._planes)
+    if _is_compiling():
         out, lse = latent_attention_op(query, *cache._planes, block_table, seq_lens, softmax_scale, query_lens, tree_mask,
                                        return_lse)
     else:
@@ -255,8 +269,10 @@ def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, 
     ``[B,S,H,576]`` bf16, ``q_nope`` times head h's key rows of
     ``kv_b_weight`` ``[H * 256, 512]`` (``kv_b_proj.weight`` as it is), and ``q_pe`` rotated as the cached keys.
     cos / sin / position_ids as in ``latent_cache_write``."""
-    _refuse_gradients("latent_query", q, kv_b_weight, cos, sin)
-    if torch.compiler.is_compiling():
+    if torch.is_grad_enabled() and (q.requires_grad or kv_b_weight.requires_grad or cos.requires_grad or sin.requires_grad) \
+            or forward_ad._current_level >= 0:
+        _refuse_gradients("latent_query", q, kv_b_weight, cos, sin)
+    if _is_compiling():
         return latent_query_op(q, kv_b_weight, cos, sin, position_ids)
     return kernels.latent_query(q, kv_b_weight, cos, sin, position_ids)
 
@@ -264,7 +280,8 @@ def latent_query(q: torch.Tensor, kv_b_weight: torch.Tensor, cos: torch.Tensor, 
 def latent_output(attn: torch.Tensor, kv_b_weight: torch.Tensor) -> torch.Tensor:
     """``latent_attention``'s result ``[B,S,H,512]`` times head h's value rows of ``kv_b_weight``: ``[B,S,H,128]`` bf16,
     contiguous, which the layer views as ``[B,S,H * 128]`` for ``o_proj``."""
-    _refuse_gradients("latent_output", attn, kv_b_weight)
-    if torch.compiler.is_compiling():
+    if torch.is_grad_enabled() and (attn.requires_grad or kv_b_weight.requires_grad) or forward_ad._current_level >= 0:
+        _refuse_gradients("latent_output", attn, kv_b_weight)
+    if _is_compiling():
         return latent_output_op(attn, kv_b_weight)
     return kernels.latent_output(attn, kv_b_weight)
