@@ -351,7 +351,7 @@ int pith_mla_assemble_bwd(const pith_mla_assemble_args* args, void* stream);
 typedef struct pith_latent_cache {
   void* latent;              /* [pages][page_size][512]: bf16, or e4m3 with one factor a row */
   void* rope;                /* [pages][page_size][64] bf16, de-interleaved and rotated */
-  float* scale;              /* [pages][page_size] fp32, e4m3 only: row = stored * scale */
+  float* scale;              /* [pages][page_size] fp32, e4m3 only: row = stored * scale; not negative, at least 2^-100 */
   int32_t dtype;             /* PITH_DTYPE_BF16 or PITH_DTYPE_E4M3 */
   int32_t pages, page_size;  /* page_size 16, 32 or a multiple of 64 */
   int64_t latent_stride[2], rope_stride[2], scale_stride[2]; /* page, row (elements); innermost contiguous */
@@ -416,8 +416,9 @@ typedef struct pith_latent_attn_args {
  * Attention in the absorbed MLA form over the cache: all H heads of the Sq new tokens of a sequence read the same keys.
  * With n keys and m new tokens, token i sees key k iff k <= n - m + i, or with a tree mask iff k < n - m or
  * tree_mask[i][k - (n - m)]. A row that sees nothing, or has no token, gives out 0, lse -inf. Keys are read up to
- * seq_lens only: pages behind it need not exist. Two launches, or one where no
- * sequence can pass 128 keys, or 1024 and cutting them over the SMs would not pay.
+ * seq_lens only: pages behind it need not exist. Softmax weights are rounded to bf16, or for an e4m3 cache to steps of 2^-17
+ * of the largest of a part of the keys at least, upwards or downwards key by key so that sums are kept; row sums and lse are fp32.
+ * Two launches, or one where no sequence can pass 128 keys, or 1024 and cutting them over the SMs would not pay.
  */
 int pith_latent_attn(const pith_latent_attn_args* args, void* stream);
 size_t pith_latent_attn_workspace_bytes(int32_t B, int32_t Sq, int32_t H, int64_t max_keys, int32_t cache_dtype);

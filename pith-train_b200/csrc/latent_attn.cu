@@ -14,8 +14,8 @@
 // An 8-bit cache stays 8-bit up to the tensor core (kind::f8f6f4). The bf16 query is split into two e4m3 terms
 // q 2^-k = hi + lo / 16 (8 significant bits, all that bf16 has, down to 2^-13 of the row's largest element, and 2^-22 of it
 // absolutely), the weights likewise, and hi and lo are separate columns of the same MMA: an MMA of 128 x N x 32 bytes costs
-// 39.5 cycles at N = 16, 40.6 at 32, 48.6 at 64 (what bounds it is reading A from shared memory), so the second half is
-// nearly free. The row factor of a key enters the score in registers and the weight as w_n = 2^(s_n + log2 scale_n - ref):
+// 39.6 cycles at N = 16, 40.6 at 32, 48.7 at 64 (what bounds it is reading A from shared memory; microbench/latent_mma_rate.cu),
+// so the second half is nearly free. The row factor of a key enters the score in registers and the weight as w_n = 2^(s_n + log2 scale_n - ref):
 // ref is the running maximum of s_n + log2 scale_n (or up to 2^4 below it). The two terms hold weights above 2^-9 of the
 // reference to 2^-9 of themselves; below that their steps are 2^-17 of the reference, whatever the weight. Rounded to the
 // nearest step, the many small weights behind one large one (a context whose first token outweighs each other one by 2^18)
@@ -24,6 +24,9 @@
 // what the weight is of a step, and sums over keys keep their value. What is left is the scatter of c over the keys that were
 // rounded up, at most sqrt(2^-17 W) of it for small weights that add up to W references, against a sum of at least 1 + W:
 // below 2^-9 of the result at any number of keys. The row sums take the weights as they were.
+// With a bf16 cache the weights are rounded to bf16, 2^-8 of each at most: both operands of that MMA have one type, and a second
+// term of 8 more bits would double the columns, which TMEM has not for 64 rows. The results are 0.0019 to 0.0021 of their norm
+// from 64 bits; their own rounding is 0.0017.
 //
 // Work split: the (sequence, row tile, 64 keys) units of the launch form one line which is cut into one equal piece per
 // CTA, so any mix of lengths is balanced without a schedule from the host (lengths are read on the device; short sequences
@@ -39,7 +42,7 @@
 //
 // Measured (16 heads, CUDA events over a captured graph): 64 sequences of 130 to 8191 keys, bf16: 65 us, 4.8 TB/s, 0.74 of
 // the measured copy rate; the loop itself streams 6 TB/s, the rest is 3 us until the first load, the pieces' ends and the
-// merge. 8 sequences of 9000 to 131071 keys, e4m3: 75 us, 5.5 TB/s, 0.86. Shorter tiles (64 keys, more of the ring in
+// merge. 8 sequences of 9000 to 131071 keys, e4m3: 76 us, 5.5 TB/s, 0.85. Shorter tiles (64 keys, more of the ring in
 // flight) were slower: 75 and 122 us. 250 tokens of a prompt over 6001 keys, bf16: 78 us, 650 TFLOP/s, the serial chain score
 // GEMM (2.2k cycles) - softmax (1.5k) - output GEMM (1.5k) of a tile; the expanded form is the one for long chunks. 16 trees
 // of 13 tokens over 500 to 4097 keys, e4m3: 48 us; a tile takes 2600 cycles (its MMAs 1750), as the slots of the tile after

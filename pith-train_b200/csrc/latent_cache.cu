@@ -7,9 +7,9 @@
 // One warp per token: a lane holds 16 of the 512 values (two 16-byte loads, 512 contiguous bytes a warp instruction), the
 // row sum and maximum are five shuffles each, and every lane rotates one pair of inputs into outputs j and 32 + j. Loads of a
 // token are issued before the first use; the kernels are bound by HBM at prompt sizes and by the launch at decode sizes.
-// Measured: 64 tokens 2.1 us; 8191 tokens into an 8-bit cache 6.3 us, back out of it 5.9 us (one token a warp, so that two
-// dependent loads and the launch are most of it); 32768 rows of a bf16 cache 13.0 us = 5.8 TB/s, 0.91 of the measured copy
-// rate.
+// Measured: 64 tokens 2.0 us; 8191 tokens into an 8-bit cache and back out of it 13 us, into a bf16 one 7.7 us (one token a warp,
+// so that two dependent loads and the launch are most of it); 32768 rows of a bf16 cache 12.6 us = 6.0 TB/s, 0.93 of the
+// measured copy rate.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
 #include "host_common.h"
@@ -98,7 +98,7 @@ __device__ __forceinline__ void unpack_e4m3x4(uint32_t v, float* f) {
   }
 }
 
-// 48 registers: five CTAs an SM, so that 8191 tokens are little more than one wave (with 16 weights and a whole rotation a lane
+// 48 registers: five CTAs an SM, so that 8191 tokens are 1.4 waves (with 16 weights and a whole rotation a lane
 // held from the start 73, and 7.2 instead of 6.3 us).
 template <bool FP8, bool CS32, bool W32>
 __global__ void __launch_bounds__(256, 5) latent_write_kernel(const LatentWriteParams p) {

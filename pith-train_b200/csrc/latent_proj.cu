@@ -7,8 +7,8 @@
 // W is used as the layer holds it: the query's B operand is read MN-major, the output's K-major; tcgen05 with accumulators in
 // TMEM, results stored by TMA, which clips the rows behind the last token. A row moves 1.5 KB (query) or 1.3 KB (output) for
 // 131 kFLOP: HBM bounds both at prompt sizes, latency at decode sizes, where narrow tiles spread the reading of W over more
-// CTAs (a kernel of one tile per CTA). Measured, 16 heads: 32 tokens 3.6 us (query) and 4.4 us (output); 4095 tokens 22.3 us
-// = 4.6 TB/s (0.71 of the measured copy rate) and 18.4 us = 4.7 TB/s (0.72), of which the launch, W and the first tile
+// CTAs (a kernel of one tile per CTA). Measured, 16 heads: 32 tokens 3.5 us (query) and 4.5 us (output); 4095 tokens 22.3 us
+// = 4.6 TB/s (0.71 of the measured copy rate) and 18.5 us = 4.7 TB/s (0.72), of which the launch, W and the first tile
 // take about 4 us.
 #include "../../include/pith_b200.h"
 #include "common.cuh"
