@@ -11,12 +11,13 @@ head h's block of ``kv_b_proj.weight``,
 so the query takes ``W_k`` in, attention runs on the latent vectors themselves, and its result goes through ``W_v``.
 
 These operators have no gradients (training keeps the expanded form): under grad mode, inputs that require one are
-refused, and so are tangents of forward-mode differentiation. Sizes are DeepSeek-V2-Lite's (latent 512, rope 64, nope 128, v 128), any number of heads; bf16, CUDA only.
-Indices are read on the device, so a slot, page, position or length out of range cannot raise at the call: nothing outside the
-tensors is touched, the error is recorded, and later kernels of the library skip their work, so that their outputs hold
-nothing. A later call of these or the attention operators raises, as soon as the news has reached the host (about ten milliseconds;
-not while a graph is being captured, and replays do not look); ``pithtrain_b200.kernels.check_device_status()`` waits and raises
-at once. A sampling loop calls it where it fetches its tokens.
+refused, and so are tangents of forward-mode differentiation. Sizes are DeepSeek-V2-Lite's (latent 512, rope 64, nope
+128, v 128), any number of heads; bf16, CUDA only. Indices are read on the device, so a slot, page, position or length
+out of range cannot raise at the call: nothing outside the tensors is touched, the error is recorded, and later kernels
+of the library skip their work, so that their outputs hold nothing. A later call of these or the attention operators
+raises as soon as the news has reached the host (about ten milliseconds; not while a graph is being captured, and
+replays do not look); ``pithtrain_b200.kernels.check_device_status()`` waits and raises at once. A sampling loop calls
+it where it fetches its tokens.
 """
 
 from __future__ import annotations
